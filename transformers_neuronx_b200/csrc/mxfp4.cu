@@ -1,0 +1,222 @@
+// Rows to microscaled 4 bits and back, and the product for sizes that no tensor map can address.  Formats: mxfp4.cuh.
+#include "mxfp4.cuh"
+
+namespace {
+
+__device__ __forceinline__ uint32_t pack_e2m1x8(const float (&v)[8]) {
+    uint32_t r;
+    asm("{\n\t.reg .b8 b0, b1, b2, b3;\n\t"
+        "cvt.rn.satfinite.e2m1x2.f32 b0, %2, %1;\n\t"
+        "cvt.rn.satfinite.e2m1x2.f32 b1, %4, %3;\n\t"
+        "cvt.rn.satfinite.e2m1x2.f32 b2, %6, %5;\n\t"
+        "cvt.rn.satfinite.e2m1x2.f32 b3, %8, %7;\n\t"
+        "mov.b32 %0, {b0, b1, b2, b3};\n\t}"
+        : "=r"(r) : "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]));
+    return r;
+}
+
+// Four neighbouring lanes hold a block, eight values each.  The block's exponent is the smallest e with max |x| <= 6 * 2^e, read off the
+// largest value's bits: m = 1.f * 2^x needs e = x - 2 up to f = 1.5 and x - 1 beyond.  Bits compared as whole numbers put infinities and
+// NaN above every finite value, so one comparison finds them.  x * 2^-e is exact (or far below the smallest code), its conversion rounds
+// to the nearest code, ties to even.
+__device__ __forceinline__ uint32_t quantize8(const float (&v)[8], uint32_t& E) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(v[i]) & 0x7FFFFFFFu);
+    m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
+    m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
+    const int e = (int)(m >> 23) - 2 + ((m & 0x7FFFFFu) > 0x400000u ? 1 : 0);
+    if (m >= 0x7F800000u) { E = 255u; return 0u; }
+    E = (uint32_t)max(e, 0);
+    const float inv = __uint_as_float((254u - E) << 23);          // E <= 253 for finite values
+    float s[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) s[i] = v[i] * inv;
+    return pack_e2m1x8(s);
+}
+
+// One read of the values, one write of codes and scales: bound by memory.  `items` = rows * blocks * 4 pieces of eight values.
+template <typename T, bool WHOLE>
+__global__ void __launch_bounds__(256) quantize_kernel(const T* __restrict__ x, long long ld, uint32_t* __restrict__ codes, uint8_t* __restrict__ scales,
+                                                       long long items, int blocks, int K) {
+    pdl_launch_dependents();             // the products read codes behind their own wait
+    pdl_wait();
+    const long long stride = (long long)gridDim.x * blockDim.x;
+    // whole warps walk the loop: the block's largest value is found by lanes together
+    for (long long i0 = (long long)blockIdx.x * blockDim.x + (threadIdx.x & ~31u); i0 < items; i0 += stride) {
+        const long long i = i0 + (threadIdx.x & 31u);
+        float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+        if (i < items) {
+            const long long row = i / (4 * blocks);
+            const int k = (int)(i - row * (4 * blocks)) * 8;
+            const T* src = x + row * ld + k;
+            if (WHOLE) { Vec8<T> q; q.load(src); q.get(v); }
+            else {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) if (k + j < K) v[j] = to_float(src[j]);
+            }
+        }
+        uint32_t E;
+        const uint32_t c = quantize8(v, E);
+        if (i < items) {
+            codes[i] = c;
+            if ((i & 3) == 0) scales[i >> 2] = (uint8_t)E;
+        }
+    }
+}
+
+// Eight values a thread; no kernel behind it starts early, because a product may take the values for a matrix that no kernel writes.  In 32 bits and in bfloat16 every value is exact; float16 rounds what lies outside its range.
+template <typename T>
+__global__ void __launch_bounds__(256) dequantize_kernel(const uint32_t* __restrict__ codes, const uint8_t* __restrict__ scales, T* __restrict__ out, long long ld,
+                                                         long long items, int blocks, int K, int vec) {
+    pdl_wait();
+    const long long stride = (long long)gridDim.x * blockDim.x;
+    for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < items; i += stride) {
+        const long long row = i / (4 * blocks);
+        const int k = (int)(i - row * (4 * blocks)) * 8;
+        if (k >= K) continue;
+        const uint32_t c = codes[i];
+        const float s = mx_scale(scales[i >> 2]);
+        float v[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = mx_code(c >> (4 * j)) * s;
+        T* dst = out + row * ld + k;
+        if (vec && k + 8 <= K) { Vec8<T> q; q.set(v); q.store(dst); }
+        else
+            for (int j = 0; j < 8 && k + j < K; ++j) dst[j] = from_float<T>(v[j]);
+    }
+}
+
+// The product on the multiply-add units, any sizes, pitches and alignments: a warp per feature (gated: per pair of them) and eight tokens,
+// its lanes walk K in pieces of eight codes, 32-bit sums, one order for every number of tokens.
+constexpr int SIMT_TOKENS = 8, SIMT_WARPS = 4;
+struct SimtParams {
+    const void* a; long long lda; int a_kind;              // 0: h16, 1: float, 2: codes (lda then counts blocks)
+    const uint8_t* a_scales;
+    const uint8_t* codes; const uint8_t* scales;
+    const float* bias; const float* residual; void* out; long long ldc;
+    int M, N, K, blocks, act, gated, out_h16;               // N: features of the result; gated: the up rows begin at row N
+};
+
+__device__ __forceinline__ uint32_t load_codes(const uint8_t* p) {
+    return ((uintptr_t)p & 3) == 0 ? *(const uint32_t*)p : (uint32_t)p[0] | (uint32_t)p[1] << 8 | (uint32_t)p[2] << 16 | (uint32_t)p[3] << 24;
+}
+
+__global__ void __launch_bounds__(32 * SIMT_WARPS) simt_kernel(const SimtParams p) {
+    pdl_wait();
+    const int lane = threadIdx.x & 31;
+    const int n = blockIdx.x * SIMT_WARPS + (threadIdx.x >> 5);
+    const int m0 = blockIdx.y * SIMT_TOKENS;
+    if (n >= p.N) return;
+    float sum[2][SIMT_TOKENS];
+#pragma unroll
+    for (int t = 0; t < SIMT_TOKENS; ++t) sum[0][t] = sum[1][t] = 0.f;
+    for (int piece = lane; piece < p.blocks * 4; piece += 32) {
+        const int k = piece * 8;
+        float w[2][8];
+#pragma unroll
+        for (int g = 0; g < 2; ++g) {
+            if (g && !p.gated) break;
+            const long long row = n + (long long)g * p.N;
+            const uint32_t c = load_codes(p.codes + row * p.blocks * 16 + piece * 4);
+            const float s = mx_scale(p.scales[row * p.blocks + (piece >> 2)]);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) w[g][j] = mx_code(c >> (4 * j)) * s;
+        }
+#pragma unroll
+        for (int t = 0; t < SIMT_TOKENS; ++t) {
+            if (m0 + t >= p.M) break;
+            const long long row = m0 + t;
+            float x[8];
+            if (p.a_kind == 2) {
+                const uint32_t c = load_codes((const uint8_t*)p.a + row * p.blocks * 16 + piece * 4);
+                const float s = mx_scale(p.a_scales[row * p.blocks + (piece >> 2)]);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) x[j] = mx_code(c >> (4 * j)) * s;
+            } else {
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    x[j] = k + j >= p.K ? 0.f : p.a_kind ? ((const float*)p.a)[row * p.lda + k + j] : h16_to_float(((const h16*)p.a)[row * p.lda + k + j]);
+            }
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                sum[0][t] = fmaf(w[0][j], x[j], sum[0][t]);
+                if (p.gated) sum[1][t] = fmaf(w[1][j], x[j], sum[1][t]);
+            }
+        }
+    }
+#pragma unroll
+    for (int t = 0; t < SIMT_TOKENS; ++t) {
+        if (m0 + t >= p.M) break;
+        float v = warp_sum(sum[0][t]), u = p.gated ? warp_sum(sum[1][t]) : 0.f;
+        if (lane == 0) {
+            if (p.bias) { v += p.bias[n]; if (p.gated) u += p.bias[p.N + n]; }
+            v = apply_activation(v, p.act);
+            if (p.gated) v *= u;
+            const long long o = (long long)(m0 + t) * p.ldc + n;
+            if (p.residual) v += p.residual[o];
+            if (p.out_h16) ((h16*)p.out)[o] = float_to_h16(v);
+            else ((float*)p.out)[o] = v;
+        }
+    }
+}
+
+template <typename T>
+int launch_quantize(const void* x, long long ld, void* codes, void* scales, int rows, int K, int sms, cudaStream_t stream) {
+    const int blocks = (K + MX_BLOCK - 1) / MX_BLOCK;
+    const long long items = (long long)rows * blocks * 4;
+    const bool whole = K % MX_BLOCK == 0 && ld % 8 == 0 && ((uintptr_t)x & 15) == 0;
+    const long long want = (items + 255) / 256, most = (long long)sms * 8;
+    const dim3 grid((unsigned)(want < most ? want : most));
+    if (whole) return tnx_launch_ex(1, quantize_kernel<T, true>, grid, dim3(256), 0, stream, (const T*)x, ld, (uint32_t*)codes, (uint8_t*)scales, items, blocks, K);
+    return tnx_launch_ex(1, quantize_kernel<T, false>, grid, dim3(256), 0, stream, (const T*)x, ld, (uint32_t*)codes, (uint8_t*)scales, items, blocks, K);
+}
+
+template <typename T>
+int launch_dequantize(const void* codes, const void* scales, void* out, long long ld, int rows, int K, int sms, cudaStream_t stream) {
+    const int blocks = (K + MX_BLOCK - 1) / MX_BLOCK;
+    const long long items = (long long)rows * blocks * 4;
+    const int vec = ld % 8 == 0 && ((uintptr_t)out & 15) == 0;
+    const long long want = (items + 255) / 256, most = (long long)sms * 8;
+    const dim3 grid((unsigned)(want < most ? want : most));
+    return tnx_launch_ex(1, dequantize_kernel<T>, grid, dim3(256), 0, stream, (const uint32_t*)codes, (const uint8_t*)scales, (T*)out, ld, items, blocks, K, vec);
+}
+
+}  // namespace
+
+// x: [rows, K] of the 16-bit type or float, row pitch ld elements; codes 4-byte aligned.
+TNX_EXPORT int tnx_mxfp4_quantize(const void* x, int x_h16, long long ld, void* codes, void* scales, int rows, int K, int sms, cudaStream_t stream) {
+    if (rows <= 0) return 0;
+    if (K <= 0 || sms <= 0 || ((uintptr_t)codes & 3)) return TNX_ERR_BAD_ARG;
+    return x_h16 ? launch_quantize<h16>(x, ld, codes, scales, rows, K, sms, stream) : launch_quantize<float>(x, ld, codes, scales, rows, K, sms, stream);
+}
+
+TNX_EXPORT int tnx_mxfp4_dequantize(const void* codes, const void* scales, void* out, int out_h16, long long ld, int rows, int K, int sms, cudaStream_t stream) {
+    if (rows <= 0) return 0;
+    if (K <= 0 || sms <= 0 || ((uintptr_t)codes & 3)) return TNX_ERR_BAD_ARG;
+    return out_h16 ? launch_dequantize<h16>(codes, scales, out, ld, rows, K, sms, stream) : launch_dequantize<float>(codes, scales, out, ld, rows, K, sms, stream);
+}
+
+TNX_EXPORT int tnx_mxfp4_gemm_simt(const void* a, int a_kind, const void* a_scales, long long lda, const void* codes, const void* scales, const float* bias,
+                                   const float* residual, void* out, int out_h16, long long ldc, int M, int N, int K, int act, int gated, cudaStream_t stream) {
+    if (M <= 0 || N <= 0) return 0;
+    if (K <= 0 || a_kind < 0 || a_kind > 2 || act < 0 || act >= TNX_ACT_COUNT) return TNX_ERR_BAD_ARG;
+    SimtParams p;
+    p.a = a; p.lda = lda; p.a_kind = a_kind; p.a_scales = (const uint8_t*)a_scales;
+    p.codes = (const uint8_t*)codes; p.scales = (const uint8_t*)scales;
+    p.bias = bias; p.residual = residual; p.out = out; p.ldc = ldc;
+    p.M = M; p.N = N; p.K = K; p.blocks = (K + MX_BLOCK - 1) / MX_BLOCK; p.act = act; p.gated = gated; p.out_h16 = out_h16;
+    // 65,535 blocks along y at most: more tokens go in slices
+    const int slice = 65535 * SIMT_TOKENS;
+    for (int m = 0; m < M; m += slice) {
+        SimtParams q = p;
+        q.M = M - m < slice ? M - m : slice;
+        q.a = a_kind == 2 ? (const void*)((const uint8_t*)a + (long long)m * p.blocks * 16) : (const void*)((const char*)a + (long long)m * lda * (a_kind ? 4 : 2));
+        if (a_scales) q.a_scales = p.a_scales + (long long)m * p.blocks;
+        if (residual) q.residual = residual + (long long)m * ldc;
+        q.out = (char*)out + (long long)m * ldc * (out_h16 ? 2 : 4);
+        const int r = tnx_launch_ex(1, simt_kernel, dim3((N + SIMT_WARPS - 1) / SIMT_WARPS, (q.M + SIMT_TOKENS - 1) / SIMT_TOKENS), dim3(32 * SIMT_WARPS), 0, stream, q);
+        if (r) return r;
+    }
+    return 0;
+}

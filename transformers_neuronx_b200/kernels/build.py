@@ -59,6 +59,7 @@ SOURCES: Dict[str, str] = {
     "ssd": "ssd.cu",
     "diff_attention": "diff_attention.cu",
     "selective_scan": "selective_scan.cu",
+    "mxfp4": "mxfp4.cu",
 }
 
 _loaded: Dict[str, ctypes.CDLL] = {}
