@@ -1,0 +1,438 @@
+// Products with a 4-bit matrix on the 5th-generation tensor cores.
+//
+//   out[t, n] = act( sum_k a[t, k] W[n, k] + bias[n] ) + residual[t, n]          W: microscaled 4 bits (mxfp4.cuh), 32-bit sums
+//   gated:  out[t, f] = act( sum_k a[t, k] W[f, k] + bias[f] ) * ( sum_k a[t, k] W[F + f, k] + bias[F + f] )
+//
+// One CTA computes a tile of 128 rows of W (gated: 64 gate rows and the 64 up rows that go with them) by BN tokens.  W's rows are the 128
+// lanes of the accumulator, the tokens its columns, so that a step of few tokens pads tokens to 16 and streams W once.  K may be split
+// over the CTAs of a cluster.
+//
+// gemm16 (16-bit activations): W's codes come through TMA into shared memory, 256 columns of K a box; eight warps turn 64 columns at a
+// time into 16-bit values and put them into tensor memory, whence the MMAs take them as their A operand; activations come through
+// TMA.  Looking the values up by byte permutation costs 2.1 instructions a value; a K block of 64 x 128 values is needed every 512 cycles at 256
+// tokens, so a quarter of the issue slots go there.
+#include "mxfp4.cuh"
+#include "tc_common.cuh"
+
+namespace {
+
+constexpr int TILE_W = 128;                  // rows of W a tile: the accumulator's lanes
+constexpr int KB = 64;                       // columns of K a pipeline stage holds in 16 bits
+constexpr int CODE_K = 256;                  // columns of K a box of codes holds: 128 bytes a row
+constexpr int CODE_BYTES = TILE_W * CODE_K / 2;
+constexpr int THREADS = 384;                 // warp 0: activations' TMA, warp 1: MMAs, warp 2: codes' TMA, warps 4..11: values, then sums
+constexpr int ROW_LD = TILE_W + 4;           // floats a token of the staged sums
+
+struct Epilogue {
+    const float* bias;
+    const float* residual;                   // [M, ldc], may be the output
+    void* out;
+    long long ldc;
+    int M, N, act, out_h16, gated;           // N: features of the result
+    int vec;                                 // rows of the output, residual and bias allow accesses of four features
+};
+
+struct Params {
+    Epilogue e;
+    const uint8_t* scales;
+    int w_rows, blocks;                      // rows of W and scales a row
+    int num_kb, boxes_per_split;             // K in stages; boxes of codes a CTA of the cluster takes
+    int splits;
+    int* err;
+};
+
+__device__ __forceinline__ uint32_t cta_rank() { uint32_t r; asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r)); return r; }
+__device__ __forceinline__ uint32_t map_to_cta(uint32_t saddr, uint32_t rank) {
+    uint32_t r;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(saddr), "r"(rank));
+    return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ float4 ld_cluster4(uint32_t a) {
+    float4 f;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(f.x), "=f"(f.y), "=f"(f.z), "=f"(f.w) : "r"(a) : "memory");
+    return f;
+}
+__device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+// D (+)= A B with A read from tensor memory (lane = row, a column = two consecutive values of K).
+__device__ __forceinline__ void umma_a_tmem(uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+        ::"r"(tmem_d), "r"(tmem_a), "l"(bdesc), "r"(idesc), "r"(accumulate) : "memory");
+}
+__host__ __device__ constexpr uint32_t idesc16(int n) {
+    return (1u << 4) | IDESC_H16_AB | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(TILE_W >> 4) << 24);
+}
+
+// x / (1 + e^-x) and the tanh form of gelu by the same few instructions; the others as everywhere (common.cuh).
+__device__ __forceinline__ float activate(float v, int act) {
+    if (act == TNX_ACT_SILU) return __fdividef(v, 1.f + __expf(fminf(-v, 80.f)));
+    if (act == TNX_ACT_GELU_NEW) return gelu_new_fast(v);
+    return apply_activation(v, act);
+}
+
+// The sums of a tile lie as [token][128 + 4 floats] at `sums` in the shared memory of every CTA of the cluster; this CTA writes every
+// splits-th token.  A warp takes a token (gated: two), a lane four neighbouring features; partial sums are added in the order of the CTAs.
+template <bool SPLIT>
+__device__ __forceinline__ void write_tile(const Epilogue& e, uint32_t sums, int splits, int row0, int token0, int tokens) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int rank = SPLIT ? (int)cta_rank() : 0;
+    if (!SPLIT) splits = 1;
+    auto load = [&](int t, int f) {
+        const uint32_t a = sums + (uint32_t)(t * ROW_LD + f) * 4u;
+        if (!SPLIT) {
+            float4 v;
+            asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(a) : "memory");
+            return v;
+        }
+        float4 v = ld_cluster4(map_to_cta(a, 0));
+        for (int s = 1; s < splits; ++s) {
+            const float4 u = ld_cluster4(map_to_cta(a, (uint32_t)s));
+            v.x += u.x; v.y += u.y; v.z += u.z; v.w += u.w;
+        }
+        return v;
+    };
+    const int f = e.gated ? 4 * (lane & 15) : 4 * lane;              // this lane's features within the tile
+    const int n = (e.gated ? row0 / 2 : row0) + f;
+    if (n >= e.N) return;
+    const bool vec = e.vec && n + 3 < e.N;
+    float b[4] = {0.f, 0.f, 0.f, 0.f}, bu[4] = {0.f, 0.f, 0.f, 0.f};
+    if (e.bias) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (n + j < e.N) { b[j] = __ldg(e.bias + n + j); if (e.gated) bu[j] = __ldg(e.bias + e.N + n + j); }
+    }
+    const int step = (THREADS / 32) * (e.gated ? 2 : 1);
+    for (int i = e.gated ? 2 * warp + (lane >> 4) : warp; i * splits + rank < tokens; i += step) {
+        const int t = i * splits + rank;
+        const long long o = (long long)(token0 + t) * e.ldc + n;
+        float res[4] = {0.f, 0.f, 0.f, 0.f};
+        if (e.residual) {
+            if (vec) { const float4 r = __ldcg((const float4*)(e.residual + o)); res[0] = r.x; res[1] = r.y; res[2] = r.z; res[3] = r.w; }
+            else
+                for (int j = 0; j < 4; ++j) if (n + j < e.N) res[j] = __ldcg(e.residual + o + j);
+        }
+        const float4 s = load(t, f);
+        float v[4] = {s.x, s.y, s.z, s.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = activate(v[j] + b[j], e.act);
+        if (e.gated) {
+            const float4 u = load(t, 64 + f);
+            v[0] *= u.x + bu[0]; v[1] *= u.y + bu[1]; v[2] *= u.z + bu[2]; v[3] *= u.w + bu[3];
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] += res[j];
+        if (vec) {
+            if (e.out_h16) {
+                const h16x2 h0 = floats_to_h16x2(v[0], v[1]), h1 = floats_to_h16x2(v[2], v[3]);
+                *(uint2*)((h16*)e.out + o) = make_uint2(*(const uint32_t*)&h0, *(const uint32_t*)&h1);
+            } else *(float4*)((float*)e.out + o) = make_float4(v[0], v[1], v[2], v[3]);
+        } else
+            for (int j = 0; j < 4; ++j)
+                if (n + j < e.N) { if (e.out_h16) ((h16*)e.out)[o + j] = float_to_h16(v[j]); else ((float*)e.out)[o + j] = v[j]; }
+    }
+}
+
+// Row `r` of a tile (gated: 64 gate rows, then their 64 up rows) in W; rows behind the last count as the last one (their sums are not written).
+__device__ __forceinline__ int tile_row(const Epilogue& e, int row0, int r, int w_rows) {
+    const int row = !e.gated ? row0 + r : r < 64 ? row0 / 2 + r : e.N + row0 / 2 + r - 64;
+    return row < w_rows ? row : w_rows - 1;
+}
+
+template <int BN> __host__ __device__ constexpr int x_stage_bytes() { return BN * KB * 2; }
+template <int BN, int STAGES, int BOXES> __host__ __device__ constexpr int gemm16_smem() { return BOXES * CODE_BYTES + STAGES * x_stage_bytes<BN>() + 1024; }
+template <int BN, int STAGES> __host__ __device__ constexpr uint32_t gemm16_tmem() { return BN + STAGES * 32 <= 256 ? 256u : 512u; }
+
+// BN tokens; STAGES: K blocks of activations and values in flight; BOXES: boxes of codes.
+template <int BN, int STAGES, int BOXES, int CTAS>
+__global__ void __launch_bounds__(THREADS, CTAS)
+gemm16_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const Params p) {
+    constexpr int X_BYTES = x_stage_bytes<BN>();
+    constexpr uint32_t TMEM_COLS = gemm16_tmem<BN, STAGES>();
+    static_assert(BN * ROW_LD * 4 <= BOXES * CODE_BYTES + STAGES * X_BYTES, "the staged sums take the place of the stages");
+    static_assert(STAGES % 2 == 0, "two groups of warps fill the stages in turn");
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+    uint8_t* sW = smem;                                   // [BOXES]
+    uint8_t* sX = smem + BOXES * CODE_BYTES;              // [STAGES]
+    __shared__ uint64_t w_full[BOXES], w_empty[BOXES], x_full[STAGES], a_full[STAGES], empty[STAGES], done;
+    __shared__ uint32_t tmem_base_smem;
+#ifdef TNX_F16
+    __shared__ int row_ref[TILE_W];
+#endif
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int token0 = blockIdx.x * BN, row0 = blockIdx.y * TILE_W;
+    const int box0 = (int)blockIdx.z * p.boxes_per_split;
+    const int kb0 = box0 * (CODE_K / KB);
+    const int num_kb = min(p.num_kb - kb0, p.boxes_per_split * (CODE_K / KB));       // at least one
+    const int num_boxes = (num_kb + CODE_K / KB - 1) / (CODE_K / KB);
+
+    pdl_launch_dependents();
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < BOXES; ++i) { mbar_init(&w_full[i], 1); mbar_init(&w_empty[i], 8); }
+        for (int i = 0; i < STAGES; ++i) { mbar_init(&x_full[i], 1); mbar_init(&a_full[i], 4); mbar_init(&empty[i], 1); }
+        mbar_init(&done, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"((unsigned long long)&map_w) : "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"((unsigned long long)&map_x) : "memory");
+    }
+    if (warp == 1) { tmem_alloc(&tmem_base_smem, TMEM_COLS); tmem_relinquish(); }
+    pdl_wait();                                           // codes, scales and activations may be the preceding kernel's
+#ifdef TNX_F16
+    if (threadIdx.x < TILE_W) row_ref[threadIdx.x] = 0;
+#endif
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem_d = tmem_base_smem, tmem_a = tmem_d + BN;
+    bool ok = true;
+
+    if (warp == 0) {
+        if (lane == 0) {
+            for (int i = 0; i < num_kb && ok; ++i) {
+                const int s = i % STAGES;
+                if (i >= STAGES) { ok = mbar_wait(&empty[s], (uint32_t)(i / STAGES - 1) & 1u, p.err, 62); if (!ok) break; }
+                mbar_expect_tx(&x_full[s], X_BYTES);
+                tma_load_2d(sX + s * X_BYTES, &map_x, &x_full[s], (kb0 + i) * KB, token0);
+            }
+        }
+        __syncwarp();
+    } else if (warp == 2) {
+        if (lane == 0) {
+            const int g0 = p.e.gated ? row0 / 2 : row0, g1 = p.e.gated ? p.e.N + row0 / 2 : row0 + 64;
+            for (int i = 0; i < num_boxes && ok; ++i) {
+                const int s = i % BOXES;
+                if (i >= BOXES) { ok = mbar_wait(&w_empty[s], (uint32_t)(i / BOXES - 1) & 1u, p.err, 61); if (!ok) break; }
+                mbar_expect_tx(&w_full[s], CODE_BYTES);
+                const int x = (box0 + i) * (CODE_K / 2);
+                tma_load_2d(sW + s * CODE_BYTES, &map_w, &w_full[s], x, g0);
+                tma_load_2d(sW + s * CODE_BYTES + CODE_BYTES / 2, &map_w, &w_full[s], x, g1);
+            }
+        }
+        __syncwarp();
+    } else if (warp == 1) {
+        constexpr uint32_t idesc = idesc16(BN);
+        const uint64_t desc0 = smem_desc_sw128(smem_u32(sX));
+        Ring<STAGES> r;
+        for (int i = 0; i < num_kb && ok; ++i) {
+            ok = __all_sync(0xffffffffu, mbar_wait(&x_full[r.slot], r.pass, p.err, 63) && mbar_wait(&a_full[r.slot], r.pass, p.err, 64));
+            if (!ok) break;
+            tc_fence_after();
+            const uint64_t bdesc = desc0 + (uint64_t)(r.slot * (X_BYTES >> 4));
+            const uint32_t a = tmem_a + (uint32_t)(r.slot * 32);
+            if (elected()) {
+#pragma unroll
+                for (int k = 0; k < KB / 16; ++k) umma_a_tmem(tmem_d, a + 8u * k, bdesc + (uint64_t)(2 * k), idesc, (i > 0 || k > 0) ? 1u : 0u);
+                umma_commit(&empty[r.slot]);
+                if (i == num_kb - 1) umma_commit(&done);
+            }
+            __syncwarp();
+            r.next();
+        }
+    } else if (warp >= 4) {
+        // Values: warp w fills the lanes of quarter w % 4 (which its tensor memory accesses are confined to), the two groups of four warps
+        // take K blocks in turn.  A thread owns a row.
+        const int quad = warp & 3, group = (warp - 4) >> 2, r = quad * 32 + lane;
+        const uint8_t* sc = p.scales + (long long)tile_row(p.e, row0, r, p.w_rows) * p.blocks;
+        const int blk0 = box0 * (CODE_K / MX_BLOCK), blk_end = min(p.blocks, blk0 + num_kb * 2);
+        const bool wide = p.blocks % 8 == 0 && ((uintptr_t)p.scales & 7) == 0;
+        auto load_scales = [&](int box) {                 // the eight scales of a box of codes
+            const int b = blk0 + box * 8;
+            if (box >= num_boxes) return make_uint2(0u, 0u);
+            if (wide) return __ldg((const uint2*)(sc + b));
+            uint32_t v[2] = {0u, 0u};
+#pragma unroll
+            for (int j = 0; j < 8; ++j) if (b + j < p.blocks) v[j >> 2] |= (uint32_t)__ldg(sc + b + j) << (8 * (j & 3));
+            return make_uint2(v[0], v[1]);
+        };
+        int ref = 0;
+#ifdef TNX_F16
+        // the largest scale of every row over this CTA's share of K, which becomes a factor of the row's sums
+        {
+            const int n = blk_end - blk0, t = (warp - 4) * 32 + lane;
+            for (int row = t >> 3; row < TILE_W; row += 32) {
+                const uint8_t* q = p.scales + (long long)tile_row(p.e, row0, row, p.w_rows) * p.blocks + blk0;
+                int m = 0;
+                if (wide)
+                    for (int j = (t & 7) * 8; j < n; j += 64) {
+                        const uint2 v = __ldg((const uint2*)(q + j));
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) { const int E = (int)(((k < 4 ? v.x : v.y) >> (8 * (k & 3))) & 255u); if (E < 255) m = max(m, E); }
+                    }
+                else
+                    for (int j = t & 7; j < n; j += 8) { const int E = __ldg(q + j); if (E < 255) m = max(m, E); }
+                m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
+                m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
+                m = max(m, __shfl_xor_sync(0xffffffffu, m, 4));
+                if ((t & 7) == 0) row_ref[row] = m;
+            }
+            asm volatile("bar.sync 1, 256;" ::: "memory");
+            ref = row_ref[r];
+        }
+#else
+        (void)blk_end;
+#endif
+        uint2 next = load_scales(0);
+        for (int box = 0; box < num_boxes && ok; ++box) {
+            const uint2 cur = next;
+            next = load_scales(box + 1);
+            const int ws = box % BOXES;
+            ok = __all_sync(0xffffffffu, mbar_wait(&w_full[ws], (uint32_t)(box / BOXES) & 1u, p.err, 65));
+            if (!ok) break;
+            const uint32_t row_addr = smem_u32(sW + ws * CODE_BYTES) + (uint32_t)r * 128u;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int j = 2 * h + group, i = box * 4 + j;                     // K block
+                if (i >= num_kb) break;
+                const uint32_t two = ((h ? cur.y : cur.x) >> (16 * group)) & 0xFFFFu;
+                uint32_t v[32];
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    uint4 q;
+                    const uint32_t at = row_addr + ((uint32_t)((2 * j + c) ^ (r & 7)) << 4);
+                    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(q.x), "=r"(q.y), "=r"(q.z), "=r"(q.w) : "r"(at) : "memory");
+                    const MxTable t = mx_table((two >> (8 * c)) & 255u, ref);
+                    mx_decode8(q.x, t, v[16 * c], v[16 * c + 1], v[16 * c + 2], v[16 * c + 3]);
+                    mx_decode8(q.y, t, v[16 * c + 4], v[16 * c + 5], v[16 * c + 6], v[16 * c + 7]);
+                    mx_decode8(q.z, t, v[16 * c + 8], v[16 * c + 9], v[16 * c + 10], v[16 * c + 11]);
+                    mx_decode8(q.w, t, v[16 * c + 12], v[16 * c + 13], v[16 * c + 14], v[16 * c + 15]);
+                }
+                if (h == 1) { __syncwarp(); if (lane == 0) mbar_arrive(&w_empty[ws]); }          // this warp has read its share of the box
+                const int s = i % STAGES;
+                if (i >= STAGES) {
+                    ok = __all_sync(0xffffffffu, mbar_wait(&empty[s], (uint32_t)(i / STAGES - 1) & 1u, p.err, 66));
+                    if (!ok) break;
+                    tc_fence_after();
+                }
+                tmem_st32(tmem_a + (uint32_t)(s * 32) + ((uint32_t)(quad * 32) << 16), v);
+                tmem_st_wait();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&a_full[s]);
+            }
+        }
+        // The sums, from tensor memory to shared memory: the stages are idle once the last MMA is done.
+        ok = __all_sync(0xffffffffu, ok && mbar_wait(&done, 0, p.err, 67));
+        tc_fence_after();
+        float* sums = (float*)smem + r;
+        constexpr int COLS = BN < 64 ? 16 : 32;
+#pragma unroll 1
+        for (int c = group * COLS; c < BN; c += 2 * COLS) {
+            uint32_t v[32];
+            if (ok) {
+                const uint32_t at = tmem_d + ((uint32_t)(quad * 32) << 16) + (uint32_t)c;
+                if (COLS == 32) tmem_ld32(at, v); else tmem_ld16(at, v);
+                tmem_ld_wait();
+            }
+#pragma unroll
+            for (int j = 0; j < COLS; ++j) {
+                float f = ok ? __uint_as_float(v[j]) : 0.f;                        // defined even if a wait ran out
+#ifdef TNX_F16
+                f = f * (1.f / (float)(1 << MX_F16_TOP)) * mx_scale((uint32_t)ref);
+#endif
+                sums[(c + j) * ROW_LD] = f;
+            }
+        }
+    }
+    if (!ok) {
+        // A wait ran out: give copies in flight time to land before the shared memory is used otherwise.
+        const unsigned long long t0 = global_ns();
+        while (global_ns() - t0 < 1000000ull) __nanosleep(1000);
+    }
+    __syncwarp();
+    tc_fence_before();
+    if (p.splits > 1) {
+        cluster_sync();
+        write_tile<true>(p.e, smem_u32(smem), p.splits, row0, token0, min(BN, p.e.M - token0));
+        __syncwarp();
+        cluster_sync();                                   // no CTA leaves while its sums may still be read
+    } else {
+        __syncthreads();
+        write_tile<false>(p.e, smem_u32(smem), 1, row0, token0, min(BN, p.e.M - token0));
+        __syncthreads();
+    }
+    if (warp == 1) { tc_fence_after(); tmem_dealloc(tmem_base_smem, TMEM_COLS); }
+}
+
+// ---- host -----------------------------------------------------------------------------------------
+// A [rows, bytes] matrix of bytes in boxes of box_rows x 128 bytes, 128-byte swizzle; and one of 16-bit values in boxes of box_rows x 64.
+bool map_bytes(CUtensorMap* out, const void* ptr, int rows, int bytes, int box_rows) {
+    EncodeTiledFn fn = encode_fn();
+    if (!fn) return false;
+    cuuint64_t dims[2] = {(cuuint64_t)bytes, (cuuint64_t)rows};
+    cuuint64_t strides[1] = {(cuuint64_t)bytes};
+    cuuint32_t box[2] = {128u, (cuuint32_t)box_rows};
+    cuuint32_t estr[2] = {1, 1};
+    return fn(out, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+bool map_h16(CUtensorMap* out, const void* ptr, int rows, int cols, long long ld, int box_rows) {
+    EncodeTiledFn fn = encode_fn();
+    if (!fn) return false;
+    cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
+    cuuint64_t strides[1] = {(cuuint64_t)ld * 2};
+    cuuint32_t box[2] = {(cuuint32_t)KB, (cuuint32_t)box_rows};
+    cuuint32_t estr[2] = {1, 1};
+    return fn(out, TNX_TMA_H16, 2, const_cast<void*>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <int BN, int STAGES, int BOXES, int CTAS>
+int launch16(const void* a, long long lda, const void* codes, int K, Params& p, int tiles_w, int splits, cudaStream_t stream) {
+    CUtensorMap mw, mx;
+    if (!map_bytes(&mw, codes, p.w_rows, p.blocks * 16, 64) || !map_h16(&mx, a, p.e.M, K, lda, BN)) return TNX_ERR_UNSUPPORTED;
+    constexpr int SMEM = gemm16_smem<BN, STAGES, BOXES>();
+    static TnxSmemLimit limit;
+    auto kernel = gemm16_kernel<BN, STAGES, BOXES, CTAS>;
+    const int r = limit.allow(kernel, SMEM);
+    if (r) return r;
+    const dim3 grid((p.e.M + BN - 1) / BN, tiles_w, splits);
+    if (splits > 1) return tnx_launch_cluster(1, dim3(1, 1, splits), kernel, grid, dim3(THREADS), SMEM, stream, mw, mx, p);
+    return tnx_launch_ex(1, kernel, grid, dim3(THREADS), SMEM, stream, mw, mx, p);
+}
+
+int g_forced_splits = 0, g_forced_bn = 0;
+
+}  // namespace
+
+// For sweeps and tests: the split of K (1, 2, 4 or 8) and the tokens of a tile whatever the sizes (0: the plan's own).
+TNX_EXPORT void tnx_gemm_mxfp4_force(int bn, int splits) { g_forced_bn = bn; g_forced_splits = splits; }
+
+// 16-bit activations [M, K] (pitch lda, a multiple of 8 elements, 16-byte aligned) by codes [w_rows][blocks * 16] (16-byte aligned).
+TNX_EXPORT int tnx_gemm_mxfp4_16(const void* a, long long lda, const void* codes, const void* scales, const float* bias, const float* residual, void* out,
+                                 int out_h16, long long ldc, int M, int N, int K, int act, int gated, int n_sms, int* err, cudaStream_t stream) {
+    if (M <= 0 || N <= 0) return 0;
+    if (K <= 0 || act < 0 || act >= TNX_ACT_COUNT || n_sms <= 0) return TNX_ERR_BAD_ARG;
+    if (lda % 8 || ((uintptr_t)a & 15) || ((uintptr_t)codes & 15)) return TNX_ERR_UNSUPPORTED;
+    Params p;
+    p.e.bias = bias; p.e.residual = residual; p.e.out = out; p.e.ldc = ldc;
+    p.e.M = M; p.e.N = N; p.e.act = act; p.e.out_h16 = out_h16; p.e.gated = gated;
+    p.e.vec = ldc % 4 == 0 && ((uintptr_t)out & 15) == 0 && ((uintptr_t)residual & 15) == 0;
+    p.scales = (const uint8_t*)scales; p.w_rows = gated ? 2 * N : N; p.blocks = (K + MX_BLOCK - 1) / MX_BLOCK; p.err = err;
+    p.num_kb = (K + KB - 1) / KB;
+    const int boxes = (K + CODE_K - 1) / CODE_K;
+    const int tiles_w = gated ? (N + 63) / 64 : (N + TILE_W - 1) / TILE_W;
+    int bn = M <= 16 ? 16 : M <= 32 ? 32 : M <= 64 ? 64 : M <= 128 ? 128 : 256;
+    if (g_forced_bn) bn = g_forced_bn;
+    const long long tiles = (long long)tiles_w * ((M + bn - 1) / bn);
+    const int room = n_sms * (bn == 256 ? 1 : 2);
+    int splits = 1;
+    while (splits < 8 && tiles * splits * 2 <= room && boxes >= splits * 2) splits *= 2;
+    if (g_forced_splits) splits = g_forced_splits;
+    p.boxes_per_split = (boxes + splits - 1) / splits;
+    while (splits > 1 && p.boxes_per_split * (splits - 1) >= boxes) { splits /= 2; p.boxes_per_split = (boxes + splits - 1) / splits; }   // no CTA without work
+    p.splits = splits;
+    if (tiles_w > 65535) return TNX_ERR_UNSUPPORTED;
+    if (bn == 16) return launch16<16, 4, 4, 2>(a, lda, codes, K, p, tiles_w, splits, stream);
+    if (bn == 32) return launch16<32, 4, 4, 2>(a, lda, codes, K, p, tiles_w, splits, stream);
+    if (bn == 64) return launch16<64, 4, 4, 2>(a, lda, codes, K, p, tiles_w, splits, stream);
+    if (bn == 128) return launch16<128, 4, 2, 2>(a, lda, codes, K, p, tiles_w, splits, stream);
+    return launch16<256, 4, 3, 1>(a, lda, codes, K, p, tiles_w, splits, stream);
+}

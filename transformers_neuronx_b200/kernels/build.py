@@ -60,6 +60,7 @@ SOURCES: Dict[str, str] = {
     "diff_attention": "diff_attention.cu",
     "selective_scan": "selective_scan.cu",
     "mxfp4": "mxfp4.cu",
+    "gemm_mxfp4": "gemm_mxfp4.cu",
 }
 
 _loaded: Dict[str, ctypes.CDLL] = {}

@@ -20,7 +20,7 @@ from typing import Optional
 
 import torch
 
-from .ops import KernelError, _FLOATS, _check, _is_h16, _lib, _need, _p, _rows_2d, _sm_count, _stream, activation_code
+from .ops import KernelError, _FLOATS, _check, _is_h16, _lib, _need, _p, _rows_2d, _sm_count, _state, _stream, activation_code
 
 BLOCK = 32                                    # values that share a scale
 
@@ -158,6 +158,13 @@ def _product(a, w, out, bias, residual, activation, gated):
         if tuple(residual.shape) != (M, N) or _rows_2d(residual, "residual")[2] != ldc or out.dtype != torch.float32:
             raise KernelError("residual must be float32 with the shape and row stride of a float32 out")
     if M == 0 or N == 0:
+        return out
+    if not quantized and _is_h16(a) and (out.dtype == a.dtype or out.dtype == torch.float32) and lda % 8 == 0 \
+            and a.data_ptr() % 16 == 0 and w.codes.data_ptr() % 16 == 0:
+        st = _state(a.device)
+        _check(_lib("gemm_mxfp4", a).tnx_gemm_mxfp4_16(_p(a), c_longlong(lda), _p(w.codes), _p(w.scales), _p(bias), _p(residual), _p(out), c_int(_is_h16(out)),
+                                                       c_longlong(ldc), c_int(M), c_int(N), c_int(K), c_int(act), c_int(1 if gated else 0),
+                                                       c_int(st["sms"]), _p(st["err"]), _stream()), "gemm_mxfp4")
         return out
     lib = _lib("mxfp4", None if quantized else a, out)
     kind = 2 if quantized else 0 if _is_h16(a) else 1
