@@ -11,6 +11,11 @@
 // time into 16-bit values and put them into tensor memory, whence the MMAs take them as their A operand; activations come through
 // TMA.  Looking the values up by byte permutation costs 2.1 instructions a value; a K block of 64 x 128 values is needed every 512 cycles at 256
 // tokens, so a quarter of the issue slots go there.
+//
+// gemm4 (activations in 4 bits too): both operands' codes come through TMA, 256 columns of K a stage, and are multiplied as they are
+// (tcgen05.mma kind::mxf4, a scale for 32 columns of K).  The MMAs read scales from tensor memory, where lane l of every quarter holds the
+// scales of rows l, 32 + l, 64 + l ... in neighbouring columns, four blocks of K a column: eight warps load them row by row, exchange
+// them through shared memory and store them there.
 #include "mxfp4.cuh"
 #include "tc_common.cuh"
 
@@ -35,6 +40,7 @@ struct Epilogue {
 struct Params {
     Epilogue e;
     const uint8_t* scales;
+    const uint8_t* a_scales;                 // gemm4
     int w_rows, blocks;                      // rows of W and scales a row
     int num_kb, boxes_per_split;             // K in stages; boxes of codes a CTA of the cluster takes
     int splits;
@@ -143,6 +149,52 @@ __device__ __forceinline__ void write_tile(const Epilogue& e, uint32_t sums, int
 __device__ __forceinline__ int tile_row(const Epilogue& e, int row0, int r, int w_rows) {
     const int row = !e.gated ? row0 + r : r < 64 ? row0 / 2 + r : e.N + row0 / 2 + r - 64;
     return row < w_rows ? row : w_rows - 1;
+}
+
+// A warp's share of the sums, from tensor memory to shared memory: the stages are idle once the last MMA is done.
+template <int BN>
+__device__ __forceinline__ void stage_sums(uint8_t* smem, uint32_t tmem_d, int quad, int group, int lane, bool ok, bool scaled = false, float factor = 1.f) {
+    float* sums = (float*)smem + quad * 32 + lane;
+    constexpr int COLS = BN < 64 ? 16 : 32;
+#pragma unroll 1
+    for (int c = group * COLS; c < BN; c += 2 * COLS) {
+        uint32_t v[32];
+        if (ok) {
+            const uint32_t at = tmem_d + ((uint32_t)(quad * 32) << 16) + (uint32_t)c;
+            if (COLS == 32) tmem_ld32(at, v); else tmem_ld16(at, v);
+            tmem_ld_wait();
+        }
+#pragma unroll
+        for (int j = 0; j < COLS; ++j) {
+            float f = ok ? __uint_as_float(v[j]) : 0.f;                            // defined even if a wait ran out
+#ifdef TNX_F16
+            if (scaled) f = f * (1.f / (float)(1 << MX_F16_TOP)) * factor;
+#endif
+            sums[(c + j) * ROW_LD] = f;
+        }
+    }
+}
+
+// What all warps do behind the sums: wait for the staged tile (of all CTAs of the cluster), write it.
+template <int BN>
+__device__ __forceinline__ void finish_tile(const Params& p, uint8_t* smem, bool ok, int row0, int token0) {
+    if (!ok) {
+        // A wait ran out: give copies in flight time to land before the shared memory is used otherwise.
+        const unsigned long long t0 = global_ns();
+        while (global_ns() - t0 < 1000000ull) __nanosleep(1000);
+    }
+    __syncwarp();
+    tc_fence_before();
+    if (p.splits > 1) {
+        cluster_sync();
+        write_tile<true>(p.e, smem_u32(smem), p.splits, row0, token0, min(BN, p.e.M - token0));
+        __syncwarp();
+        cluster_sync();                                   // no CTA leaves while its sums may still be read
+    } else {
+        __syncthreads();
+        write_tile<false>(p.e, smem_u32(smem), 1, row0, token0, min(BN, p.e.M - token0));
+        __syncthreads();
+    }
 }
 
 template <int BN> __host__ __device__ constexpr int x_stage_bytes() { return BN * KB * 2; }
@@ -318,46 +370,193 @@ gemm16_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__
                 if (lane == 0) mbar_arrive(&a_full[s]);
             }
         }
-        // The sums, from tensor memory to shared memory: the stages are idle once the last MMA is done.
         ok = __all_sync(0xffffffffu, ok && mbar_wait(&done, 0, p.err, 67));
         tc_fence_after();
-        float* sums = (float*)smem + r;
-        constexpr int COLS = BN < 64 ? 16 : 32;
-#pragma unroll 1
-        for (int c = group * COLS; c < BN; c += 2 * COLS) {
-            uint32_t v[32];
-            if (ok) {
-                const uint32_t at = tmem_d + ((uint32_t)(quad * 32) << 16) + (uint32_t)c;
-                if (COLS == 32) tmem_ld32(at, v); else tmem_ld16(at, v);
-                tmem_ld_wait();
-            }
-#pragma unroll
-            for (int j = 0; j < COLS; ++j) {
-                float f = ok ? __uint_as_float(v[j]) : 0.f;                        // defined even if a wait ran out
 #ifdef TNX_F16
-                f = f * (1.f / (float)(1 << MX_F16_TOP)) * mx_scale((uint32_t)ref);
+        stage_sums<BN>(smem, tmem_d, quad, group, lane, ok, true, mx_scale((uint32_t)ref));
+#else
+        stage_sums<BN>(smem, tmem_d, quad, group, lane, ok);
 #endif
-                sums[(c + j) * ROW_LD] = f;
+    }
+    finish_tile<BN>(p, smem, ok, row0, token0);
+    if (warp == 1) { tc_fence_after(); tmem_dealloc(tmem_base_smem, TMEM_COLS); }
+}
+
+// ---- both operands in 4 bits -----------------------------------------------------------------------
+__device__ __forceinline__ void umma_mxf4(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t sfa, uint32_t sfb, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %6, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
+        ::"r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate) : "memory");
+}
+// D = f32, A = B = e2m1, scales 2^(E - 127), both operands K-major, M = 128, N = n; `id`: which half of a column's four scales (0 or 2).
+__host__ __device__ constexpr uint32_t idesc4(int n, uint32_t id) {
+    return (id << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) | (1u << 23) | ((uint32_t)(TILE_W >> 7) << 27) | (id << 29);
+}
+__device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&r)[8]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
+                 ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]) : "memory");
+}
+// Eight bytes from any address: two aligned words and a shift; `end`: the first address behind the tensor, `n`: how many bytes are wanted (the
+// rest is zero).
+__device__ __forceinline__ uint2 load8(const uint8_t* p, const uint8_t* end, int n) {
+    if (n <= 0) return make_uint2(0u, 0u);
+    const uint32_t off = (uint32_t)((uintptr_t)p & 3u);
+    uint32_t v0, v1;
+    if (n >= 8 && off == 0 && ((uintptr_t)p & 7u) == 0) return __ldg((const uint2*)p);
+    if (n >= 8 && p - off + 12 <= end) {
+        const uint32_t* q = (const uint32_t*)(p - off);
+        const uint32_t a = __ldg(q), b = __ldg(q + 1), c = off ? __ldg(q + 2) : 0u;
+        v0 = __funnelshift_r(a, b, 8 * off); v1 = __funnelshift_r(b, c, 8 * off);
+    } else {
+        v0 = v1 = 0u;
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            if (j < n) { const uint32_t E = (uint32_t)__ldg(p + j) << (8 * (j & 3)); if (j < 4) v0 |= E; else v1 |= E; }
+    }
+    return make_uint2(v0, v1);
+}
+
+template <int BN> __host__ __device__ constexpr int sf_cols_x() { return BN < 32 ? 1 : BN / 32; }         // columns of an atom (four blocks of K) with rows in them
+template <int BN> __host__ __device__ constexpr int sf_step_x() { return BN < 128 ? 4 : BN / 32; }         // columns from one atom to the next
+template <int BN> __host__ __device__ constexpr int sf_stage_cols() { return BN == 256 ? 32 : 16; }       // W: 8 columns, activations: 2 atoms
+template <int BN, int STAGES> __host__ __device__ constexpr int gemm4_smem() { return STAGES * (CODE_BYTES + BN * CODE_K / 2) + 1024; }
+template <int BN, int STAGES> __host__ __device__ constexpr uint32_t gemm4_tmem() {
+    return BN + STAGES * sf_stage_cols<BN>() <= 128 ? 128u : BN + STAGES * sf_stage_cols<BN>() <= 256 ? 256u : 512u;
+}
+
+__device__ __forceinline__ void group_sync(int group) {
+    if (group) asm volatile("bar.sync 2, 128;" ::: "memory");
+    else asm volatile("bar.sync 1, 128;" ::: "memory");
+}
+
+template <int BN, int STAGES, int CTAS>
+__global__ void __launch_bounds__(THREADS, CTAS)
+gemm4_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const Params p) {
+    constexpr int STAGE_BYTES = CODE_BYTES + BN * CODE_K / 2;
+    constexpr uint32_t TMEM_COLS = gemm4_tmem<BN, STAGES>();
+    constexpr int XC = sf_cols_x<BN>(), XS = sf_step_x<BN>(), SF_COLS = sf_stage_cols<BN>();
+    static_assert(BN * ROW_LD * 4 <= STAGES * STAGE_BYTES, "the staged sums take the place of the stages");
+    static_assert(STAGES % 2 == 0, "two groups of warps fill the scales in turn");
+    static_assert(8 + 2 * XS <= SF_COLS, "a stage's scales");
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+    __shared__ uint64_t full[STAGES], sf_full[STAGES], empty[STAGES], done;
+    __shared__ uint32_t tmem_base_smem;
+    __shared__ uint32_t sf_smem[2][(8 + 2 * XS) * 32];
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int token0 = blockIdx.x * BN, row0 = blockIdx.y * TILE_W;
+    const int st0 = (int)blockIdx.z * p.boxes_per_split;                           // stages of 256 columns
+    const int num = min((p.blocks + 7) / 8 - st0, p.boxes_per_split);               // at least one
+
+    pdl_launch_dependents();
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < STAGES; ++i) { mbar_init(&full[i], 1); mbar_init(&sf_full[i], 4); mbar_init(&empty[i], 1); }
+        mbar_init(&done, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"((unsigned long long)&map_w) : "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"((unsigned long long)&map_x) : "memory");
+    }
+    if (warp == 1) { tmem_alloc(&tmem_base_smem, TMEM_COLS); tmem_relinquish(); }
+    pdl_wait();
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem_d = tmem_base_smem, tmem_sf = tmem_d + BN;
+    bool ok = true;
+
+    if (warp == 0) {
+        if (lane == 0) {
+            const int g0 = p.e.gated ? row0 / 2 : row0, g1 = p.e.gated ? p.e.N + row0 / 2 : row0 + 64;
+            for (int i = 0; i < num && ok; ++i) {
+                const int s = i % STAGES;
+                if (i >= STAGES) { ok = mbar_wait(&empty[s], (uint32_t)(i / STAGES - 1) & 1u, p.err, 71); if (!ok) break; }
+                mbar_expect_tx(&full[s], STAGE_BYTES);
+                uint8_t* at = smem + s * STAGE_BYTES;
+                const int x = (st0 + i) * (CODE_K / 2);
+                tma_load_2d(at, &map_w, &full[s], x, g0);
+                tma_load_2d(at + CODE_BYTES / 2, &map_w, &full[s], x, g1);
+                tma_load_2d(at + CODE_BYTES, &map_x, &full[s], x, token0);
             }
         }
-    }
-    if (!ok) {
-        // A wait ran out: give copies in flight time to land before the shared memory is used otherwise.
-        const unsigned long long t0 = global_ns();
-        while (global_ns() - t0 < 1000000ull) __nanosleep(1000);
-    }
-    __syncwarp();
-    tc_fence_before();
-    if (p.splits > 1) {
-        cluster_sync();
-        write_tile<true>(p.e, smem_u32(smem), p.splits, row0, token0, min(BN, p.e.M - token0));
         __syncwarp();
-        cluster_sync();                                   // no CTA leaves while its sums may still be read
-    } else {
-        __syncthreads();
-        write_tile<false>(p.e, smem_u32(smem), 1, row0, token0, min(BN, p.e.M - token0));
-        __syncthreads();
+    } else if (warp == 1) {
+        const uint64_t desc0 = smem_desc_sw128(smem_u32(smem));
+        Ring<STAGES> r;
+        for (int i = 0; i < num && ok; ++i) {
+            ok = __all_sync(0xffffffffu, mbar_wait(&full[r.slot], r.pass, p.err, 72) && mbar_wait(&sf_full[r.slot], r.pass, p.err, 73));
+            if (!ok) break;
+            tc_fence_after();
+            const uint64_t adesc = desc0 + (uint64_t)(r.slot * (STAGE_BYTES >> 4)), bdesc = adesc + (uint64_t)(CODE_BYTES >> 4);
+            const uint32_t sf = tmem_sf + (uint32_t)(r.slot * SF_COLS);
+            if (elected()) {
+#pragma unroll
+                for (int k = 0; k < 4; ++k)               // 64 columns of K = 32 bytes = 2 units of the address field
+                    umma_mxf4(tmem_d, adesc + (uint64_t)(2 * k), bdesc + (uint64_t)(2 * k), idesc4(BN, (k & 1) * 2), sf + 4u * (k >> 1),
+                              sf + 8u + (uint32_t)(XS * (k >> 1)), (i > 0 || k > 0) ? 1u : 0u);
+                umma_commit(&empty[r.slot]);
+                if (i == num - 1) umma_commit(&done);
+            }
+            __syncwarp();
+            r.next();
+        }
+    } else if (warp >= 4) {
+        // Scales: two groups of four warps take stages in turn; a thread loads a row of W's and up to two of the activations', eight scales each,
+        // a turn ahead; then every warp stores all of them to the lanes of its quarter.
+        const int quad = warp & 3, group = (warp - 4) >> 2, r = quad * 32 + lane;
+        const uint8_t* w_end = p.scales + (long long)p.w_rows * p.blocks;
+        const uint8_t* x_end = p.a_scales + (long long)p.e.M * p.blocks;
+        const uint8_t* ws = p.scales + (long long)tile_row(p.e, row0, r, p.w_rows) * p.blocks;
+        const uint8_t* xs[2];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) { const int t = token0 + r + 128 * j; xs[j] = p.a_scales + (long long)(t < p.e.M ? t : p.e.M - 1) * p.blocks; }
+        uint2 w, x[2];
+        auto load = [&](int i) {
+            const int b = (st0 + i) * 8, n = i < num ? p.blocks - b : 0;
+            w = load8(ws + b, w_end, n);
+#pragma unroll
+            for (int j = 0; j < 2; ++j) if (r + 128 * j < 32 * XC) x[j] = load8(xs[j] + b, x_end, n);
+        };
+        uint32_t* buf = sf_smem[group];
+        load(group);
+        for (int i = group; i < num; i += 2) {            // whole even if a wait ran out: the groups' warps meet at their barrier
+            buf[quad * 32 + lane] = w.x; buf[(4 + quad) * 32 + lane] = w.y;
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+                if (r + 128 * j < 32 * XC) { buf[(8 + 4 * j + quad) * 32 + lane] = x[j].x; buf[(8 + XS + 4 * j + quad) * 32 + lane] = x[j].y; }
+            group_sync(group);
+            load(i + 2);
+            uint32_t v[8 + 2 * XS];
+#pragma unroll
+            for (int c = 0; c < 8 + 2 * XS; ++c) v[c] = c < 8 || (c - 8) % XS < XC ? buf[c * 32 + lane] : 0u;
+            const int s = i % STAGES;
+            if (ok && i >= STAGES) {
+                ok = __all_sync(0xffffffffu, mbar_wait(&empty[s], (uint32_t)(i / STAGES - 1) & 1u, p.err, 74));
+                tc_fence_after();
+            }
+            if (ok) {
+                const uint32_t at = tmem_sf + (uint32_t)(s * SF_COLS) + ((uint32_t)(quad * 32) << 16);
+#pragma unroll
+                for (int c = 0; c < 8 + 2 * XS; c += 8) {
+                    uint32_t q[8];
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) q[j] = v[c + j];
+                    tmem_st8(at + (uint32_t)c, q);
+                }
+                tmem_st_wait();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sf_full[s]);
+            }
+            group_sync(group);                            // the buffer has been read by all four
+        }
+        ok = __all_sync(0xffffffffu, ok && mbar_wait(&done, 0, p.err, 75));
+        tc_fence_after();
+        stage_sums<BN>(smem, tmem_d, quad, group, lane, ok);
     }
+    finish_tile<BN>(p, smem, ok, row0, token0);
     if (warp == 1) { tc_fence_after(); tmem_dealloc(tmem_base_smem, TMEM_COLS); }
 }
 
@@ -384,21 +583,55 @@ bool map_h16(CUtensorMap* out, const void* ptr, int rows, int cols, long long ld
               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+template <typename Kernel>
+int launch(Kernel kernel, TnxSmemLimit& limit, int smem, int bn, const CUtensorMap& mw, const CUtensorMap& mx, const Params& p, int tiles_w, cudaStream_t stream) {
+    const int r = limit.allow(kernel, smem);
+    if (r) return r;
+    const dim3 grid((p.e.M + bn - 1) / bn, tiles_w, p.splits);
+    if (p.splits > 1) return tnx_launch_cluster(1, dim3(1, 1, p.splits), kernel, grid, dim3(THREADS), smem, stream, mw, mx, p);
+    return tnx_launch_ex(1, kernel, grid, dim3(THREADS), smem, stream, mw, mx, p);
+}
 template <int BN, int STAGES, int BOXES, int CTAS>
-int launch16(const void* a, long long lda, const void* codes, int K, Params& p, int tiles_w, int splits, cudaStream_t stream) {
+int launch16(const void* a, long long lda, const void* codes, int K, const Params& p, int tiles_w, cudaStream_t stream) {
     CUtensorMap mw, mx;
     if (!map_bytes(&mw, codes, p.w_rows, p.blocks * 16, 64) || !map_h16(&mx, a, p.e.M, K, lda, BN)) return TNX_ERR_UNSUPPORTED;
-    constexpr int SMEM = gemm16_smem<BN, STAGES, BOXES>();
     static TnxSmemLimit limit;
-    auto kernel = gemm16_kernel<BN, STAGES, BOXES, CTAS>;
-    const int r = limit.allow(kernel, SMEM);
-    if (r) return r;
-    const dim3 grid((p.e.M + BN - 1) / BN, tiles_w, splits);
-    if (splits > 1) return tnx_launch_cluster(1, dim3(1, 1, splits), kernel, grid, dim3(THREADS), SMEM, stream, mw, mx, p);
-    return tnx_launch_ex(1, kernel, grid, dim3(THREADS), SMEM, stream, mw, mx, p);
+    return launch(gemm16_kernel<BN, STAGES, BOXES, CTAS>, limit, gemm16_smem<BN, STAGES, BOXES>(), BN, mw, mx, p, tiles_w, stream);
+}
+template <int BN, int STAGES, int CTAS>
+int launch4(const void* a, const void* codes, const Params& p, int tiles_w, cudaStream_t stream) {
+    CUtensorMap mw, mx;
+    if (!map_bytes(&mw, codes, p.w_rows, p.blocks * 16, 64) || !map_bytes(&mx, a, p.e.M, p.blocks * 16, BN)) return TNX_ERR_UNSUPPORTED;
+    static TnxSmemLimit limit;
+    return launch(gemm4_kernel<BN, STAGES, CTAS>, limit, gemm4_smem<BN, STAGES>(), BN, mw, mx, p, tiles_w, stream);
 }
 
 int g_forced_splits = 0, g_forced_bn = 0;
+
+void fill(Params& p, const void* scales, const void* a_scales, const float* bias, const float* residual, void* out, int out_h16, long long ldc, int M, int N,
+          int K, int act, int gated, int* err) {
+    p.e.bias = bias; p.e.residual = residual; p.e.out = out; p.e.ldc = ldc;
+    p.e.M = M; p.e.N = N; p.e.act = act; p.e.out_h16 = out_h16; p.e.gated = gated;
+    p.e.vec = ldc % 4 == 0 && ((uintptr_t)out & 15) == 0 && ((uintptr_t)residual & 15) == 0;
+    p.scales = (const uint8_t*)scales; p.a_scales = (const uint8_t*)a_scales;
+    p.w_rows = gated ? 2 * N : N; p.blocks = (K + MX_BLOCK - 1) / MX_BLOCK; p.err = err;
+    p.num_kb = (K + KB - 1) / KB;
+}
+// Tokens of a tile and the split of K over a cluster's CTAs.
+int plan(Params& p, int K, int n_sms, int tiles_w) {
+    const int M = p.e.M, boxes = (K + CODE_K - 1) / CODE_K;
+    int bn = M <= 16 ? 16 : M <= 32 ? 32 : M <= 64 ? 64 : M <= 128 ? 128 : 256;
+    if (g_forced_bn) bn = g_forced_bn;
+    const long long tiles = (long long)tiles_w * ((M + bn - 1) / bn);
+    const int room = n_sms * (bn == 256 ? 1 : 2);
+    int splits = 1;
+    while (splits < 8 && tiles * splits * 2 <= room && boxes >= splits * 2) splits *= 2;
+    if (g_forced_splits) splits = g_forced_splits;
+    p.boxes_per_split = (boxes + splits - 1) / splits;
+    while (splits > 1 && p.boxes_per_split * (splits - 1) >= boxes) { splits /= 2; p.boxes_per_split = (boxes + splits - 1) / splits; }   // no CTA without work
+    p.splits = splits;
+    return bn;
+}
 
 }  // namespace
 
@@ -410,29 +643,33 @@ TNX_EXPORT int tnx_gemm_mxfp4_16(const void* a, long long lda, const void* codes
                                  int out_h16, long long ldc, int M, int N, int K, int act, int gated, int n_sms, int* err, cudaStream_t stream) {
     if (M <= 0 || N <= 0) return 0;
     if (K <= 0 || act < 0 || act >= TNX_ACT_COUNT || n_sms <= 0) return TNX_ERR_BAD_ARG;
-    if (lda % 8 || ((uintptr_t)a & 15) || ((uintptr_t)codes & 15)) return TNX_ERR_UNSUPPORTED;
-    Params p;
-    p.e.bias = bias; p.e.residual = residual; p.e.out = out; p.e.ldc = ldc;
-    p.e.M = M; p.e.N = N; p.e.act = act; p.e.out_h16 = out_h16; p.e.gated = gated;
-    p.e.vec = ldc % 4 == 0 && ((uintptr_t)out & 15) == 0 && ((uintptr_t)residual & 15) == 0;
-    p.scales = (const uint8_t*)scales; p.w_rows = gated ? 2 * N : N; p.blocks = (K + MX_BLOCK - 1) / MX_BLOCK; p.err = err;
-    p.num_kb = (K + KB - 1) / KB;
-    const int boxes = (K + CODE_K - 1) / CODE_K;
     const int tiles_w = gated ? (N + 63) / 64 : (N + TILE_W - 1) / TILE_W;
-    int bn = M <= 16 ? 16 : M <= 32 ? 32 : M <= 64 ? 64 : M <= 128 ? 128 : 256;
-    if (g_forced_bn) bn = g_forced_bn;
-    const long long tiles = (long long)tiles_w * ((M + bn - 1) / bn);
-    const int room = n_sms * (bn == 256 ? 1 : 2);
-    int splits = 1;
-    while (splits < 8 && tiles * splits * 2 <= room && boxes >= splits * 2) splits *= 2;
-    if (g_forced_splits) splits = g_forced_splits;
-    p.boxes_per_split = (boxes + splits - 1) / splits;
-    while (splits > 1 && p.boxes_per_split * (splits - 1) >= boxes) { splits /= 2; p.boxes_per_split = (boxes + splits - 1) / splits; }   // no CTA without work
-    p.splits = splits;
-    if (tiles_w > 65535) return TNX_ERR_UNSUPPORTED;
-    if (bn == 16) return launch16<16, 4, 4, 2>(a, lda, codes, K, p, tiles_w, splits, stream);
-    if (bn == 32) return launch16<32, 4, 4, 2>(a, lda, codes, K, p, tiles_w, splits, stream);
-    if (bn == 64) return launch16<64, 4, 4, 2>(a, lda, codes, K, p, tiles_w, splits, stream);
-    if (bn == 128) return launch16<128, 4, 2, 2>(a, lda, codes, K, p, tiles_w, splits, stream);
-    return launch16<256, 4, 3, 1>(a, lda, codes, K, p, tiles_w, splits, stream);
+    if (lda % 8 || ((uintptr_t)a & 15) || ((uintptr_t)codes & 15) || tiles_w > 65535) return TNX_ERR_UNSUPPORTED;
+    Params p;
+    fill(p, scales, nullptr, bias, residual, out, out_h16, ldc, M, N, K, act, gated, err);
+    switch (plan(p, K, n_sms, tiles_w)) {
+        case 16: return launch16<16, 4, 4, 2>(a, lda, codes, K, p, tiles_w, stream);
+        case 32: return launch16<32, 4, 4, 2>(a, lda, codes, K, p, tiles_w, stream);
+        case 64: return launch16<64, 4, 4, 2>(a, lda, codes, K, p, tiles_w, stream);
+        case 128: return launch16<128, 4, 2, 2>(a, lda, codes, K, p, tiles_w, stream);
+        default: return launch16<256, 4, 3, 1>(a, lda, codes, K, p, tiles_w, stream);
+    }
+}
+
+// 4-bit activations: codes [M][blocks * 16] (16-byte aligned) and scales [M][blocks].
+TNX_EXPORT int tnx_gemm_mxfp4_4(const void* a, const void* a_scales, const void* codes, const void* scales, const float* bias, const float* residual, void* out,
+                                int out_h16, long long ldc, int M, int N, int K, int act, int gated, int n_sms, int* err, cudaStream_t stream) {
+    if (M <= 0 || N <= 0) return 0;
+    if (K <= 0 || act < 0 || act >= TNX_ACT_COUNT || n_sms <= 0) return TNX_ERR_BAD_ARG;
+    const int tiles_w = gated ? (N + 63) / 64 : (N + TILE_W - 1) / TILE_W;
+    if (((uintptr_t)a & 15) || ((uintptr_t)codes & 15) || tiles_w > 65535) return TNX_ERR_UNSUPPORTED;
+    Params p;
+    fill(p, scales, a_scales, bias, residual, out, out_h16, ldc, M, N, K, act, gated, err);
+    switch (plan(p, K, n_sms, tiles_w)) {
+        case 16: return launch4<16, 4, 2>(a, codes, p, tiles_w, stream);
+        case 32: return launch4<32, 4, 2>(a, codes, p, tiles_w, stream);
+        case 64: return launch4<64, 4, 2>(a, codes, p, tiles_w, stream);
+        case 128: return launch4<128, 4, 1>(a, codes, p, tiles_w, stream);
+        default: return launch4<256, 4, 1>(a, codes, p, tiles_w, stream);
+    }
 }

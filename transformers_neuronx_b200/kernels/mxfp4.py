@@ -166,6 +166,12 @@ def _product(a, w, out, bias, residual, activation, gated):
                                                        c_longlong(ldc), c_int(M), c_int(N), c_int(K), c_int(act), c_int(1 if gated else 0),
                                                        c_int(st["sms"]), _p(st["err"]), _stream()), "gemm_mxfp4")
         return out
+    if quantized and a.codes.data_ptr() % 16 == 0 and w.codes.data_ptr() % 16 == 0:
+        st = _state(w.device)
+        _check(_lib("gemm_mxfp4", out).tnx_gemm_mxfp4_4(_p(a.codes), _p(a.scales), _p(w.codes), _p(w.scales), _p(bias), _p(residual), _p(out),
+                                                        c_int(_is_h16(out)), c_longlong(ldc), c_int(M), c_int(N), c_int(K), c_int(act),
+                                                        c_int(1 if gated else 0), c_int(st["sms"]), _p(st["err"]), _stream()), "gemm_mxfp4")
+        return out
     lib = _lib("mxfp4", None if quantized else a, out)
     kind = 2 if quantized else 0 if _is_h16(a) else 1
     _check(lib.tnx_mxfp4_gemm_simt(_p(a.codes if quantized else a), c_int(kind), _p(a.scales if quantized else None), c_longlong(lda), _p(w.codes),
