@@ -15,12 +15,14 @@ keeps 8-bit matrices beside scales per column (src/transformers_neuronx/quantize
 """
 from __future__ import annotations
 
-from ctypes import c_int, c_longlong
+from ctypes import c_int, c_longlong, c_void_p
 from typing import Optional
 
 import torch
 
-from .ops import KernelError, _FLOATS, _check, _is_h16, _lib, _need, _p, _rows_2d, _sm_count, _state, _stream, activation_code
+from . import build as _build
+from . import ops as _ops
+from .ops import KernelError, _FLOATS, _H16, _check, _sm_count, _state, activation_code
 
 BLOCK = 32                                    # values that share a scale
 
@@ -62,58 +64,103 @@ class Mxfp4Matrix:
         return f"Mxfp4Matrix({self.codes.shape[0]} x {self.columns}, {self.device})"
 
 
-def _here(device, *tensors) -> None:
-    """All on one device, and it is the current one: the stream is the current device's."""
-    if device.type != "cuda":
-        raise KernelError("the 4-bit matrices' kernels need CUDA tensors: the engine has no CPU path")
-    if device.index != torch.cuda.current_device():
-        raise KernelError(f"the tensors are on {device}, the current device is cuda:{torch.cuda.current_device()}")
-    for t in tensors:
-        if t is not None and t.device != device:
-            raise KernelError(f"tensors on {device} and {t.device} in one call")
+# The entry points' parameters: p a pointer, l a 64-bit number, i an int; every one ends with the stream.
+_SIGNATURES = {
+    ("mxfp4", "tnx_mxfp4_quantize"): "pilppiii", ("mxfp4", "tnx_mxfp4_dequantize"): "pppiliii",
+    ("mxfp4", "tnx_mxfp4_gemm_simt"): "piplpppppiliiiii",
+    ("gemm_mxfp4", "tnx_gemm_mxfp4_16"): "plpppppiliiiiiip", ("gemm_mxfp4", "tnx_gemm_mxfp4_4"): "pppppppiliiiiiip",
+}
+_TYPES = {"p": c_void_p, "l": c_longlong, "i": c_int}
+_entries = {}
+
+
+def _entry(library: str, name: str, dtype):
+    """The entry point in the flavour of `dtype`'s 16-bit type, its parameter types set once: building a ctypes object for every argument of
+    every call costs more than a launch."""
+    fn = _entries.get((name, dtype))
+    if fn is None:
+        lib = _build.load(library, dtype if dtype in _H16 else None)
+        fn = getattr(lib, name)
+        if not fn.argtypes:
+            fn.argtypes = [_TYPES[c] for c in _SIGNATURES[(library, name)]] + [c_void_p]
+        _entries[(name, dtype)] = fn
+    return fn
+
+
+def _stream(device: int):
+    scoped = _ops._scoped_stream
+    return scoped if scoped is not None else torch._C._cuda_getCurrentRawStream(device)
+
+
+def _device_of(t: torch.Tensor, name: str) -> int:
+    """The number of the tensor's device, which has to be the current one: the stream is the current device's."""
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        raise KernelError(f"{name} must be a CUDA tensor: the engine has no CPU path")
+    d = t.get_device()
+    if d != torch._C._cuda_getDevice():
+        raise KernelError(f"{name} is on cuda:{d}, the current device is cuda:{torch._C._cuda_getDevice()}")
+    return d
+
+
+def _floats(t, name: str, device: int):
+    """(rows, columns, row pitch) of a 2-D tensor of 16- or 32-bit floats on `device` whose rows are contiguous."""
+    if not isinstance(t, torch.Tensor) or t.dtype not in _FLOATS:
+        raise KernelError(f"{name} must be a tensor of bfloat16, float16 or float32")
+    if t.get_device() != device:
+        raise KernelError(f"{name} is on {t.device}, other tensors of the call on cuda:{device}")
+    if t.dim() != 2:
+        raise KernelError(f"{name} has {t.dim()} dimensions, expected 2")
+    rows, columns = t.shape
+    pitch, step = t.stride()
+    if step != 1 and columns > 1:
+        raise KernelError(f"{name} must have contiguous rows")
+    return rows, columns, pitch
 
 
 def quantize_mxfp4(x: torch.Tensor, out: Optional[Mxfp4Matrix] = None) -> Mxfp4Matrix:
     """The rows of x [rows, columns] (16- or 32-bit floats; any row pitch) in 4 bits; `out`: the matrix to write."""
-    _need(x, "x", _FLOATS, None, contiguous=False)
-    rows, columns, pitch = _rows_2d(x, "x")
-    _here(x.device)
+    device = _device_of(x, "x")
+    rows, columns, pitch = _floats(x, "x", device)
     if columns < 1:
         raise KernelError("x has no columns")
     if out is None:
-        blocks = -(-columns // BLOCK)
-        out = Mxfp4Matrix(torch.empty((rows, blocks * 16), dtype=torch.uint8, device=x.device),
-                          torch.empty((rows, blocks), dtype=torch.uint8, device=x.device), columns)
+        blocks = (columns + BLOCK - 1) // BLOCK
+        out = object.__new__(Mxfp4Matrix)
+        out.codes = torch.empty((rows, blocks * 16), dtype=torch.uint8, device=x.device)
+        out.scales = torch.empty((rows, blocks), dtype=torch.uint8, device=x.device)
+        out.columns = columns
     else:
-        _here(x.device, out.codes)
-        if out.shape != x.shape:
-            raise KernelError(f"out is {tuple(out.shape)}, x {tuple(x.shape)}")
+        if not isinstance(out, Mxfp4Matrix) or out.shape != x.shape or out.codes.get_device() != device:
+            raise KernelError(f"out must be an Mxfp4Matrix of {rows} x {columns} on the device of x")
         if out.codes.data_ptr() % 4:
             raise KernelError("out's codes must be 4-byte aligned")
     if rows:
-        _check(_lib("mxfp4", x).tnx_mxfp4_quantize(_p(x), c_int(_is_h16(x)), c_longlong(pitch), _p(out.codes), _p(out.scales), c_int(rows),
-                                                   c_int(columns), c_int(_sm_count(x.device)), _stream()), "quantize_mxfp4")
+        _check(_entry("mxfp4", "tnx_mxfp4_quantize", x.dtype)(
+            x.data_ptr(), 0 if x.dtype == torch.float32 else 1, pitch, out.codes.data_ptr(), out.scales.data_ptr(), rows, columns,
+            _sm_count(x.device), _stream(device)), "quantize_mxfp4")
     return out
 
 
 def dequantize_mxfp4(m: Mxfp4Matrix, dtype=torch.bfloat16, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """The values of m: exact in float32 and bfloat16; float16 rounds what lies outside its range (infinity, subnormal numbers)."""
-    _here(m.device)
+    if not isinstance(m, Mxfp4Matrix):
+        raise KernelError("m must be an Mxfp4Matrix")
+    device = _device_of(m.codes, "the matrix")
     if m.codes.data_ptr() % 4:
         raise KernelError("the codes must be 4-byte aligned")
+    rows, columns = m.shape
     if out is None:
         if dtype not in _FLOATS:
             raise KernelError(f"dtype {dtype}: expected one of {_FLOATS}")
-        out = torch.empty(m.shape, dtype=dtype, device=m.device)
+        out, pitch = torch.empty((rows, columns), dtype=dtype, device=m.device), columns
     else:
-        _need(out, "out", _FLOATS, None, contiguous=False)
-        _here(m.device, out)
-        if out.shape != m.shape:
-            raise KernelError(f"out is {tuple(out.shape)}, the matrix {tuple(m.shape)}")
-    rows, columns, pitch = _rows_2d(out, "out")
+        have, width, pitch = _floats(out, "out", device)
+        if have != rows or width != columns:
+            raise KernelError(f"out is {tuple(out.shape)}, the matrix {rows} x {columns}")
     if rows:
-        _check(_lib("mxfp4", out).tnx_mxfp4_dequantize(_p(m.codes), _p(m.scales), _p(out), c_int(_is_h16(out)), c_longlong(pitch), c_int(rows),
-                                                       c_int(columns), c_int(_sm_count(m.device)), _stream()), "dequantize_mxfp4")
+        _check(_entry("mxfp4", "tnx_mxfp4_dequantize", out.dtype)(
+            m.codes.data_ptr(), m.scales.data_ptr(), out.data_ptr(), 0 if out.dtype == torch.float32 else 1, pitch, rows, columns,
+            _sm_count(m.device), _stream(device)), "dequantize_mxfp4")
     return out
 
 
@@ -134,47 +181,53 @@ def _product(a, w, out, bias, residual, activation, gated):
     act = activation_code(activation)
     if not isinstance(w, Mxfp4Matrix):
         raise KernelError("w must be an Mxfp4Matrix")
+    codes = w.codes
+    device = _device_of(codes, "w")
+    rows, Kw = codes.shape[0], w.columns
     quantized = isinstance(a, Mxfp4Matrix)
     if quantized:
-        (M, K), lda = a.shape, 0
+        if a.codes.get_device() != device:
+            raise KernelError(f"a is on {a.device}, w on {w.device}")
+        (M, K), lda, kind = a.shape, 0, out.dtype if isinstance(out, torch.Tensor) else None
     else:
-        _need(a, "a", _FLOATS, None, contiguous=False)
-        M, K, lda = _rows_2d(a, "a")
-    _need(out, "out", _FLOATS, None, contiguous=False)
-    Mo, No, ldc = _rows_2d(out, "out")
-    rows, Kw = w.shape
+        M, K, lda = _floats(a, "a", device)
+        kind = a.dtype
+    Mo, No, ldc = _floats(out, "out", device)
     if gated and rows % 2:
         raise KernelError(f"a gated product needs as many gate rows as up rows, got {rows} in all")
     N = rows // 2 if gated else rows
     if Kw != K or Mo != M or No != N:
         raise KernelError(f"shapes do not fit: a {(M, K)}, w {(rows, Kw)}{' (gated)' if gated else ''}, out {tuple(out.shape)}")
-    _here(w.device, a.codes if quantized else a, out, bias, residual)
+    out_h16 = 0 if out.dtype == torch.float32 else 1
+    if out_h16 and kind != out.dtype:
+        if kind != torch.float32:
+            raise KernelError(f"a is {kind}, out {out.dtype}: 16-bit activations and results must agree")
+        kind = out.dtype
+    bias_p = res_p = 0
     if bias is not None:
-        _need(bias, "bias", torch.float32, 1)
+        if not isinstance(bias, torch.Tensor) or bias.dtype != torch.float32 or bias.dim() != 1 or bias.get_device() != device or not bias.is_contiguous():
+            raise KernelError("bias must be a contiguous 1-D float32 tensor on the device of w")
         if bias.shape[0] != rows:
             raise KernelError("bias length differs from the matrix's rows")
+        bias_p = bias.data_ptr()
     if residual is not None:
-        _need(residual, "residual", torch.float32, None, contiguous=False)
-        if tuple(residual.shape) != (M, N) or _rows_2d(residual, "residual")[2] != ldc or out.dtype != torch.float32:
+        if _floats(residual, "residual", device) != (M, N, ldc) or residual.dtype != torch.float32 or out_h16:
             raise KernelError("residual must be float32 with the shape and row stride of a float32 out")
+        res_p = residual.data_ptr()
     if M == 0 or N == 0:
         return out
-    if not quantized and _is_h16(a) and (out.dtype == a.dtype or out.dtype == torch.float32) and lda % 8 == 0 \
-            and a.data_ptr() % 16 == 0 and w.codes.data_ptr() % 16 == 0:
-        st = _state(a.device)
-        _check(_lib("gemm_mxfp4", a).tnx_gemm_mxfp4_16(_p(a), c_longlong(lda), _p(w.codes), _p(w.scales), _p(bias), _p(residual), _p(out), c_int(_is_h16(out)),
-                                                       c_longlong(ldc), c_int(M), c_int(N), c_int(K), c_int(act), c_int(1 if gated else 0),
-                                                       c_int(st["sms"]), _p(st["err"]), _stream()), "gemm_mxfp4")
-        return out
-    if quantized and a.codes.data_ptr() % 16 == 0 and w.codes.data_ptr() % 16 == 0:
+    a_p, w_p, out_p = (a.codes if quantized else a).data_ptr(), codes.data_ptr(), out.data_ptr()
+    if (a_p | w_p) % 16 == 0 and (quantized or (a.dtype != torch.float32 and lda % 8 == 0)):
         st = _state(w.device)
-        _check(_lib("gemm_mxfp4", out).tnx_gemm_mxfp4_4(_p(a.codes), _p(a.scales), _p(w.codes), _p(w.scales), _p(bias), _p(residual), _p(out),
-                                                        c_int(_is_h16(out)), c_longlong(ldc), c_int(M), c_int(N), c_int(K), c_int(act),
-                                                        c_int(1 if gated else 0), c_int(st["sms"]), _p(st["err"]), _stream()), "gemm_mxfp4")
-        return out
-    lib = _lib("mxfp4", None if quantized else a, out)
-    kind = 2 if quantized else 0 if _is_h16(a) else 1
-    _check(lib.tnx_mxfp4_gemm_simt(_p(a.codes if quantized else a), c_int(kind), _p(a.scales if quantized else None), c_longlong(lda), _p(w.codes),
-                                   _p(w.scales), _p(bias), _p(residual), _p(out), c_int(_is_h16(out)), c_longlong(ldc), c_int(M), c_int(N), c_int(K),
-                                   c_int(act), c_int(1 if gated else 0), _stream()), "gemm_mxfp4")
+        if quantized:
+            code = _entry("gemm_mxfp4", "tnx_gemm_mxfp4_4", kind)(a_p, a.scales.data_ptr(), w_p, w.scales.data_ptr(), bias_p, res_p, out_p, out_h16, ldc, M, N,
+                                                                 K, act, 1 if gated else 0, st["sms"], st["err"].data_ptr(), _stream(device))
+        else:
+            code = _entry("gemm_mxfp4", "tnx_gemm_mxfp4_16", kind)(a_p, lda, w_p, w.scales.data_ptr(), bias_p, res_p, out_p, out_h16, ldc, M, N,
+                                                                  K, act, 1 if gated else 0, st["sms"], st["err"].data_ptr(), _stream(device))
+    else:
+        code = _entry("mxfp4", "tnx_mxfp4_gemm_simt", kind)(a_p, 2 if quantized else 1 if a.dtype == torch.float32 else 0,
+                                                           a.scales.data_ptr() if quantized else 0, lda, w_p, w.scales.data_ptr(), bias_p, res_p, out_p,
+                                                           out_h16, ldc, M, N, K, act, 1 if gated else 0, _stream(device))
+    _check(code, "gemm_mxfp4")
     return out
