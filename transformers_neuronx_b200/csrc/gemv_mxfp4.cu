@@ -1,71 +1,68 @@
-// Products of a few tokens with a 4-bit matrix (formats: mxfp4.cuh; what is computed: gemm_mxfp4.cu).  The matrix is streamed once, straight
-// into registers: no stage lies between memory and the multiplications.
+// Products of a few tokens with a 4-bit matrix (formats: mxfp4.cuh; what is computed: gemm_mxfp4.cu).  The matrix is streamed once; what
+// bounds them is memory, or else the instructions that turn codes into operands, so these are few.
 //
-// A warp takes 16 rows of W and walks K in chunks of 128 columns: four blocks of 32, one for each of the four lanes that share a row of
-// an MMA (mma.sync m16n8k16).  Which column of K stands where in an MMA is free as long as both operands agree, so a lane multiplies
-// its own block: 16 bytes of codes and one scale byte a row, loaded as they lie.  The block's eight magnitudes times its scale are a
-// table in registers, bytes are looked up by permutation (15 instructions for eight values), and the lanes of a column find eight
-// neighbouring activations of their block as one 16-byte piece in shared memory.
+// A warp takes 16 rows of W (gated: 8 gate rows and their 8 up rows) and a share of K, and works for itself: its lane 0 fetches boxes of
+// 256 columns through TMA into a ring of its own, four ahead.  A block of 32 columns is two MMAs (mma.sync m16n8k16, 16 rows by 8
+// tokens): which column of K stands where in an MMA is free as long as both operands agree, so a lane multiplies eight neighbouring columns
+// of its two rows, one 32-bit word of codes each.  The conversion e2m1x2 -> f16x2 makes them operands, two an instruction and without their
+// scale: an MMA's columns belong to one block, so its 32-bit sums are multiplied by the block's scale when they are added up.  (Codes looked
+// up in a table of the block's scaled magnitudes by byte permutation took 15 instructions for eight values, which the half-rate unit that
+// executes them all bounded: 24 us for one token by 16,384 x 4,096, at 1.5 TB/s.)
 //
-// Values and activations are multiplied as bfloat16, which holds a code times its scale exactly; activations of other types are the
-// exact sum of two (float16) or three (32 bits) bfloat16 terms, which share the looked-up values.
+// Activations are float16 operands too: float16 as they are, others divided by a power of two that brings the largest of a box's 256 to
+// 2^14..2^15, in one term (bfloat16's eight bits and 4-bit values fit) or three (32 bits).  What is lost is below 2^-39 of the largest of
+// the 256, where float16 ends.
 //
-// A block of eight warps: wf groups of 16 rows by 8 / wf shares of K, whose sums meet in shared memory; K may be split further over the
-// blocks of a cluster.  More rows a block means activations are fetched less often, fewer that small matrices reach all SMs.
+// The warps of a block: wf groups of 16 rows by wk shares of K, whose sums meet in shared memory; K may be split further over the blocks of a
+// cluster.  The plan chooses them so that one round of blocks, one an SM, covers the GPU as evenly as the sizes allow.
 #include "mxfp4.cuh"
+#include "tc_common.cuh"
 
 namespace {
 
-constexpr int WARPS = 8, THREADS = 32 * WARPS;
-constexpr int CHUNK = 128;                   // columns of K: four blocks
-constexpr int AHEAD = 4;                     // chunks a warp has asked for
+constexpr int MAX_WARPS = 16;
+constexpr int SLOT_K = 256, SLOT_BLOCKS = SLOT_K / MX_BLOCK, SLOT_BYTES = 16 * SLOT_K / 2;
+constexpr int AHEAD = 4;                     // boxes a warp has asked for
 
 struct Params {
     const void* a; const uint8_t* a_scales; long long lda;
     int a_kind, a_vec;                       // 0: h16, 1: float, 2: codes; rows can be read 16 bytes at a time
-    const uint8_t* codes; const uint8_t* scales;
+    const uint8_t* scales;
     const float* bias; const float* residual; void* out; long long ldc;
-    int M, N, K, w_rows, blocks, chunks, act, out_h16, gated;
-    int wf, splits, chunks_per_split, phase; // phase: chunks whose activations lie in shared memory at a time
+    int M, N, K, w_rows, blocks, slots, act, out_h16, gated;
+    int wf, wk, splits, slots_per_split, phase; // phase: boxes of K whose activations lie in shared memory at a time
+    int x_at, sx_at;                         // places in shared memory
+    int* err;
 };
 
-struct Table { uint32_t h0, h1, l0, l1; };
-__device__ __forceinline__ uint32_t mul_bf16x2(uint32_t a, uint32_t b) {
-    __nv_bfloat162 r = __hmul2(*(__nv_bfloat162*)&a, *(__nv_bfloat162*)&b);
-    return *(uint32_t*)&r;
-}
-__device__ __forceinline__ Table make_table(uint32_t E) {
-    uint32_t s = E ? E << 7 : 0x0040u;
-    if (E == 255u) s = 0x7FC0u;
-    s |= s << 16;
-    const uint32_t p0 = mul_bf16x2(0x3F000000u, s), p1 = mul_bf16x2(0x3FC03F80u, s), p2 = mul_bf16x2(0x40404000u, s), p3 = mul_bf16x2(0x40C04080u, s);
-    Table t;
-    t.l0 = prmt(p0, p1, 0x6420); t.h0 = prmt(p0, p1, 0x7531);
-    t.l1 = prmt(p2, p3, 0x6420); t.h1 = prmt(p2, p3, 0x7531);
-    return t;
-}
-__device__ __forceinline__ void decode8(uint32_t w, const Table& t, uint32_t (&o)[4]) {
-    const uint32_t s = w & 0x77777777u, s2 = s >> 16, w4 = w << 4;
-    const uint32_t ha = prmt(t.h0, t.h1, s) | (prmt(w, w4, 0x9D8C) & 0x80808080u), la = prmt(t.l0, t.l1, s);
-    const uint32_t hb = prmt(t.h0, t.h1, s2) | (prmt(w, w4, 0xBFAE) & 0x80808080u), lb = prmt(t.l0, t.l1, s2);
-    o[0] = prmt(la, ha, 0x5140); o[1] = prmt(la, ha, 0x7362);
-    o[2] = prmt(lb, hb, 0x5140); o[3] = prmt(lb, hb, 0x7362);
-}
 __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
-    __nv_bfloat162 r = __floats2bfloat162_rn(a, b);
-    return *(uint32_t*)&r;
+__device__ __forceinline__ void mma_first(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+        : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
 }
-__device__ __forceinline__ float2 unpack_bf16(uint32_t v) { return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xFFFF0000u)); }
+// Eight codes as eight float16 numbers, without a scale.
+__device__ __forceinline__ void codes_to_f16(uint32_t w, uint32_t (&o)[4]) {
+    asm("{\n\t.reg .b8 b0, b1, b2, b3;\n\t"
+        "mov.b32 {b0, b1, b2, b3}, %4;\n\t"
+        "cvt.rn.f16x2.e2m1x2 %0, b0;\n\t"
+        "cvt.rn.f16x2.e2m1x2 %1, b1;\n\t"
+        "cvt.rn.f16x2.e2m1x2 %2, b2;\n\t"
+        "cvt.rn.f16x2.e2m1x2 %3, b3;\n\t}"
+        : "=r"(o[0]), "=r"(o[1]), "=r"(o[2]), "=r"(o[3]) : "r"(w));
+}
+__device__ __forceinline__ uint32_t pack_f16(float a, float b) {
+    const __half2 r = __floats2half2_rn(a, b);
+    return *(const uint32_t*)&r;
+}
 
 __device__ __forceinline__ uint32_t cta_rank() { uint32_t r; asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r)); return r; }
 __device__ __forceinline__ float ld_cluster(const float* p, uint32_t rank) {
     uint32_t a;
     float v;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"((uint32_t)__cvta_generic_to_shared(p)), "r"(rank));
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
     asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(a) : "memory");
     return v;
 }
@@ -73,130 +70,225 @@ __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
-// Eight activations of a token from column k on as TERMS pieces of eight bfloat16 values whose sum they are; zeros behind the last column.
-template <int TERMS>
-__device__ __forceinline__ void load_terms(const Params& p, int token, int k, uint4 (&out)[TERMS]) {
+// Eight activations of a token from column k on, as they lie in memory.
+struct Raw { uint4 a, b; };
+__device__ __forceinline__ Raw load_raw(const Params& p, int token, int k) {
+    Raw r;
+    r.a = r.b = make_uint4(0u, 0u, 0u, 0u);
+    if (p.a_kind == 2) {
+        if (k < p.blocks * MX_BLOCK) {
+            const long long b = (long long)token * p.blocks + (k >> 5);
+            r.a.x = __ldg((const uint32_t*)((const uint8_t*)p.a + b * 16 + ((k & 31) >> 1)));
+            r.a.y = __ldg(p.a_scales + b);
+        }
+    } else if (p.a_vec && k + 8 <= p.K) {
+        const char* at = (const char*)p.a + (token * p.lda + k) * (p.a_kind ? 4 : 2);
+        r.a = __ldg((const uint4*)at);
+        if (p.a_kind) r.b = __ldg((const uint4*)at + 1);
+    } else if (p.a_kind) {
+        const float* src = (const float*)p.a + token * p.lda + k;
+        float v[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = k + j < p.K ? __ldg(src + j) : 0.f;
+        r.a = *(const uint4*)&v[0]; r.b = *(const uint4*)&v[4];
+    } else {
+        const h16* src = (const h16*)p.a + token * p.lda + k;
+        h16 v[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = k + j < p.K ? src[j] : float_to_h16(0.f);
+        r.a = *(const uint4*)&v[0];
+    }
+    return r;
+}
+
+// A warp's pieces of eight columns are the 256 of a box.  They become TERMS float16 numbers each whose sum times `scale`, a power of two that
+// all 256 share, they are: the largest lies between 2^14 and 2^15.
+template <int TERMS, bool SCALED>
+__device__ __forceinline__ void make_terms(const Params& p, const Raw& r, uint4 (&out)[TERMS], float& scale) {
+    if (!SCALED) { out[0] = r.a; scale = 1.f; return; }
     float v[8];
     if (p.a_kind == 2) {
-        uint32_t c = 0u;
-        float s = 0.f;
-        if (k < p.blocks * 32) {
-            const long long b = (long long)token * p.blocks + (k >> 5);
-            c = *(const uint32_t*)((const uint8_t*)p.a + b * 16 + ((k & 31) >> 1));
-            s = mx_scale(p.a_scales[b]);
-        }
+        const float s = mx_scale(r.a.y);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = mx_code(c >> (4 * j)) * s;
-    } else if (p.a_kind == 0 && p.a_vec && k + 8 <= p.K) {
-        const h16* src = (const h16*)p.a + token * p.lda + k;
-        if (TERMS == 1) { out[0] = __ldg((const uint4*)src); return; }
-        Vec8<h16> q;
-        q.raw = __ldg((const uint4*)src);
-        q.get(v);
-    } else if (p.a_kind == 1 && p.a_vec && k + 8 <= p.K) {
-        const float* src = (const float*)p.a + token * p.lda + k;
-        const float4 x = __ldg((const float4*)src), y = __ldg((const float4*)src + 1);
-        v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w; v[4] = y.x; v[5] = y.y; v[6] = y.z; v[7] = y.w;
+        for (int j = 0; j < 8; ++j) v[j] = mx_code(r.a.x >> (4 * j)) * s;
+    } else if (p.a_kind) {
+        v[0] = __uint_as_float(r.a.x); v[1] = __uint_as_float(r.a.y); v[2] = __uint_as_float(r.a.z); v[3] = __uint_as_float(r.a.w);
+        v[4] = __uint_as_float(r.b.x); v[5] = __uint_as_float(r.b.y); v[6] = __uint_as_float(r.b.z); v[7] = __uint_as_float(r.b.w);
     } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-            v[j] = k + j >= p.K ? 0.f : p.a_kind ? ((const float*)p.a)[token * p.lda + k + j] : h16_to_float(((const h16*)p.a)[token * p.lda + k + j]);
+        Vec8<h16> q;
+        q.raw = r.a;
+        q.get(v);
     }
+    uint32_t m = 0u;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) m = max(m, __float_as_uint(v[j]) & 0x7FFFFFFFu);
+    m = __reduce_max_sync(0xffffffffu, m);
+    const uint32_t f = min(268u - (m >> 23), 254u);                  // 2^(14 - exponent of the largest), a normal number
+    const float by = __uint_as_float(f << 23);
+    scale = __uint_as_float(f < 254u ? (254u - f) << 23 : 0x00400000u);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] *= by;
 #pragma unroll
     for (int t = 0; t < TERMS; ++t) {
         uint32_t w[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            w[j] = pack_bf16(v[2 * j], v[2 * j + 1]);
-            const float2 r = unpack_bf16(w[j]);
-            // what is not finite is whole in the first term (a rest would be NaN for an infinity)
-            v[2 * j] = fabsf(r.x) < INFINITY ? v[2 * j] - r.x : 0.f;
-            v[2 * j + 1] = fabsf(r.y) < INFINITY ? v[2 * j + 1] - r.y : 0.f;
+            w[j] = pack_f16(v[2 * j], v[2 * j + 1]);
+            if (t + 1 < TERMS) {
+                const float2 h = __half22float2(*(const __half2*)&w[j]);
+                // what is not finite is whole in the first term (a rest would be NaN for an infinity)
+                v[2 * j] = fabsf(h.x) < INFINITY ? v[2 * j] - h.x : 0.f;
+                v[2 * j + 1] = fabsf(h.y) < INFINITY ? v[2 * j + 1] - h.y : 0.f;
+            }
         }
         out[t] = make_uint4(w[0], w[1], w[2], w[3]);
     }
 }
 
-// NT: groups of eight tokens.
-template <int TERMS, int NT>
-__global__ void __launch_bounds__(THREADS, 2) gemv_kernel(const Params p) {
-    extern __shared__ __align__(16) uint8_t smem[];
+// NT: groups of eight tokens; SCALED: the activations have scales.
+template <int TERMS, int NT, bool SCALED>
+__global__ void __launch_bounds__(32 * MAX_WARPS, 1) gemv_kernel(const __grid_constant__ CUtensorMap map_w, const Params p) {
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+    __shared__ uint64_t full[MAX_WARPS][AHEAD];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const int wk_n = WARPS / p.wf, wf = warp % p.wf, wk = warp / p.wf;
-    const int c_begin = (int)blockIdx.z * p.chunks_per_split, c_end = min(p.chunks, c_begin + p.chunks_per_split);
-    // rows of W behind a lane's two MMA rows; gated: a gate row and its up row
+    const int wf = warp % p.wf, wk = warp / p.wf;
+    const int s_begin = (int)blockIdx.z * p.slots_per_split, s_end = min(p.slots, s_begin + p.slots_per_split);
+    const int per = (s_end - s_begin + p.wk - 1) / p.wk, b = min(s_begin + wk * per, s_end), e = min(b + per, s_end);
+    // rows of W behind a lane's two MMA rows
     const int tile = blockIdx.x * p.wf + wf;
-    const int ra = min(p.gated ? tile * 8 + g : tile * 16 + g, p.w_rows - 1);
-    const int rb = min(p.gated ? p.N + tile * 8 + g : tile * 16 + 8 + g, p.w_rows - 1);
-    const uint8_t* ca = p.codes + (long long)ra * p.blocks * 16 + t * 16;
-    const uint8_t* cb = p.codes + (long long)rb * p.blocks * 16 + t * 16;
-    const uint8_t* sa = p.scales + (long long)ra * p.blocks + t;
-    const uint8_t* sb = p.scales + (long long)rb * p.blocks + t;
+    const int r0 = p.gated ? tile * 8 : tile * 16, r1 = p.gated ? p.N + tile * 8 : tile * 16 + 8;
+    const uint8_t* sa = p.scales + (long long)min(r0 + g, p.w_rows - 1) * p.blocks;
+    const uint8_t* sb = p.scales + (long long)min(r1 + g, p.w_rows - 1) * p.blocks;
+    uint8_t* ring = smem + warp * AHEAD * SLOT_BYTES;
+
+    pdl_launch_dependents();
+    auto fetch = [&](int s) {                             // box s into its place of the ring
+        uint64_t* bar = &full[warp][(s - b) % AHEAD];
+        uint8_t* at = ring + (s - b) % AHEAD * SLOT_BYTES;
+        mbar_expect_tx(bar, SLOT_BYTES);
+        tma_load_2d(at, &map_w, bar, s * (SLOT_K / 2), r0);
+        tma_load_2d(at + SLOT_BYTES / 2, &map_w, bar, s * (SLOT_K / 2), r1);
+    };
+    if (lane == 0) {
+        for (int i = 0; i < AHEAD; ++i) mbar_init(&full[warp][i], 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    pdl_wait();
+    if (lane == 0)
+        for (int s = b; s < e && s < b + AHEAD; ++s) fetch(s);
+    __syncwarp();
+    // the scales of a box: lane t of a row holds blocks 2t and 2t + 1 of both rows
+    uint32_t na[2], nb[2];
+    auto load_scales = [&](int s) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const int blk = s * SLOT_BLOCKS + 2 * t + j;
+            const bool in = s < e && blk < p.blocks;
+            na[j] = in ? __ldg(sa + blk) : 0u;
+            nb[j] = in ? __ldg(sb + blk) : 0u;
+        }
+    };
+    load_scales(b);
 
     float acc[NT][4];
 #pragma unroll
     for (int n = 0; n < NT; ++n) acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.f;
-
-    pdl_launch_dependents();
-    pdl_wait();
-    uint4* xs = (uint4*)smem;                             // [term][chunk of the phase][piece of a block][token][lane t]
-    const int term_step = p.phase * 16 * p.M;
-    for (int p0 = c_begin; p0 < c_end; p0 += p.phase) {
-        const int p1 = min(c_end, p0 + p.phase);
-        const int per = (p1 - p0 + wk_n - 1) / wk_n, b = min(p0 + wk * per, p1), e = min(b + per, p1);
-        uint4 qa[AHEAD], qb[AHEAD];
-        uint32_t ea[AHEAD], eb[AHEAD];
-        auto load = [&](int j, int c) {
-            const bool in = c < e && 4 * c + t < p.blocks;
-            qa[j] = qb[j] = make_uint4(0u, 0u, 0u, 0u);
-            ea[j] = eb[j] = 0u;
-            if (in) {
-                qa[j] = __ldg((const uint4*)(ca + (long long)c * 64));
-                qb[j] = __ldg((const uint4*)(cb + (long long)c * 64));
-                ea[j] = __ldg(sa + 4 * c);
-                eb[j] = __ldg(sb + 4 * c);
+    uint4* xs = (uint4*)(smem + p.x_at);                  // [term][block of the phase][token][lane t]
+    float* sx = (float*)(smem + p.sx_at);                 // [box of the phase][NT * 8 tokens]
+    const int term_step = p.phase * p.wk * SLOT_BLOCKS * p.M * 4;
+    int token[NT];                                        // places behind the last token: its sums again, which are not written
+#pragma unroll
+    for (int n = 0; n < NT; ++n) token[n] = min(n * 8 + g, p.M - 1) * 4 + t;
+    bool ok = true;
+    // A phase is the next p.phase boxes of every share of K.
+    for (int f0 = 0; f0 < per; f0 += p.phase) {
+        if (f0) __syncthreads();
+        const int len = min(p.phase, per - f0);           // boxes of a share
+        // A warp brings a token's share of a box, a lane eight columns; four boxes are asked for before the first is used.
+        const int units = len * p.wk * p.M, warps = p.wf * p.wk;
+        for (int q0 = warp; q0 < units; q0 += 4 * warps) {
+            Raw raw[4];
+            int place[4], tok[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int q = min(q0 + j * warps, units - 1), box = q / p.M, share = box / len;
+                tok[j] = q - box * p.M;
+                place[j] = share * p.phase + box - share * len;
+                raw[j] = load_raw(p, tok[j], (s_begin + share * per + f0 + box - share * len) * SLOT_K + lane * 8);
             }
-        };
 #pragma unroll
-        for (int j = 0; j < AHEAD; ++j) load(j, b + j);
-        // this phase's activations: pieces of eight columns
-        if (p0 != c_begin) __syncthreads();
-        for (int i = threadIdx.x; i < (p1 - p0) * 16 * p.M; i += THREADS) {
-            const int u = i % ((p1 - p0) * 16), token = i / ((p1 - p0) * 16);
-            const int c = u >> 4, tt = (u >> 2) & 3, piece = u & 3;
-            uint4 v[TERMS];
-            load_terms<TERMS>(p, token, (p0 * 16 + u) * 8, v);
+            for (int j = 0; j < 4; ++j) {
+                if (q0 + j * warps >= units) break;
+                uint4 v[TERMS];
+                float scale;
+                make_terms<TERMS, SCALED>(p, raw[j], v, scale);
 #pragma unroll
-            for (int k = 0; k < TERMS; ++k) xs[k * term_step + ((c * 4 + piece) * p.M + token) * 4 + tt] = v[k];
+                for (int k = 0; k < TERMS; ++k) xs[k * term_step + ((place[j] * SLOT_BLOCKS + (lane >> 2)) * p.M + tok[j]) * 4 + (lane & 3)] = v[k];
+                if (SCALED && lane == 0) sx[place[j] * (NT * 8) + tok[j]] = scale;
+            }
         }
         __syncthreads();
-        for (int c = b; c < e; c += AHEAD) {
+        const int last = min(e, b + f0 + len);
+        for (int s = b + f0; s < last; ++s) {
+            float fa[2], fb[2];
 #pragma unroll
-            for (int j = 0; j < AHEAD; ++j) {
-                if (c + j >= e) break;
-                const Table ta = make_table(ea[j]), tb = make_table(eb[j]);
-                const uint32_t wa[4] = {qa[j].x, qa[j].y, qa[j].z, qa[j].w}, wb[4] = {qb[j].x, qb[j].y, qb[j].z, qb[j].w};
-                load(j, c + j + AHEAD);
-                const uint4* xc = xs + (c + j - p0) * 16 * p.M;
+            for (int j = 0; j < 2; ++j) { fa[j] = mx_scale(na[j]); fb[j] = mx_scale(nb[j]); }
+            load_scales(s + 1);
+            const int place = (s - b) % AHEAD;
+            if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&full[warp][place], (uint32_t)((s - b) / AHEAD) & 1u, p.err, 81));
+            if (!ok) break;
+            const uint8_t* row = ring + place * SLOT_BYTES + g * 128 + t * 4;
+            uint32_t wa[SLOT_BLOCKS], wb[SLOT_BLOCKS];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    uint32_t A[4], B[4];
-                    decode8(wa[i], ta, A);
-                    decode8(wb[i], tb, B);
+            for (int i = 0; i < SLOT_BLOCKS; ++i) {
+                const int at = (i ^ g) << 4;
+                wa[i] = *(const uint32_t*)(row + at);
+                wb[i] = *(const uint32_t*)(row + at + SLOT_BYTES / 2);
+            }
+            __syncwarp();
+            if (lane == 0 && s + AHEAD < e) fetch(s + AHEAD);        // the place has been read
+            const int box = wk * p.phase + s - b - f0;
+            const uint4* xb = xs + box * SLOT_BLOCKS * p.M * 4;
+            float sum[NT][4];
 #pragma unroll
-                    for (int n = 0; n < NT; ++n) {
-                        const int token = n * 8 + g;
+            for (int i = 0; i < SLOT_BLOCKS; ++i) {
+                uint32_t A[4], B[4];
+                codes_to_f16(wa[i], A);
+                codes_to_f16(wb[i], B);
+                const float ga = __shfl_sync(0xffffffffu, fa[i & 1], (lane & ~3) | (i >> 1)), gb = __shfl_sync(0xffffffffu, fb[i & 1], (lane & ~3) | (i >> 1));
 #pragma unroll
-                        for (int k = 0; k < TERMS; ++k) {
-                            uint4 x = make_uint4(0u, 0u, 0u, 0u);
-                            if (token < p.M) x = xc[k * term_step + (i * p.M + token) * 4 + t];
-                            mma(acc[n], A[0], B[0], A[1], B[1], x.x, x.y);
-                            mma(acc[n], A[2], B[2], A[3], B[3], x.z, x.w);
-                        }
+                for (int n = 0; n < NT; ++n) {
+                    float c[4];
+#pragma unroll
+                    for (int k = 0; k < TERMS; ++k) {
+                        const uint4 x = xb[k * term_step + i * p.M * 4 + token[n]];
+                        if (k == 0) mma_first(c, A[0], B[0], A[1], B[1], x.x, x.y);
+                        else mma(c, A[0], B[0], A[1], B[1], x.x, x.y);
+                        mma(c, A[2], B[2], A[3], B[3], x.z, x.w);
+                    }
+                    if (SCALED && i == 0) {
+                        sum[n][0] = c[0] * ga; sum[n][1] = c[1] * ga; sum[n][2] = c[2] * gb; sum[n][3] = c[3] * gb;
+                    } else {
+                        float (&to)[4] = SCALED ? sum[n] : acc[n];
+                        to[0] = fmaf(c[0], ga, to[0]); to[1] = fmaf(c[1], ga, to[1]); to[2] = fmaf(c[2], gb, to[2]); to[3] = fmaf(c[3], gb, to[3]);
                     }
                 }
             }
+            if (SCALED) {
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    const float2 f = *(const float2*)&sx[box * (NT * 8) + n * 8 + 2 * t];
+                    acc[n][0] = fmaf(sum[n][0], f.x, acc[n][0]); acc[n][1] = fmaf(sum[n][1], f.y, acc[n][1]);
+                    acc[n][2] = fmaf(sum[n][2], f.x, acc[n][2]); acc[n][3] = fmaf(sum[n][3], f.y, acc[n][3]);
+                }
+            }
         }
+    }
+    if (!ok) {
+        // A wait ran out: give copies in flight time to land before the shared memory is used otherwise.
+        const unsigned long long t0 = global_ns();
+        while (global_ns() - t0 < 1000000ull) __nanosleep(1000);
     }
     // The shares' sums: [share][token][rows + 4], the lanes of a warp in 32 banks.
     const int rows = p.wf * 16, ld = rows + 4;
@@ -214,14 +306,14 @@ __global__ void __launch_bounds__(THREADS, 2) gemv_kernel(const Params p) {
     auto total = [&](int token, int row) {                // shares in their order, then the cluster's blocks in theirs
         float v = 0.f;
         for (int s = 0; s < splits; ++s)
-            for (int w = 0; w < wk_n; ++w) {
+            for (int w = 0; w < p.wk; ++w) {
                 const float* at = red + (w * p.M + token) * ld + row;
                 v += splits > 1 ? ld_cluster(at, (uint32_t)s) : *at;
             }
         return v;
     };
     const int feats = p.gated ? rows / 2 : rows;
-    for (int i = threadIdx.x * splits + rank; i < feats * p.M; i += THREADS * splits) {
+    for (int i = threadIdx.x * splits + rank; i < feats * p.M; i += blockDim.x * splits) {
         const int f = i % feats, token = i / feats, n = blockIdx.x * feats + f;
         if (n >= p.N) continue;
         const long long o = (long long)token * p.ldc + n;
@@ -241,27 +333,41 @@ __global__ void __launch_bounds__(THREADS, 2) gemv_kernel(const Params p) {
         if (p.out_h16) ((h16*)p.out)[o] = float_to_h16(v);
         else ((float*)p.out)[o] = v;
     }
-    if (splits > 1) cluster_sync();                       // no block leaves while its sums may still be read
+    if (splits > 1) { __syncwarp(); cluster_sync(); }     // no block leaves while its sums may still be read
 }
 
-constexpr int SMEM_MOST = 96 * 1024;
+// ---- host -----------------------------------------------------------------------------------------
+constexpr int SMEM_MOST = 224 * 1024;
 
-template <int TERMS, int NT>
-int launch(const Params& p, int smem, cudaStream_t stream) {
+bool map_codes(CUtensorMap* out, const void* ptr, int rows, int bytes) {
+    EncodeTiledFn fn = encode_fn();
+    if (!fn) return false;
+    cuuint64_t dims[2] = {(cuuint64_t)bytes, (cuuint64_t)rows};
+    cuuint64_t strides[1] = {(cuuint64_t)bytes};
+    cuuint32_t box[2] = {128u, 8u};
+    cuuint32_t estr[2] = {1, 1};
+    return fn(out, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <int TERMS, int NT, bool SCALED>
+int launch(const void* codes, const Params& p, int smem, cudaStream_t stream) {
+    CUtensorMap map;
+    if (!map_codes(&map, codes, p.w_rows, p.blocks * 16)) return TNX_ERR_UNSUPPORTED;
     static TnxSmemLimit limit;
-    auto kernel = gemv_kernel<TERMS, NT>;
+    auto kernel = gemv_kernel<TERMS, NT, SCALED>;
     const int r = limit.allow(kernel, SMEM_MOST);
     if (r) return r;
     const int per = (p.gated ? 8 : 16) * p.wf;
-    const dim3 grid((p.N + per - 1) / per, 1, p.splits);
-    if (p.splits > 1) return tnx_launch_cluster(1, dim3(1, 1, p.splits), kernel, grid, dim3(THREADS), smem, stream, p);
-    return tnx_launch_ex(1, kernel, grid, dim3(THREADS), smem, stream, p);
+    const dim3 grid((p.N + per - 1) / per, 1, p.splits), block(32 * p.wf * p.wk);
+    if (p.splits > 1) return tnx_launch_cluster(1, dim3(1, 1, p.splits), kernel, grid, block, smem, stream, map, p);
+    return tnx_launch_ex(1, kernel, grid, block, smem, stream, map, p);
 }
-template <int TERMS>
-int launch_terms(const Params& p, int smem, cudaStream_t stream) {
-    if (p.M <= 8) return launch<TERMS, 1>(p, smem, stream);
-    if (p.M <= 16) return launch<TERMS, 2>(p, smem, stream);
-    return launch<TERMS, 4>(p, smem, stream);
+template <int TERMS, bool SCALED>
+int launch_terms(const void* codes, const Params& p, int smem, cudaStream_t stream) {
+    if (p.M <= 8) return launch<TERMS, 1, SCALED>(codes, p, smem, stream);
+    if (p.M <= 16) return launch<TERMS, 2, SCALED>(codes, p, smem, stream);
+    return launch<TERMS, 4, SCALED>(codes, p, smem, stream);
 }
 
 int g_forced_wf = 0, g_forced_splits = 0;
@@ -269,13 +375,12 @@ int g_forced_wf = 0, g_forced_splits = 0;
 }  // namespace
 
 constexpr int FEW_TOKENS = 32;
-TNX_EXPORT int tnx_gemv_mxfp4_tokens() { return FEW_TOKENS; }
-// For sweeps and tests: groups of 16 rows a block (1, 2, 4 or 8) and the split of K (1, 2, 4 or 8) whatever the sizes (0: the plan's own).
+// For sweeps and tests: groups of 16 rows a block (1 to 16) and the split of K (1, 2, 4 or 8) whatever the sizes (0: the plan's own).
 TNX_EXPORT void tnx_gemv_mxfp4_force(int wf, int splits) { g_forced_wf = wf; g_forced_splits = splits; }
 
 // a_kind: 0 16-bit, 1 32-bit activations (pitch lda), 2 codes (4-byte aligned) with a_scales; codes of W 16-byte aligned.
 TNX_EXPORT int tnx_gemv_mxfp4(const void* a, int a_kind, const void* a_scales, long long lda, const void* codes, const void* scales, const float* bias,
-                              const float* residual, void* out, int out_h16, long long ldc, int M, int N, int K, int act, int gated, int n_sms,
+                              const float* residual, void* out, int out_h16, long long ldc, int M, int N, int K, int act, int gated, int n_sms, int* err,
                               cudaStream_t stream) {
     if (M <= 0 || N <= 0) return 0;
     if (K <= 0 || a_kind < 0 || a_kind > 2 || act < 0 || act >= TNX_ACT_COUNT || n_sms <= 0) return TNX_ERR_BAD_ARG;
@@ -283,29 +388,43 @@ TNX_EXPORT int tnx_gemv_mxfp4(const void* a, int a_kind, const void* a_scales, l
     Params p;
     p.a = a; p.a_scales = (const uint8_t*)a_scales; p.lda = lda; p.a_kind = a_kind;
     p.a_vec = ((uintptr_t)a & 15) == 0 && lda % (a_kind == 1 ? 4 : 8) == 0;
-    p.codes = (const uint8_t*)codes; p.scales = (const uint8_t*)scales; p.bias = bias; p.residual = residual; p.out = out; p.ldc = ldc;
-    p.M = M; p.N = N; p.K = K; p.w_rows = gated ? 2 * N : N; p.blocks = (K + MX_BLOCK - 1) / MX_BLOCK; p.chunks = (p.blocks + 3) / 4;
+    p.scales = (const uint8_t*)scales; p.bias = bias; p.residual = residual; p.out = out; p.ldc = ldc; p.err = err;
+    p.M = M; p.N = N; p.K = K; p.w_rows = gated ? 2 * N : N; p.blocks = (K + MX_BLOCK - 1) / MX_BLOCK;
+    p.slots = (p.blocks + SLOT_BLOCKS - 1) / SLOT_BLOCKS;
     p.act = act; p.out_h16 = out_h16; p.gated = gated;
+    const int terms = a_kind == 1 ? 3 : 1, groups = (N + (gated ? 8 : 16) - 1) / (gated ? 8 : 16);
+    const int nt = M <= 8 ? 1 : M <= 16 ? 2 : 4;
+    const int box_x = SLOT_K * 2 * M * terms, box_s = nt * 8 * 4;      // shared memory of a box's activations, for one share of K
+    // The busiest SM's boxes of codes, and what a block costs beside them (its activations, sums and barriers: as much as 16 boxes).
+    long long best = -1;
+    for (int splits = 1; splits <= 8; splits *= 2) {
+        if (g_forced_splits && splits != g_forced_splits) continue;
+        const int sps = (p.slots + splits - 1) / splits;
+        if (splits > 1 && sps * (splits - 1) >= p.slots) continue;                 // no block without work
+        for (int wf = 1; wf <= MAX_WARPS; ++wf) {
+            if (g_forced_wf && wf != g_forced_wf) continue;
+            int wk = MAX_WARPS / wf;
+            if (wk > sps) wk = sps;
+            while (wk > 1 && wk * (wf * AHEAD * SLOT_BYTES + box_x + box_s) > SMEM_MOST - 1024) --wk;
+            if (wk * (wf * AHEAD * SLOT_BYTES + box_x + box_s) > SMEM_MOST - 1024) continue;
+            const long long blocks = (long long)((groups + wf - 1) / wf) * splits;
+            const long long rounds = (blocks + n_sms - 1) / n_sms;
+            const long long cost = rounds * ((long long)wf * wk * ((sps + wk - 1) / wk) + 16 + (splits > 1 ? 8 : 0));
+            if (best < 0 || cost < best) { best = cost; p.splits = splits; p.wf = wf; p.wk = wk; p.slots_per_split = sps; }
+        }
+    }
+    if (best < 0) return TNX_ERR_UNSUPPORTED;
+    const int ring = p.wf * p.wk * AHEAD * SLOT_BYTES;
+    const int per = (p.slots_per_split + p.wk - 1) / p.wk, most = (SMEM_MOST - 1024 - ring) / (p.wk * (box_x + box_s));
+    const int phases = (per + most - 1) / most;
+    p.phase = (per + phases - 1) / phases;
+    p.x_at = ring;
+    p.sx_at = ring + p.phase * p.wk * box_x;
+    const int sums = p.wk * M * (p.wf * 16 + 4) * 4, used = p.sx_at + p.phase * p.wk * box_s;
+    const int smem = (used > sums ? used : sums) + 1024;
+    if (terms == 3) return launch_terms<3, true>(codes, p, smem, stream);
 #ifdef TNX_F16
-    const int terms = a_kind == 2 ? 1 : a_kind == 1 ? 3 : 2;
-#else
-    const int terms = a_kind == 1 ? 3 : 1;
+    if (a_kind == 0) return launch_terms<1, false>(codes, p, smem, stream);
 #endif
-    p.wf = g_forced_wf ? g_forced_wf : M <= 2 ? 1 : M <= 4 ? 2 : M <= 8 ? 4 : 8;
-    const int per = (gated ? 8 : 16) * p.wf;
-    const long long tiles = (N + per - 1) / per;
-    p.splits = 1;
-    while (p.splits < 8 && tiles * p.splits < 2 * n_sms && p.chunks >= 2 * p.splits * (WARPS / p.wf)) p.splits *= 2;
-    if (g_forced_splits) p.splits = g_forced_splits;
-    p.chunks_per_split = (p.chunks + p.splits - 1) / p.splits;
-    while (p.splits > 1 && p.chunks_per_split * (p.splits - 1) >= p.chunks) { p.splits /= 2; p.chunks_per_split = (p.chunks + p.splits - 1) / p.splits; }
-    // a phase's activations: 256 bytes a chunk, token and term
-    const int chunk_bytes = CHUNK * 2 * M * terms, most = SMEM_MOST / chunk_bytes;
-    const int phases = (p.chunks_per_split + most - 1) / most;
-    p.phase = (p.chunks_per_split + phases - 1) / phases;
-    const int x_bytes = p.phase * chunk_bytes, red = WARPS / p.wf * M * (p.wf * 16 + 4) * 4;
-    const int smem = x_bytes > red ? x_bytes : red;
-    if (terms == 1) return launch_terms<1>(p, smem, stream);
-    if (terms == 2) return launch_terms<2>(p, smem, stream);
-    return launch_terms<3>(p, smem, stream);
+    return launch_terms<1, true>(codes, p, smem, stream);
 }

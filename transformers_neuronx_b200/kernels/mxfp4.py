@@ -69,7 +69,7 @@ class Mxfp4Matrix:
 _SIGNATURES = {
     ("mxfp4", "tnx_mxfp4_quantize"): "pilppiii", ("mxfp4", "tnx_mxfp4_dequantize"): "pppiliii",
     ("mxfp4", "tnx_mxfp4_gemm_simt"): "piplpppppiliiiii",
-    ("gemv_mxfp4", "tnx_gemv_mxfp4"): "piplpppppiliiiiii",
+    ("gemv_mxfp4", "tnx_gemv_mxfp4"): "piplpppppiliiiiiip",
     ("gemm_mxfp4", "tnx_gemm_mxfp4_16"): "plpppppiliiiiiip", ("gemm_mxfp4", "tnx_gemm_mxfp4_4"): "pppppppiliiiiiip",
 }
 _TYPES = {"p": c_void_p, "l": c_longlong, "i": c_int}
@@ -220,9 +220,10 @@ def _product(a, w, out, bias, residual, activation, gated):
         return out
     a_p, w_p, out_p = (a.codes if quantized else a).data_ptr(), codes.data_ptr(), out.data_ptr()
     if M <= FEW_TOKENS and w_p % 16 == 0 and (not quantized or a_p % 4 == 0):
+        st = _state(w.device)
         code = _entry("gemv_mxfp4", "tnx_gemv_mxfp4", kind)(a_p, 2 if quantized else 1 if a.dtype == torch.float32 else 0,
                                                            a.scales.data_ptr() if quantized else 0, lda, w_p, w.scales.data_ptr(), bias_p, res_p, out_p,
-                                                           out_h16, ldc, M, N, K, act, 1 if gated else 0, _sm_count(w.device), _stream(device))
+                                                           out_h16, ldc, M, N, K, act, 1 if gated else 0, st["sms"], st["err"].data_ptr(), _stream(device))
     elif (a_p | w_p) % 16 == 0 and (quantized or (a.dtype != torch.float32 and lda % 8 == 0)):
         st = _state(w.device)
         if quantized:
