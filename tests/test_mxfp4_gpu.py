@@ -301,3 +301,28 @@ def test_refusals():
         with pytest.raises(m.KernelError):
             call()
             pytest.fail(f"call {i} was taken")
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("M,N,K", [(700, 9001, 96), (1040, 6000, 288), (385, 20000, 64), (2048, 4100, 1312), (150, 60000, 32)])
+def test_many_tiles(M, N, K, dtype):
+    """Blocks that walk over several tiles: all kinds of operands, plain and gated, every element."""
+    m = mx()
+    w, wv = _matrix(N, K, M + N + K)
+    g = torch.Generator().manual_seed(K)
+    a = torch.randn(M, K, generator=g).to(dtype).to(DEV)
+    bias = torch.randn(N, generator=g).to(DEV)
+    for x, av in ((a, a.double()), (m.quantize_mxfp4(a), plain.rounded(a))):
+        exact, bound = av @ wv.t() + bias.double(), _sum_bound(av, wv)
+        bound = bound + 2.0 ** -23 * (exact.abs() + bias.double().abs())
+        out = torch.full((M, N), float("nan"), device=DEV, dtype=dtype)
+        m.gemm_mxfp4(x, w, out, bias=bias)
+        ops().raise_on_device_error()
+        _check(out, exact, bound, dtype)
+        if N % 2 == 0:
+            F = N // 2
+            out = torch.full((M, F), float("nan"), device=DEV, dtype=dtype)
+            m.gated_gemm_mxfp4(x, w, out, bias=bias, activation="relu")
+            gate, up = exact[:, :F].clamp_min(0), exact[:, F:]
+            both = bound[:, :F] * up.abs() + gate * bound[:, F:] + bound[:, :F] * bound[:, F:] + 2.0 ** -23 * (gate * up).abs()
+            _check(out, gate * up, both, dtype)

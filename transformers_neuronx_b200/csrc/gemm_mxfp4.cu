@@ -16,26 +16,14 @@
 // (tcgen05.mma kind::mxf4, a scale for 32 columns of K).  The MMAs read scales from tensor memory, where lane l of every quarter holds the
 // scales of rows l, 32 + l, 64 + l ... in neighbouring columns, four blocks of K a column: eight warps load them row by row, exchange
 // them through shared memory and store them there.
-#include "mxfp4.cuh"
-#include "tc_common.cuh"
+#include "gemm_mxfp4.cuh"
 
 namespace {
 
-constexpr int TILE_W = 128;                  // rows of W a tile: the accumulator's lanes
-constexpr int KB = 64;                       // columns of K a pipeline stage holds in 16 bits
-constexpr int CODE_K = 256;                  // columns of K a box of codes holds: 128 bytes a row
-constexpr int CODE_BYTES = TILE_W * CODE_K / 2;
-constexpr int THREADS = 384;                 // warp 0: activations' TMA, warp 1: MMAs, warp 2: codes' TMA, warps 4..11: values, then sums
+constexpr int THREADS4 = 384;                // gemm4: warp 0: TMA, warp 1: MMAs, warps 4..11: scales, then sums
+constexpr int GROUPS16 = 4;                  // gemm16: groups of four warps that make values
+constexpr int THREADS16 = 128 + 128 * GROUPS16;      // warp 0: activations' TMA, warp 1: MMAs, warp 2: codes' TMA, warps 4..: values, then sums
 constexpr int ROW_LD = TILE_W + 4;           // floats a token of the staged sums
-
-struct Epilogue {
-    const float* bias;
-    const float* residual;                   // [M, ldc], may be the output
-    void* out;
-    long long ldc;
-    int M, N, act, out_h16, gated;           // N: features of the result
-    int vec;                                 // rows of the output, residual and bias allow accesses of four features
-};
 
 struct Params {
     Epilogue e;
@@ -61,31 +49,9 @@ __device__ __forceinline__ float4 ld_cluster4(uint32_t a) {
     asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(f.x), "=f"(f.y), "=f"(f.z), "=f"(f.w) : "r"(a) : "memory");
     return f;
 }
-__device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
-    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
-}
-// D (+)= A B with A read from tensor memory (lane = row, a column = two consecutive values of K).
-__device__ __forceinline__ void umma_a_tmem(uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
-        ::"r"(tmem_d), "r"(tmem_a), "l"(bdesc), "r"(idesc), "r"(accumulate) : "memory");
-}
-__host__ __device__ constexpr uint32_t idesc16(int n) {
-    return (1u << 4) | IDESC_H16_AB | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(TILE_W >> 4) << 24);
-}
-
-// x / (1 + e^-x) and the tanh form of gelu by the same few instructions; the others as everywhere (common.cuh).
-__device__ __forceinline__ float activate(float v, int act) {
-    if (act == TNX_ACT_SILU) return __fdividef(v, 1.f + __expf(fminf(-v, 80.f)));
-    if (act == TNX_ACT_GELU_NEW) return gelu_new_fast(v);
-    return apply_activation(v, act);
-}
-
 // The sums of a tile lie as [token][128 + 4 floats] at `sums` in the shared memory of every CTA of the cluster; this CTA writes every
 // splits-th token.  A warp takes a token (gated: two), a lane four neighbouring features; partial sums are added in the order of the CTAs.
-template <bool SPLIT>
+template <bool SPLIT, int THREADS>
 __device__ __forceinline__ void write_tile(const Epilogue& e, uint32_t sums, int splits, int row0, int token0, int tokens) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int rank = SPLIT ? (int)cta_rank() : 0;
@@ -152,17 +118,25 @@ __device__ __forceinline__ int tile_row(const Epilogue& e, int row0, int r, int 
 }
 
 // A warp's share of the sums, from tensor memory to shared memory: the stages are idle once the last MMA is done.
-template <int BN>
+template <int BN, int GROUPS, int ACCS = 1>
 __device__ __forceinline__ void stage_sums(uint8_t* smem, uint32_t tmem_d, int quad, int group, int lane, bool ok, bool scaled = false, float factor = 1.f) {
     float* sums = (float*)smem + quad * 32 + lane;
-    constexpr int COLS = BN < 64 ? 16 : 32;
+    constexpr int COLS = BN < 32 * GROUPS ? 16 : 32;
 #pragma unroll 1
-    for (int c = group * COLS; c < BN; c += 2 * COLS) {
+    for (int c = group * COLS; c < BN; c += GROUPS * COLS) {
         uint32_t v[32];
         if (ok) {
             const uint32_t at = tmem_d + ((uint32_t)(quad * 32) << 16) + (uint32_t)c;
             if (COLS == 32) tmem_ld32(at, v); else tmem_ld16(at, v);
             tmem_ld_wait();
+#pragma unroll
+            for (int a = 1; a < ACCS; ++a) {
+                uint32_t u[32];
+                if (COLS == 32) tmem_ld32(at + (uint32_t)(a * BN), u); else tmem_ld16(at + (uint32_t)(a * BN), u);
+                tmem_ld_wait();
+#pragma unroll
+                for (int j = 0; j < COLS; ++j) v[j] = __float_as_uint(__uint_as_float(v[j]) + __uint_as_float(u[j]));
+            }
         }
 #pragma unroll
         for (int j = 0; j < COLS; ++j) {
@@ -176,7 +150,7 @@ __device__ __forceinline__ void stage_sums(uint8_t* smem, uint32_t tmem_d, int q
 }
 
 // What all warps do behind the sums: wait for the staged tile (of all CTAs of the cluster), write it.
-template <int BN>
+template <int BN, int THREADS>
 __device__ __forceinline__ void finish_tile(const Params& p, uint8_t* smem, bool ok, int row0, int token0) {
     if (!ok) {
         // A wait ran out: give copies in flight time to land before the shared memory is used otherwise.
@@ -187,28 +161,30 @@ __device__ __forceinline__ void finish_tile(const Params& p, uint8_t* smem, bool
     tc_fence_before();
     if (p.splits > 1) {
         cluster_sync();
-        write_tile<true>(p.e, smem_u32(smem), p.splits, row0, token0, min(BN, p.e.M - token0));
+        write_tile<true, THREADS>(p.e, smem_u32(smem), p.splits, row0, token0, min(BN, p.e.M - token0));
         __syncwarp();
         cluster_sync();                                   // no CTA leaves while its sums may still be read
     } else {
         __syncthreads();
-        write_tile<false>(p.e, smem_u32(smem), 1, row0, token0, min(BN, p.e.M - token0));
+        write_tile<false, THREADS>(p.e, smem_u32(smem), 1, row0, token0, min(BN, p.e.M - token0));
         __syncthreads();
     }
 }
 
 template <int BN> __host__ __device__ constexpr int x_stage_bytes() { return BN * KB * 2; }
 template <int BN, int STAGES, int BOXES> __host__ __device__ constexpr int gemm16_smem() { return BOXES * CODE_BYTES + STAGES * x_stage_bytes<BN>() + 1024; }
-template <int BN, int STAGES> __host__ __device__ constexpr uint32_t gemm16_tmem() { return BN + STAGES * 32 <= 256 ? 256u : 512u; }
+template <int BN> __host__ __device__ constexpr int gemm16_accs() { return BN <= 32 ? 4 : BN <= 64 ? 2 : 1; }
+template <int BN, int STAGES> __host__ __device__ constexpr uint32_t gemm16_tmem() { return gemm16_accs<BN>() * BN + STAGES * 32 <= 256 ? 256u : 512u; }
 
 // BN tokens; STAGES: K blocks of activations and values in flight; BOXES: boxes of codes.
 template <int BN, int STAGES, int BOXES, int CTAS>
-__global__ void __launch_bounds__(THREADS, CTAS)
+__global__ void __launch_bounds__(THREADS16, CTAS)
 gemm16_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const Params p) {
     constexpr int X_BYTES = x_stage_bytes<BN>();
     constexpr uint32_t TMEM_COLS = gemm16_tmem<BN, STAGES>();
+    constexpr int ACCS = gemm16_accs<BN>();
+    static_assert(GROUPS16 == CODE_K / KB, "a group of warps for every K block of a box");
     static_assert(BN * ROW_LD * 4 <= BOXES * CODE_BYTES + STAGES * X_BYTES, "the staged sums take the place of the stages");
-    static_assert(STAGES % 2 == 0, "two groups of warps fill the stages in turn");
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
     uint8_t* sW = smem;                                   // [BOXES]
@@ -228,7 +204,7 @@ gemm16_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__
 
     pdl_launch_dependents();
     if (threadIdx.x == 0) {
-        for (int i = 0; i < BOXES; ++i) { mbar_init(&w_full[i], 1); mbar_init(&w_empty[i], 8); }
+        for (int i = 0; i < BOXES; ++i) { mbar_init(&w_full[i], 1); mbar_init(&w_empty[i], 4 * GROUPS16); }
         for (int i = 0; i < STAGES; ++i) { mbar_init(&x_full[i], 1); mbar_init(&a_full[i], 4); mbar_init(&empty[i], 1); }
         mbar_init(&done, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -243,7 +219,7 @@ gemm16_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem_d = tmem_base_smem, tmem_a = tmem_d + BN;
+    const uint32_t tmem_d = tmem_base_smem, tmem_a = tmem_d + ACCS * BN;
     bool ok = true;
 
     if (warp == 0) {
@@ -281,7 +257,7 @@ gemm16_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__
             const uint32_t a = tmem_a + (uint32_t)(r.slot * 32);
             if (elected()) {
 #pragma unroll
-                for (int k = 0; k < KB / 16; ++k) umma_a_tmem(tmem_d, a + 8u * k, bdesc + (uint64_t)(2 * k), idesc, (i > 0 || k > 0) ? 1u : 0u);
+                for (int k = 0; k < KB / 16; ++k) umma_a_tmem(tmem_d + (uint32_t)(k % ACCS * BN), a + 8u * k, bdesc + (uint64_t)(2 * k), idesc, (i > 0 || k >= ACCS) ? 1u : 0u);
                 umma_commit(&empty[r.slot]);
                 if (i == num_kb - 1) umma_commit(&done);
             }
@@ -289,27 +265,25 @@ gemm16_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__
             r.next();
         }
     } else if (warp >= 4) {
-        // Values: warp w fills the lanes of quarter w % 4 (which its tensor memory accesses are confined to), the two groups of four warps
-        // take K blocks in turn.  A thread owns a row.
+        // Values: warp w fills the lanes of quarter w % 4 (which its tensor memory accesses are confined to), each group of four
+        // warps takes one of a box's four K blocks.  A thread owns a row.
         const int quad = warp & 3, group = (warp - 4) >> 2, r = quad * 32 + lane;
         const uint8_t* sc = p.scales + (long long)tile_row(p.e, row0, r, p.w_rows) * p.blocks;
         const int blk0 = box0 * (CODE_K / MX_BLOCK), blk_end = min(p.blocks, blk0 + num_kb * 2);
-        const bool wide = p.blocks % 8 == 0 && ((uintptr_t)p.scales & 7) == 0;
-        auto load_scales = [&](int box) {                 // the eight scales of a box of codes
-            const int b = blk0 + box * 8;
-            if (box >= num_boxes) return make_uint2(0u, 0u);
-            if (wide) return __ldg((const uint2*)(sc + b));
-            uint32_t v[2] = {0u, 0u};
-#pragma unroll
-            for (int j = 0; j < 8; ++j) if (b + j < p.blocks) v[j >> 2] |= (uint32_t)__ldg(sc + b + j) << (8 * (j & 3));
-            return make_uint2(v[0], v[1]);
+        const bool even = p.blocks % 2 == 0 && ((uintptr_t)p.scales & 1) == 0;
+        auto load_scales = [&](int box) -> uint32_t {     // the two scales of this group's K block of a box
+            const int b = blk0 + box * 8 + 2 * group;
+            if (b >= blk_end) return 0u;
+            if (even) return __ldg((const uint16_t*)(sc + b));
+            return (uint32_t)__ldg(sc + b) | (b + 1 < p.blocks ? (uint32_t)__ldg(sc + b + 1) << 8 : 0u);
         };
         int ref = 0;
 #ifdef TNX_F16
         // the largest scale of every row over this CTA's share of K, which becomes a factor of the row's sums
         {
+            const bool wide = p.blocks % 8 == 0 && ((uintptr_t)p.scales & 7) == 0;
             const int n = blk_end - blk0, t = (warp - 4) * 32 + lane;
-            for (int row = t >> 3; row < TILE_W; row += 32) {
+            for (int row = t >> 3; row < TILE_W; row += 16 * GROUPS16) {
                 const uint8_t* q = p.scales + (long long)tile_row(p.e, row0, row, p.w_rows) * p.blocks + blk0;
                 int m = 0;
                 if (wide)
@@ -325,99 +299,72 @@ gemm16_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__
                 m = max(m, __shfl_xor_sync(0xffffffffu, m, 4));
                 if ((t & 7) == 0) row_ref[row] = m;
             }
-            asm volatile("bar.sync 1, 256;" ::: "memory");
+            asm volatile("bar.sync 1, %0;" ::"n"(128 * GROUPS16) : "memory");
             ref = row_ref[r];
         }
-#else
-        (void)blk_end;
 #endif
-        uint2 next = load_scales(0);
-        for (int box = 0; box < num_boxes && ok; ++box) {
-            const uint2 cur = next;
-            next = load_scales(box + 1);
+        // Asked for four boxes ahead: one box ahead, every box took a trip to memory (one token by 16,384 x 4,096 24 us).
+        // (The loop is unrolled so that a register waits for its load where the scale is used: handing the values on would wait for the newest.)
+        uint32_t ahead[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) ahead[j] = load_scales(j);
+        for (int box4 = 0; box4 < num_boxes && ok; box4 += 4) {
+#pragma unroll
+          for (int u = 0; u < 4; ++u) {
+            const int box = box4 + u;
+            if (box >= num_boxes || !ok) break;
+            const uint32_t two = ahead[u];
+            ahead[u] = load_scales(box + 4);
             const int ws = box % BOXES;
             ok = __all_sync(0xffffffffu, mbar_wait(&w_full[ws], (uint32_t)(box / BOXES) & 1u, p.err, 65));
             if (!ok) break;
+            // group j takes the box's K block j
             const uint32_t row_addr = smem_u32(sW + ws * CODE_BYTES) + (uint32_t)r * 128u;
+            const int i = box * 4 + group;
+            if (i >= num_kb) break;
+            uint4 q[2];
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const int j = 2 * h + group, i = box * 4 + j;                     // K block
-                if (i >= num_kb) break;
-                const uint32_t two = ((h ? cur.y : cur.x) >> (16 * group)) & 0xFFFFu;
-                uint32_t v[32];
-#pragma unroll
-                for (int c = 0; c < 2; ++c) {
-                    uint4 q;
-                    const uint32_t at = row_addr + ((uint32_t)((2 * j + c) ^ (r & 7)) << 4);
-                    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(q.x), "=r"(q.y), "=r"(q.z), "=r"(q.w) : "r"(at) : "memory");
-                    const MxTable t = mx_table((two >> (8 * c)) & 255u, ref);
-                    mx_decode8(q.x, t, v[16 * c], v[16 * c + 1], v[16 * c + 2], v[16 * c + 3]);
-                    mx_decode8(q.y, t, v[16 * c + 4], v[16 * c + 5], v[16 * c + 6], v[16 * c + 7]);
-                    mx_decode8(q.z, t, v[16 * c + 8], v[16 * c + 9], v[16 * c + 10], v[16 * c + 11]);
-                    mx_decode8(q.w, t, v[16 * c + 12], v[16 * c + 13], v[16 * c + 14], v[16 * c + 15]);
-                }
-                if (h == 1) { __syncwarp(); if (lane == 0) mbar_arrive(&w_empty[ws]); }          // this warp has read its share of the box
-                const int s = i % STAGES;
-                if (i >= STAGES) {
-                    ok = __all_sync(0xffffffffu, mbar_wait(&empty[s], (uint32_t)(i / STAGES - 1) & 1u, p.err, 66));
-                    if (!ok) break;
-                    tc_fence_after();
-                }
-                tmem_st32(tmem_a + (uint32_t)(s * 32) + ((uint32_t)(quad * 32) << 16), v);
-                tmem_st_wait();
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&a_full[s]);
+            for (int c = 0; c < 2; ++c) {
+                const uint32_t at = row_addr + ((uint32_t)((2 * group + c) ^ (r & 7)) << 4);
+                asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(q[c].x), "=r"(q[c].y), "=r"(q[c].z), "=r"(q[c].w) : "r"(at) : "memory");
             }
+            uint32_t v[32];
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                const MxValues t((two >> (8 * c)) & 255u, ref);
+                t.decode8(q[c].x, &v[16 * c]);
+                t.decode8(q[c].y, &v[16 * c + 4]);
+                t.decode8(q[c].z, &v[16 * c + 8]);
+                t.decode8(q[c].w, &v[16 * c + 12]);
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&w_empty[ws]);                             // this warp has read its share of the box
+            const int s = i % STAGES;
+            if (i >= STAGES) {
+                ok = __all_sync(0xffffffffu, mbar_wait(&empty[s], (uint32_t)(i / STAGES - 1) & 1u, p.err, 66));
+                if (!ok) break;
+                tc_fence_after();
+            }
+            tmem_st32(tmem_a + (uint32_t)(s * 32) + ((uint32_t)(quad * 32) << 16), v);
+            tmem_st_wait();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&a_full[s]);
+          }
         }
         ok = __all_sync(0xffffffffu, ok && mbar_wait(&done, 0, p.err, 67));
         tc_fence_after();
 #ifdef TNX_F16
-        stage_sums<BN>(smem, tmem_d, quad, group, lane, ok, true, mx_scale((uint32_t)ref));
+        stage_sums<BN, GROUPS16, ACCS>(smem, tmem_d, quad, group, lane, ok, true, mx_scale((uint32_t)ref));
 #else
-        stage_sums<BN>(smem, tmem_d, quad, group, lane, ok);
+        stage_sums<BN, GROUPS16, ACCS>(smem, tmem_d, quad, group, lane, ok);
 #endif
     }
-    finish_tile<BN>(p, smem, ok, row0, token0);
+    finish_tile<BN, THREADS16>(p, smem, ok, row0, token0);
     if (warp == 1) { tc_fence_after(); tmem_dealloc(tmem_base_smem, TMEM_COLS); }
 }
 
 // ---- both operands in 4 bits -----------------------------------------------------------------------
-__device__ __forceinline__ void umma_mxf4(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t sfa, uint32_t sfb, uint32_t accumulate) {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %6, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
-        ::"r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate) : "memory");
-}
-// D = f32, A = B = e2m1, scales 2^(E - 127), both operands K-major, M = 128, N = n; `id`: which half of a column's four scales (0 or 2).
-__host__ __device__ constexpr uint32_t idesc4(int n, uint32_t id) {
-    return (id << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) | (1u << 23) | ((uint32_t)(TILE_W >> 7) << 27) | (id << 29);
-}
-__device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&r)[8]) {
-    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
-                 ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]) : "memory");
-}
-// Eight bytes from any address: two aligned words and a shift; `end`: the first address behind the tensor, `n`: how many bytes are wanted (the
-// rest is zero).
-__device__ __forceinline__ uint2 load8(const uint8_t* p, const uint8_t* end, int n) {
-    if (n <= 0) return make_uint2(0u, 0u);
-    const uint32_t off = (uint32_t)((uintptr_t)p & 3u);
-    uint32_t v0, v1;
-    if (n >= 8 && off == 0 && ((uintptr_t)p & 7u) == 0) return __ldg((const uint2*)p);
-    if (n >= 8 && p - off + 12 <= end) {
-        const uint32_t* q = (const uint32_t*)(p - off);
-        const uint32_t a = __ldg(q), b = __ldg(q + 1), c = off ? __ldg(q + 2) : 0u;
-        v0 = __funnelshift_r(a, b, 8 * off); v1 = __funnelshift_r(b, c, 8 * off);
-    } else {
-        v0 = v1 = 0u;
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-            if (j < n) { const uint32_t E = (uint32_t)__ldg(p + j) << (8 * (j & 3)); if (j < 4) v0 |= E; else v1 |= E; }
-    }
-    return make_uint2(v0, v1);
-}
-
 template <int BN> __host__ __device__ constexpr int sf_cols_x() { return BN < 32 ? 1 : BN / 32; }         // columns of an atom (four blocks of K) with rows in them
 template <int BN> __host__ __device__ constexpr int sf_step_x() { return BN < 128 ? 4 : BN / 32; }         // columns from one atom to the next
 template <int BN> __host__ __device__ constexpr int sf_stage_cols() { return BN == 256 ? 32 : 16; }       // W: 8 columns, activations: 2 atoms
@@ -432,7 +379,7 @@ __device__ __forceinline__ void group_sync(int group) {
 }
 
 template <int BN, int STAGES, int CTAS>
-__global__ void __launch_bounds__(THREADS, CTAS)
+__global__ void __launch_bounds__(THREADS4, CTAS)
 gemm4_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const Params p) {
     constexpr int STAGE_BYTES = CODE_BYTES + BN * CODE_K / 2;
     constexpr uint32_t TMEM_COLS = gemm4_tmem<BN, STAGES>();
@@ -504,7 +451,7 @@ gemm4_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ 
         }
     } else if (warp >= 4) {
         // Scales: two groups of four warps take stages in turn; a thread loads a row of W's and up to two of the activations', eight scales each,
-        // a turn ahead; then every warp stores all of them to the lanes of its quarter.
+        // three turns ahead (a trip to memory takes longer than a stage); then every warp stores all of them to the lanes of its quarter.
         const int quad = warp & 3, group = (warp - 4) >> 2, r = quad * 32 + lane;
         const uint8_t* w_end = p.scales + (long long)p.w_rows * p.blocks;
         const uint8_t* x_end = p.a_scales + (long long)p.e.M * p.blocks;
@@ -512,22 +459,29 @@ gemm4_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ 
         const uint8_t* xs[2];
 #pragma unroll
         for (int j = 0; j < 2; ++j) { const int t = token0 + r + 128 * j; xs[j] = p.a_scales + (long long)(t < p.e.M ? t : p.e.M - 1) * p.blocks; }
-        uint2 w, x[2];
+        struct Scales { uint2 w, x[2]; };
         auto load = [&](int i) {
+            Scales q;
             const int b = (st0 + i) * 8, n = i < num ? p.blocks - b : 0;
-            w = load8(ws + b, w_end, n);
+            q.w = load8(ws + b, p.scales, w_end, n);
 #pragma unroll
-            for (int j = 0; j < 2; ++j) if (r + 128 * j < 32 * XC) x[j] = load8(xs[j] + b, x_end, n);
+            for (int j = 0; j < 2; ++j) if (r + 128 * j < 32 * XC) q.x[j] = load8(xs[j] + b, p.a_scales, x_end, n);
+            return q;
         };
         uint32_t* buf = sf_smem[group];
-        load(group);
-        for (int i = group; i < num; i += 2) {            // whole even if a wait ran out: the groups' warps meet at their barrier
-            buf[quad * 32 + lane] = w.x; buf[(4 + quad) * 32 + lane] = w.y;
+        Scales ahead[3] = {load(group), load(group + 2), load(group + 4)};
+        for (int i0 = group; i0 < num; i0 += 6) {         // whole even if a wait ran out: the groups' warps meet at their barrier
+#pragma unroll
+          for (int u = 0; u < 3; ++u) {                   // (unrolled so that a register waits for its load where it is used)
+            const int i = i0 + 2 * u;
+            if (i >= num) break;
+            const Scales now = ahead[u];
+            ahead[u] = load(i + 6);
+            buf[quad * 32 + lane] = now.w.x; buf[(4 + quad) * 32 + lane] = now.w.y;
 #pragma unroll
             for (int j = 0; j < 2; ++j)
-                if (r + 128 * j < 32 * XC) { buf[(8 + 4 * j + quad) * 32 + lane] = x[j].x; buf[(8 + XS + 4 * j + quad) * 32 + lane] = x[j].y; }
+                if (r + 128 * j < 32 * XC) { buf[(8 + 4 * j + quad) * 32 + lane] = now.x[j].x; buf[(8 + XS + 4 * j + quad) * 32 + lane] = now.x[j].y; }
             group_sync(group);
-            load(i + 2);
             uint32_t v[8 + 2 * XS];
 #pragma unroll
             for (int c = 0; c < 8 + 2 * XS; ++c) v[c] = c < 8 || (c - 8) % XS < XC ? buf[c * 32 + lane] : 0u;
@@ -551,79 +505,56 @@ gemm4_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ 
                 if (lane == 0) mbar_arrive(&sf_full[s]);
             }
             group_sync(group);                            // the buffer has been read by all four
+          }
         }
         ok = __all_sync(0xffffffffu, ok && mbar_wait(&done, 0, p.err, 75));
         tc_fence_after();
-        stage_sums<BN>(smem, tmem_d, quad, group, lane, ok);
+        stage_sums<BN, 2>(smem, tmem_d, quad, group, lane, ok);
     }
-    finish_tile<BN>(p, smem, ok, row0, token0);
+    finish_tile<BN, THREADS4>(p, smem, ok, row0, token0);
     if (warp == 1) { tc_fence_after(); tmem_dealloc(tmem_base_smem, TMEM_COLS); }
 }
 
 // ---- host -----------------------------------------------------------------------------------------
-// A [rows, bytes] matrix of bytes in boxes of box_rows x 128 bytes, 128-byte swizzle; and one of 16-bit values in boxes of box_rows x 64.
-bool map_bytes(CUtensorMap* out, const void* ptr, int rows, int bytes, int box_rows) {
-    EncodeTiledFn fn = encode_fn();
-    if (!fn) return false;
-    cuuint64_t dims[2] = {(cuuint64_t)bytes, (cuuint64_t)rows};
-    cuuint64_t strides[1] = {(cuuint64_t)bytes};
-    cuuint32_t box[2] = {128u, (cuuint32_t)box_rows};
-    cuuint32_t estr[2] = {1, 1};
-    return fn(out, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
-bool map_h16(CUtensorMap* out, const void* ptr, int rows, int cols, long long ld, int box_rows) {
-    EncodeTiledFn fn = encode_fn();
-    if (!fn) return false;
-    cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
-    cuuint64_t strides[1] = {(cuuint64_t)ld * 2};
-    cuuint32_t box[2] = {(cuuint32_t)KB, (cuuint32_t)box_rows};
-    cuuint32_t estr[2] = {1, 1};
-    return fn(out, TNX_TMA_H16, 2, const_cast<void*>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
-
 template <typename Kernel>
-int launch(Kernel kernel, TnxSmemLimit& limit, int smem, int bn, const CUtensorMap& mw, const CUtensorMap& mx, const Params& p, int tiles_w, cudaStream_t stream) {
+int launch(Kernel kernel, TnxSmemLimit& limit, int threads, int smem, int bn, const CUtensorMap& mw, const CUtensorMap& mx, const Params& p, int tiles_w, cudaStream_t stream) {
     const int r = limit.allow(kernel, smem);
     if (r) return r;
     const dim3 grid((p.e.M + bn - 1) / bn, tiles_w, p.splits);
-    if (p.splits > 1) return tnx_launch_cluster(1, dim3(1, 1, p.splits), kernel, grid, dim3(THREADS), smem, stream, mw, mx, p);
-    return tnx_launch_ex(1, kernel, grid, dim3(THREADS), smem, stream, mw, mx, p);
+    if (p.splits > 1) return tnx_launch_cluster(1, dim3(1, 1, p.splits), kernel, grid, dim3(threads), smem, stream, mw, mx, p);
+    return tnx_launch_ex(1, kernel, grid, dim3(threads), smem, stream, mw, mx, p);
 }
 template <int BN, int STAGES, int BOXES, int CTAS>
 int launch16(const void* a, long long lda, const void* codes, int K, const Params& p, int tiles_w, cudaStream_t stream) {
     CUtensorMap mw, mx;
     if (!map_bytes(&mw, codes, p.w_rows, p.blocks * 16, 64) || !map_h16(&mx, a, p.e.M, K, lda, BN)) return TNX_ERR_UNSUPPORTED;
     static TnxSmemLimit limit;
-    return launch(gemm16_kernel<BN, STAGES, BOXES, CTAS>, limit, gemm16_smem<BN, STAGES, BOXES>(), BN, mw, mx, p, tiles_w, stream);
+    return launch(gemm16_kernel<BN, STAGES, BOXES, CTAS>, limit, THREADS16, gemm16_smem<BN, STAGES, BOXES>(), BN, mw, mx, p, tiles_w, stream);
 }
 template <int BN, int STAGES, int CTAS>
 int launch4(const void* a, const void* codes, const Params& p, int tiles_w, cudaStream_t stream) {
     CUtensorMap mw, mx;
     if (!map_bytes(&mw, codes, p.w_rows, p.blocks * 16, 64) || !map_bytes(&mx, a, p.e.M, p.blocks * 16, BN)) return TNX_ERR_UNSUPPORTED;
     static TnxSmemLimit limit;
-    return launch(gemm4_kernel<BN, STAGES, CTAS>, limit, gemm4_smem<BN, STAGES>(), BN, mw, mx, p, tiles_w, stream);
+    return launch(gemm4_kernel<BN, STAGES, CTAS>, limit, THREADS4, gemm4_smem<BN, STAGES>(), BN, mw, mx, p, tiles_w, stream);
 }
 
 int g_forced_splits = 0, g_forced_bn = 0;
 
 void fill(Params& p, const void* scales, const void* a_scales, const float* bias, const float* residual, void* out, int out_h16, long long ldc, int M, int N,
           int K, int act, int gated, int* err) {
-    p.e.bias = bias; p.e.residual = residual; p.e.out = out; p.e.ldc = ldc;
-    p.e.M = M; p.e.N = N; p.e.act = act; p.e.out_h16 = out_h16; p.e.gated = gated;
-    p.e.vec = ldc % 4 == 0 && ((uintptr_t)out & 15) == 0 && ((uintptr_t)residual & 15) == 0;
+    fill_epilogue(p.e, bias, residual, out, out_h16, ldc, M, N, act, gated);
     p.scales = (const uint8_t*)scales; p.a_scales = (const uint8_t*)a_scales;
     p.w_rows = gated ? 2 * N : N; p.blocks = (K + MX_BLOCK - 1) / MX_BLOCK; p.err = err;
     p.num_kb = (K + KB - 1) / KB;
 }
 // Tokens of a tile and the split of K over a cluster's CTAs.
-int plan(Params& p, int K, int n_sms, int tiles_w) {
+int plan(Params& p, int K, int n_sms, int tiles_w, int ctas_few) {
     const int M = p.e.M, boxes = (K + CODE_K - 1) / CODE_K;
     int bn = M <= 16 ? 16 : M <= 32 ? 32 : M <= 64 ? 64 : M <= 128 ? 128 : 256;
     if (g_forced_bn) bn = g_forced_bn;
     const long long tiles = (long long)tiles_w * ((M + bn - 1) / bn);
-    const int room = n_sms * (bn == 256 ? 1 : 2);
+    const int room = n_sms * (bn >= 128 ? 1 : ctas_few);
     int splits = 1;
     while (splits < 8 && tiles * splits * 2 <= room && boxes >= splits * 2) splits *= 2;
     if (g_forced_splits) splits = g_forced_splits;
@@ -647,12 +578,12 @@ TNX_EXPORT int tnx_gemm_mxfp4_16(const void* a, long long lda, const void* codes
     if (lda % 8 || ((uintptr_t)a & 15) || ((uintptr_t)codes & 15) || tiles_w > 65535) return TNX_ERR_UNSUPPORTED;
     Params p;
     fill(p, scales, nullptr, bias, residual, out, out_h16, ldc, M, N, K, act, gated, err);
-    switch (plan(p, K, n_sms, tiles_w)) {
-        case 16: return launch16<16, 4, 4, 2>(a, lda, codes, K, p, tiles_w, stream);
-        case 32: return launch16<32, 4, 4, 2>(a, lda, codes, K, p, tiles_w, stream);
-        case 64: return launch16<64, 4, 4, 2>(a, lda, codes, K, p, tiles_w, stream);
-        case 128: return launch16<128, 4, 2, 2>(a, lda, codes, K, p, tiles_w, stream);
-        default: return launch16<256, 4, 3, 1>(a, lda, codes, K, p, tiles_w, stream);
+    switch (plan(p, K, n_sms, tiles_w, 1)) {
+        case 16: return launch16<16, 8, 6, 1>(a, lda, codes, K, p, tiles_w, stream);
+        case 32: return launch16<32, 8, 6, 1>(a, lda, codes, K, p, tiles_w, stream);
+        case 64: return launch16<64, 8, 6, 1>(a, lda, codes, K, p, tiles_w, stream);
+        case 128: return launch16<128, 8, 4, 1>(a, lda, codes, K, p, tiles_w, stream);
+        default: return launch16<256, 5, 3, 1>(a, lda, codes, K, p, tiles_w, stream);
     }
 }
 
@@ -665,7 +596,7 @@ TNX_EXPORT int tnx_gemm_mxfp4_4(const void* a, const void* a_scales, const void*
     if (((uintptr_t)a & 15) || ((uintptr_t)codes & 15) || tiles_w > 65535) return TNX_ERR_UNSUPPORTED;
     Params p;
     fill(p, scales, a_scales, bias, residual, out, out_h16, ldc, M, N, K, act, gated, err);
-    switch (plan(p, K, n_sms, tiles_w)) {
+    switch (plan(p, K, n_sms, tiles_w, 2)) {
         case 16: return launch4<16, 4, 2>(a, codes, p, tiles_w, stream);
         case 32: return launch4<32, 4, 2>(a, codes, p, tiles_w, stream);
         case 64: return launch4<64, 4, 2>(a, codes, p, tiles_w, stream);

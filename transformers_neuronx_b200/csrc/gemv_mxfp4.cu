@@ -1,8 +1,8 @@
 // Products of a few tokens with a 4-bit matrix (formats: mxfp4.cuh; what is computed: gemm_mxfp4.cu).  The matrix is streamed once; what
 // bounds them is memory, or else the instructions that turn codes into operands, so these are few.
 //
-// A warp takes 16 rows of W (gated: 8 gate rows and their 8 up rows) and a share of K, and works for itself: its lane 0 fetches boxes of
-// 256 columns through TMA into a ring of its own, four ahead.  A block of 32 columns is two MMAs (mma.sync m16n8k16, 16 rows by 8
+// A warp takes 16 rows of W (gated: 8 gate rows and their 8 up rows) and a share of K, which one more warp fetches through TMA in boxes of
+// 256 columns, four ahead.  A block of 32 columns is two MMAs (mma.sync m16n8k16, 16 rows by 8
 // tokens): which column of K stands where in an MMA is free as long as both operands agree, so a lane multiplies eight neighbouring columns
 // of its two rows, one 32-bit word of codes each.  The conversion e2m1x2 -> f16x2 makes them operands, two an instruction and without their
 // scale: an MMA's columns belong to one block, so its 32-bit sums are multiplied by the block's scale when they are added up.  (Codes looked
@@ -20,7 +20,7 @@
 
 namespace {
 
-constexpr int MAX_WARPS = 16;
+constexpr int MAX_WARPS = 15;               // and one that fetches
 constexpr int SLOT_K = 256, SLOT_BLOCKS = SLOT_K / MX_BLOCK, SLOT_BYTES = 16 * SLOT_K / 2;
 constexpr int AHEAD = 4;                     // boxes a warp has asked for
 
@@ -32,6 +32,7 @@ struct Params {
     int M, N, K, w_rows, blocks, slots, act, out_h16, gated;
     int wf, wk, splits, slots_per_split, phase; // phase: boxes of K whose activations lie in shared memory at a time
     int x_at, sx_at;                         // places in shared memory
+    int pairs;                               // two neighbouring scales are one aligned word
     int* err;
 };
 
@@ -65,6 +66,9 @@ __device__ __forceinline__ float ld_cluster(const float* p, uint32_t rank) {
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
     asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(a) : "memory");
     return v;
+}
+__device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
 __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
@@ -145,142 +149,168 @@ __device__ __forceinline__ void make_terms(const Params& p, const Raw& r, uint4 
     }
 }
 
-// NT: groups of eight tokens; SCALED: the activations have scales.
+// A scale byte as a 32-bit number, in the byte's place `at` of w: 2^-127 is half of the smallest normal number; 255, an infinity by its bits,
+// becomes NaN.
+__device__ __forceinline__ float scale_at(uint32_t w, int at) {
+    const float f = __uint_as_float(max((at < 3 ? w << (23 - 8 * at) : w >> 1) & 0x7F800000u, 0x00400000u));
+    return fmaf(f, 0.f, f);
+}
+
+// NT: groups of eight tokens; SCALED: the activations have scales.  Warps 0 .. wf * wk - 1 multiply, the last one fetches codes.
 template <int TERMS, int NT, bool SCALED>
-__global__ void __launch_bounds__(32 * MAX_WARPS, 1) gemv_kernel(const __grid_constant__ CUtensorMap map_w, const Params p) {
+__global__ void __launch_bounds__(32 * (MAX_WARPS + 1), 1) gemv_kernel(const __grid_constant__ CUtensorMap map_w, const Params p) {
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
-    __shared__ uint64_t full[MAX_WARPS][AHEAD];
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    __shared__ uint64_t full[MAX_WARPS][AHEAD], empty[MAX_WARPS][AHEAD];
+    const int warps = p.wf * p.wk, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const int wf = warp % p.wf, wk = warp / p.wf;
     const int s_begin = (int)blockIdx.z * p.slots_per_split, s_end = min(p.slots, s_begin + p.slots_per_split);
-    const int per = (s_end - s_begin + p.wk - 1) / p.wk, b = min(s_begin + wk * per, s_end), e = min(b + per, s_end);
-    // rows of W behind a lane's two MMA rows
-    const int tile = blockIdx.x * p.wf + wf;
-    const int r0 = p.gated ? tile * 8 : tile * 16, r1 = p.gated ? p.N + tile * 8 : tile * 16 + 8;
-    const uint8_t* sa = p.scales + (long long)min(r0 + g, p.w_rows - 1) * p.blocks;
-    const uint8_t* sb = p.scales + (long long)min(r1 + g, p.w_rows - 1) * p.blocks;
-    uint8_t* ring = smem + warp * AHEAD * SLOT_BYTES;
+    const int per = (s_end - s_begin + p.wk - 1) / p.wk;              // boxes of a share of K
+    const int step = p.gated ? 8 : 16, first = blockIdx.x * p.wf * step;             // this block's first feature
+    const int box_bytes = p.wf * SLOT_BYTES;                          // a share's boxes: rows first.., then rows second.. of all its warps
+    bool ok = true;
 
     pdl_launch_dependents();
-    auto fetch = [&](int s) {                             // box s into its place of the ring
-        uint64_t* bar = &full[warp][(s - b) % AHEAD];
-        uint8_t* at = ring + (s - b) % AHEAD * SLOT_BYTES;
-        mbar_expect_tx(bar, SLOT_BYTES);
-        tma_load_2d(at, &map_w, bar, s * (SLOT_K / 2), r0);
-        tma_load_2d(at + SLOT_BYTES / 2, &map_w, bar, s * (SLOT_K / 2), r1);
-    };
-    if (lane == 0) {
-        for (int i = 0; i < AHEAD; ++i) mbar_init(&full[warp][i], 1);
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < p.wk; ++i)
+            for (int j = 0; j < AHEAD; ++j) { mbar_init(&full[i][j], 1); mbar_init(&empty[i][j], p.wf); }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     pdl_wait();
-    if (lane == 0)
-        for (int s = b; s < e && s < b + AHEAD; ++s) fetch(s);
-    __syncwarp();
-    // the scales of a box: lane t of a row holds blocks 2t and 2t + 1 of both rows
-    uint32_t na[2], nb[2];
-    auto load_scales = [&](int s) {
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            const int blk = s * SLOT_BLOCKS + 2 * t + j;
-            const bool in = s < e && blk < p.blocks;
-            na[j] = in ? __ldg(sa + blk) : 0u;
-            nb[j] = in ? __ldg(sb + blk) : 0u;
-        }
-    };
-    load_scales(b);
-
+    __syncthreads();
     float acc[NT][4];
 #pragma unroll
     for (int n = 0; n < NT; ++n) acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.f;
-    uint4* xs = (uint4*)(smem + p.x_at);                  // [term][block of the phase][token][lane t]
-    float* sx = (float*)(smem + p.sx_at);                 // [box of the phase][NT * 8 tokens]
-    const int term_step = p.phase * p.wk * SLOT_BLOCKS * p.M * 4;
-    int token[NT];                                        // places behind the last token: its sums again, which are not written
+
+    if (warp == warps) {
+        if (lane == 0)
+            for (int i = 0; i < per && ok; ++i)
+                for (int share = 0; share < p.wk && ok; ++share) {
+                    const int s = s_begin + share * per + i, place = i % AHEAD;
+                    if (s >= s_end) break;
+                    if (i >= AHEAD) { ok = mbar_wait(&empty[share][place], (uint32_t)(i / AHEAD - 1) & 1u, p.err, 82); if (!ok) break; }
+                    uint8_t* at = smem + (share * AHEAD + place) * box_bytes;
+                    mbar_expect_tx(&full[share][place], (uint32_t)box_bytes);
+                    tma_load_2d(at, &map_w, &full[share][place], s * (SLOT_K / 2), first);
+                    tma_load_2d(at + box_bytes / 2, &map_w, &full[share][place], s * (SLOT_K / 2), p.gated ? p.N + first : first + 8 * p.wf);
+                }
+        __syncwarp();
+    } else {
+        const int b = min(s_begin + wk * per, s_end), e = min(b + per, s_end);
+        // The rows of W behind a lane's two MMA rows: 8 of the first half of the block's rows and 8 of the second.
+        const int ra = first + wf * 8 + g, rb = (p.gated ? p.N + first : first + 8 * p.wf) + wf * 8 + g;
+        const uint8_t* sa = p.scales + (long long)min(ra, p.w_rows - 1) * p.blocks;
+        const uint8_t* sb = p.scales + (long long)min(rb, p.w_rows - 1) * p.blocks;
+        // The scales of a box: lane t of a row holds blocks 2t and 2t + 1 of both rows in one word.
+        auto load_scales = [&](int s) -> uint32_t {
+            const int blk = s * SLOT_BLOCKS + 2 * t;
+            uint32_t v = 0u;
+            if (s >= e) return v;
+            if (p.pairs) {
+                if (blk < p.blocks) v = (uint32_t)__ldg((const uint16_t*)(sa + blk)) | (uint32_t)__ldg((const uint16_t*)(sb + blk)) << 16;
+            } else {
 #pragma unroll
-    for (int n = 0; n < NT; ++n) token[n] = min(n * 8 + g, p.M - 1) * 4 + t;
-    bool ok = true;
-    // A phase is the next p.phase boxes of every share of K.
-    for (int f0 = 0; f0 < per; f0 += p.phase) {
-        if (f0) __syncthreads();
-        const int len = min(p.phase, per - f0);           // boxes of a share
-        // A warp brings a token's share of a box, a lane eight columns; four boxes are asked for before the first is used.
-        const int units = len * p.wk * p.M, warps = p.wf * p.wk;
-        for (int q0 = warp; q0 < units; q0 += 4 * warps) {
-            Raw raw[4];
-            int place[4], tok[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const int q = min(q0 + j * warps, units - 1), box = q / p.M, share = box / len;
-                tok[j] = q - box * p.M;
-                place[j] = share * p.phase + box - share * len;
-                raw[j] = load_raw(p, tok[j], (s_begin + share * per + f0 + box - share * len) * SLOT_K + lane * 8);
+                for (int j = 0; j < 2; ++j)
+                    if (blk + j < p.blocks) v |= (uint32_t)__ldg(sa + blk + j) << (8 * j) | (uint32_t)__ldg(sb + blk + j) << (16 + 8 * j);
             }
+            return v;
+        };
+        uint32_t ahead[AHEAD];                            // as far ahead as the codes: a trip to memory takes longer than a box
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                if (q0 + j * warps >= units) break;
-                uint4 v[TERMS];
-                float scale;
-                make_terms<TERMS, SCALED>(p, raw[j], v, scale);
+        for (int j = 0; j < AHEAD; ++j) ahead[j] = load_scales(b + j);
+        uint4* xs = (uint4*)(smem + p.x_at);              // [term][box of the phase][block][NT * 8 tokens][lane t]; rows of no token are never read out
+        float* sx = (float*)(smem + p.sx_at);             // [box of the phase][NT * 8 tokens]
+        constexpr int BLOCK_X = NT * 8 * 4, BOX_X = SLOT_BLOCKS * BLOCK_X;
+        const int term_step = p.phase * p.wk * BOX_X;
+        uint32_t pass = 0u;
+        // A phase is the next p.phase boxes of every share of K.
+        for (int f0 = 0; f0 < per; f0 += p.phase) {
+            if (f0) asm volatile("bar.sync 1, %0;" ::"r"(32 * warps) : "memory");
+            const int len = min(p.phase, per - f0);       // boxes of a share
+            // A warp brings a token's share of a box, a lane eight columns; four boxes are asked for before the first is used.
+            const int units = len * p.wk * p.M;
+            for (int q0 = warp; q0 < units; q0 += 4 * warps) {
+                Raw raw[4];
+                int at[4], tok[4];
 #pragma unroll
-                for (int k = 0; k < TERMS; ++k) xs[k * term_step + ((place[j] * SLOT_BLOCKS + (lane >> 2)) * p.M + tok[j]) * 4 + (lane & 3)] = v[k];
-                if (SCALED && lane == 0) sx[place[j] * (NT * 8) + tok[j]] = scale;
-            }
-        }
-        __syncthreads();
-        const int last = min(e, b + f0 + len);
-        for (int s = b + f0; s < last; ++s) {
-            float fa[2], fb[2];
+                for (int j = 0; j < 4; ++j) {
+                    const int q = min(q0 + j * warps, units - 1), box = q / p.M, share = box / len;
+                    tok[j] = q - box * p.M;
+                    at[j] = share * p.phase + box - share * len;
+                    raw[j] = load_raw(p, tok[j], (s_begin + share * per + f0 + box - share * len) * SLOT_K + lane * 8);
+                }
 #pragma unroll
-            for (int j = 0; j < 2; ++j) { fa[j] = mx_scale(na[j]); fb[j] = mx_scale(nb[j]); }
-            load_scales(s + 1);
-            const int place = (s - b) % AHEAD;
-            if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&full[warp][place], (uint32_t)((s - b) / AHEAD) & 1u, p.err, 81));
-            if (!ok) break;
-            const uint8_t* row = ring + place * SLOT_BYTES + g * 128 + t * 4;
-            uint32_t wa[SLOT_BLOCKS], wb[SLOT_BLOCKS];
+                for (int j = 0; j < 4; ++j) {
+                    if (q0 + j * warps >= units) break;
+                    uint4 v[TERMS];
+                    float scale;
+                    make_terms<TERMS, SCALED>(p, raw[j], v, scale);
 #pragma unroll
-            for (int i = 0; i < SLOT_BLOCKS; ++i) {
-                const int at = (i ^ g) << 4;
-                wa[i] = *(const uint32_t*)(row + at);
-                wb[i] = *(const uint32_t*)(row + at + SLOT_BYTES / 2);
-            }
-            __syncwarp();
-            if (lane == 0 && s + AHEAD < e) fetch(s + AHEAD);        // the place has been read
-            const int box = wk * p.phase + s - b - f0;
-            const uint4* xb = xs + box * SLOT_BLOCKS * p.M * 4;
-            float sum[NT][4];
-#pragma unroll
-            for (int i = 0; i < SLOT_BLOCKS; ++i) {
-                uint32_t A[4], B[4];
-                codes_to_f16(wa[i], A);
-                codes_to_f16(wb[i], B);
-                const float ga = __shfl_sync(0xffffffffu, fa[i & 1], (lane & ~3) | (i >> 1)), gb = __shfl_sync(0xffffffffu, fb[i & 1], (lane & ~3) | (i >> 1));
-#pragma unroll
-                for (int n = 0; n < NT; ++n) {
-                    float c[4];
-#pragma unroll
-                    for (int k = 0; k < TERMS; ++k) {
-                        const uint4 x = xb[k * term_step + i * p.M * 4 + token[n]];
-                        if (k == 0) mma_first(c, A[0], B[0], A[1], B[1], x.x, x.y);
-                        else mma(c, A[0], B[0], A[1], B[1], x.x, x.y);
-                        mma(c, A[2], B[2], A[3], B[3], x.z, x.w);
-                    }
-                    if (SCALED && i == 0) {
-                        sum[n][0] = c[0] * ga; sum[n][1] = c[1] * ga; sum[n][2] = c[2] * gb; sum[n][3] = c[3] * gb;
-                    } else {
-                        float (&to)[4] = SCALED ? sum[n] : acc[n];
-                        to[0] = fmaf(c[0], ga, to[0]); to[1] = fmaf(c[1], ga, to[1]); to[2] = fmaf(c[2], gb, to[2]); to[3] = fmaf(c[3], gb, to[3]);
-                    }
+                    for (int k = 0; k < TERMS; ++k) xs[k * term_step + at[j] * BOX_X + (lane >> 2) * BLOCK_X + tok[j] * 4 + (lane & 3)] = v[k];
+                    if (SCALED && lane == 0) sx[at[j] * (NT * 8) + tok[j]] = scale;
                 }
             }
-            if (SCALED) {
+            asm volatile("bar.sync 1, %0;" ::"r"(32 * warps) : "memory");
+            const int last = min(e, b + f0 + len);
+            const uint4* xb = xs + wk * p.phase * BOX_X + lane;
+            const float* sxb = sx + wk * p.phase * (NT * 8) + 2 * t;
+            // Unrolled so that a register waits for its load where the scale is used; phases are whole turns.
+            for (int s0 = b + f0; s0 < last && ok; s0 += AHEAD)
 #pragma unroll
-                for (int n = 0; n < NT; ++n) {
-                    const float2 f = *(const float2*)&sx[box * (NT * 8) + n * 8 + 2 * t];
-                    acc[n][0] = fmaf(sum[n][0], f.x, acc[n][0]); acc[n][1] = fmaf(sum[n][1], f.y, acc[n][1]);
-                    acc[n][2] = fmaf(sum[n][2], f.x, acc[n][2]); acc[n][3] = fmaf(sum[n][3], f.y, acc[n][3]);
+              for (int place = 0; place < AHEAD; ++place, xb += BOX_X, sxb += NT * 8) {
+                const int s = s0 + place;
+                if (s >= last) break;
+                float fs[4];                              // lane t: blocks 2t, 2t + 1 of the first row, then of the second
+#pragma unroll
+                for (int j = 0; j < 4; ++j) fs[j] = scale_at(ahead[place], j);
+                ahead[place] = load_scales(s + AHEAD);
+                if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&full[wk][place], pass, p.err, 81));
+                if (!ok) break;
+                const uint8_t* row = smem + (wk * AHEAD + place) * box_bytes + (wf * 8 + g) * 128 + t * 4;
+                const uint8_t* row_b = row + box_bytes / 2;
+                uint32_t wa[SLOT_BLOCKS], wb[SLOT_BLOCKS];
+#pragma unroll
+                for (int i = 0; i < SLOT_BLOCKS; ++i) {
+                    const int at = (i ^ g) << 4;
+                    wa[i] = *(const uint32_t*)(row + at);
+                    wb[i] = *(const uint32_t*)(row_b + at);
+                }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&empty[wk][place]);       // the box has been read
+                if (place == AHEAD - 1) pass ^= 1u;
+                float sum[NT][4];
+#pragma unroll
+                for (int i = 0; i < SLOT_BLOCKS; ++i) {
+                    uint32_t A[4], B[4];
+                    codes_to_f16(wa[i], A);
+                    codes_to_f16(wb[i], B);
+                    const float ga = __shfl_sync(0xffffffffu, fs[i & 1], (lane & ~3) | (i >> 1));
+                    const float gb = __shfl_sync(0xffffffffu, fs[2 + (i & 1)], (lane & ~3) | (i >> 1));
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) {
+                        float c[4];
+#pragma unroll
+                        for (int k = 0; k < TERMS; ++k) {
+                            const uint4 x = xb[k * term_step + i * BLOCK_X + n * 32];
+                            if (k == 0) mma_first(c, A[0], B[0], A[1], B[1], x.x, x.y);
+                            else mma(c, A[0], B[0], A[1], B[1], x.x, x.y);
+                            mma(c, A[2], B[2], A[3], B[3], x.z, x.w);
+                        }
+                        if (SCALED && i == 0) {
+                            sum[n][0] = c[0] * ga; sum[n][1] = c[1] * ga; sum[n][2] = c[2] * gb; sum[n][3] = c[3] * gb;
+                        } else {
+                            float (&to)[4] = SCALED ? sum[n] : acc[n];
+                            to[0] = fmaf(c[0], ga, to[0]); to[1] = fmaf(c[1], ga, to[1]); to[2] = fmaf(c[2], gb, to[2]); to[3] = fmaf(c[3], gb, to[3]);
+                        }
+                    }
+                }
+                if (SCALED) {
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) {
+                        const float2 f = *(const float2*)&sxb[n * 8];
+                        acc[n][0] = fmaf(sum[n][0], f.x, acc[n][0]); acc[n][1] = fmaf(sum[n][1], f.y, acc[n][1]);
+                        acc[n][2] = fmaf(sum[n][2], f.x, acc[n][2]); acc[n][3] = fmaf(sum[n][3], f.y, acc[n][3]);
+                    }
                 }
             }
         }
@@ -290,48 +320,46 @@ __global__ void __launch_bounds__(32 * MAX_WARPS, 1) gemv_kernel(const __grid_co
         const unsigned long long t0 = global_ns();
         while (global_ns() - t0 < 1000000ull) __nanosleep(1000);
     }
-    // The shares' sums: [share][token][rows + 4], the lanes of a warp in 32 banks.
+    // The shares' sums: [share][token][rows + 4], the lanes of a warp in 32 banks.  Gated: a warp's 8 gate rows stand in the first half of the rows,
+    // its 8 up rows in the second; otherwise the two halves are neighbours.
     const int rows = p.wf * 16, ld = rows + 4;
     float* red = (float*)smem;
     __syncthreads();
+    if (warp < warps) {
 #pragma unroll
-    for (int n = 0; n < NT; ++n)
+        for (int n = 0; n < NT; ++n)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int token = n * 8 + 2 * t + (j & 1);
-            if (token < p.M) red[(wk * p.M + token) * ld + wf * 16 + g + 8 * (j >> 1)] = acc[n][j];
-        }
+            for (int j = 0; j < 4; ++j) {
+                const int token = n * 8 + 2 * t + (j & 1);
+                if (token < p.M) red[(wk * p.M + token) * ld + (j >> 1) * (rows / 2) + wf * 8 + g] = acc[n][j];
+            }
+    }
     const int splits = p.splits, rank = splits > 1 ? (int)cta_rank() : 0;
     if (splits > 1) cluster_sync(); else __syncthreads();
     auto total = [&](int token, int row) {                // shares in their order, then the cluster's blocks in theirs
         float v = 0.f;
-        for (int s = 0; s < splits; ++s)
-            for (int w = 0; w < p.wk; ++w) {
-                const float* at = red + (w * p.M + token) * ld + row;
-                v += splits > 1 ? ld_cluster(at, (uint32_t)s) : *at;
-            }
+        const float* at = red + token * ld + row;
+        if (splits == 1) {
+            for (int w = 0; w < p.wk; ++w) v += at[w * p.M * ld];
+        } else
+            for (int s = 0; s < splits; ++s)
+                for (int w = 0; w < p.wk; ++w) v += ld_cluster(at + w * p.M * ld, (uint32_t)s);
         return v;
     };
     const int feats = p.gated ? rows / 2 : rows;
-    for (int i = threadIdx.x * splits + rank; i < feats * p.M; i += blockDim.x * splits) {
-        const int f = i % feats, token = i / feats, n = blockIdx.x * feats + f;
-        if (n >= p.N) continue;
-        const long long o = (long long)token * p.ldc + n;
-        const float res = p.residual ? __ldcg(p.residual + o) : 0.f;
-        float v;
-        if (p.gated) {
-            const int row = (f >> 3) * 16 + (f & 7);
-            float gate = total(token, row), up = total(token, row + 8);
-            if (p.bias) { gate += __ldg(p.bias + n); up += __ldg(p.bias + p.N + n); }
-            v = apply_activation(gate, p.act) * up;
-        } else {
-            v = total(token, f);
-            if (p.bias) v += __ldg(p.bias + n);
-            v = apply_activation(v, p.act);
+    const int f = threadIdx.x % feats;                    // a thread keeps its feature: blocks have at least as many threads as features
+    const int n = first + f, groups = blockDim.x / feats;
+    if ((int)threadIdx.x < groups * feats && n < p.N) {
+        const float bias = p.bias ? __ldg(p.bias + n) : 0.f, bias_up = p.gated && p.bias ? __ldg(p.bias + p.N + n) : 0.f;
+        for (int token = (threadIdx.x / feats) * splits + rank; token < p.M; token += groups * splits) {
+            const long long o = (long long)token * p.ldc + n;
+            const float res = p.residual ? __ldcg(p.residual + o) : 0.f;
+            float v = apply_activation(total(token, f) + bias, p.act);
+            if (p.gated) v *= total(token, feats + f) + bias_up;
+            v += res;
+            if (p.out_h16) ((h16*)p.out)[o] = float_to_h16(v);
+            else ((float*)p.out)[o] = v;
         }
-        v += res;
-        if (p.out_h16) ((h16*)p.out)[o] = float_to_h16(v);
-        else ((float*)p.out)[o] = v;
     }
     if (splits > 1) { __syncwarp(); cluster_sync(); }     // no block leaves while its sums may still be read
 }
@@ -339,12 +367,12 @@ __global__ void __launch_bounds__(32 * MAX_WARPS, 1) gemv_kernel(const __grid_co
 // ---- host -----------------------------------------------------------------------------------------
 constexpr int SMEM_MOST = 224 * 1024;
 
-bool map_codes(CUtensorMap* out, const void* ptr, int rows, int bytes) {
+bool map_codes(CUtensorMap* out, const void* ptr, int rows, int bytes, int box_rows) {
     EncodeTiledFn fn = encode_fn();
     if (!fn) return false;
     cuuint64_t dims[2] = {(cuuint64_t)bytes, (cuuint64_t)rows};
     cuuint64_t strides[1] = {(cuuint64_t)bytes};
-    cuuint32_t box[2] = {128u, 8u};
+    cuuint32_t box[2] = {128u, (cuuint32_t)box_rows};
     cuuint32_t estr[2] = {1, 1};
     return fn(out, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
@@ -353,13 +381,13 @@ bool map_codes(CUtensorMap* out, const void* ptr, int rows, int bytes) {
 template <int TERMS, int NT, bool SCALED>
 int launch(const void* codes, const Params& p, int smem, cudaStream_t stream) {
     CUtensorMap map;
-    if (!map_codes(&map, codes, p.w_rows, p.blocks * 16)) return TNX_ERR_UNSUPPORTED;
+    if (!map_codes(&map, codes, p.w_rows, p.blocks * 16, 8 * p.wf)) return TNX_ERR_UNSUPPORTED;
     static TnxSmemLimit limit;
     auto kernel = gemv_kernel<TERMS, NT, SCALED>;
     const int r = limit.allow(kernel, SMEM_MOST);
     if (r) return r;
     const int per = (p.gated ? 8 : 16) * p.wf;
-    const dim3 grid((p.N + per - 1) / per, 1, p.splits), block(32 * p.wf * p.wk);
+    const dim3 grid((p.N + per - 1) / per, 1, p.splits), block(32 * (p.wf * p.wk + 1));
     if (p.splits > 1) return tnx_launch_cluster(1, dim3(1, 1, p.splits), kernel, grid, block, smem, stream, map, p);
     return tnx_launch_ex(1, kernel, grid, block, smem, stream, map, p);
 }
@@ -392,9 +420,10 @@ TNX_EXPORT int tnx_gemv_mxfp4(const void* a, int a_kind, const void* a_scales, l
     p.M = M; p.N = N; p.K = K; p.w_rows = gated ? 2 * N : N; p.blocks = (K + MX_BLOCK - 1) / MX_BLOCK;
     p.slots = (p.blocks + SLOT_BLOCKS - 1) / SLOT_BLOCKS;
     p.act = act; p.out_h16 = out_h16; p.gated = gated;
+    p.pairs = p.blocks % 2 == 0 && ((uintptr_t)scales & 1) == 0;
     const int terms = a_kind == 1 ? 3 : 1, groups = (N + (gated ? 8 : 16) - 1) / (gated ? 8 : 16);
     const int nt = M <= 8 ? 1 : M <= 16 ? 2 : 4;
-    const int box_x = SLOT_K * 2 * M * terms, box_s = nt * 8 * 4;      // shared memory of a box's activations, for one share of K
+    const int box_x = SLOT_K * 2 * nt * 8 * terms, box_s = nt * 8 * 4;      // shared memory of a box's activations, for one share of K
     // The busiest SM's boxes of codes, and what a block costs beside them (its activations, sums and barriers: as much as 16 boxes).
     long long best = -1;
     for (int splits = 1; splits <= 8; splits *= 2) {
@@ -405,8 +434,8 @@ TNX_EXPORT int tnx_gemv_mxfp4(const void* a, int a_kind, const void* a_scales, l
             if (g_forced_wf && wf != g_forced_wf) continue;
             int wk = MAX_WARPS / wf;
             if (wk > sps) wk = sps;
-            while (wk > 1 && wk * (wf * AHEAD * SLOT_BYTES + box_x + box_s) > SMEM_MOST - 1024) --wk;
-            if (wk * (wf * AHEAD * SLOT_BYTES + box_x + box_s) > SMEM_MOST - 1024) continue;
+            while (wk > 1 && wk * (wf * AHEAD * SLOT_BYTES + AHEAD * (box_x + box_s)) > SMEM_MOST - 1024) --wk;
+            if (wk * (wf * AHEAD * SLOT_BYTES + AHEAD * (box_x + box_s)) > SMEM_MOST - 1024) continue;      // a turn's activations at least
             const long long blocks = (long long)((groups + wf - 1) / wf) * splits;
             const long long rounds = (blocks + n_sms - 1) / n_sms;
             const long long cost = rounds * ((long long)wf * wk * ((sps + wk - 1) / wk) + 16 + (splits > 1 ? 8 : 0));
@@ -416,8 +445,8 @@ TNX_EXPORT int tnx_gemv_mxfp4(const void* a, int a_kind, const void* a_scales, l
     if (best < 0) return TNX_ERR_UNSUPPORTED;
     const int ring = p.wf * p.wk * AHEAD * SLOT_BYTES;
     const int per = (p.slots_per_split + p.wk - 1) / p.wk, most = (SMEM_MOST - 1024 - ring) / (p.wk * (box_x + box_s));
-    const int phases = (per + most - 1) / most;
-    p.phase = (per + phases - 1) / phases;
+    // all of a share, or whole turns of the ring
+    p.phase = per <= most ? per : most / AHEAD * AHEAD;
     p.x_at = ring;
     p.sx_at = ring + p.phase * p.wk * box_x;
     const int sums = p.wk * M * (p.wf * 16 + 4) * 4, used = p.sx_at + p.phase * p.wk * box_s;

@@ -27,56 +27,60 @@ __device__ __forceinline__ float mx_code(uint32_t c) {
     return __uint_as_float(((c & 8u) << 28) | ((c & 7u) << 22)) * 8.507059173023462e37f;
 }
 
-// The eight magnitudes of a block times its scale in the 16-bit type, their high and low bytes apart: a byte permutation then looks
-// four codes up at once.  What 16 bits cannot hold exactly is rounded here (bfloat16: only beyond 2^127 and below 2^-133, where no
-// matrix's block lies that this library made from finite numbers but the largest; float16: see `shift`).
-struct MxTable { uint32_t h0, h1, l0, l1; };
-
-#ifdef TNX_F16
-// The scale relative to the largest of its row, `ref`: 2^(E - ref + 13), so that 6 * 2^13 is the largest magnitude and blocks down to
-// 2^-36 of the row's largest scale keep every bit in float16's normal and subnormal numbers; the rest of the scale is the row's (mx_row_factor).
-constexpr int MX_F16_TOP = 13;
-__device__ __forceinline__ uint32_t mx_scale_h16(uint32_t E, int ref) {
-    const int d = (int)E - ref + MX_F16_TOP;
-    uint32_t b = d >= -14 ? (uint32_t)(d + 15) << 10 : d >= -24 ? 1u << (d + 24) : 0u;
-    if (E == 255u) b = 0x7E00u;
-    return b | (b << 16);
-}
-#define MX_PAIR_0_1 0x38000000u          /* 0.5 : 0   */
-#define MX_PAIR_2_3 0x3E003C00u          /* 1.5 : 1   */
-#define MX_PAIR_4_5 0x42004000u          /* 3   : 2   */
-#define MX_PAIR_6_7 0x46004400u          /* 6   : 4   */
-#else
-__device__ __forceinline__ uint32_t mx_scale_h16(uint32_t E, int) {
-    uint32_t b = E ? E << 7 : 0x0040u;
-    if (E == 255u) b = 0x7FC0u;
-    return b | (b << 16);
-}
-#define MX_PAIR_0_1 0x3F000000u
-#define MX_PAIR_2_3 0x3FC03F80u
-#define MX_PAIR_4_5 0x40404000u
-#define MX_PAIR_6_7 0x40C04080u
-#endif
 __device__ __forceinline__ uint32_t mul_h16x2(uint32_t a, uint32_t b) {
     h16x2 r = __hmul2(*(h16x2*)&a, *(h16x2*)&b);
     return *(uint32_t*)&r;
 }
-__device__ __forceinline__ MxTable mx_table(uint32_t E, int ref) {
-    const uint32_t s = mx_scale_h16(E, ref);
-    const uint32_t p0 = mul_h16x2(MX_PAIR_0_1, s), p1 = mul_h16x2(MX_PAIR_2_3, s), p2 = mul_h16x2(MX_PAIR_4_5, s), p3 = mul_h16x2(MX_PAIR_6_7, s);
-    MxTable t;
-    t.l0 = prmt(p0, p1, 0x6420); t.h0 = prmt(p0, p1, 0x7531);
-    t.l1 = prmt(p2, p3, 0x6420); t.h1 = prmt(p2, p3, 0x7531);
-    return t;
-}
-// Eight codes -> eight 16-bit values in their order: 17 instructions with the table's share (two lookups of four magnitudes' high bytes and
-// low bytes each, the signs spread by the permutation's sign mode, bytes put together).
-__device__ __forceinline__ void mx_decode8(uint32_t w, const MxTable& t, uint32_t& o0, uint32_t& o1, uint32_t& o2, uint32_t& o3) {
-    const uint32_t s = w & 0x77777777u, s2 = s >> 16, w4 = w << 4;
-    const uint32_t ha = prmt(t.h0, t.h1, s) | (prmt(w, w4, 0x9D8C) & 0x80808080u), la = prmt(t.l0, t.l1, s);
-    const uint32_t hb = prmt(t.h0, t.h1, s2) | (prmt(w, w4, 0xBFAE) & 0x80808080u), lb = prmt(t.l0, t.l1, s2);
-    o0 = prmt(la, ha, 0x5140); o1 = prmt(la, ha, 0x7362);
-    o2 = prmt(lb, hb, 0x5140); o3 = prmt(lb, hb, 0x7362);
-}
+
+// A block's codes -> 16-bit values, code times scale, eight at a time in their order.
+#ifdef TNX_F16
+// float16: the conversion e2m1x2 -> f16x2 and a multiplication, by the scale relative to the largest of its row, `ref`: 2^(E - ref + 13), so that
+// 6 * 2^13 is the largest value and blocks down to 2^-36 of the row's largest scale keep every bit in float16's normal and
+// subnormal numbers; the rest of the scale is a factor of the row's sums.
+constexpr int MX_F16_TOP = 13;
+struct MxValues {
+    uint32_t s;
+    __device__ __forceinline__ MxValues(uint32_t E, int ref) {
+        const int d = (int)E - ref + MX_F16_TOP;
+        uint32_t b = d >= -14 ? (uint32_t)(d + 15) << 10 : d >= -24 ? 1u << (d + 24) : 0u;
+        if (E == 255u) b = 0x7E00u;
+        s = b | (b << 16);
+    }
+    __device__ __forceinline__ void decode8(uint32_t w, uint32_t* o) const {
+        uint32_t c[4];
+        asm("{\n\t.reg .b8 b0, b1, b2, b3;\n\t"
+            "mov.b32 {b0, b1, b2, b3}, %4;\n\t"
+            "cvt.rn.f16x2.e2m1x2 %0, b0;\n\t"
+            "cvt.rn.f16x2.e2m1x2 %1, b1;\n\t"
+            "cvt.rn.f16x2.e2m1x2 %2, b2;\n\t"
+            "cvt.rn.f16x2.e2m1x2 %3, b3;\n\t}"
+            : "=r"(c[0]), "=r"(c[1]), "=r"(c[2]), "=r"(c[3]) : "r"(w));
+#pragma unroll
+        for (int j = 0; j < 4; ++j) o[j] = mul_h16x2(c[j], s);
+    }
+};
+#else
+// bfloat16: the eight magnitudes times the scale are a table, high and low bytes apart; a byte permutation looks four codes up at once, signs
+// are spread by the permutation's sign mode, bytes put together: 17 instructions for eight values with the table's share.  Every value is
+// exact but those beyond 2^127 and below 2^-133.
+struct MxValues {
+    uint32_t h0, h1, l0, l1;
+    __device__ __forceinline__ MxValues(uint32_t E, int) {
+        uint32_t s = E ? E << 7 : 0x0040u;
+        if (E == 255u) s = 0x7FC0u;
+        s |= s << 16;
+        const uint32_t p0 = mul_h16x2(0x3F000000u, s), p1 = mul_h16x2(0x3FC03F80u, s), p2 = mul_h16x2(0x40404000u, s), p3 = mul_h16x2(0x40C04080u, s);
+        l0 = prmt(p0, p1, 0x6420); h0 = prmt(p0, p1, 0x7531);
+        l1 = prmt(p2, p3, 0x6420); h1 = prmt(p2, p3, 0x7531);
+    }
+    __device__ __forceinline__ void decode8(uint32_t w, uint32_t* o) const {
+        const uint32_t s = w & 0x77777777u, s2 = s >> 16, w4 = w << 4;
+        const uint32_t ha = prmt(h0, h1, s) | (prmt(w, w4, 0x9D8C) & 0x80808080u), la = prmt(l0, l1, s);
+        const uint32_t hb = prmt(h0, h1, s2) | (prmt(w, w4, 0xBFAE) & 0x80808080u), lb = prmt(l0, l1, s2);
+        o[0] = prmt(la, ha, 0x5140); o[1] = prmt(la, ha, 0x7362);
+        o[2] = prmt(lb, hb, 0x5140); o[3] = prmt(lb, hb, 0x7362);
+    }
+};
+#endif
 
 }  // namespace

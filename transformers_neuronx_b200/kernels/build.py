@@ -61,6 +61,7 @@ SOURCES: Dict[str, str] = {
     "selective_scan": "selective_scan.cu",
     "mxfp4": "mxfp4.cu",
     "gemm_mxfp4": "gemm_mxfp4.cu",
+    "gemm_mxfp4_tiles": "gemm_mxfp4_tiles.cu",
     "gemv_mxfp4": "gemv_mxfp4.cu",
 }
 

@@ -25,6 +25,7 @@ from . import ops as _ops
 from .ops import KernelError, _FLOATS, _H16, _check, _sm_count, _state, activation_code
 
 BLOCK = 32                                    # values that share a scale
+TILE_TOKENS = 128                             # beyond these persistent blocks walk over tiles of up to 192 tokens (gemm_mxfp4_tiles.cu)
 FEW_TOKENS = 16                               # up to here the matrix is streamed through registers (gemv_mxfp4.cu)
 
 
@@ -71,6 +72,7 @@ _SIGNATURES = {
     ("mxfp4", "tnx_mxfp4_gemm_simt"): "piplpppppiliiiii",
     ("gemv_mxfp4", "tnx_gemv_mxfp4"): "piplpppppiliiiiiip",
     ("gemm_mxfp4", "tnx_gemm_mxfp4_16"): "plpppppiliiiiiip", ("gemm_mxfp4", "tnx_gemm_mxfp4_4"): "pppppppiliiiiiip",
+    ("gemm_mxfp4_tiles", "tnx_gemm_mxfp4_tiles_16"): "plpppppiliiiiiip", ("gemm_mxfp4_tiles", "tnx_gemm_mxfp4_tiles_4"): "pppppppiliiiiiip",
 }
 _TYPES = {"p": c_void_p, "l": c_longlong, "i": c_int}
 _entries = {}
@@ -226,12 +228,13 @@ def _product(a, w, out, bias, residual, activation, gated):
                                                            out_h16, ldc, M, N, K, act, 1 if gated else 0, st["sms"], st["err"].data_ptr(), _stream(device))
     elif (a_p | w_p) % 16 == 0 and (quantized or (a.dtype != torch.float32 and lda % 8 == 0)):
         st = _state(w.device)
+        library = "gemm_mxfp4_tiles" if M > TILE_TOKENS else "gemm_mxfp4"
         if quantized:
-            code = _entry("gemm_mxfp4", "tnx_gemm_mxfp4_4", kind)(a_p, a.scales.data_ptr(), w_p, w.scales.data_ptr(), bias_p, res_p, out_p, out_h16, ldc, M, N,
-                                                                 K, act, 1 if gated else 0, st["sms"], st["err"].data_ptr(), _stream(device))
+            code = _entry(library, f"tnx_{library}_4", kind)(a_p, a.scales.data_ptr(), w_p, w.scales.data_ptr(), bias_p, res_p, out_p, out_h16, ldc, M, N, K,
+                                                             act, 1 if gated else 0, st["sms"], st["err"].data_ptr(), _stream(device))
         else:
-            code = _entry("gemm_mxfp4", "tnx_gemm_mxfp4_16", kind)(a_p, lda, w_p, w.scales.data_ptr(), bias_p, res_p, out_p, out_h16, ldc, M, N,
-                                                                  K, act, 1 if gated else 0, st["sms"], st["err"].data_ptr(), _stream(device))
+            code = _entry(library, f"tnx_{library}_16", kind)(a_p, lda, w_p, w.scales.data_ptr(), bias_p, res_p, out_p, out_h16, ldc, M, N, K,
+                                                              act, 1 if gated else 0, st["sms"], st["err"].data_ptr(), _stream(device))
     else:
         code = _entry("mxfp4", "tnx_mxfp4_gemm_simt", kind)(a_p, 2 if quantized else 1 if a.dtype == torch.float32 else 0,
                                                            a.scales.data_ptr() if quantized else 0, lda, w_p, w.scales.data_ptr(), bias_p, res_p, out_p,
