@@ -249,20 +249,27 @@ gemm16_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__
         constexpr uint32_t idesc = idesc16(BN);
         const uint64_t desc0 = smem_desc_sw128(smem_u32(sX));
         Ring<STAGES> r;
-        for (int i = 0; i < num_kb && ok; ++i) {
-            ok = __all_sync(0xffffffffu, mbar_wait(&x_full[r.slot], r.pass, p.err, 63) && mbar_wait(&a_full[r.slot], r.pass, p.err, 64));
-            if (!ok) break;
-            tc_fence_after();
-            const uint64_t bdesc = desc0 + (uint64_t)(r.slot * (X_BYTES >> 4));
-            const uint32_t a = tmem_a + (uint32_t)(r.slot * 32);
-            if (elected()) {
-#pragma unroll
-                for (int k = 0; k < KB / 16; ++k) umma_a_tmem(tmem_d + (uint32_t)(k % ACCS * BN), a + 8u * k, bdesc + (uint64_t)(2 * k), idesc, (i > 0 || k >= ACCS) ? 1u : 0u);
-                umma_commit(&empty[r.slot]);
-                if (i == num_kb - 1) umma_commit(&done);
+        for (int i = 0; i < num_kb && ok;) {
+            int ready = min(ready_stages(x_full, r.slot, r.pass, STAGES, a_full, r.slot, r.pass, STAGES), num_kb - i);
+            if (ready == 0) {
+                ok = __all_sync(0xffffffffu, mbar_wait(&x_full[r.slot], r.pass, p.err, 63) && mbar_wait(&a_full[r.slot], r.pass, p.err, 64));
+                if (!ok) break;
+                ready = 1;
             }
-            __syncwarp();
-            r.next();
+            tc_fence_after();
+            for (; ready > 0; --ready, ++i) {
+                const uint64_t bdesc = desc0 + (uint64_t)(r.slot * (X_BYTES >> 4));
+                const uint32_t a = tmem_a + (uint32_t)(r.slot * 32);
+                if (elected()) {
+#pragma unroll
+                    for (int k = 0; k < KB / 16; ++k)
+                        umma_a_tmem(tmem_d + (uint32_t)(k % ACCS * BN), a + 8u * k, bdesc + (uint64_t)(2 * k), idesc, (i > 0 || k >= ACCS) ? 1u : 0u);
+                    umma_commit(&empty[r.slot]);
+                    if (i == num_kb - 1) umma_commit(&done);
+                }
+                __syncwarp();
+                r.next();
+            }
         }
     } else if (warp >= 4) {
         // Values: warp w fills the lanes of quarter w % 4 (which its tensor memory accesses are confined to), each group of four
@@ -432,22 +439,28 @@ gemm4_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ 
     } else if (warp == 1) {
         const uint64_t desc0 = smem_desc_sw128(smem_u32(smem));
         Ring<STAGES> r;
-        for (int i = 0; i < num && ok; ++i) {
-            ok = __all_sync(0xffffffffu, mbar_wait(&full[r.slot], r.pass, p.err, 72) && mbar_wait(&sf_full[r.slot], r.pass, p.err, 73));
-            if (!ok) break;
-            tc_fence_after();
-            const uint64_t adesc = desc0 + (uint64_t)(r.slot * (STAGE_BYTES >> 4)), bdesc = adesc + (uint64_t)(CODE_BYTES >> 4);
-            const uint32_t sf = tmem_sf + (uint32_t)(r.slot * SF_COLS);
-            if (elected()) {
-#pragma unroll
-                for (int k = 0; k < 4; ++k)               // 64 columns of K = 32 bytes = 2 units of the address field
-                    umma_mxf4(tmem_d, adesc + (uint64_t)(2 * k), bdesc + (uint64_t)(2 * k), idesc4(BN, (k & 1) * 2), sf + 4u * (k >> 1),
-                              sf + 8u + (uint32_t)(XS * (k >> 1)), (i > 0 || k > 0) ? 1u : 0u);
-                umma_commit(&empty[r.slot]);
-                if (i == num - 1) umma_commit(&done);
+        for (int i = 0; i < num && ok;) {
+            int ready = min(ready_stages(full, r.slot, r.pass, STAGES, sf_full, r.slot, r.pass, STAGES), num - i);
+            if (ready == 0) {
+                ok = __all_sync(0xffffffffu, mbar_wait(&full[r.slot], r.pass, p.err, 72) && mbar_wait(&sf_full[r.slot], r.pass, p.err, 73));
+                if (!ok) break;
+                ready = 1;
             }
-            __syncwarp();
-            r.next();
+            tc_fence_after();
+            for (; ready > 0; --ready, ++i) {
+                const uint64_t adesc = desc0 + (uint64_t)(r.slot * (STAGE_BYTES >> 4)), bdesc = adesc + (uint64_t)(CODE_BYTES >> 4);
+                const uint32_t sf = tmem_sf + (uint32_t)(r.slot * SF_COLS);
+                if (elected()) {
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)           // 64 columns of K = 32 bytes = 2 units of the address field
+                        umma_mxf4(tmem_d, adesc + (uint64_t)(2 * k), bdesc + (uint64_t)(2 * k), idesc4(BN, (k & 1) * 2), sf + 4u * (k >> 1),
+                                  sf + 8u + (uint32_t)(XS * (k >> 1)), (i > 0 || k > 0) ? 1u : 0u);
+                    umma_commit(&empty[r.slot]);
+                    if (i == num - 1) umma_commit(&done);
+                }
+                __syncwarp();
+                r.next();
+            }
         }
     } else if (warp >= 4) {
         // Scales: two groups of four warps take stages in turn; a thread loads a row of W's and up to two of the activations', eight scales each,

@@ -22,6 +22,26 @@ struct Epilogue {
 __device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
+// How many of the next stages (up to four) are ready: lane j looks at stage j of one ring, lane 4 + j at stage j of the other, all in one trip
+// to shared memory.  An MMA's issue blocks until the ones ahead of it have almost been executed, and a look at a barrier takes 150 to 200
+// cycles even when it is ready: a look at both rings for every stage left the tensor cores idle for half of the time.
+__device__ __forceinline__ int ready_stages(uint64_t* a, int a_slot, uint32_t a_pass, int a_stages, uint64_t* b, int b_slot, uint32_t b_pass, int b_stages) {
+    const int lane = threadIdx.x & 31;
+    const bool second = lane & 4;
+    int s = (second ? b_slot : a_slot) + (lane & 3);
+    uint32_t parity = second ? b_pass : a_pass;
+    const int n = second ? b_stages : a_stages;
+    if (s >= n) { s -= n; parity ^= 1u; }
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok) : "r"(smem_u32((second ? b : a) + s)), "r"(parity) : "memory");
+    const uint32_t ready = __ballot_sync(0xffffffffu, ok);
+    __syncwarp();
+    return __ffs(~(ready & (ready >> 4) & 15u)) - 1;
+}
 // D (+)= A B with A read from tensor memory (lane = row, a column = two consecutive values of K).
 __device__ __forceinline__ void umma_a_tmem(uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
     asm volatile(

@@ -110,9 +110,9 @@ struct Rings {                               // both kernels' barriers between M
     uint64_t full[2], empty[2];
 };
 
-// The four epilogue warps: accumulator `it & 1` of the CTA's it-th tile.
-template <typename Factor>
-__device__ __forceinline__ bool epilogue(const Params& p, Rings& d, uint32_t tmem_d, int step, Factor factor_of) {
+// The epilogue's warps, SETS of four, take sixteen columns in turn: accumulator `it & 1` of the CTA's it-th tile.
+template <int SETS, typename Factor>
+__device__ __forceinline__ bool epilogue(const Params& p, Rings& d, uint32_t tmem_d, int step, int set, Factor factor_of) {
     const int quad = (threadIdx.x >> 5) & 3, lane = threadIdx.x & 31, r = quad * 32 + lane;
     bool ok = true;
     int it = 0;
@@ -131,14 +131,15 @@ __device__ __forceinline__ bool epilogue(const Params& p, Rings& d, uint32_t tme
         const uint32_t at = tmem_d + (uint32_t)(buf * step) + ((uint32_t)(quad * 32) << 16);
         const int token0 = tt * p.bn, cols = min(p.bn, (p.e.M - token0 + 15) & ~15);
         uint32_t raw[32];
-        tmem_ld16(at, raw);
+        const int c0 = set * 16;
+        if (c0 < cols) tmem_ld16(at + (uint32_t)c0, raw);
 #pragma unroll 1
-        for (int c = 0; c < cols; c += 16) {
+        for (int c = c0; c < cols; c += 16 * SETS) {
             tmem_ld_wait();
             float v[16];
 #pragma unroll
             for (int j = 0; j < 16; ++j) v[j] = __uint_as_float(raw[j]) * factor;
-            if (c + 16 < cols) tmem_ld16(at + (uint32_t)(c + 16), raw);               // on its way while these are written
+            if (c + 16 * SETS < cols) tmem_ld16(at + (uint32_t)(c + 16 * SETS), raw);               // on its way while these are written
             switch (p.e.act) {
                 case TNX_ACT_NONE: write16<TNX_ACT_NONE>(p.e, v, n, token0 + c, bias, bias_up); break;
                 case TNX_ACT_RELU: write16<TNX_ACT_RELU>(p.e, v, n, token0 + c, bias, bias_up); break;
@@ -168,11 +169,10 @@ __device__ __forceinline__ void teardown(bool ok, uint32_t tmem, int warp) {
 }
 
 // ---- 16-bit activations ------------------------------------------------------------------------------
-constexpr int X_STAGES = 6, BOXES = 3, GROUPS = 4;
+constexpr int STAGES16 = 4, BOXES = 4, GROUPS = 4;
 constexpr int THREADS16 = 256 + 128 * GROUPS;        // warps 0: activations, 1: MMAs, 2: codes, 3: rows' references, 4..7: epilogue, 8..23: values
 constexpr int X16_BYTES = MAX_BN * KB * 2;
-constexpr int SMEM16 = BOXES * CODE_BYTES + X_STAGES * X16_BYTES + 1024;
-constexpr int MAX_A_STAGES = 8;              // stages of values in tensor memory: what two accumulators of bn columns leave
+constexpr int SMEM16 = BOXES * CODE_BYTES + STAGES16 * X16_BYTES + 1024;
 
 __global__ void __launch_bounds__(THREADS16, 1)
 gemm16_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const Params p) {
@@ -180,7 +180,7 @@ gemm16_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__
     uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
     uint8_t* sW = smem;
     uint8_t* sX = smem + BOXES * CODE_BYTES;
-    __shared__ uint64_t w_full[BOXES], w_empty[BOXES], x_full[X_STAGES], x_empty[X_STAGES], a_full[MAX_A_STAGES], a_empty[MAX_A_STAGES];
+    __shared__ uint64_t w_full[BOXES], w_empty[BOXES], full[STAGES16], empty[STAGES16];
     __shared__ Rings d;
     __shared__ uint32_t tmem_base_smem;
 #ifdef TNX_F16
@@ -193,8 +193,7 @@ gemm16_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__
     pdl_launch_dependents();
     if (threadIdx.x == 0) {
         for (int i = 0; i < BOXES; ++i) { mbar_init(&w_full[i], 1); mbar_init(&w_empty[i], 4 * GROUPS); }
-        for (int i = 0; i < X_STAGES; ++i) { mbar_init(&x_full[i], 1); mbar_init(&x_empty[i], 1); }
-        for (int i = 0; i < MAX_A_STAGES; ++i) { mbar_init(&a_full[i], 4); mbar_init(&a_empty[i], 1); }
+        for (int i = 0; i < STAGES16; ++i) { mbar_init(&full[i], 5); mbar_init(&empty[i], 1); }       // full: activations and four warps' values
         for (int i = 0; i < 2; ++i) { mbar_init(&d.full[i], 1); mbar_init(&d.empty[i], 4); }
 #ifdef TNX_F16
         for (int i = 0; i < 2; ++i) { mbar_init(&ref_full[i], 1); mbar_init(&ref_empty[i], 4 + 4 * GROUPS); }
@@ -208,19 +207,20 @@ gemm16_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem_d = tmem_base_smem, tmem_a = tmem_d + 2 * p.bn;
-    const int a_stages = min((512 - 2 * p.bn) / 32, MAX_A_STAGES);
-    bool ok = true;
-
-    if (warp == 0) {
+    // The whole of tensor memory is this CTA's, so it begins at column 0: addresses that the compiler knows.
+    constexpr uint32_t tmem_d = 0u, tmem_a = 2 * MAX_BN;
+    bool ok = tmem_base_smem == 0u;                       // never anything else
+    if (!ok) {
+        if (threadIdx.x == 0) atomicExch(p.err, 90);
+    } else if (warp == 0) {
         if (lane == 0) {
-            Ring<X_STAGES> r;
+            Ring<STAGES16> r;
             int n = 0;
             for (int tile = blockIdx.x; tile < p.tiles && ok; tile += gridDim.x)
                 for (int i = 0; i < num; ++i, ++n) {
-                    if (n >= X_STAGES) { ok = mbar_wait(&x_empty[r.slot], r.pass ^ 1u, p.err, 92); if (!ok) break; }
-                    mbar_expect_tx(&x_full[r.slot], (uint32_t)(p.bn * KB * 2));
-                    tma_load_2d(sX + r.slot * X16_BYTES, &map_x, &x_full[r.slot], i * KB, tile % p.tiles_t * p.bn);
+                    if (n >= STAGES16) { ok = mbar_wait(&empty[r.slot], r.pass ^ 1u, p.err, 92); if (!ok) break; }
+                    mbar_expect_tx(&full[r.slot], (uint32_t)(p.bn * KB * 2));
+                    tma_load_2d(sX + r.slot * X16_BYTES, &map_x, &full[r.slot], i * KB, tile % p.tiles_t * p.bn);
                     r.next();
                 }
         }
@@ -238,33 +238,39 @@ gemm16_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__
         }
         __syncwarp();
     } else if (warp == 1) {
+        // Two stages a turn: a wait costs this warp 200 cycles even where the barrier is ready (it queues behind the MMAs issued before it), the
+        // MMAs of a stage take 256 to 384; a wait and other turn's work for every stage took 600 to 700.
         const uint32_t idesc = idesc16(p.bn);
         const uint64_t desc0 = smem_desc_sw128(smem_u32(sX));
-        Ring<X_STAGES> r;
-        int it = 0, as = 0;
-        uint32_t apass = 0u;
-        for (int tile = blockIdx.x; tile < p.tiles && ok; tile += gridDim.x, ++it) {
-            const int buf = it & 1;
-            if (it >= 2) ok = __all_sync(0xffffffffu, mbar_wait(&d.empty[buf], (uint32_t)((it >> 1) - 1) & 1u, p.err, 94));
-            if (!ok) break;
-            tc_fence_after();
-            const uint32_t acc = tmem_d + (uint32_t)(buf * p.bn);
-            for (int i = 0; i < num && ok; ++i) {
-                ok = __all_sync(0xffffffffu, mbar_wait(&x_full[r.slot], r.pass, p.err, 95) && mbar_wait(&a_full[as], apass, p.err, 96));
-                if (!ok) break;
-                tc_fence_after();
-                const uint64_t bdesc = desc0 + (uint64_t)(r.slot * (X16_BYTES >> 4));
-                const uint32_t a = tmem_a + (uint32_t)(as * 32);
-                if (elected()) {
+        const int total = (p.tiles - (int)blockIdx.x + (int)gridDim.x - 1) / (int)gridDim.x * num;
+        int i = 0, it = 0;
+        for (int n0 = 0; n0 < total && ok; n0 += STAGES16) {
+            const uint32_t pass = (uint32_t)(n0 / STAGES16) & 1u;
 #pragma unroll
-                    for (int k = 0; k < KB / 16; ++k) umma_a_tmem(acc, a + 8u * k, bdesc + (uint64_t)(2 * k), idesc, (i > 0 || k > 0) ? 1u : 0u);
-                    umma_commit(&x_empty[r.slot]);
-                    umma_commit(&a_empty[as]);
-                    if (i == num - 1) umma_commit(&d.full[buf]);
+            for (int s0 = 0; s0 < STAGES16; s0 += 2) {
+                if (n0 + s0 >= total || !ok) break;
+                const bool both = n0 + s0 + 1 < total;
+                ok = mbar_wait(&full[s0], pass, p.err, 95) && (!both || mbar_wait(&full[s0 + 1], pass, p.err, 96));
+                ok = __all_sync(0xffffffffu, ok);
+#pragma unroll
+                for (int s = s0; s < s0 + 2; ++s) {
+                    if (!ok || (s > s0 && !both)) break;
+                    if (i == 0 && it >= 2) {
+                        ok = __all_sync(0xffffffffu, mbar_wait(&d.empty[it & 1], (uint32_t)((it >> 1) - 1) & 1u, p.err, 94));
+                        if (!ok) break;
+                    }
+                    tc_fence_after();
+                    if (elected()) {
+                        const uint32_t acc = tmem_d + (it & 1 ? MAX_BN : 0);
+#pragma unroll
+                        for (int k = 0; k < KB / 16; ++k)
+                            umma_a_tmem(acc, tmem_a + (uint32_t)(s * 32 + 8 * k), desc0 + (uint64_t)(s * (X16_BYTES >> 4) + 2 * k), idesc, (i > 0 || k > 0) ? 1u : 0u);
+                        umma_commit(&empty[s]);
+                        if (i == num - 1) umma_commit(&d.full[it & 1]);
+                    }
+                    __syncwarp();
+                    if (++i == num) { i = 0; ++it; }
                 }
-                __syncwarp();
-                r.next();
-                if (++as == a_stages) { as = 0; apass ^= 1u; }
             }
         }
     } else if (warp == 3) {
@@ -296,7 +302,7 @@ gemm16_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__
         }
 #endif
     } else if (warp < 8) {
-        ok = epilogue(p, d, tmem_d, p.bn, [&](int it) {
+        ok = epilogue<1>(p, d, tmem_d, MAX_BN, 0, [&](int it) {
 #ifdef TNX_F16
             const int buf = it & 1;
             if (!__all_sync(0xffffffffu, mbar_wait(&ref_full[buf], (uint32_t)(it >> 1) & 1u, p.err, 98))) return 0.f;
@@ -374,9 +380,9 @@ gemm16_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&w_empty[ws]);                 // this warp has read its share of the box
                 if (i >= num) continue;
-                const int turn = n / a_stages, s = n - turn * a_stages;
-                if (turn > 0) {
-                    ok = __all_sync(0xffffffffu, mbar_wait(&a_empty[s], (uint32_t)(turn - 1) & 1u, p.err, 101));
+                const int s = n % STAGES16;
+                if (n >= STAGES16) {
+                    ok = __all_sync(0xffffffffu, mbar_wait(&empty[s], (uint32_t)(n / STAGES16 - 1) & 1u, p.err, 101));
                     if (!ok) break;
                     tc_fence_after();
                 }
@@ -384,7 +390,7 @@ gemm16_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__
                 tmem_st_wait();
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&a_full[s]);
+                if (lane == 0) mbar_arrive(&full[s]);
             }
         }
     }
@@ -393,10 +399,11 @@ gemm16_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__
 
 // ---- 4-bit activations -------------------------------------------------------------------------------
 constexpr int STAGES4 = 5;
-constexpr int THREADS4 = 512;                // warps 0: TMA, 1: MMAs, 4..7: epilogue, 8..15: scales
+constexpr int THREADS4 = 640;                // warps 0: TMA, 1: MMAs, 4..11: epilogue, 12..19: scales
 constexpr int X4_BYTES = MAX_BN * CODE_K / 2, STAGE4_BYTES = CODE_BYTES + X4_BYTES;
 constexpr int SMEM4 = STAGES4 * STAGE4_BYTES + 1024;
 constexpr int SF_COLS = 24;                  // a stage's scales: 2 x 4 columns for W, 2 x 8 for up to 256 tokens
+constexpr int SF_LD = SF_COLS + 4;           // a lane's scales in shared memory: 16-byte loads of eight lanes lie in all banks
 
 __device__ __forceinline__ void group_sync(int group) {
     if (group) asm volatile("bar.sync 2, 128;" ::: "memory");
@@ -408,17 +415,17 @@ gemm4_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ 
     static_assert(2 * MAX_BN + STAGES4 * SF_COLS <= 512, "tensor memory");
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
-    __shared__ uint64_t full[STAGES4], sf_full[STAGES4], empty[STAGES4];
+    __shared__ uint64_t full[STAGES4], empty[STAGES4];
     __shared__ Rings d;
     __shared__ uint32_t tmem_base_smem;
-    __shared__ uint32_t sf_smem[2][SF_COLS * 32];
+    __shared__ __align__(16) uint32_t sf_smem[2][2][32 * SF_LD];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int num = p.num;
 
     pdl_launch_dependents();
     if (threadIdx.x == 0) {
-        for (int i = 0; i < STAGES4; ++i) { mbar_init(&full[i], 1); mbar_init(&sf_full[i], 4); mbar_init(&empty[i], 1); }
-        for (int i = 0; i < 2; ++i) { mbar_init(&d.full[i], 1); mbar_init(&d.empty[i], 4); }
+        for (int i = 0; i < STAGES4; ++i) { mbar_init(&full[i], 5); mbar_init(&empty[i], 1); }         // full: codes and four warps' scales
+        for (int i = 0; i < 2; ++i) { mbar_init(&d.full[i], 1); mbar_init(&d.empty[i], 8); }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("prefetch.tensormap [%0];" ::"l"((unsigned long long)&map_w) : "memory");
         asm volatile("prefetch.tensormap [%0];" ::"l"((unsigned long long)&map_x) : "memory");
@@ -428,10 +435,11 @@ gemm4_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ 
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem_d = tmem_base_smem, tmem_sf = tmem_d + 2 * MAX_BN;
-    bool ok = true;
-
-    if (warp == 0) {
+    constexpr uint32_t tmem_d = 0u, tmem_sf = 2 * MAX_BN;            // the whole of tensor memory is this CTA's
+    bool ok = tmem_base_smem == 0u;                       // never anything else
+    if (!ok) {
+        if (threadIdx.x == 0) atomicExch(p.err, 90);
+    } else if (warp == 0) {
         if (lane == 0) {
             Ring<STAGES4> r;
             int n = 0;
@@ -449,65 +457,81 @@ gemm4_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ 
     } else if (warp == 1) {
         const uint32_t idesc0 = idesc4(p.bn, 0), idesc2 = idesc4(p.bn, 2);
         const uint64_t desc0 = smem_desc_sw128(smem_u32(smem));
+        const int total = (p.tiles - (int)blockIdx.x + (int)gridDim.x - 1) / (int)gridDim.x * num;
+        int i = 0, it = 0;
         Ring<STAGES4> r;
-        int it = 0;
-        for (int tile = blockIdx.x; tile < p.tiles && ok; tile += gridDim.x, ++it) {
-            const int buf = it & 1;
-            if (it >= 2) ok = __all_sync(0xffffffffu, mbar_wait(&d.empty[buf], (uint32_t)((it >> 1) - 1) & 1u, p.err, 112));
-            if (!ok) break;
-            tc_fence_after();
-            const uint32_t acc = tmem_d + (uint32_t)(buf * MAX_BN);
-            for (int i = 0; i < num && ok; ++i) {
-                ok = __all_sync(0xffffffffu, mbar_wait(&full[r.slot], r.pass, p.err, 113) && mbar_wait(&sf_full[r.slot], r.pass, p.err, 114));
-                if (!ok) break;
+        for (int n = 0; n < total && ok; n += 2) {        // two stages a turn, as above
+            Ring<STAGES4> q = r;
+            q.next();
+            const bool both = n + 1 < total;
+            ok = mbar_wait(&full[r.slot], r.pass, p.err, 113) && (!both || mbar_wait(&full[q.slot], q.pass, p.err, 114));
+            ok = __all_sync(0xffffffffu, ok);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                if (!ok || (h && !both)) break;
+                if (i == 0 && it >= 2) {
+                    ok = __all_sync(0xffffffffu, mbar_wait(&d.empty[it & 1], (uint32_t)((it >> 1) - 1) & 1u, p.err, 112));
+                    if (!ok) break;
+                }
                 tc_fence_after();
                 const uint64_t adesc = desc0 + (uint64_t)(r.slot * (STAGE4_BYTES >> 4)), bdesc = adesc + (uint64_t)(CODE_BYTES >> 4);
-                const uint32_t sf = tmem_sf + (uint32_t)(r.slot * SF_COLS);
+                const uint32_t sf = tmem_sf + (uint32_t)(r.slot * SF_COLS), acc = tmem_d + (it & 1 ? MAX_BN : 0);
                 if (elected()) {
 #pragma unroll
                     for (int k = 0; k < 4; ++k)           // 64 columns of K = 32 bytes = 2 units of the address field
                         umma_mxf4(acc, adesc + (uint64_t)(2 * k), bdesc + (uint64_t)(2 * k), k & 1 ? idesc2 : idesc0, sf + 4u * (k >> 1),
                                   sf + 8u + 8u * (k >> 1), (i > 0 || k > 0) ? 1u : 0u);
                     umma_commit(&empty[r.slot]);
-                    if (i == num - 1) umma_commit(&d.full[buf]);
+                    if (i == num - 1) umma_commit(&d.full[it & 1]);
                 }
                 __syncwarp();
                 r.next();
+                if (++i == num) { i = 0; ++it; }
             }
         }
-    } else if (warp >= 8) {
+    } else if (warp >= 12) {
         // Scales: two groups of four warps take stages in turn; a thread loads a row of W's and up to two of the activations', eight scales each,
-        // three turns ahead (a trip to memory takes longer than a stage); then every warp stores all of them to the lanes of its quarter.
-        const int quad = warp & 3, group = (warp - 8) >> 2, r = quad * 32 + lane;
+        // three turns ahead (a trip to memory takes longer than a stage); they meet in shared memory, whence every warp takes all of them
+        // to the lanes of its quarter.
+        const int quad = warp & 3, group = (warp - 12) >> 2, r = quad * 32 + lane;
+        const bool words = p.blocks % 8 == 0 && (((uintptr_t)p.scales | (uintptr_t)p.a_scales) & 7) == 0;        // eight scales are one aligned load
+        const bool second = r + 128 < p.bn, first = r < p.bn;
         const uint8_t* w_end = p.scales + (long long)p.w_rows * p.blocks;
         const uint8_t* x_end = p.a_scales + (long long)p.e.M * p.blocks;
         struct Scales { uint2 w, x[2]; };
         int ptile = blockIdx.x, pi = group;
-        const uint8_t* ws = nullptr;
-        const uint8_t* xs[2] = {nullptr, nullptr};
+        const uint8_t *ws = nullptr, *xs0 = nullptr, *xs1 = nullptr;
         auto aim = [&]() {                                // over the tiles' ends
             while (pi >= num) { pi -= num; ptile += gridDim.x; }
             if (ptile >= p.tiles) return;
-            ws = p.scales + (long long)tile_row(p, ptile / p.tiles_t, r) * p.blocks;
-#pragma unroll
-            for (int j = 0; j < 2; ++j) xs[j] = p.a_scales + (long long)min(ptile % p.tiles_t * p.bn + r + 128 * j, p.e.M - 1) * p.blocks;
+            const int token = ptile % p.tiles_t * p.bn + r;
+            ws = p.scales + (long long)tile_row(p, ptile / p.tiles_t, r) * p.blocks + pi * 8;
+            xs0 = p.a_scales + (long long)min(token, p.e.M - 1) * p.blocks + pi * 8;
+            xs1 = p.a_scales + (long long)min(token + 128, p.e.M - 1) * p.blocks + pi * 8;
         };
         auto load = [&]() {
             Scales q;
             q.w = q.x[0] = q.x[1] = make_uint2(0u, 0u);
             if (ptile >= p.tiles) return q;
-            const int b = pi * 8, n = p.blocks - b;
-            q.w = load8(ws + b, p.scales, w_end, n);
-#pragma unroll
-            for (int j = 0; j < 2; ++j) if (r + 128 * j < p.bn) q.x[j] = load8(xs[j] + b, p.a_scales, x_end, n);
-            pi += 2;
+            if (words) {
+                q.w = __ldg((const uint2*)ws);
+                if (first) q.x[0] = __ldg((const uint2*)xs0);
+                if (second) q.x[1] = __ldg((const uint2*)xs1);
+            } else {
+                const int n = p.blocks - pi * 8;
+                q.w = load8(ws, p.scales, w_end, n);
+                if (first) q.x[0] = load8(xs0, p.a_scales, x_end, n);
+                if (second) q.x[1] = load8(xs1, p.a_scales, x_end, n);
+            }
+            pi += 2; ws += 16; xs0 += 16; xs1 += 16;
             if (pi >= num) aim();
             return q;
         };
         aim();
-        uint32_t* buf = sf_smem[group];
         Scales ahead[3] = {load(), load(), load()};
         const int total = (p.tiles - (int)blockIdx.x + (int)gridDim.x - 1) / (int)gridDim.x * num;
+        int turn = 0, s = group;
+        uint32_t pass = 1u;                               // of the stage's last use, from its second use on
         for (int i0 = group; i0 < total; i0 += 6) {       // whole even if a wait ran out: the groups' warps meet at their barrier
 #pragma unroll
             for (int u = 0; u < 3; ++u) {                 // (unrolled so that a register waits for its load where it is used)
@@ -515,16 +539,21 @@ gemm4_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ 
                 if (i >= total) break;
                 const Scales now = ahead[u];
                 ahead[u] = load();
-                buf[quad * 32 + lane] = now.w.x; buf[(4 + quad) * 32 + lane] = now.w.y;
-#pragma unroll
-                for (int j = 0; j < 2; ++j) { buf[(8 + 4 * j + quad) * 32 + lane] = now.x[j].x; buf[(16 + 4 * j + quad) * 32 + lane] = now.x[j].y; }
+                uint32_t* buf = &sf_smem[group][turn][0]; // two in turn: one barrier a stage
+                turn ^= 1;
+                uint32_t* mine = buf + lane * SF_LD + quad;
+                mine[0] = now.w.x; mine[4] = now.w.y;
+                mine[8] = now.x[0].x; mine[16] = now.x[0].y;
+                mine[12] = now.x[1].x; mine[20] = now.x[1].y;
                 group_sync(group);
                 uint32_t v[SF_COLS];
 #pragma unroll
-                for (int c = 0; c < SF_COLS; ++c) v[c] = buf[c * 32 + lane];
-                const int s = i % STAGES4;
+                for (int c = 0; c < SF_COLS; c += 4) {
+                    const uint4 q = *(const uint4*)(buf + lane * SF_LD + c);
+                    v[c] = q.x; v[c + 1] = q.y; v[c + 2] = q.z; v[c + 3] = q.w;
+                }
                 if (ok && i >= STAGES4) {
-                    ok = __all_sync(0xffffffffu, mbar_wait(&empty[s], (uint32_t)(i / STAGES4 - 1) & 1u, p.err, 115));
+                    ok = __all_sync(0xffffffffu, mbar_wait(&empty[s], pass, p.err, 115));
                     tc_fence_after();
                 }
                 if (ok) {
@@ -539,13 +568,14 @@ gemm4_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ 
                     tmem_st_wait();
                     tc_fence_before();
                     __syncwarp();
-                    if (lane == 0) mbar_arrive(&sf_full[s]);
+                    if (lane == 0) mbar_arrive(&full[s]);
                 }
-                group_sync(group);                        // the buffer has been read by all four
+                s += 2;
+                if (s >= STAGES4) { s -= STAGES4; pass ^= 1u; }
             }
         }
     } else if (warp >= 4) {
-        ok = epilogue(p, d, tmem_d, MAX_BN, [](int) { return 1.f; });
+        ok = epilogue<2>(p, d, tmem_d, MAX_BN, (warp - 4) >> 2, [](int) { return 1.f; });
     }
     teardown(ok, tmem_base_smem, warp);
 }
