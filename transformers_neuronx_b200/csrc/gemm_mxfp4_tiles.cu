@@ -583,7 +583,7 @@ gemm4_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ 
 // ---- host -----------------------------------------------------------------------------------------
 int g_forced_bn = 0;
 
-// Tokens of a tile: the busiest CTA's rounds of tiles, each as long as its columns (and what a tile costs beside them: `extra` columns).
+// Tokens of a tile: the busiest CTA's rounds of tiles, each as long as its columns and what a stage costs whatever its columns are, `extra` of them.
 void plan(Params& p, int n_sms, int tiles_w, int extra) {
     long long best = -1;
     const int most = (p.e.M + 15) / 16 * 16;
@@ -619,7 +619,7 @@ TNX_EXPORT int tnx_gemm_mxfp4_tiles_16(const void* a, long long lda, const void*
     fill_epilogue(p.e, bias, residual, out, out_h16, ldc, M, N, act, gated);
     p.scales = (const uint8_t*)scales; p.a_scales = nullptr; p.err = err;
     p.w_rows = gated ? 2 * N : N; p.blocks = (K + MX_BLOCK - 1) / MX_BLOCK; p.num = (K + KB - 1) / KB;
-    plan(p, n_sms, tiles_w, 16);
+    plan(p, n_sms, tiles_w, 400);
     CUtensorMap mw, mx;
     if (!map_bytes(&mw, codes, p.w_rows, p.blocks * 16, gated ? 16 : TILE_W) || !map_h16(&mx, a, M, K, lda, p.bn)) return TNX_ERR_UNSUPPORTED;
     static TnxSmemLimit limit;
@@ -637,7 +637,7 @@ TNX_EXPORT int tnx_gemm_mxfp4_tiles_4(const void* a, const void* a_scales, const
     fill_epilogue(p.e, bias, residual, out, out_h16, ldc, M, N, act, gated);
     p.scales = (const uint8_t*)scales; p.a_scales = (const uint8_t*)a_scales; p.err = err;
     p.w_rows = gated ? 2 * N : N; p.blocks = (K + MX_BLOCK - 1) / MX_BLOCK; p.num = (K + CODE_K - 1) / CODE_K;
-    plan(p, n_sms, tiles_w, 16);
+    plan(p, n_sms, tiles_w, 400);
     CUtensorMap mw, mx;
     if (!map_bytes(&mw, codes, p.w_rows, p.blocks * 16, gated ? 16 : TILE_W) || !map_bytes(&mx, a, M, p.blocks * 16, p.bn)) return TNX_ERR_UNSUPPORTED;
     static TnxSmemLimit limit;

@@ -32,7 +32,7 @@ struct Params {
     int M, N, K, w_rows, blocks, slots, act, out_h16, gated;
     int wf, wk, splits, slots_per_split, phase; // phase: boxes of K whose activations lie in shared memory at a time
     int x_at, sx_at;                         // places in shared memory
-    int pairs;                               // two neighbouring scales are one aligned word
+    int sw_at, sw_ld, words;                 // scales' place, bytes a row of them; eight of them are one aligned load
     int* err;
 };
 
@@ -197,36 +197,33 @@ __global__ void __launch_bounds__(32 * (MAX_WARPS + 1), 1) gemv_kernel(const __g
         __syncwarp();
     } else {
         const int b = min(s_begin + wk * per, s_end), e = min(b + per, s_end);
-        // The rows of W behind a lane's two MMA rows: 8 of the first half of the block's rows and 8 of the second.
-        const int ra = first + wf * 8 + g, rb = (p.gated ? p.N + first : first + 8 * p.wf) + wf * 8 + g;
-        const uint8_t* sa = p.scales + (long long)min(ra, p.w_rows - 1) * p.blocks;
-        const uint8_t* sb = p.scales + (long long)min(rb, p.w_rows - 1) * p.blocks;
-        // The scales of a box: lane t of a row holds blocks 2t and 2t + 1 of both rows in one word.
-        auto load_scales = [&](int s) -> uint32_t {
-            const int blk = s * SLOT_BLOCKS + 2 * t;
-            uint32_t v = 0u;
-            if (s >= e) return v;
-            if (p.pairs) {
-                if (blk < p.blocks) v = (uint32_t)__ldg((const uint16_t*)(sa + blk)) | (uint32_t)__ldg((const uint16_t*)(sb + blk)) << 16;
-            } else {
-#pragma unroll
-                for (int j = 0; j < 2; ++j)
-                    if (blk + j < p.blocks) v |= (uint32_t)__ldg(sa + blk + j) << (8 * j) | (uint32_t)__ldg(sb + blk + j) << (16 + 8 * j);
-            }
-            return v;
-        };
-        uint32_t ahead[AHEAD];                            // as far ahead as the codes: a trip to memory takes longer than a box
-#pragma unroll
-        for (int j = 0; j < AHEAD; ++j) ahead[j] = load_scales(b + j);
         uint4* xs = (uint4*)(smem + p.x_at);              // [term][box of the phase][block][NT * 8 tokens][lane t]; rows of no token are never read out
         float* sx = (float*)(smem + p.sx_at);             // [box of the phase][NT * 8 tokens]
+        uint8_t* sw = smem + p.sw_at;                     // [row: the first half's, then the second's][box of the phase][8 scales]
         constexpr int BLOCK_X = NT * 8 * 4, BOX_X = SLOT_BLOCKS * BLOCK_X;
         const int term_step = p.phase * p.wk * BOX_X;
+        int place = 0;
         uint32_t pass = 0u;
         // A phase is the next p.phase boxes of every share of K.
         for (int f0 = 0; f0 < per; f0 += p.phase) {
             if (f0) asm volatile("bar.sync 1, %0;" ::"r"(32 * warps) : "memory");
             const int len = min(p.phase, per - f0);       // boxes of a share
+            // W's scales, as they lie in memory: a trip there for every box would take longer than the box.
+            for (int q = threadIdx.x; q < 16 * p.wf * p.wk * len; q += 32 * warps) {
+                const int row = q / (p.wk * len), rest = q - row * (p.wk * len), share = rest / len, f = rest - share * len;
+                const int w_row = min(row < 8 * p.wf ? first + row : (p.gated ? p.N + first : first + 8 * p.wf) + row - 8 * p.wf, p.w_rows - 1);
+                const int blk = (s_begin + share * per + f0 + f) * SLOT_BLOCKS;
+                const uint8_t* src = p.scales + (long long)w_row * p.blocks + blk;
+                uint2 v = make_uint2(0u, 0u);
+                if (p.words) {
+                    if (blk < p.blocks) v = __ldg((const uint2*)src);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j)
+                        if (blk + j < p.blocks) { const uint32_t E = (uint32_t)__ldg(src + j) << (8 * (j & 3)); if (j < 4) v.x |= E; else v.y |= E; }
+                }
+                *(uint2*)(sw + row * p.sw_ld + (share * p.phase + f) * 8) = v;
+            }
             // A warp brings a token's share of a box, a lane eight columns; four boxes are asked for before the first is used.
             const int units = len * p.wk * p.M;
             for (int q0 = warp; q0 < units; q0 += 4 * warps) {
@@ -254,16 +251,14 @@ __global__ void __launch_bounds__(32 * (MAX_WARPS + 1), 1) gemv_kernel(const __g
             const int last = min(e, b + f0 + len);
             const uint4* xb = xs + wk * p.phase * BOX_X + lane;
             const float* sxb = sx + wk * p.phase * (NT * 8) + 2 * t;
-            // Unrolled so that a register waits for its load where the scale is used; phases are whole turns.
-            for (int s0 = b + f0; s0 < last && ok; s0 += AHEAD)
+            const uint8_t* swa = sw + (wf * 8 + g) * p.sw_ld + wk * p.phase * 8 + 2 * t;
+#pragma unroll 1
+            for (int s = b + f0; s < last; ++s, xb += BOX_X, sxb += NT * 8, swa += 8) {
+                // lane t: the scales of blocks 2t, 2t + 1 of its first row, then of its second
+                const uint32_t two = *(const uint16_t*)swa | (uint32_t)*(const uint16_t*)(swa + 8 * p.wf * p.sw_ld) << 16;
+                float fs[4];
 #pragma unroll
-              for (int place = 0; place < AHEAD; ++place, xb += BOX_X, sxb += NT * 8) {
-                const int s = s0 + place;
-                if (s >= last) break;
-                float fs[4];                              // lane t: blocks 2t, 2t + 1 of the first row, then of the second
-#pragma unroll
-                for (int j = 0; j < 4; ++j) fs[j] = scale_at(ahead[place], j);
-                ahead[place] = load_scales(s + AHEAD);
+                for (int j = 0; j < 4; ++j) fs[j] = scale_at(two, j);
                 if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&full[wk][place], pass, p.err, 81));
                 if (!ok) break;
                 const uint8_t* row = smem + (wk * AHEAD + place) * box_bytes + (wf * 8 + g) * 128 + t * 4;
@@ -277,7 +272,7 @@ __global__ void __launch_bounds__(32 * (MAX_WARPS + 1), 1) gemv_kernel(const __g
                 }
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&empty[wk][place]);       // the box has been read
-                if (place == AHEAD - 1) pass ^= 1u;
+                if (++place == AHEAD) { place = 0; pass ^= 1u; }
                 float sum[NT][4];
 #pragma unroll
                 for (int i = 0; i < SLOT_BLOCKS; ++i) {
@@ -420,10 +415,11 @@ TNX_EXPORT int tnx_gemv_mxfp4(const void* a, int a_kind, const void* a_scales, l
     p.M = M; p.N = N; p.K = K; p.w_rows = gated ? 2 * N : N; p.blocks = (K + MX_BLOCK - 1) / MX_BLOCK;
     p.slots = (p.blocks + SLOT_BLOCKS - 1) / SLOT_BLOCKS;
     p.act = act; p.out_h16 = out_h16; p.gated = gated;
-    p.pairs = p.blocks % 2 == 0 && ((uintptr_t)scales & 1) == 0;
+    p.words = p.blocks % 8 == 0 && ((uintptr_t)scales & 7) == 0;
     const int terms = a_kind == 1 ? 3 : 1, groups = (N + (gated ? 8 : 16) - 1) / (gated ? 8 : 16);
     const int nt = M <= 8 ? 1 : M <= 16 ? 2 : 4;
     const int box_x = SLOT_K * 2 * nt * 8 * terms, box_s = nt * 8 * 4;      // shared memory of a box's activations, for one share of K
+    auto scale_bytes = [&](int wf, int boxes) { return 16 * wf * ((boxes * 8 + 127) / 128 * 128 + 8); };        // eight rows lie in all banks
     // The busiest SM's boxes of codes, and what a block costs beside them (its activations, sums and barriers: as much as 16 boxes).
     long long best = -1;
     for (int splits = 1; splits <= 8; splits *= 2) {
@@ -434,8 +430,9 @@ TNX_EXPORT int tnx_gemv_mxfp4(const void* a, int a_kind, const void* a_scales, l
             if (g_forced_wf && wf != g_forced_wf) continue;
             int wk = MAX_WARPS / wf;
             if (wk > sps) wk = sps;
-            while (wk > 1 && wk * (wf * AHEAD * SLOT_BYTES + AHEAD * (box_x + box_s)) > SMEM_MOST - 1024) --wk;
-            if (wk * (wf * AHEAD * SLOT_BYTES + AHEAD * (box_x + box_s)) > SMEM_MOST - 1024) continue;      // a turn's activations at least
+            auto least = [&]() { return wk * (wf * AHEAD * SLOT_BYTES + box_x + box_s) + scale_bytes(wf, wk) + 1024; };
+            while (wk > 1 && least() > SMEM_MOST) --wk;
+            if (least() > SMEM_MOST) continue;
             const long long blocks = (long long)((groups + wf - 1) / wf) * splits;
             const long long rounds = (blocks + n_sms - 1) / n_sms;
             const long long cost = rounds * ((long long)wf * wk * ((sps + wk - 1) / wk) + 16 + (splits > 1 ? 8 : 0));
@@ -444,12 +441,16 @@ TNX_EXPORT int tnx_gemv_mxfp4(const void* a, int a_kind, const void* a_scales, l
     }
     if (best < 0) return TNX_ERR_UNSUPPORTED;
     const int ring = p.wf * p.wk * AHEAD * SLOT_BYTES;
-    const int per = (p.slots_per_split + p.wk - 1) / p.wk, most = (SMEM_MOST - 1024 - ring) / (p.wk * (box_x + box_s));
-    // all of a share, or whole turns of the ring
-    p.phase = per <= most ? per : most / AHEAD * AHEAD;
+    const int per = (p.slots_per_split + p.wk - 1) / p.wk;
+    p.phase = per;
+    while (p.phase > 1 && ring + p.phase * p.wk * (box_x + box_s) + scale_bytes(p.wf, p.phase * p.wk) + 1024 > SMEM_MOST) --p.phase;
+    p.phase = (per + (per + p.phase - 1) / p.phase - 1) / ((per + p.phase - 1) / p.phase);           // as many phases, equal ones
     p.x_at = ring;
     p.sx_at = ring + p.phase * p.wk * box_x;
-    const int sums = p.wk * M * (p.wf * 16 + 4) * 4, used = p.sx_at + p.phase * p.wk * box_s;
+    const int sums = p.wk * M * (p.wf * 16 + 4) * 4, sx_end = p.sx_at + p.phase * p.wk * box_s;
+    p.sw_at = sx_end;
+    p.sw_ld = scale_bytes(1, p.phase * p.wk) / 16;
+    const int used = sx_end + scale_bytes(p.wf, p.phase * p.wk);
     const int smem = (used > sums ? used : sums) + 1024;
     if (terms == 3) return launch_terms<3, true>(codes, p, smem, stream);
 #ifdef TNX_F16
