@@ -399,32 +399,82 @@ gemm16_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__
 
 // ---- 4-bit activations -------------------------------------------------------------------------------
 constexpr int STAGES4 = 5;
-constexpr int THREADS4 = 640;                // warps 0: TMA, 1: MMAs, 4..11: epilogue, 12..19: scales
+constexpr int THREADS4 = 384;                // warps 0: TMA, 1: MMAs, 4..11: epilogue
 constexpr int X4_BYTES = MAX_BN * CODE_K / 2, STAGE4_BYTES = CODE_BYTES + X4_BYTES;
-constexpr int SMEM4 = STAGES4 * STAGE4_BYTES + 1024;
-constexpr int SF_COLS = 24;                  // a stage's scales: 2 x 4 columns for W, 2 x 8 for up to 256 tokens
-constexpr int SF_LD = SF_COLS + 4;           // a lane's scales in shared memory: 16-byte loads of eight lanes lie in all banks
+constexpr int SF_ATOM = 512;                 // scales of 128 rows and 128 columns of K: [32 lanes][rows l, 32 + l, 64 + l, 96 + l][4 blocks]
+constexpr int SFW_BYTES = 2 * SF_ATOM, SFX_BYTES = 4 * SF_ATOM;        // a stage's for W and for up to 256 tokens
+constexpr int SMEM4 = STAGES4 * (STAGE4_BYTES + SFW_BYTES + SFX_BYTES) + 1024;
+constexpr int SF_COLS = 24;                  // tensor memory of a stage's scales: 2 x 4 columns for W, 2 x 8 for up to 256 tokens
 
-__device__ __forceinline__ void group_sync(int group) {
-    if (group) asm volatile("bar.sync 2, 128;" ::: "memory");
-    else asm volatile("bar.sync 1, 128;" ::: "memory");
+// The scales as the MMAs read them, from rows of bytes to atoms: W's for every tile and stage (1 KB), then the activations' (1 or 2 KB).  Gathered
+// row by row by the product's own warps, eight bytes of 320 rows a stage, they were what the product waited for (2,048 tokens by
+// 16,384 x 4,096: 103 us, 70 without them); here they are moved once, a warp's lanes side by side.
+__global__ void __launch_bounds__(256) scales_kernel(const Params p, uint8_t* __restrict__ sfw, uint8_t* __restrict__ sfx, int tiles_w, int groups) {
+    pdl_launch_dependents();
+    pdl_wait();
+    const int pairs = (p.num + 1) / 2;                    // a thread takes two stages: 16 scales of four rows
+    const int units = (tiles_w + p.tiles_t * groups) * pairs;
+    const int lane = threadIdx.x & 31;
+    for (int u = blockIdx.x * 8 + (threadIdx.x >> 5); u < units; u += gridDim.x * 8) {
+        const int unit = u / pairs, pair = u - unit * pairs;
+        const bool of_w = unit < tiles_w;
+        const int tt = (unit - tiles_w) / groups, group = (unit - tiles_w) - tt * groups;
+        const uint8_t* base = of_w ? p.scales : p.a_scales;
+        const uint8_t* end = base + (long long)(of_w ? p.w_rows : p.e.M) * p.blocks;
+        const int b = pair * 16, n = p.blocks - b;
+        uint32_t v[4][4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const int r = q * 32 + lane;
+            const int row = of_w ? tile_row(p, unit, r) : min(tt * p.bn + group * 128 + r, p.e.M - 1);
+            const uint8_t* src = base + (long long)row * p.blocks + b;
+            if (n >= 16 && ((uintptr_t)src & 15) == 0) {
+                const uint4 w = __ldg((const uint4*)src);
+                v[q][0] = w.x; v[q][1] = w.y; v[q][2] = w.z; v[q][3] = w.w;
+            } else {
+                const uint2 lo = load8(src, base, end, n), hi = load8(src + 8, base, end, n - 8);
+                v[q][0] = lo.x; v[q][1] = lo.y; v[q][2] = hi.x; v[q][3] = hi.y;
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {                     // atoms of the two stages
+            const int stage = pair * 2 + (j >> 1);
+            if (stage >= p.num) break;
+            uint8_t* at = of_w ? sfw + ((long long)unit * p.num + stage) * SFW_BYTES + (j & 1) * SF_ATOM
+                               : sfx + (((long long)tt * p.num + stage) * 2 + (j & 1)) * groups * SF_ATOM + group * SF_ATOM;
+            *(uint4*)(at + lane * 16) = make_uint4(v[0][j], v[1][j], v[2][j], v[3][j]);
+        }
+    }
+}
+
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                 ::"r"(smem_u32(dst)), "l"(src), "r"(bytes), "r"(smem_u32(bar)) : "memory");
+}
+// An atom of scales from shared memory (32 rows of 16 bytes, groups of eight rows 128 bytes apart) to four columns of all four quarters.
+__device__ __forceinline__ void copy_atom(uint32_t taddr, uint64_t desc) {
+    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+}
+__device__ __forceinline__ uint64_t atom_desc(uint32_t saddr) {
+    return (uint64_t)((saddr & 0x3FFFF) >> 4) | (uint64_t)1 << 16 | (uint64_t)(128 >> 4) << 32 | (uint64_t)1 << 46;
 }
 
 __global__ void __launch_bounds__(THREADS4, 1)
-gemm4_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const Params p) {
+gemm4_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const Params p, const uint8_t* __restrict__ sfw,
+             const uint8_t* __restrict__ sfx, int groups) {
     static_assert(2 * MAX_BN + STAGES4 * SF_COLS <= 512, "tensor memory");
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+    uint8_t* sSF = smem + STAGES4 * STAGE4_BYTES;         // [STAGES4][W's two atoms, the activations' two times `groups`]
     __shared__ uint64_t full[STAGES4], empty[STAGES4];
     __shared__ Rings d;
     __shared__ uint32_t tmem_base_smem;
-    __shared__ __align__(16) uint32_t sf_smem[2][2][32 * SF_LD];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int num = p.num;
 
     pdl_launch_dependents();
     if (threadIdx.x == 0) {
-        for (int i = 0; i < STAGES4; ++i) { mbar_init(&full[i], 5); mbar_init(&empty[i], 1); }         // full: codes and four warps' scales
+        for (int i = 0; i < STAGES4; ++i) { mbar_init(&full[i], 1); mbar_init(&empty[i], 1); }
         for (int i = 0; i < 2; ++i) { mbar_init(&d.full[i], 1); mbar_init(&d.empty[i], 8); }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("prefetch.tensormap [%0];" ::"l"((unsigned long long)&map_w) : "memory");
@@ -443,24 +493,31 @@ gemm4_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ 
         if (lane == 0) {
             Ring<STAGES4> r;
             int n = 0;
-            for (int tile = blockIdx.x; tile < p.tiles && ok; tile += gridDim.x)
+            const uint32_t x_scales = (uint32_t)(2 * groups * SF_ATOM);
+            for (int tile = blockIdx.x; tile < p.tiles && ok; tile += gridDim.x) {
+                const int tw = tile / p.tiles_t, tt = tile - tw * p.tiles_t;
                 for (int i = 0; i < num; ++i, ++n) {
                     if (n >= STAGES4) { ok = mbar_wait(&empty[r.slot], r.pass ^ 1u, p.err, 111); if (!ok) break; }
                     uint8_t* at = smem + r.slot * STAGE4_BYTES;
-                    mbar_expect_tx(&full[r.slot], (uint32_t)(CODE_BYTES + p.bn * (CODE_K / 2)));
-                    load_codes(p, at, &map_w, &full[r.slot], i * (CODE_K / 2), tile / p.tiles_t);
-                    tma_load_2d(at + CODE_BYTES, &map_x, &full[r.slot], i * (CODE_K / 2), tile % p.tiles_t * p.bn);
+                    uint8_t* sf = sSF + r.slot * (SFW_BYTES + SFX_BYTES);
+                    mbar_expect_tx(&full[r.slot], (uint32_t)(CODE_BYTES + p.bn * (CODE_K / 2) + SFW_BYTES) + x_scales);
+                    load_codes(p, at, &map_w, &full[r.slot], i * (CODE_K / 2), tw);
+                    tma_load_2d(at + CODE_BYTES, &map_x, &full[r.slot], i * (CODE_K / 2), tt * p.bn);
+                    bulk_load(sf, sfw + ((long long)tw * num + i) * SFW_BYTES, SFW_BYTES, &full[r.slot]);
+                    bulk_load(sf + SFW_BYTES, sfx + ((long long)tt * num + i) * x_scales, x_scales, &full[r.slot]);
                     r.next();
                 }
+            }
         }
         __syncwarp();
     } else if (warp == 1) {
+        // Two stages a turn, as above.  Copies of scales and MMAs are carried out in the order in which they are issued.
         const uint32_t idesc0 = idesc4(p.bn, 0), idesc2 = idesc4(p.bn, 2);
-        const uint64_t desc0 = smem_desc_sw128(smem_u32(smem));
+        const uint64_t desc0 = smem_desc_sw128(smem_u32(smem)), sfdesc0 = atom_desc(smem_u32(sSF));
         const int total = (p.tiles - (int)blockIdx.x + (int)gridDim.x - 1) / (int)gridDim.x * num;
         int i = 0, it = 0;
         Ring<STAGES4> r;
-        for (int n = 0; n < total && ok; n += 2) {        // two stages a turn, as above
+        for (int n = 0; n < total && ok; n += 2) {
             Ring<STAGES4> q = r;
             q.next();
             const bool both = n + 1 < total;
@@ -475,8 +532,15 @@ gemm4_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ 
                 }
                 tc_fence_after();
                 const uint64_t adesc = desc0 + (uint64_t)(r.slot * (STAGE4_BYTES >> 4)), bdesc = adesc + (uint64_t)(CODE_BYTES >> 4);
+                const uint64_t sfdesc = sfdesc0 + (uint64_t)(r.slot * ((SFW_BYTES + SFX_BYTES) >> 4));
                 const uint32_t sf = tmem_sf + (uint32_t)(r.slot * SF_COLS), acc = tmem_d + (it & 1 ? MAX_BN : 0);
                 if (elected()) {
+#pragma unroll
+                    for (int k = 0; k < 2; ++k) {         // 128 columns of K
+                        copy_atom(sf + 4u * k, sfdesc + (uint64_t)(k * (SF_ATOM >> 4)));
+                        copy_atom(sf + 8u + 8u * k, sfdesc + (uint64_t)((SFW_BYTES + k * groups * SF_ATOM) >> 4));
+                        if (groups == 2) copy_atom(sf + 12u + 8u * k, sfdesc + (uint64_t)((SFW_BYTES + (2 * k + 1) * SF_ATOM) >> 4));
+                    }
 #pragma unroll
                     for (int k = 0; k < 4; ++k)           // 64 columns of K = 32 bytes = 2 units of the address field
                         umma_mxf4(acc, adesc + (uint64_t)(2 * k), bdesc + (uint64_t)(2 * k), k & 1 ? idesc2 : idesc0, sf + 4u * (k >> 1),
@@ -487,91 +551,6 @@ gemm4_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ 
                 __syncwarp();
                 r.next();
                 if (++i == num) { i = 0; ++it; }
-            }
-        }
-    } else if (warp >= 12) {
-        // Scales: two groups of four warps take stages in turn; a thread loads a row of W's and up to two of the activations', eight scales each,
-        // three turns ahead (a trip to memory takes longer than a stage); they meet in shared memory, whence every warp takes all of them
-        // to the lanes of its quarter.
-        const int quad = warp & 3, group = (warp - 12) >> 2, r = quad * 32 + lane;
-        const bool words = p.blocks % 8 == 0 && (((uintptr_t)p.scales | (uintptr_t)p.a_scales) & 7) == 0;        // eight scales are one aligned load
-        const bool second = r + 128 < p.bn, first = r < p.bn;
-        const uint8_t* w_end = p.scales + (long long)p.w_rows * p.blocks;
-        const uint8_t* x_end = p.a_scales + (long long)p.e.M * p.blocks;
-        struct Scales { uint2 w, x[2]; };
-        int ptile = blockIdx.x, pi = group;
-        const uint8_t *ws = nullptr, *xs0 = nullptr, *xs1 = nullptr;
-        auto aim = [&]() {                                // over the tiles' ends
-            while (pi >= num) { pi -= num; ptile += gridDim.x; }
-            if (ptile >= p.tiles) return;
-            const int token = ptile % p.tiles_t * p.bn + r;
-            ws = p.scales + (long long)tile_row(p, ptile / p.tiles_t, r) * p.blocks + pi * 8;
-            xs0 = p.a_scales + (long long)min(token, p.e.M - 1) * p.blocks + pi * 8;
-            xs1 = p.a_scales + (long long)min(token + 128, p.e.M - 1) * p.blocks + pi * 8;
-        };
-        auto load = [&]() {
-            Scales q;
-            q.w = q.x[0] = q.x[1] = make_uint2(0u, 0u);
-            if (ptile >= p.tiles) return q;
-            if (words) {
-                q.w = __ldg((const uint2*)ws);
-                if (first) q.x[0] = __ldg((const uint2*)xs0);
-                if (second) q.x[1] = __ldg((const uint2*)xs1);
-            } else {
-                const int n = p.blocks - pi * 8;
-                q.w = load8(ws, p.scales, w_end, n);
-                if (first) q.x[0] = load8(xs0, p.a_scales, x_end, n);
-                if (second) q.x[1] = load8(xs1, p.a_scales, x_end, n);
-            }
-            pi += 2; ws += 16; xs0 += 16; xs1 += 16;
-            if (pi >= num) aim();
-            return q;
-        };
-        aim();
-        Scales ahead[3] = {load(), load(), load()};
-        const int total = (p.tiles - (int)blockIdx.x + (int)gridDim.x - 1) / (int)gridDim.x * num;
-        int turn = 0, s = group;
-        uint32_t pass = 1u;                               // of the stage's last use, from its second use on
-        for (int i0 = group; i0 < total; i0 += 6) {       // whole even if a wait ran out: the groups' warps meet at their barrier
-#pragma unroll
-            for (int u = 0; u < 3; ++u) {                 // (unrolled so that a register waits for its load where it is used)
-                const int i = i0 + 2 * u;
-                if (i >= total) break;
-                const Scales now = ahead[u];
-                ahead[u] = load();
-                uint32_t* buf = &sf_smem[group][turn][0]; // two in turn: one barrier a stage
-                turn ^= 1;
-                uint32_t* mine = buf + lane * SF_LD + quad;
-                mine[0] = now.w.x; mine[4] = now.w.y;
-                mine[8] = now.x[0].x; mine[16] = now.x[0].y;
-                mine[12] = now.x[1].x; mine[20] = now.x[1].y;
-                group_sync(group);
-                uint32_t v[SF_COLS];
-#pragma unroll
-                for (int c = 0; c < SF_COLS; c += 4) {
-                    const uint4 q = *(const uint4*)(buf + lane * SF_LD + c);
-                    v[c] = q.x; v[c + 1] = q.y; v[c + 2] = q.z; v[c + 3] = q.w;
-                }
-                if (ok && i >= STAGES4) {
-                    ok = __all_sync(0xffffffffu, mbar_wait(&empty[s], pass, p.err, 115));
-                    tc_fence_after();
-                }
-                if (ok) {
-                    const uint32_t at = tmem_sf + (uint32_t)(s * SF_COLS) + ((uint32_t)(quad * 32) << 16);
-#pragma unroll
-                    for (int c = 0; c < SF_COLS; c += 8) {
-                        uint32_t q[8];
-#pragma unroll
-                        for (int j = 0; j < 8; ++j) q[j] = v[c + j];
-                        tmem_st8(at + (uint32_t)c, q);
-                    }
-                    tmem_st_wait();
-                    tc_fence_before();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(&full[s]);
-                }
-                s += 2;
-                if (s >= STAGES4) { s -= STAGES4; pass ^= 1u; }
             }
         }
     } else if (warp >= 4) {
@@ -596,13 +575,6 @@ void plan(Params& p, int n_sms, int tiles_w, int extra) {
     }
 }
 
-template <typename Kernel>
-int launch(Kernel kernel, TnxSmemLimit& limit, int threads, int smem, const CUtensorMap& mw, const CUtensorMap& mx, const Params& p, int n_sms, cudaStream_t stream) {
-    const int r = limit.allow(kernel, smem);
-    if (r) return r;
-    return tnx_launch_ex(1, kernel, dim3(p.tiles < n_sms ? p.tiles : n_sms), dim3(threads), smem, stream, mw, mx, p);
-}
-
 }  // namespace
 
 // For sweeps: the tokens of a tile (a multiple of 16 from 64 to 192) whatever the sizes (0: the plan's own).
@@ -623,23 +595,48 @@ TNX_EXPORT int tnx_gemm_mxfp4_tiles_16(const void* a, long long lda, const void*
     CUtensorMap mw, mx;
     if (!map_bytes(&mw, codes, p.w_rows, p.blocks * 16, gated ? 16 : TILE_W) || !map_h16(&mx, a, M, K, lda, p.bn)) return TNX_ERR_UNSUPPORTED;
     static TnxSmemLimit limit;
-    return launch(gemm16_kernel, limit, THREADS16, SMEM16, mw, mx, p, n_sms, stream);
+    const int r = limit.allow(gemm16_kernel, SMEM16);
+    if (r) return r;
+    return tnx_launch_ex(1, gemm16_kernel, dim3(p.tiles < n_sms ? p.tiles : n_sms), dim3(THREADS16), SMEM16, stream, mw, mx, p);
 }
 
-// 4-bit activations: codes [M][blocks * 16] (16-byte aligned) and scales [M][blocks].
+// 4-bit activations: codes [M][blocks * 16] (16-byte aligned) and scales [M][blocks]; scratch: 16-byte aligned, for every 256 columns of K 1,024 bytes
+// for 128 rows of W and 2,048 for 64 tokens.
 TNX_EXPORT int tnx_gemm_mxfp4_tiles_4(const void* a, const void* a_scales, const void* codes, const void* scales, const float* bias, const float* residual,
-                                      void* out, int out_h16, long long ldc, int M, int N, int K, int act, int gated, int n_sms, int* err, cudaStream_t stream) {
+                                      void* out, int out_h16, long long ldc, int M, int N, int K, int act, int gated, void* scratch, int n_sms, int* err,
+                                      cudaStream_t stream) {
     if (M <= 0 || N <= 0) return 0;
-    if (K <= 0 || act < 0 || act >= TNX_ACT_COUNT || n_sms <= 0) return TNX_ERR_BAD_ARG;
+    if (K <= 0 || act < 0 || act >= TNX_ACT_COUNT || n_sms <= 0 || ((uintptr_t)scratch & 15)) return TNX_ERR_BAD_ARG;
     const int tiles_w = gated ? (N + 63) / 64 : (N + TILE_W - 1) / TILE_W;
     if (((uintptr_t)a & 15) || ((uintptr_t)codes & 15) || (long long)tiles_w * ((M + 63) / 64) > 0x3FFFFFFF) return TNX_ERR_UNSUPPORTED;
     Params p;
     fill_epilogue(p.e, bias, residual, out, out_h16, ldc, M, N, act, gated);
     p.scales = (const uint8_t*)scales; p.a_scales = (const uint8_t*)a_scales; p.err = err;
     p.w_rows = gated ? 2 * N : N; p.blocks = (K + MX_BLOCK - 1) / MX_BLOCK; p.num = (K + CODE_K - 1) / CODE_K;
-    plan(p, n_sms, tiles_w, 400);
+    plan(p, n_sms, tiles_w, 100);
     CUtensorMap mw, mx;
     if (!map_bytes(&mw, codes, p.w_rows, p.blocks * 16, gated ? 16 : TILE_W) || !map_bytes(&mx, a, M, p.blocks * 16, p.bn)) return TNX_ERR_UNSUPPORTED;
     static TnxSmemLimit limit;
-    return launch(gemm4_kernel, limit, THREADS4, SMEM4, mw, mx, p, n_sms, stream);
+    int r = limit.allow(gemm4_kernel, SMEM4);
+    if (r) return r;
+    const int groups = p.bn > 128 ? 2 : 1;
+    uint8_t* sfw = (uint8_t*)scratch;
+    uint8_t* sfx = sfw + (long long)tiles_w * p.num * SFW_BYTES;
+    const long long units = (long long)(tiles_w + p.tiles_t * groups) * ((p.num + 1) / 2), blocks = (units + 7) / 8, most = (long long)n_sms * 8;
+    r = tnx_launch_ex(1, scales_kernel, dim3((unsigned)(blocks < most ? blocks : most)), dim3(256), 0, stream, p, sfw, sfx, tiles_w, groups);
+    if (r) return r;
+    return tnx_launch_ex(1, gemm4_kernel, dim3(p.tiles < n_sms ? p.tiles : n_sms), dim3(THREADS4), SMEM4, stream, mw, mx, p, (const uint8_t*)sfw,
+                         (const uint8_t*)sfx, groups);
+}
+
+// The same with the parameters in one array (the stream last): a call through ctypes costs 0.1 us a parameter.
+TNX_EXPORT int tnx_gemm_mxfp4_tiles_16_packed(const long long* v) {
+    return tnx_gemm_mxfp4_tiles_16((const void*)v[0], (long long)v[1], (const void*)v[2], (const void*)v[3], (const float*)v[4], (const float*)v[5],
+                                   (void*)v[6], (int)v[7], (long long)v[8], (int)v[9], (int)v[10], (int)v[11], (int)v[12], (int)v[13], (int)v[14],
+                                   (int*)v[15], (cudaStream_t)v[16]);
+}
+TNX_EXPORT int tnx_gemm_mxfp4_tiles_4_packed(const long long* v) {
+    return tnx_gemm_mxfp4_tiles_4((const void*)v[0], (const void*)v[1], (const void*)v[2], (const void*)v[3], (const float*)v[4], (const float*)v[5],
+                                  (void*)v[6], (int)v[7], (long long)v[8], (int)v[9], (int)v[10], (int)v[11], (int)v[12], (int)v[13], (void*)v[14],
+                                  (int)v[15], (int*)v[16], (cudaStream_t)v[17]);
 }

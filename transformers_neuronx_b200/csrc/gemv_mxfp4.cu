@@ -54,6 +54,17 @@ __device__ __forceinline__ void codes_to_f16(uint32_t w, uint32_t (&o)[4]) {
         "cvt.rn.f16x2.e2m1x2 %3, b3;\n\t}"
         : "=r"(o[0]), "=r"(o[1]), "=r"(o[2]), "=r"(o[3]) : "r"(w));
 }
+// Shared memory by its own addresses: a pointer made from a rounded-up address is a generic one to the compiler, and 64-bit arithmetic on those and
+// generic loads were a third of the main loop's instructions.
+__device__ __forceinline__ uint32_t lds32(uint32_t a) { uint32_t v; asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(a)); return v; }
+__device__ __forceinline__ uint32_t lds16(uint32_t a) { uint16_t v; asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(a)); return v; }
+__device__ __forceinline__ uint4 lds128(uint32_t a) {
+    uint4 v;
+    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a));
+    return v;
+}
+__device__ __forceinline__ float2 lds_f2(uint32_t a) { float2 v; asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(a)); return v; }
+
 __device__ __forceinline__ uint32_t pack_f16(float a, float b) {
     const __half2 r = __floats2half2_rn(a, b);
     return *(const uint32_t*)&r;
@@ -249,26 +260,27 @@ __global__ void __launch_bounds__(32 * (MAX_WARPS + 1), 1) gemv_kernel(const __g
             }
             asm volatile("bar.sync 1, %0;" ::"r"(32 * warps) : "memory");
             const int last = min(e, b + f0 + len);
-            const uint4* xb = xs + wk * p.phase * BOX_X + lane;
-            const float* sxb = sx + wk * p.phase * (NT * 8) + 2 * t;
-            const uint8_t* swa = sw + (wf * 8 + g) * p.sw_ld + wk * p.phase * 8 + 2 * t;
+            uint32_t xb = smem_u32(xs) + (uint32_t)(wk * p.phase * BOX_X + lane) * 16u;
+            uint32_t sxb = smem_u32(sx) + (uint32_t)(wk * p.phase * (NT * 8) + 2 * t) * 4u;
+            uint32_t swa = smem_u32(sw) + (uint32_t)((wf * 8 + g) * p.sw_ld + wk * p.phase * 8 + 2 * t);
+            const uint32_t sw_half = (uint32_t)(8 * p.wf * p.sw_ld), x_term = (uint32_t)term_step * 16u;
+            const uint32_t ring = smem_u32(smem) + (uint32_t)(wk * AHEAD * box_bytes + (wf * 8 + g) * 128 + t * 4), half = (uint32_t)box_bytes / 2;
 #pragma unroll 1
-            for (int s = b + f0; s < last; ++s, xb += BOX_X, sxb += NT * 8, swa += 8) {
+            for (int s = b + f0; s < last; ++s, xb += BOX_X * 16, sxb += NT * 8 * 4, swa += 8) {
                 // lane t: the scales of blocks 2t, 2t + 1 of its first row, then of its second
-                const uint32_t two = *(const uint16_t*)swa | (uint32_t)*(const uint16_t*)(swa + 8 * p.wf * p.sw_ld) << 16;
+                const uint32_t two = lds16(swa) | lds16(swa + sw_half) << 16;
                 float fs[4];
 #pragma unroll
                 for (int j = 0; j < 4; ++j) fs[j] = scale_at(two, j);
                 if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&full[wk][place], pass, p.err, 81));
                 if (!ok) break;
-                const uint8_t* row = smem + (wk * AHEAD + place) * box_bytes + (wf * 8 + g) * 128 + t * 4;
-                const uint8_t* row_b = row + box_bytes / 2;
+                const uint32_t row = ring + (uint32_t)(place * box_bytes);
                 uint32_t wa[SLOT_BLOCKS], wb[SLOT_BLOCKS];
 #pragma unroll
                 for (int i = 0; i < SLOT_BLOCKS; ++i) {
-                    const int at = (i ^ g) << 4;
-                    wa[i] = *(const uint32_t*)(row + at);
-                    wb[i] = *(const uint32_t*)(row_b + at);
+                    const uint32_t at = row + (uint32_t)((i ^ g) << 4);
+                    wa[i] = lds32(at);
+                    wb[i] = lds32(at + half);
                 }
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&empty[wk][place]);       // the box has been read
@@ -286,7 +298,7 @@ __global__ void __launch_bounds__(32 * (MAX_WARPS + 1), 1) gemv_kernel(const __g
                         float c[4];
 #pragma unroll
                         for (int k = 0; k < TERMS; ++k) {
-                            const uint4 x = xb[k * term_step + i * BLOCK_X + n * 32];
+                            const uint4 x = lds128(xb + k * x_term + (uint32_t)(i * BLOCK_X + n * 32) * 16u);
                             if (k == 0) mma_first(c, A[0], B[0], A[1], B[1], x.x, x.y);
                             else mma(c, A[0], B[0], A[1], B[1], x.x, x.y);
                             mma(c, A[2], B[2], A[3], B[3], x.z, x.w);
@@ -302,7 +314,7 @@ __global__ void __launch_bounds__(32 * (MAX_WARPS + 1), 1) gemv_kernel(const __g
                 if (SCALED) {
 #pragma unroll
                     for (int n = 0; n < NT; ++n) {
-                        const float2 f = *(const float2*)&sxb[n * 8];
+                        const float2 f = lds_f2(sxb + (uint32_t)n * 32u);
                         acc[n][0] = fmaf(sum[n][0], f.x, acc[n][0]); acc[n][1] = fmaf(sum[n][1], f.y, acc[n][1]);
                         acc[n][2] = fmaf(sum[n][2], f.x, acc[n][2]); acc[n][3] = fmaf(sum[n][3], f.y, acc[n][3]);
                     }
@@ -434,7 +446,9 @@ TNX_EXPORT int tnx_gemv_mxfp4(const void* a, int a_kind, const void* a_scales, l
             while (wk > 1 && least() > SMEM_MOST) --wk;
             if (least() > SMEM_MOST) continue;
             const long long blocks = (long long)((groups + wf - 1) / wf) * splits;
-            const long long rounds = (blocks + n_sms - 1) / n_sms;
+            // clusters of four find places on nine SMs in ten at a time, of eight on seven
+            const int places = splits <= 2 ? n_sms : splits == 4 ? n_sms * 9 / 10 : n_sms * 7 / 10;
+            const long long rounds = (blocks + places - 1) / places;
             const long long cost = rounds * ((long long)wf * wk * ((sps + wk - 1) / wk) + 16 + (splits > 1 ? 8 : 0));
             if (best < 0 || cost < best) { best = cost; p.splits = splits; p.wf = wf; p.wk = wk; p.slots_per_split = sps; }
         }
@@ -457,4 +471,11 @@ TNX_EXPORT int tnx_gemv_mxfp4(const void* a, int a_kind, const void* a_scales, l
     if (a_kind == 0) return launch_terms<1, false>(codes, p, smem, stream);
 #endif
     return launch_terms<1, true>(codes, p, smem, stream);
+}
+
+// The same with the parameters in one array (the stream last): a call through ctypes costs 0.1 us a parameter.
+TNX_EXPORT int tnx_gemv_mxfp4_packed(const long long* v) {
+    return tnx_gemv_mxfp4((const void*)v[0], (int)v[1], (const void*)v[2], (long long)v[3], (const void*)v[4], (const void*)v[5], (const float*)v[6],
+                          (const float*)v[7], (void*)v[8], (int)v[9], (long long)v[10], (int)v[11], (int)v[12], (int)v[13], (int)v[14], (int)v[15],
+                          (int)v[16], (int*)v[17], (cudaStream_t)v[18]);
 }

@@ -220,3 +220,16 @@ TNX_EXPORT int tnx_mxfp4_gemm_simt(const void* a, int a_kind, const void* a_scal
     }
     return 0;
 }
+
+// The same with the parameters in one array (the stream last): a call through ctypes costs 0.1 us a parameter.
+TNX_EXPORT int tnx_mxfp4_quantize_packed(const long long* v) {
+    return tnx_mxfp4_quantize((const void*)v[0], (int)v[1], (long long)v[2], (void*)v[3], (void*)v[4], (int)v[5], (int)v[6], (int)v[7], (cudaStream_t)v[8]);
+}
+TNX_EXPORT int tnx_mxfp4_dequantize_packed(const long long* v) {
+    return tnx_mxfp4_dequantize((const void*)v[0], (const void*)v[1], (void*)v[2], (int)v[3], (long long)v[4], (int)v[5], (int)v[6], (int)v[7], (cudaStream_t)v[8]);
+}
+TNX_EXPORT int tnx_mxfp4_gemm_simt_packed(const long long* v) {
+    return tnx_mxfp4_gemm_simt((const void*)v[0], (int)v[1], (const void*)v[2], (long long)v[3], (const void*)v[4], (const void*)v[5],
+                               (const float*)v[6], (const float*)v[7], (void*)v[8], (int)v[9], (long long)v[10], (int)v[11], (int)v[12], (int)v[13],
+                               (int)v[14], (int)v[15], (cudaStream_t)v[16]);
+}

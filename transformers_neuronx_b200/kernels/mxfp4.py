@@ -15,14 +15,15 @@ keeps 8-bit matrices beside scales per column (src/transformers_neuronx/quantize
 """
 from __future__ import annotations
 
-from ctypes import c_int, c_longlong, c_void_p
+from ctypes import c_char_p
+from struct import Struct
 from typing import Optional
 
 import torch
 
 from . import build as _build
 from . import ops as _ops
-from .ops import KernelError, _FLOATS, _H16, _check, _sm_count, _state, activation_code
+from .ops import ACTIVATIONS, KernelError, _FLOATS, _H16, _check, _state, activation_code
 
 BLOCK = 32                                    # values that share a scale
 TILE_TOKENS = 128                             # beyond these persistent blocks walk over tiles of up to 192 tokens (gemm_mxfp4_tiles.cu)
@@ -34,66 +35,101 @@ class Mxfp4Matrix:
     blocks = ceil(columns / 32).  Both contiguous and on one device; codes behind the last column are zeros (0 times whatever stands there
     is what the products add).  The tensors are used as they are, not copied."""
 
-    __slots__ = ("codes", "scales", "columns")
+    __slots__ = ("_codes", "_scales", "_buffer", "_device", "_blocks", "rows", "columns")
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor, columns: Optional[int] = None):
         for t, name in ((codes, "codes"), (scales, "scales")):
             if not isinstance(t, torch.Tensor) or t.dtype != torch.uint8 or t.dim() != 2 or not t.is_contiguous():
                 raise KernelError(f"{name} must be a contiguous 2-D uint8 tensor")
         rows, blocks = scales.shape
-        if codes.shape[0] != rows or codes.shape[1] != blocks * 16 or codes.device != scales.device:
+        if codes.shape != (rows, blocks * 16) or codes.device != scales.device:
             raise KernelError(f"codes {tuple(codes.shape)} and scales {tuple(scales.shape)} do not fit: 16 bytes of codes a scale, one device")
         columns = blocks * BLOCK if columns is None else int(columns)
         if blocks < 1 or not (blocks - 1) * BLOCK < columns <= blocks * BLOCK:
             raise KernelError(f"{columns} columns do not make {blocks} blocks of {BLOCK}")
-        self.codes, self.scales, self.columns = codes, scales, columns
+        self._codes, self._scales, self._buffer = codes, scales, None
+        self._device, self._blocks, self.rows, self.columns = codes.get_device(), blocks, rows, columns
+
+    @classmethod
+    def _empty(cls, rows: int, columns: int, device: torch.device, number: int) -> "Mxfp4Matrix":
+        """Codes and scales behind them in one allocation; the two tensors are made when they are asked for."""
+        self = object.__new__(cls)
+        blocks = (columns + BLOCK - 1) // BLOCK
+        self._codes = self._scales = None
+        self._buffer = torch.empty_strided((rows * blocks * 17,), (1,), dtype=torch.uint8, device=device)
+        self._device, self._blocks, self.rows, self.columns = number, blocks, rows, columns
+        return self
+
+    def _split(self) -> None:
+        n = self.rows * self._blocks * 16
+        self._codes = self._buffer[:n].view(self.rows, self._blocks * 16)
+        self._scales = self._buffer[n:].view(self.rows, self._blocks)
+
+    @property
+    def codes(self) -> torch.Tensor:
+        if self._codes is None:
+            self._split()
+        return self._codes
+
+    @property
+    def scales(self) -> torch.Tensor:
+        if self._scales is None:
+            self._split()
+        return self._scales
+
+    def _pointers(self):
+        if self._buffer is not None:
+            p = self._buffer.data_ptr()
+            return p, p + self.rows * self._blocks * 16
+        return self._codes.data_ptr(), self._scales.data_ptr()
 
     @property
     def shape(self):
-        return torch.Size((self.codes.shape[0], self.columns))
+        return torch.Size((self.rows, self.columns))
 
     @property
     def device(self):
-        return self.codes.device
+        return (self._buffer if self._buffer is not None else self._codes).device
 
     def numel(self) -> int:
-        return self.codes.shape[0] * self.columns
+        return self.rows * self.columns
 
     def nbytes(self) -> int:
-        return self.codes.numel() + self.scales.numel()
+        return self.rows * self._blocks * 17
 
     def __repr__(self) -> str:
-        return f"Mxfp4Matrix({self.codes.shape[0]} x {self.columns}, {self.device})"
+        return f"Mxfp4Matrix({self.rows} x {self.columns}, {self.device})"
 
 
-# The entry points' parameters: p a pointer, l a 64-bit number, i an int; every one ends with the stream.
-_SIGNATURES = {
-    ("mxfp4", "tnx_mxfp4_quantize"): "pilppiii", ("mxfp4", "tnx_mxfp4_dequantize"): "pppiliii",
-    ("mxfp4", "tnx_mxfp4_gemm_simt"): "piplpppppiliiiii",
-    ("gemv_mxfp4", "tnx_gemv_mxfp4"): "piplpppppiliiiiiip",
-    ("gemm_mxfp4", "tnx_gemm_mxfp4_16"): "plpppppiliiiiiip", ("gemm_mxfp4", "tnx_gemm_mxfp4_4"): "pppppppiliiiiiip",
-    ("gemm_mxfp4_tiles", "tnx_gemm_mxfp4_tiles_16"): "plpppppiliiiiiip", ("gemm_mxfp4_tiles", "tnx_gemm_mxfp4_tiles_4"): "pppppppiliiiiiip",
-}
-_TYPES = {"p": c_void_p, "l": c_longlong, "i": c_int}
+# Entry points take their parameters in one array, the stream last: a parameter of a ctypes call costs 0.1 us.
+_PACK = {n: Struct(f"{n}q").pack for n in range(1, 24)}
 _entries = {}
 
 
 def _entry(library: str, name: str, dtype):
-    """The entry point in the flavour of `dtype`'s 16-bit type, its parameter types set once: building a ctypes object for every argument of
-    every call costs more than a launch."""
+    """The entry point in the flavour of `dtype`'s 16-bit type."""
     fn = _entries.get((name, dtype))
     if fn is None:
-        lib = _build.load(library, dtype if dtype in _H16 else None)
-        fn = getattr(lib, name)
-        if not fn.argtypes:
-            fn.argtypes = [_TYPES[c] for c in _SIGNATURES[(library, name)]] + [c_void_p]
+        fn = getattr(_build.load(library, dtype if dtype in _H16 else None), name + "_packed")
+        fn.argtypes = [c_char_p]
         _entries[(name, dtype)] = fn
     return fn
 
 
-def _stream(device: int):
+_devices = {}                                 # number -> (SMs, address of the error word)
+
+
+def _device_info(number: int, device: torch.device):
+    have = _devices.get(number)
+    if have is None:
+        st = _state(device)
+        have = _devices[number] = (st["sms"], st["err"].data_ptr())
+    return have
+
+
+def _stream(device: int) -> int:
     scoped = _ops._scoped_stream
-    return scoped if scoped is not None else torch._C._cuda_getCurrentRawStream(device)
+    return (scoped.value or 0) if scoped is not None else torch._C._cuda_getCurrentRawStream(device)
 
 
 def _device_of(t: torch.Tensor, name: str) -> int:
@@ -101,6 +137,15 @@ def _device_of(t: torch.Tensor, name: str) -> int:
     if not isinstance(t, torch.Tensor) or not t.is_cuda:
         raise KernelError(f"{name} must be a CUDA tensor: the engine has no CPU path")
     d = t.get_device()
+    if d != torch._C._cuda_getDevice():
+        raise KernelError(f"{name} is on cuda:{d}, the current device is cuda:{torch._C._cuda_getDevice()}")
+    return d
+
+
+def _matrix_device(m: Mxfp4Matrix, name: str) -> int:
+    d = m._device
+    if d < 0:
+        raise KernelError(f"{name} must be on a CUDA device: the engine has no CPU path")
     if d != torch._C._cuda_getDevice():
         raise KernelError(f"{name} is on cuda:{d}, the current device is cuda:{torch._C._cuda_getDevice()}")
     return d
@@ -128,20 +173,17 @@ def quantize_mxfp4(x: torch.Tensor, out: Optional[Mxfp4Matrix] = None) -> Mxfp4M
     if columns < 1:
         raise KernelError("x has no columns")
     if out is None:
-        blocks = (columns + BLOCK - 1) // BLOCK
-        out = object.__new__(Mxfp4Matrix)
-        out.codes = torch.empty((rows, blocks * 16), dtype=torch.uint8, device=x.device)
-        out.scales = torch.empty((rows, blocks), dtype=torch.uint8, device=x.device)
-        out.columns = columns
-    else:
-        if not isinstance(out, Mxfp4Matrix) or out.shape != x.shape or out.codes.get_device() != device:
-            raise KernelError(f"out must be an Mxfp4Matrix of {rows} x {columns} on the device of x")
-        if out.codes.data_ptr() % 4:
-            raise KernelError("out's codes must be 4-byte aligned")
+        out = Mxfp4Matrix._empty(rows, columns, x.device, device)
+    elif not isinstance(out, Mxfp4Matrix) or (out.rows, out.columns, out._device) != (rows, columns, device):
+        raise KernelError(f"out must be an Mxfp4Matrix of {rows} x {columns} on the device of x")
+    codes, scales = out._pointers()
+    if codes % 4:
+        raise KernelError("out's codes must be 4-byte aligned")
     if rows:
-        _check(_entry("mxfp4", "tnx_mxfp4_quantize", x.dtype)(
-            x.data_ptr(), 0 if x.dtype == torch.float32 else 1, pitch, out.codes.data_ptr(), out.scales.data_ptr(), rows, columns,
-            _sm_count(x.device), _stream(device)), "quantize_mxfp4")
+        dtype = x.dtype
+        _check(_entry("mxfp4", "tnx_mxfp4_quantize", dtype)(_PACK[9](
+            x.data_ptr(), 0 if dtype is torch.float32 else 1, pitch, codes, scales, rows, columns, _device_info(device, x.device)[0], _stream(device))),
+            "quantize_mxfp4")
     return out
 
 
@@ -149,22 +191,24 @@ def dequantize_mxfp4(m: Mxfp4Matrix, dtype=torch.bfloat16, out: Optional[torch.T
     """The values of m: exact in float32 and bfloat16; float16 rounds what lies outside its range (infinity, subnormal numbers)."""
     if not isinstance(m, Mxfp4Matrix):
         raise KernelError("m must be an Mxfp4Matrix")
-    device = _device_of(m.codes, "the matrix")
-    if m.codes.data_ptr() % 4:
+    device = _matrix_device(m, "m")
+    codes, scales = m._pointers()
+    if codes % 4:
         raise KernelError("the codes must be 4-byte aligned")
-    rows, columns = m.shape
+    rows, columns = m.rows, m.columns
     if out is None:
         if dtype not in _FLOATS:
             raise KernelError(f"dtype {dtype}: expected one of {_FLOATS}")
-        out, pitch = torch.empty((rows, columns), dtype=dtype, device=m.device), columns
+        out, pitch = torch.empty_strided((rows, columns), (columns, 1), dtype=dtype, device=m.device), columns
     else:
         have, width, pitch = _floats(out, "out", device)
         if have != rows or width != columns:
             raise KernelError(f"out is {tuple(out.shape)}, the matrix {rows} x {columns}")
+        dtype = out.dtype
     if rows:
-        _check(_entry("mxfp4", "tnx_mxfp4_dequantize", out.dtype)(
-            m.codes.data_ptr(), m.scales.data_ptr(), out.data_ptr(), 0 if out.dtype == torch.float32 else 1, pitch, rows, columns,
-            _sm_count(m.device), _stream(device)), "dequantize_mxfp4")
+        _check(_entry("mxfp4", "tnx_mxfp4_dequantize", dtype)(_PACK[9](
+            codes, scales, out.data_ptr(), 0 if dtype is torch.float32 else 1, pitch, rows, columns, _device_info(device, out.device)[0], _stream(device))),
+            "dequantize_mxfp4")
     return out
 
 
@@ -182,62 +226,69 @@ def gated_gemm_mxfp4(a, w: Mxfp4Matrix, out: torch.Tensor, bias=None, activation
 
 
 def _product(a, w, out, bias, residual, activation, gated):
-    act = activation_code(activation)
+    act = ACTIVATIONS.get(activation)
+    if act is None:
+        act = activation_code(activation)                     # raises
     if not isinstance(w, Mxfp4Matrix):
         raise KernelError("w must be an Mxfp4Matrix")
-    codes = w.codes
-    device = _device_of(codes, "w")
-    rows, Kw = codes.shape[0], w.columns
+    device = _matrix_device(w, "w")
+    rows = w.rows
     quantized = isinstance(a, Mxfp4Matrix)
     if quantized:
-        if a.codes.get_device() != device:
+        if a._device != device:
             raise KernelError(f"a is on {a.device}, w on {w.device}")
-        (M, K), lda, kind = a.shape, 0, out.dtype if isinstance(out, torch.Tensor) else None
+        M, K, lda, kind, a_kind = a.rows, a.columns, 0, None, 2
+        a_p, as_p = a._pointers()
     else:
         M, K, lda = _floats(a, "a", device)
         kind = a.dtype
-    Mo, No, ldc = _floats(out, "out", device)
+        a_kind = 1 if kind is torch.float32 else 0
+        a_p, as_p = a.data_ptr(), 0
+    Mo, N, ldc = _floats(out, "out", device)
     if gated and rows % 2:
         raise KernelError(f"a gated product needs as many gate rows as up rows, got {rows} in all")
-    N = rows // 2 if gated else rows
-    if Kw != K or Mo != M or No != N:
-        raise KernelError(f"shapes do not fit: a {(M, K)}, w {(rows, Kw)}{' (gated)' if gated else ''}, out {tuple(out.shape)}")
-    out_h16 = 0 if out.dtype == torch.float32 else 1
-    if out_h16 and kind != out.dtype:
-        if kind != torch.float32:
-            raise KernelError(f"a is {kind}, out {out.dtype}: 16-bit activations and results must agree")
-        kind = out.dtype
+    if w.columns != K or Mo != M or (2 * N if gated else N) != rows:
+        raise KernelError(f"shapes do not fit: a {(M, K)}, w {(rows, w.columns)}{' (gated)' if gated else ''}, out {tuple(out.shape)}")
+    out_kind = out.dtype
+    out_h16 = 0 if out_kind is torch.float32 else 1
+    if out_h16:
+        if a_kind == 0 and kind is not out_kind:
+            raise KernelError(f"a is {kind}, out {out_kind}: 16-bit activations and results must agree")
+        kind = out_kind
     bias_p = res_p = 0
     if bias is not None:
-        if not isinstance(bias, torch.Tensor) or bias.dtype != torch.float32 or bias.dim() != 1 or bias.get_device() != device or not bias.is_contiguous():
+        if not isinstance(bias, torch.Tensor) or bias.dtype is not torch.float32 or bias.dim() != 1 or bias.get_device() != device or not bias.is_contiguous():
             raise KernelError("bias must be a contiguous 1-D float32 tensor on the device of w")
         if bias.shape[0] != rows:
             raise KernelError("bias length differs from the matrix's rows")
         bias_p = bias.data_ptr()
     if residual is not None:
-        if _floats(residual, "residual", device) != (M, N, ldc) or residual.dtype != torch.float32 or out_h16:
+        if _floats(residual, "residual", device) != (M, N, ldc) or residual.dtype is not torch.float32 or out_h16:
             raise KernelError("residual must be float32 with the shape and row stride of a float32 out")
         res_p = residual.data_ptr()
     if M == 0 or N == 0:
         return out
-    a_p, w_p, out_p = (a.codes if quantized else a).data_ptr(), codes.data_ptr(), out.data_ptr()
-    if M <= FEW_TOKENS and w_p % 16 == 0 and (not quantized or a_p % 4 == 0):
-        st = _state(w.device)
-        code = _entry("gemv_mxfp4", "tnx_gemv_mxfp4", kind)(a_p, 2 if quantized else 1 if a.dtype == torch.float32 else 0,
-                                                           a.scales.data_ptr() if quantized else 0, lda, w_p, w.scales.data_ptr(), bias_p, res_p, out_p,
-                                                           out_h16, ldc, M, N, K, act, 1 if gated else 0, st["sms"], st["err"].data_ptr(), _stream(device))
-    elif (a_p | w_p) % 16 == 0 and (quantized or (a.dtype != torch.float32 and lda % 8 == 0)):
-        st = _state(w.device)
-        library = "gemm_mxfp4_tiles" if M > TILE_TOKENS else "gemm_mxfp4"
-        if quantized:
-            code = _entry(library, f"tnx_{library}_4", kind)(a_p, a.scales.data_ptr(), w_p, w.scales.data_ptr(), bias_p, res_p, out_p, out_h16, ldc, M, N, K,
-                                                             act, 1 if gated else 0, st["sms"], st["err"].data_ptr(), _stream(device))
+    w_p, s_p = w._pointers()
+    sms, err = _device_info(device, out.device)
+    kernels = 1
+    tail = (w_p, s_p, bias_p, res_p, out.data_ptr(), out_h16, ldc, M, N, K, act, 1 if gated else 0)
+    if M <= FEW_TOKENS and w_p % 16 == 0 and (a_kind != 2 or a_p % 4 == 0):
+        code = _entry("gemv_mxfp4", "tnx_gemv_mxfp4", kind)(_PACK[19](a_p, a_kind, as_p, lda, *tail, sms, err, _stream(device)))
+    elif (a_p | w_p) % 16 == 0 and (a_kind == 2 or (a_kind == 0 and lda % 8 == 0)):
+        if M > TILE_TOKENS and quantized:
+            # scales as the tensor cores read them: 1,024 bytes for 128 rows of W, 2,048 for 64 tokens, for every 256 columns
+            nbytes = ((rows + 127) // 128 * 1024 + (M + 63) // 64 * 2048) * ((K + 255) // 256)
+            scratch = torch.empty_strided((nbytes,), (1,), dtype=torch.uint8, device=out.device)
+            code = _entry("gemm_mxfp4_tiles", "tnx_gemm_mxfp4_tiles_4", kind)(
+                _PACK[18](a_p, as_p, *tail, scratch.data_ptr(), sms, err, _stream(device)))
+            kernels = 2
+        elif M > TILE_TOKENS:
+            code = _entry("gemm_mxfp4_tiles", "tnx_gemm_mxfp4_tiles_16", kind)(_PACK[17](a_p, lda, *tail, sms, err, _stream(device)))
+        elif quantized:
+            code = _entry("gemm_mxfp4", "tnx_gemm_mxfp4_4", kind)(_PACK[17](a_p, as_p, *tail, sms, err, _stream(device)))
         else:
-            code = _entry(library, f"tnx_{library}_16", kind)(a_p, lda, w_p, w.scales.data_ptr(), bias_p, res_p, out_p, out_h16, ldc, M, N, K,
-                                                              act, 1 if gated else 0, st["sms"], st["err"].data_ptr(), _stream(device))
+            code = _entry("gemm_mxfp4", "tnx_gemm_mxfp4_16", kind)(_PACK[17](a_p, lda, *tail, sms, err, _stream(device)))
     else:
-        code = _entry("mxfp4", "tnx_mxfp4_gemm_simt", kind)(a_p, 2 if quantized else 1 if a.dtype == torch.float32 else 0,
-                                                           a.scales.data_ptr() if quantized else 0, lda, w_p, w.scales.data_ptr(), bias_p, res_p, out_p,
-                                                           out_h16, ldc, M, N, K, act, 1 if gated else 0, _stream(device))
-    _check(code, "gemm_mxfp4")
+        code = _entry("mxfp4", "tnx_mxfp4_gemm_simt", kind)(_PACK[17](a_p, a_kind, as_p, lda, *tail, _stream(device)))
+    _check(code, "gemm_mxfp4", kernels)
     return out
