@@ -4,7 +4,7 @@
 // while one is written out by four warps of their own, the MMAs fill the other.  (A CTA a tile, whose sums went through shared memory,
 // spent 11 us a tile outside of its main loop: 2,048 tokens by 16,384 x 4,096 229 us with 16-bit activations, 153 with 4-bit ones.)
 // Sums go straight from tensor memory to memory: a warp's lanes are 32 neighbouring features, so that a token's store is 64 or 128 bytes.
-// Gated tiles hold 16 gate rows and their 16 up rows for each of the four warps: gate and up values meet by one exchange of lanes 16 apart.
+// Gated tiles alternate eight gate rows and their eight up rows: gate and up values meet by one exchange of lanes eight apart.
 //
 // gemm16 (16-bit activations): codes come through TMA, 256 columns of K a box; sixteen warps turn them into 16-bit values in tensor memory, 64 columns a
 // group of four warps; the MMAs take them from there as their A operand, activations from shared memory.
@@ -23,6 +23,7 @@ struct Params {
     int w_rows, blocks;
     int num;                                 // stages of K a tile
     int tiles_t, tiles, bn;                  // tiles of tokens, tiles in all, tokens of a tile (a multiple of 16)
+    int one_box;                             // gated: a tile's gate and up rows are one box of a map of four dimensions
     int* err;
 };
 
@@ -30,20 +31,23 @@ struct Params {
 __device__ __forceinline__ int tile_row(const Params& p, int tw, int r) {
     int row;
     if (!p.e.gated) row = tw * TILE_W + r;
-    else row = tw * 64 + (r >> 5) * 16 + (r & 15) + ((r & 16) ? p.e.N : 0);
+    else row = tw * 64 + (r >> 4) * 8 + (r & 7) + ((r & 8) ? p.e.N : 0);
     return row < p.w_rows ? row : p.w_rows - 1;
+}
+__device__ __forceinline__ void tma_load_4d(void* dst, const CUtensorMap* map, uint64_t* bar, int x, int y, int z, int w) {
+    asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];"
+                 ::"r"(smem_u32(dst)), "l"((unsigned long long)map), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
 }
 // A box of 256 columns of tile tw's codes from column x (bytes) on.
 __device__ __forceinline__ void load_codes(const Params& p, uint8_t* at, const CUtensorMap* map, uint64_t* bar, int x, int tw) {
-    if (!p.e.gated) {
-        tma_load_2d(at, map, bar, x, tw * TILE_W);
-    } else {
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            tma_load_2d(at + q * 4096, map, bar, x, tw * 64 + q * 16);
-            tma_load_2d(at + q * 4096 + 2048, map, bar, x, p.e.N + tw * 64 + q * 16);
+    if (!p.e.gated) tma_load_2d(at, map, bar, x, tw * TILE_W);
+    else if (p.one_box) tma_load_4d(at, map, bar, x, 0, 0, tw * 8);
+    else
+#pragma unroll 1
+        for (int q = 0; q < 8; ++q) {
+            tma_load_2d(at + q * 2048, map, bar, x, tw * 64 + q * 8);
+            tma_load_2d(at + q * 2048 + 1024, map, bar, x, p.e.N + tw * 64 + q * 8);
         }
-    }
 }
 
 // Sixteen columns (tokens from `token` on) of this lane's row.
@@ -79,13 +83,13 @@ template <int ACT>
 __device__ __forceinline__ void write16(const Epilogue& e, const float (&v)[16], int n, int token, float bias, float bias_up) {
     const int lane = threadIdx.x & 31;
     if (e.gated) {
-        const bool low = lane < 16;
+        const bool low = !(lane & 8);
         const long long step = 2 * e.ldc * (e.out_h16 ? 2 : 4);
         const int tokens = n < e.N ? e.M - token - (low ? 0 : 1) : 0;
         char* at = (char*)e.out + ((long long)(token + (low ? 0 : 1)) * e.ldc + n) * (e.out_h16 ? 2 : 4);
 #pragma unroll
         for (int j = 0; j < 16; j += 2, at += step) {
-            const float other = __shfl_xor_sync(0xffffffffu, low ? v[j + 1] : v[j], 16);
+            const float other = __shfl_xor_sync(0xffffffffu, low ? v[j + 1] : v[j], 8);
             const float gate = (low ? v[j] : other) + bias, up = (low ? other : v[j + 1]) + bias_up;
             const float r = act_of<ACT>(gate, e.act) * up;
             if (j < tokens) put(at, r, e.out_h16);
@@ -118,7 +122,7 @@ __device__ __forceinline__ bool epilogue(const Params& p, Rings& d, uint32_t tme
     int it = 0;
     for (int tile = blockIdx.x; tile < p.tiles && ok; tile += gridDim.x, ++it) {
         const int tt = tile % p.tiles_t, tw = tile / p.tiles_t, buf = it & 1;
-        const int n = p.e.gated ? tw * 64 + quad * 16 + (lane & 15) : tw * TILE_W + r;
+        const int n = p.e.gated ? tw * 64 + quad * 16 + (lane >> 4) * 8 + (lane & 7) : tw * TILE_W + r;
         float bias = 0.f, bias_up = 0.f;
         if (p.e.bias && n < p.e.N) {
             bias = __ldg(p.e.bias + n);
@@ -399,7 +403,7 @@ gemm16_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__
 
 // ---- 4-bit activations -------------------------------------------------------------------------------
 constexpr int STAGES4 = 5;
-constexpr int THREADS4 = 384;                // warps 0: TMA, 1: MMAs, 4..11: epilogue
+constexpr int THREADS4 = 384;                // warps 0, 2: TMA, 1: MMAs, 4..11: epilogue
 constexpr int X4_BYTES = MAX_BN * CODE_K / 2, STAGE4_BYTES = CODE_BYTES + X4_BYTES;
 constexpr int SF_ATOM = 512;                 // scales of 128 rows and 128 columns of K: [32 lanes][rows l, 32 + l, 64 + l, 96 + l][4 blocks]
 constexpr int SFW_BYTES = 2 * SF_ATOM, SFX_BYTES = 4 * SF_ATOM;        // a stage's for W and for up to 256 tokens
@@ -474,7 +478,7 @@ gemm4_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ 
 
     pdl_launch_dependents();
     if (threadIdx.x == 0) {
-        for (int i = 0; i < STAGES4; ++i) { mbar_init(&full[i], 1); mbar_init(&empty[i], 1); }
+        for (int i = 0; i < STAGES4; ++i) { mbar_init(&full[i], 2); mbar_init(&empty[i], 1); }
         for (int i = 0; i < 2; ++i) { mbar_init(&d.full[i], 1); mbar_init(&d.empty[i], 8); }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("prefetch.tensormap [%0];" ::"l"((unsigned long long)&map_w) : "memory");
@@ -489,7 +493,8 @@ gemm4_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ 
     bool ok = tmem_base_smem == 0u;                       // never anything else
     if (!ok) {
         if (threadIdx.x == 0) atomicExch(p.err, 90);
-    } else if (warp == 0) {
+    } else if (warp == 0 || warp == 2) {
+        // W's share of a stage and the activations', a thread each: a copy costs its thread about 100 cycles.
         if (lane == 0) {
             Ring<STAGES4> r;
             int n = 0;
@@ -500,11 +505,15 @@ gemm4_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ 
                     if (n >= STAGES4) { ok = mbar_wait(&empty[r.slot], r.pass ^ 1u, p.err, 111); if (!ok) break; }
                     uint8_t* at = smem + r.slot * STAGE4_BYTES;
                     uint8_t* sf = sSF + r.slot * (SFW_BYTES + SFX_BYTES);
-                    mbar_expect_tx(&full[r.slot], (uint32_t)(CODE_BYTES + p.bn * (CODE_K / 2) + SFW_BYTES) + x_scales);
-                    load_codes(p, at, &map_w, &full[r.slot], i * (CODE_K / 2), tw);
-                    tma_load_2d(at + CODE_BYTES, &map_x, &full[r.slot], i * (CODE_K / 2), tt * p.bn);
-                    bulk_load(sf, sfw + ((long long)tw * num + i) * SFW_BYTES, SFW_BYTES, &full[r.slot]);
-                    bulk_load(sf + SFW_BYTES, sfx + ((long long)tt * num + i) * x_scales, x_scales, &full[r.slot]);
+                    if (warp == 0) {
+                        mbar_expect_tx(&full[r.slot], (uint32_t)(CODE_BYTES + SFW_BYTES));
+                        load_codes(p, at, &map_w, &full[r.slot], i * (CODE_K / 2), tw);
+                        bulk_load(sf, sfw + ((long long)tw * num + i) * SFW_BYTES, SFW_BYTES, &full[r.slot]);
+                    } else {
+                        mbar_expect_tx(&full[r.slot], (uint32_t)(p.bn * (CODE_K / 2)) + x_scales);
+                        tma_load_2d(at + CODE_BYTES, &map_x, &full[r.slot], i * (CODE_K / 2), tt * p.bn);
+                        bulk_load(sf + SFW_BYTES, sfx + ((long long)tt * num + i) * x_scales, x_scales, &full[r.slot]);
+                    }
                     r.next();
                 }
             }
@@ -562,6 +571,28 @@ gemm4_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ 
 // ---- host -----------------------------------------------------------------------------------------
 int g_forced_bn = 0;
 
+// W's codes: rows in boxes of a tile's; gated, as [features / 8][gate, up][8 rows], so that a box is the tile's eight times eight gate rows and their up
+// rows in turn (a box for every eight rows cost a thread more than the stage's MMAs took).  Features beside a multiple of eight: eight rows a box.
+bool map_w(CUtensorMap* out, const void* codes, Params& p) {
+    const int bytes = p.blocks * 16;
+    p.one_box = 0;
+    if (!p.e.gated) return map_bytes(out, codes, p.w_rows, bytes, TILE_W);
+    if (p.e.N % 8 == 0) {
+        EncodeTiledFn fn = encode_fn();
+        if (!fn) return false;
+        cuuint64_t dims[4] = {(cuuint64_t)bytes, 8u, 2u, (cuuint64_t)p.e.N / 8};
+        cuuint64_t strides[3] = {(cuuint64_t)bytes, (cuuint64_t)bytes * p.e.N, (cuuint64_t)bytes * 8};
+        cuuint32_t box[4] = {128u, 8u, 2u, 8u};
+        cuuint32_t estr[4] = {1, 1, 1, 1};
+        if (fn(out, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, const_cast<void*>(codes), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS) {
+            p.one_box = 1;
+            return true;
+        }
+    }
+    return map_bytes(out, codes, p.w_rows, bytes, 8);
+}
+
 // Tokens of a tile: the busiest CTA's rounds of tiles, each as long as its columns and what a stage costs whatever its columns are, `extra` of them.
 void plan(Params& p, int n_sms, int tiles_w, int extra) {
     long long best = -1;
@@ -593,7 +624,7 @@ TNX_EXPORT int tnx_gemm_mxfp4_tiles_16(const void* a, long long lda, const void*
     p.w_rows = gated ? 2 * N : N; p.blocks = (K + MX_BLOCK - 1) / MX_BLOCK; p.num = (K + KB - 1) / KB;
     plan(p, n_sms, tiles_w, 400);
     CUtensorMap mw, mx;
-    if (!map_bytes(&mw, codes, p.w_rows, p.blocks * 16, gated ? 16 : TILE_W) || !map_h16(&mx, a, M, K, lda, p.bn)) return TNX_ERR_UNSUPPORTED;
+    if (!map_w(&mw, codes, p) || !map_h16(&mx, a, M, K, lda, p.bn)) return TNX_ERR_UNSUPPORTED;
     static TnxSmemLimit limit;
     const int r = limit.allow(gemm16_kernel, SMEM16);
     if (r) return r;
@@ -613,9 +644,9 @@ TNX_EXPORT int tnx_gemm_mxfp4_tiles_4(const void* a, const void* a_scales, const
     fill_epilogue(p.e, bias, residual, out, out_h16, ldc, M, N, act, gated);
     p.scales = (const uint8_t*)scales; p.a_scales = (const uint8_t*)a_scales; p.err = err;
     p.w_rows = gated ? 2 * N : N; p.blocks = (K + MX_BLOCK - 1) / MX_BLOCK; p.num = (K + CODE_K - 1) / CODE_K;
-    plan(p, n_sms, tiles_w, 100);
+    plan(p, n_sms, tiles_w, 200);
     CUtensorMap mw, mx;
-    if (!map_bytes(&mw, codes, p.w_rows, p.blocks * 16, gated ? 16 : TILE_W) || !map_bytes(&mx, a, M, p.blocks * 16, p.bn)) return TNX_ERR_UNSUPPORTED;
+    if (!map_w(&mw, codes, p) || !map_bytes(&mx, a, M, p.blocks * 16, p.bn)) return TNX_ERR_UNSUPPORTED;
     static TnxSmemLimit limit;
     int r = limit.allow(gemm4_kernel, SMEM4);
     if (r) return r;

@@ -432,28 +432,38 @@ TNX_EXPORT int tnx_gemv_mxfp4(const void* a, int a_kind, const void* a_scales, l
     const int nt = M <= 8 ? 1 : M <= 16 ? 2 : 4;
     const int box_x = SLOT_K * 2 * nt * 8 * terms, box_s = nt * 8 * 4;      // shared memory of a box's activations, for one share of K
     auto scale_bytes = [&](int wf, int boxes) { return 16 * wf * ((boxes * 8 + 127) / 128 * 128 + 8); };        // eight rows lie in all banks
-    // The busiest SM's boxes of codes, and what a block costs beside them (its activations, sums and barriers: as much as 16 boxes).
-    long long best = -1;
-    for (int splits = 1; splits <= 8; splits *= 2) {
-        if (g_forced_splits && splits != g_forced_splits) continue;
-        const int sps = (p.slots + splits - 1) / splits;
-        if (splits > 1 && sps * (splits - 1) >= p.slots) continue;                 // no block without work
-        for (int wf = 1; wf <= MAX_WARPS; ++wf) {
-            if (g_forced_wf && wf != g_forced_wf) continue;
-            int wk = MAX_WARPS / wf;
-            if (wk > sps) wk = sps;
-            auto least = [&]() { return wk * (wf * AHEAD * SLOT_BYTES + box_x + box_s) + scale_bytes(wf, wk) + 1024; };
-            while (wk > 1 && least() > SMEM_MOST) --wk;
-            if (least() > SMEM_MOST) continue;
-            const long long blocks = (long long)((groups + wf - 1) / wf) * splits;
-            // clusters of four find places on nine SMs in ten at a time, of eight on seven
-            const int places = splits <= 2 ? n_sms : splits == 4 ? n_sms * 9 / 10 : n_sms * 7 / 10;
-            const long long rounds = (blocks + places - 1) / places;
-            const long long cost = rounds * ((long long)wf * wk * ((sps + wk - 1) / wk) + 16 + (splits > 1 ? 8 : 0));
-            if (best < 0 || cost < best) { best = cost; p.splits = splits; p.wf = wf; p.wk = wk; p.slots_per_split = sps; }
+    // The last plans by their sizes: working one out takes longer than a launch.
+    struct Plan { int M, N, slots, gated, terms, sms, wf, wk, splits, sps; };
+    static thread_local Plan known[64];
+    Plan& k = known[((unsigned)M * 31u + (unsigned)N * 7u + (unsigned)p.slots * 13u + (unsigned)gated * 3u + (unsigned)terms) % 64u];
+    const bool forced = g_forced_wf || g_forced_splits;
+    if (!forced && k.M == M && k.N == N && k.slots == p.slots && k.gated == gated && k.terms == terms && k.sms == n_sms) {
+        p.wf = k.wf; p.wk = k.wk; p.splits = k.splits; p.slots_per_split = k.sps;
+    } else {
+        // The busiest SM's boxes of codes, and what a block costs beside them (its activations, sums and barriers: as much as 16 boxes).
+        long long best = -1;
+        for (int splits = 1; splits <= 8; splits *= 2) {
+            if (g_forced_splits && splits != g_forced_splits) continue;
+            const int sps = (p.slots + splits - 1) / splits;
+            if (splits > 1 && sps * (splits - 1) >= p.slots) continue;                 // no block without work
+            for (int wf = 1; wf <= MAX_WARPS; ++wf) {
+                if (g_forced_wf && wf != g_forced_wf) continue;
+                int wk = MAX_WARPS / wf;
+                if (wk > sps) wk = sps;
+                auto least = [&]() { return wk * (wf * AHEAD * SLOT_BYTES + box_x + box_s) + scale_bytes(wf, wk) + 1024; };
+                while (wk > 1 && least() > SMEM_MOST) --wk;
+                if (least() > SMEM_MOST) continue;
+                const long long blocks = (long long)((groups + wf - 1) / wf) * splits;
+                // clusters of four find places on nine SMs in ten at a time, of eight on seven
+                const int places = splits <= 2 ? n_sms : splits == 4 ? n_sms * 9 / 10 : n_sms * 7 / 10;
+                const long long rounds = (blocks + places - 1) / places;
+                const long long cost = rounds * ((long long)wf * wk * ((sps + wk - 1) / wk) + 16 + (splits > 1 ? 8 : 0));
+                if (best < 0 || cost < best) { best = cost; p.splits = splits; p.wf = wf; p.wk = wk; p.slots_per_split = sps; }
+            }
         }
+        if (best < 0) return TNX_ERR_UNSUPPORTED;
+        if (!forced) k = {M, N, p.slots, gated, terms, n_sms, p.wf, p.wk, p.splits, p.slots_per_split};
     }
-    if (best < 0) return TNX_ERR_UNSUPPORTED;
     const int ring = p.wf * p.wk * AHEAD * SLOT_BYTES;
     const int per = (p.slots_per_split + p.wk - 1) / p.wk;
     p.phase = per;
