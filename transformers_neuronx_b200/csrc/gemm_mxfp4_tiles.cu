@@ -286,20 +286,44 @@ gemm16_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__
             const int buf = it & 1, tw = tile / p.tiles_t;
             if (it >= 2) ok = __all_sync(0xffffffffu, mbar_wait(&ref_empty[buf], (uint32_t)((it >> 1) - 1) & 1u, p.err, 97));
             if (!ok) break;
-            for (int row = lane >> 2; row < TILE_W; row += 8) {
-                const uint8_t* q = p.scales + (long long)tile_row(p, tw, row) * p.blocks;
-                uint32_t m = 0u;
-                auto take = [&](uint32_t w) {                         // four bytes; 255 (NaN) is no size
+            auto largest = [](uint32_t m, uint32_t w) {               // of four bytes; 255 (NaN) is no size
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) { const uint32_t E = (w >> (8 * k)) & 255u; m = max(m, E == 255u ? 0u : E); }
-                };
-                if (wide)
-                    for (int j = (lane & 3) * 16; j < p.blocks; j += 64) { const uint4 v = __ldg((const uint4*)(q + j)); take(v.x); take(v.y); take(v.z); take(v.w); }
-                else
-                    for (int j = lane & 3; j < p.blocks; j += 4) take((uint32_t)__ldg(q + j));
-                m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
-                m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
-                if ((lane & 3) == 0) row_ref[buf][row] = (int)m;
+                for (int k = 0; k < 4; ++k) { const uint32_t E = (w >> (8 * k)) & 255u; m = max(m, E == 255u ? 0u : E); }
+                return m;
+            };
+            // eight rows of four lanes at a time and eight of those in flight: the first tile waits for this
+#pragma unroll 1
+            for (int half = 0; half < 2; ++half) {
+                const uint8_t* q[8];
+                uint32_t m[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    q[e] = p.scales + (long long)tile_row(p, tw, half * 64 + e * 8 + (lane >> 2)) * p.blocks;
+                    m[e] = 0u;
+                }
+                if (wide) {
+                    for (int j = (lane & 3) * 16; j < p.blocks; j += 64) {
+                        uint4 v[8];
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) v[e] = __ldg((const uint4*)(q[e] + j));
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) m[e] = largest(largest(largest(largest(m[e], v[e].x), v[e].y), v[e].z), v[e].w);
+                    }
+                } else {
+                    for (int j = lane & 3; j < p.blocks; j += 4) {
+                        uint32_t v[8];
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) v[e] = __ldg(q[e] + j);
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) m[e] = max(m[e], v[e] == 255u ? 0u : v[e]);
+                    }
+                }
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    m[e] = max(m[e], __shfl_xor_sync(0xffffffffu, m[e], 1));
+                    m[e] = max(m[e], __shfl_xor_sync(0xffffffffu, m[e], 2));
+                    if ((lane & 3) == 0) row_ref[buf][half * 64 + e * 8 + (lane >> 2)] = (int)m[e];
+                }
             }
             __syncwarp();
             if (lane == 0) mbar_arrive(&ref_full[buf]);
