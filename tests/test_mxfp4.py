@@ -46,3 +46,29 @@ def test_plain_rounding():
     assert torch.equal(plain.unpack(plain.pack(code)), code)
     tiny = torch.full((1, 32), 2.0 ** -140)
     assert plain.quantize(tiny)[1].tolist() == [[0]] and float(plain.rounded(tiny).abs().max()) == 0.0
+
+
+def test_quantization_config():
+    from transformers_neuronx_b200 import NeuronConfig, QuantizationConfig
+    q = QuantizationConfig(no_quantize_list=["fc2"])
+    assert (q.quant_dtype, q.activation_quant_dtype, q.quantize_attn, q.no_quantize_list) == ("mxfp4", None, True, ["fc2"])
+    assert NeuronConfig(quant=q).quant is q and NeuronConfig(quant=q).ignored == {} and NeuronConfig().quant is None
+    for bad, error in ((dict(quant_dtype="s8"), NotImplementedError), (dict(activation_quant_dtype="s8"), NotImplementedError),
+                       (dict(no_quantize_list="fc2"), TypeError)):
+        with pytest.raises(error):
+            QuantizationConfig(**bad)
+
+
+def test_quantized_models_need_16_bits():
+    from helpers import TinyModel
+    from transformers_neuronx_b200 import QuantizationConfig
+    from transformers_neuronx_b200.models import opt as opt_arch
+    from transformers_neuronx_b200.models.decoder import DecoderModel
+    tiny = TinyModel("A", seed=1)
+    model = DecoderModel(opt_arch.build_spec(tiny.cfg))
+    assert "gemv_mxfp4" not in model.libraries(torch.bfloat16)
+    model.act_dtype = torch.float32
+    with pytest.raises(ValueError):
+        model.quantize(QuantizationConfig())
+    model.quantization = QuantizationConfig()
+    assert {"mxfp4", "gemv_mxfp4", "gemm_mxfp4", "gemm_mxfp4_tiles"} <= set(model.libraries(torch.bfloat16))

@@ -4,7 +4,7 @@ sampling, and hand-written CUDA kernels.  Capabilities follow aws-neuron/transfo
 support; the design does not."""
 __version__ = "0.1.0"
 
-from .config.generation_config import (BlkSparseAttnConfig, ContinuousBatchingConfig, GenerationConfig, NeuronConfig,
+from .config.generation_config import (BlkSparseAttnConfig, ContinuousBatchingConfig, GenerationConfig, NeuronConfig, QuantizationConfig,
                                        SlidingWindowAttnConfig, SparseAttnConfig)      # as `from transformers_neuronx import ...`
 
 _LAZY = {"OPTForSampling": ".opt.model", "OPTForGreedySearch": ".opt.model", "VononexForSampling": ".vononex.model", "PifelixForSampling": ".pifelix.model",

@@ -8,5 +8,5 @@ from .taborax_config import TaboraxConfig
 from .engine_config import EngineConfig, canonical_dtype
 from .registry import (Architecture, register_architecture, resolve_architecture, architectures,
                        load_config, config_from_dict)
-from .generation_config import (BlkSparseAttnConfig, ContinuousBatchingConfig, GenerationConfig, NeuronConfig,
+from .generation_config import (BlkSparseAttnConfig, ContinuousBatchingConfig, GenerationConfig, NeuronConfig, QuantizationConfig,
                                 SlidingWindowAttnConfig, SparseAttnConfig)

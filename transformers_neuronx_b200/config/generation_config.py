@@ -177,9 +177,35 @@ class ContinuousBatchingConfig:
         return self.max_num_seqs
 
 
+class QuantizationConfig:
+    """How matrices are stored, under the reference's name (its class of that name: an 8-bit type, a method, quantize_attn, no_quantize_list).
+    This engine has one format, microscaled 4 bits (kernels/mxfp4.py); another `quant_dtype` is refused.
+
+    quant_dtype             'mxfp4'
+    activation_quant_dtype  None: 16-bit activations; 'mxfp4': they are brought into 4 bits too, ahead of every product
+    quantize_attn           whether the mixers' projections are quantized beside the feed-forwards'
+    no_quantize_list        parts of tensor names whose matrices stay as they are (one of them keeps all that are joined with it)
+    """
+
+    def __init__(self, quant_dtype: str = "mxfp4", activation_quant_dtype: Optional[str] = None, quantize_attn: bool = True,
+                 no_quantize_list: Optional[Sequence[str]] = None):
+        if quant_dtype != "mxfp4":
+            raise NotImplementedError(f"quant_dtype {quant_dtype!r} is not built: the engine's quantized matrices are 'mxfp4'")
+        if activation_quant_dtype not in (None, "mxfp4"):
+            raise NotImplementedError(f"activation_quant_dtype {activation_quant_dtype!r} is not built: None or 'mxfp4'")
+        if isinstance(no_quantize_list, str):
+            raise TypeError("no_quantize_list is a list of names")
+        self.quant_dtype, self.activation_quant_dtype = quant_dtype, activation_quant_dtype
+        self.quantize_attn = bool(quantize_attn)
+        self.no_quantize_list = [str(n) for n in (no_quantize_list or [])]
+
+    def __repr__(self) -> str:
+        return "QuantizationConfig(" + ", ".join(f"{k}={v!r}" for k, v in self.__dict__.items()) + ")"
+
+
 class NeuronConfig:
     """The reference's bag of options (config.py:160-330).  `on_device_generation`,
-    `output_all_logits`, `continuous_batching`, `cast_logits_dtype` and `sparse_attn` (sliding window) have a
+    `output_all_logits`, `continuous_batching`, `cast_logits_dtype`, `sparse_attn` (sliding window) and `quant` (a QuantizationConfig) have a
     meaning here; `on_device_embedding`, `fuse_qkv` and
     `padding_side='left'` name what this engine does anyway.  Anything else set to a value of its own is kept in
     `ignored` and reported once."""
@@ -203,6 +229,7 @@ class NeuronConfig:
         if sparse_attn is not None and not isinstance(sparse_attn, SparseAttnConfig):
             raise TypeError("sparse_attn must be a SparseAttnConfig")
         self.sparse_attn = sparse_attn                        # a causal sliding window for every attention layer
+        self.quant = options.pop("quant") if isinstance(options.get("quant"), QuantizationConfig) else None
         self.output_all_logits = bool(output_all_logits)      # forward() of a prompt returns every position's logits
         self.ignored = {k: v for k, v in options.items()
                         if k not in self._AS_BUILT and v not in (None, False)}

@@ -26,8 +26,9 @@ def require_cuda(device="cuda:0") -> torch.device:
     return dev
 
 
-def build_model(spec, tensors, dtype: str, device="cuda:0", verbose=True) -> DecoderModel:
-    """A ModelSpec and its {name: tensor} -> a DecoderModel on the device, kernels compiled."""
+def build_model(spec, tensors, dtype: str, device="cuda:0", verbose=True, quant=None) -> DecoderModel:
+    """A ModelSpec and its {name: tensor} -> a DecoderModel on the device, kernels compiled; quant (QuantizationConfig): its dense
+    projections in 4 bits."""
     dev = require_cuda(device)
     torch.cuda.set_device(dev)
     model = DecoderModel(spec)
@@ -35,6 +36,9 @@ def build_model(spec, tensors, dtype: str, device="cuda:0", verbose=True) -> Dec
     # the libraries' flavour: the engine's 16-bit type, or (32-bit engine) that of the stored matrices
     sixteen = act if act != torch.float32 else (
         torch.float16 if any(t.dtype == torch.float16 for t in tensors.values()) else torch.bfloat16)
+    if quant is not None and act == torch.float32:
+        raise ValueError("4-bit matrices need a 16-bit engine: dtype bfloat16 or float16")
+    model.quantization = quant
     kbuild.build_many(kbuild.with_flavour(model.libraries(act), sixteen), verbose=verbose)
     rounding_report()
     model.load(tensors, dev, act)
@@ -43,13 +47,19 @@ def build_model(spec, tensors, dtype: str, device="cuda:0", verbose=True) -> Dec
         warnings.warn(f"{n} tensors are stored in another 16-bit type than the engine's and were rounded to "
                       f"{canonical_dtype(dtype)} (e.g. {example}): the logits are no longer the checkpoint's own; "
                       f"run the engine in the checkpoint's type, or in float32, to avoid this")
+    if quant is not None:
+        n = model.quantize(quant)
+        if n == 0:
+            warnings.warn("quantization was asked for, but the model has no 16-bit matrix that could be brought into 4 bits")
+        elif verbose:
+            print(f"[tnx-b200] {n} matrices in 4 bits", file=sys.stderr, flush=True)
     return model
 
 
-def load_model(folder: str, dtype: str = "bfloat16", device="cuda:0", verbose=True, spec_hook=None):
+def load_model(folder: str, dtype: str = "bfloat16", device="cuda:0", verbose=True, spec_hook=None, quant=None):
     """Returns (model, typed config).  The model class is chosen by config.json.  `spec_hook`, when given,
     takes the architecture's ModelSpec and returns the one to build (a run-time option that changes a part's
-    parameters, such as a sliding window for every attention layer)."""
+    parameters, such as a sliding window for every attention layer).  quant: a QuantizationConfig, or None."""
     arch, cfg = load_config(folder)
     spec = arch.build_spec(cfg)
     if spec_hook is not None:
@@ -57,7 +67,7 @@ def load_model(folder: str, dtype: str = "bfloat16", device="cuda:0", verbose=Tr
     probe = DecoderModel(spec)                       # host-only: lists the tensors the model reads
     t0 = time.time()
     tensors = load_tensors(folder, probe.tensor_specs())
-    model = build_model(spec, tensors, dtype, device, verbose)
+    model = build_model(spec, tensors, dtype, device, verbose, quant)
     if verbose:
         print(f"[tnx-b200] {arch.name} loaded from {folder} as {canonical_dtype(dtype)} in "
               f"{time.time() - t0:.1f} s ({model.parameter_bytes() / 1e9:.2f} GB of weights)",

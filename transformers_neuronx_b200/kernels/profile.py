@@ -16,7 +16,7 @@ from collections import OrderedDict
 
 import torch
 
-from . import ops
+from . import mxfp4, ops
 
 _NAMES = ("embed", "gather_rows", "patch_tokens", "layer_norm", "pick_rows", "gemm_simt", "gemm_split", "gemm_tc", "gemv_layer_norm", "kv_append",
           "attention_simt", "attention_decode", "attention_prefill", "attention_prefill_tc", "sample", "sample_packed",
@@ -25,6 +25,7 @@ _NAMES = ("embed", "gather_rows", "patch_tokens", "layer_norm", "pick_rows", "ge
           "gemm_tc_grouped", "gemm_tc_batched", "moe_activation", "moe_combine", "latent_prep", "headwise_product", "delta_prep", "delta_scan",
           "ssd_prep", "ssd_gate_norm", "diff_qkv_prep", "diff_combine", "rms_norm_pair", "scaled_residual_add", "causal_conv",
           "selective_scan", "gated_rms_norm")
+_WHERE = [(ops, name) for name in _NAMES] + [(mxfp4, name) for name in ("quantize_mxfp4", "dequantize_mxfp4", "gemm_mxfp4", "gated_gemm_mxfp4")]
 
 
 class KernelProfile:
@@ -65,11 +66,11 @@ def kernel_profile():
                 prof.events.append((name, a, b))
         return timed
 
-    for name in _NAMES:
-        saved[name] = getattr(ops, name)
-        setattr(ops, name, wrap(name, saved[name]))
+    for module, name in _WHERE:
+        saved[(module, name)] = getattr(module, name)
+        setattr(module, name, wrap(name, saved[(module, name)]))
     try:
         yield prof
     finally:
-        for name, fn in saved.items():
-            setattr(ops, name, fn)
+        for (module, name), fn in saved.items():
+            setattr(module, name, fn)

@@ -33,6 +33,7 @@ class DecoderModel:
                 raise ValueError(f"a join of width {j.weight.out_features} in a model of width {spec.hidden_size}")
         self.device = None
         self.act_dtype = None
+        self.quantization = None              # QuantizationConfig: dense projections in 4 bits (quantize())
         self._taps: Optional[Dict[str, torch.Tensor]] = None
 
     # ---- taps -----------------------------------------------------------------------------------
@@ -78,6 +79,8 @@ class DecoderModel:
                                                  "moe_grouped")]
         else:
             libs = [l for l in libs if l != "gemm_split"]            # for 32-bit activations
+        if self.quantization is not None:
+            libs += ["mxfp4", "gemv_mxfp4", "gemm_mxfp4", "gemm_mxfp4_tiles"]
         return list(dict.fromkeys(libs))
 
     @property
@@ -110,6 +113,21 @@ class DecoderModel:
         for j in self.joins.values():
             j.load(tensors, device, act_dtype)
         self.head.load(tensors, device, act_dtype, shared={self.spec.embedding.table: self.embedding.table})
+
+    def quantize(self, config) -> int:
+        """Brings the layers' dense projections into 4 bits (config: QuantizationConfig; call it behind load()); returns how many matrices.
+        Embeddings, heads, norms, routed experts' matrices and whatever is not a 16-bit matrix of whole blocks stay as they are."""
+        if self.act_dtype not in (torch.bfloat16, torch.float16):
+            raise ValueError("4-bit matrices need a 16-bit engine (bfloat16 or float16 activations)")
+        self.quantization = config
+        count = 0
+        for b in self.blocks:
+            parts = [b.feed_forward] + ([b.mixer] if config.quantize_attn else [])
+            for p in parts:
+                for linear in (p.linears() if p is not None else ()):
+                    if not any(skip in name for skip in config.no_quantize_list for name in linear.names):
+                        count += linear.quantize(activations=config.activation_quant_dtype is not None)
+        return count
 
     def parameter_bytes(self) -> int:
         """Bytes of every weight one step reads once (a tied table counted once)."""

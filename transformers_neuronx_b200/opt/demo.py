@@ -54,6 +54,9 @@ def _parser():
     rp.add_argument("--sparse_attn", type=str, default=None, choices=[None, "blk_sparse", "custom", "window"],
                     help="'window': sliding-window attention (the other patterns are not built)")
     rp.add_argument("--window_size", type=int, default=128, help="Window size for sliding-window attention.")
+    rp.add_argument("--weight_format", default=None, choices=["mxfp4"],
+                    help="the layers' dense projections in microscaled 4 bits, quantized as the model is loaded (bf16 or f16)")
+    rp.add_argument("--activation_format", default=None, choices=["mxfp4"], help="their inputs in 4 bits too (needs --weight_format)")
     for name in ("--tp_degree", "--unroll", "--context_length_estimate", "--blk_size",
                  "--num_global_blks", "--num_local_blks", "--num_random_blks"):
         rp.add_argument(name, type=int, default=None, help=argparse.SUPPRESS)
@@ -103,13 +106,20 @@ def run(args):
     torch.manual_seed(15213)
     from ..modeling_auto import NeuronAutoModelForCausalLM      # the entry-point class is chosen by config.json
     print("running NeuronAutoModelForCausalLM.from_pretrained")
-    neuron_config = None
+    options = {}
+    if args.activation_format and not args.weight_format:
+        raise SystemExit("--activation_format needs --weight_format")
+    if args.weight_format:
+        from ..config import QuantizationConfig
+        options["quant"] = QuantizationConfig(quant_dtype=args.weight_format, activation_quant_dtype=args.activation_format)
     if args.sparse_attn:                                    # gpt_demo.py:107-123
         if args.sparse_attn != "window":
             raise NotImplementedError("Interface for other attention patterns not implemented yet!")
-        from ..config import NeuronConfig, SlidingWindowAttnConfig, SparseAttnConfig
-        neuron_config = NeuronConfig(sparse_attn=SparseAttnConfig(
-            attn_type="window", causal=True, sparse_attn_config=SlidingWindowAttnConfig(window_size=args.window_size)))
+        from ..config import SlidingWindowAttnConfig, SparseAttnConfig
+        options["sparse_attn"] = SparseAttnConfig(
+            attn_type="window", causal=True, sparse_attn_config=SlidingWindowAttnConfig(window_size=args.window_size))
+    from ..config import NeuronConfig
+    neuron_config = NeuronConfig(**options) if options else None
     model = NeuronAutoModelForCausalLM.from_pretrained(args.load, batch_size=args.batch_size, amp=args.amp,
                                            n_positions=args.n_positions, neuron_config=neuron_config)
     print("running model.to_neuron")

@@ -78,7 +78,7 @@ class OPTForSampling:
         """Weights to the GPU, kernels compiled, cache made.  Kept under the reference's name."""
         if self.engine is not None:
             return self
-        self.model, _ = load_model(self.folder, self.dtype, spec_hook=self._spec_hook())
+        self.model, _ = load_model(self.folder, self.dtype, spec_hook=self._spec_hook(), quant=self.neuron_config.quant)
         ec = EngineConfig(dtype=self.dtype, max_num_seqs=max(self.batch_size, 1), max_model_len=self.n_positions,
                           max_tokens=self.batch_size * (-(-self.n_positions // 16) * 16),
                           max_batch_tokens=max(2048, self.batch_size))
@@ -124,7 +124,9 @@ class OPTForSampling:
             libs = self.model.libraries(self.model.act_dtype)
         else:
             arch, cfg = load_config(self.folder)
-            libs = DecoderModel(arch.build_spec(cfg)).libraries(act)
+            probe = DecoderModel(arch.build_spec(cfg))
+            probe.quantization = self.neuron_config.quant
+            libs = probe.libraries(act)
         return all(os.path.isfile(kbuild.library_path(n)) for n in kbuild.with_flavour(libs, act))
 
     def profile(self, profile_dir: str, ntff_count_limit=None) -> str:

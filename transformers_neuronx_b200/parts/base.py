@@ -123,6 +123,25 @@ class Part:
     def parameter_bytes(self) -> int:
         return 0
 
+    def linears(self):
+        """The matrices this part multiplies through Linear.forward once it is loaded, its own and those of the parts it holds."""
+        from .linear import Linear
+        out = []
+
+        def look(v):
+            if isinstance(v, Linear):
+                if v.weight is not None and all(v is not o for o in out):
+                    out.append(v)
+            elif isinstance(v, Part):
+                for o in v.linears():
+                    look(o)
+            elif isinstance(v, (list, tuple)):
+                for o in v:
+                    look(o)
+        for v in vars(self).values():
+            look(v)
+        return out
+
 
 class Norm(Part):
     def forward(self, ctx, x, out_f32=None, out_act=None, rows=None):

@@ -3,7 +3,7 @@
 (hlo.py:485-501).  The activation and the residual add run in the epilogues of the two products."""
 from __future__ import annotations
 
-from ..kernels import ops
+from ..kernels import mxfp4, ops
 from ..kernels.ops import activation_code
 from .base import FeedForward
 from .linear import Linear, fuse_linears
@@ -40,7 +40,7 @@ class DenseFeedForward(FeedForward):
 
 class GatedDenseFeedForward(FeedForward):
     """down(act(gate(h)) * up(h)), all three with optional biases: gate and up are one product, the
-    activation and the multiplication one elementwise kernel in 32-bit on its output."""
+    activation and the multiplication one elementwise kernel in 32-bit on its output, or (4-bit matrices) the product's own epilogue."""
     graph_safe = True
     can_overwrite = True
     libraries = ("gemm_simt", "gemm_split", "gemm_tc", "gemv", "gated_act")
@@ -69,10 +69,13 @@ class GatedDenseFeedForward(FeedForward):
     def forward(self, ctx, h, out, accumulate=True, row_scale=None):
         """row_scale (32-bit [tokens]): a number per token that multiplies the result."""
         N, F = h.shape[0], self.spec.up.out_features
-        gu = ctx.scratch(N, 2 * F)
-        self.gate_up.forward(h, gu)
         a = ctx.scratch(N, F)
-        ops.gated_activation(gu, a, self.spec.activation, row_scale)
+        if self.gate_up.quantized and row_scale is None:
+            mxfp4.gated_gemm_mxfp4(self.gate_up.input_of(h), self.gate_up.weight, a, bias=self.gate_up.bias, activation=self.spec.activation)
+        else:
+            gu = ctx.scratch(N, 2 * F)
+            self.gate_up.forward(h, gu)
+            ops.gated_activation(gu, a, self.spec.activation, row_scale)
         self.down.forward(a, out, residual=out if accumulate else None)
 
 

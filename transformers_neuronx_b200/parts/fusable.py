@@ -32,6 +32,7 @@ def fuse_linears_along_k(parts: List[Linear], scales, device) -> Linear:
     spec = LinearSpec(sum(p.spec.in_features for p in parts), parts[0].spec.out_features, "<fused>",
                       "<fused>" if bias is not None else None)
     fused = Linear(spec)
+    fused.names = tuple(n for p in parts for n in p.names)
     fused.set_weight(weight, bias)
     return fused
 

@@ -7,6 +7,10 @@ Kernel choice: 16-bit activations with a matrix of the same 16-bit type go to th
 kernel when its size rules hold (the row length in bytes a multiple of 16, for its TMA descriptors);
 32-bit activations with a 16-bit matrix go to the tensor cores as three exact 16-bit terms (all but small matrices);
 everything else goes to the CUDA-core kernel with 32-bit FMA accumulation.
+
+quantize() brings a loaded 16-bit matrix into microscaled 4 bits (kernels/mxfp4.py), the counterpart of the reference's 8-bit matrices
+(src/transformers_neuronx/quantize.py, decoder.py: quantized weights beside their scales); with `activations` its input is brought into 4 bits
+in every call as well.
 """
 from __future__ import annotations
 
@@ -14,7 +18,7 @@ from typing import Dict, List, Optional
 
 import torch
 
-from ..kernels import ops
+from ..kernels import mxfp4, ops
 from ..weights.loader import TensorSpec
 from .base import NormedInput, Part, to_device, weight_to_device
 from .spec import LinearSpec
@@ -28,6 +32,26 @@ class Linear(Part):
         self.spec = spec
         self.weight: Optional[torch.Tensor] = None
         self.bias: Optional[torch.Tensor] = None
+        self.names = (spec.weight,)                # of the checkpoint's matrices this one is made of
+        self.quantize_input = False                # 4-bit matrix: the activations are brought into 4 bits too
+
+    @property
+    def quantized(self) -> bool:
+        return isinstance(self.weight, mxfp4.Mxfp4Matrix)
+
+    def quantize(self, activations: bool = False) -> bool:
+        """The matrix in 4 bits, if it is a 16-bit one whose columns are whole blocks; whether it was."""
+        w = self.weight
+        if not isinstance(w, torch.Tensor) or w.dtype not in (torch.bfloat16, torch.float16) or w.dim() != 2 or w.shape[1] % mxfp4.BLOCK:
+            return False
+        self.weight, self.quantize_input = mxfp4.quantize_mxfp4(w), bool(activations)
+        return True
+
+    def input_of(self, a):
+        """What a 4-bit matrix is multiplied by: the activations, or their 4-bit form."""
+        if isinstance(a, NormedInput):
+            a = a.tensor()
+        return mxfp4.quantize_mxfp4(a) if self.quantize_input else a
 
     @property
     def libraries(self):
@@ -48,7 +72,7 @@ class Linear(Part):
         self.weight, self.bias = weight, bias
 
     def parameter_bytes(self) -> int:
-        n = self.weight.numel() * self.weight.element_size()
+        n = self.weight.nbytes() if self.quantized else self.weight.numel() * self.weight.element_size()
         if self.bias is not None:
             n += self.bias.numel() * 4
         return n
@@ -56,6 +80,9 @@ class Linear(Part):
     def forward(self, a, out: torch.Tensor, residual: Optional[torch.Tensor] = None,
                 activation: Optional[str] = None) -> torch.Tensor:
         """`a`: the activations, or a NormedInput (rows of the residual stream and the norm still to apply)."""
+        if self.quantized:
+            mxfp4.gemm_mxfp4(self.input_of(a), self.weight, out, bias=self.bias, residual=residual, activation=activation)
+            return out
         if isinstance(a, NormedInput):
             fused = a.norm.fused_params()
             if (fused is not None and a.ctx.act_dtype == self.weight.dtype
@@ -91,5 +118,6 @@ def fuse_linears(parts: List[Linear], device) -> Linear:
     spec = LinearSpec(parts[0].spec.in_features, sum(p.spec.out_features for p in parts), "<fused>",
                       "<fused>" if bias is not None else None)
     fused = Linear(spec)
+    fused.names = tuple(n for p in parts for n in p.names)
     fused.set_weight(weight, bias)
     return fused
