@@ -35,55 +35,91 @@ __device__ __forceinline__ uint32_t quantize8(const float (&v)[8], uint32_t& E) 
     return pack_e2m1x8(s);
 }
 
-// One read of the values, one write of codes and scales: bound by memory.  `items` = rows * blocks * 4 pieces of eight values.
-template <typename T, bool WHOLE>
+// Rows to 4 bits: one read of the values, one write of codes and scales; bound by memory.  `items` = rows * blocks * 4 pieces of eight values, whose
+// codes lie in their order.  FLAT: so do the values (whole blocks, no gap between rows, 16-byte aligned), and a thread asks for four pieces
+// before it uses the first.  Otherwise a piece's row and column are worked out, and values are read one by one where 16 bytes at a time cannot be.
+constexpr int PIECES = 4;
+
+template <typename T, bool FLAT>
 __global__ void __launch_bounds__(256) quantize_kernel(const T* __restrict__ x, long long ld, uint32_t* __restrict__ codes, uint8_t* __restrict__ scales,
-                                                       long long items, int blocks, int K) {
+                                                       long long items, int blocks, int K, int vec) {
     pdl_launch_dependents();             // the products read codes behind their own wait
     pdl_wait();
     const long long stride = (long long)gridDim.x * blockDim.x;
+    constexpr int U = FLAT ? PIECES : 1;
     // whole warps walk the loop: the block's largest value is found by lanes together
-    for (long long i0 = (long long)blockIdx.x * blockDim.x + (threadIdx.x & ~31u); i0 < items; i0 += stride) {
+    for (long long i0 = (long long)blockIdx.x * blockDim.x + (threadIdx.x & ~31u); i0 < items; i0 += stride * U) {
         const long long i = i0 + (threadIdx.x & 31u);
-        float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-        if (i < items) {
-            const long long row = i / (4 * blocks);
-            const int k = (int)(i - row * (4 * blocks)) * 8;
-            const T* src = x + row * ld + k;
-            if (WHOLE) { Vec8<T> q; q.load(src); q.get(v); }
-            else {
+        float v[U][8];
+        if (FLAT) {
+            Vec8<T> q[U];
 #pragma unroll
-                for (int j = 0; j < 8; ++j) if (k + j < K) v[j] = to_float(src[j]);
+            for (int u = 0; u < U; ++u) { q[u].zero(); if (i + u * stride < items) q[u].load(x + (i + u * stride) * 8); }
+#pragma unroll
+            for (int u = 0; u < U; ++u) q[u].get(v[u]);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[0][j] = 0.f;
+            if (i < items) {
+                const long long row = i / (4 * blocks);
+                const int k = (int)(i - row * (4 * blocks)) * 8;
+                const T* src = x + row * ld + k;
+                if (vec && k + 8 <= K) { Vec8<T> q; q.load(src); q.get(v[0]); }
+                else {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) if (k + j < K) v[0][j] = to_float(src[j]);
+                }
             }
         }
-        uint32_t E;
-        const uint32_t c = quantize8(v, E);
-        if (i < items) {
-            codes[i] = c;
-            if ((i & 3) == 0) scales[i >> 2] = (uint8_t)E;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const long long at = i + u * stride;
+            uint32_t E;
+            const uint32_t c = quantize8(v[u], E);
+            if (at < items) {
+                codes[at] = c;
+                if ((at & 3) == 0) scales[at >> 2] = (uint8_t)E;
+            }
         }
     }
 }
 
 // Eight values a thread; no kernel behind it starts early, because a product may take the values for a matrix that no kernel writes.  In 32 bits and in bfloat16 every value is exact; float16 rounds what lies outside its range.
-template <typename T>
+template <typename T, bool FLAT>
 __global__ void __launch_bounds__(256) dequantize_kernel(const uint32_t* __restrict__ codes, const uint8_t* __restrict__ scales, T* __restrict__ out, long long ld,
                                                          long long items, int blocks, int K, int vec) {
     pdl_wait();
     const long long stride = (long long)gridDim.x * blockDim.x;
-    for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < items; i += stride) {
-        const long long row = i / (4 * blocks);
-        const int k = (int)(i - row * (4 * blocks)) * 8;
-        if (k >= K) continue;
-        const uint32_t c = codes[i];
-        const float s = mx_scale(scales[i >> 2]);
-        float v[8];
+    constexpr int U = FLAT ? PIECES : 1;
+    for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < items; i += stride * U) {
+        uint32_t c[U], E[U];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = mx_code(c >> (4 * j)) * s;
-        T* dst = out + row * ld + k;
-        if (vec && k + 8 <= K) { Vec8<T> q; q.set(v); q.store(dst); }
-        else
-            for (int j = 0; j < 8 && k + j < K; ++j) dst[j] = from_float<T>(v[j]);
+        for (int u = 0; u < U; ++u) {
+            const long long at = i + u * stride;
+            c[u] = E[u] = 0u;
+            if (at < items) { c[u] = __ldg(codes + at); E[u] = __ldg(scales + (at >> 2)); }
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const long long at = i + u * stride;
+            if (at >= items) break;
+            const float s = mx_scale(E[u]);
+            float v[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] = mx_code(c[u] >> (4 * j)) * s;
+            if (FLAT) {
+                Vec8<T> q;
+                q.set(v);
+                q.store(out + at * 8);
+                continue;
+            }
+            const long long row = at / (4 * blocks);
+            const int k = (int)(at - row * (4 * blocks)) * 8;
+            T* dst = out + row * ld + k;
+            if (vec && k + 8 <= K) { Vec8<T> q; q.set(v); q.store(dst); }
+            else
+                for (int j = 0; j < 8 && k + j < K; ++j) dst[j] = from_float<T>(v[j]);
+        }
     }
 }
 
@@ -161,15 +197,23 @@ __global__ void __launch_bounds__(32 * SIMT_WARPS) simt_kernel(const SimtParams 
     }
 }
 
+// Blocks of 256 threads: enough for one piece a thread, at most eight an SM.
+inline unsigned grid_for(long long items, int pieces, int sms) {
+    const long long want = (items + 256 * pieces - 1) / (256 * pieces), most = (long long)sms * 8;
+    return (unsigned)(want < most ? want : most);
+}
+
 template <typename T>
 int launch_quantize(const void* x, long long ld, void* codes, void* scales, int rows, int K, int sms, cudaStream_t stream) {
     const int blocks = (K + MX_BLOCK - 1) / MX_BLOCK;
     const long long items = (long long)rows * blocks * 4;
-    const bool whole = K % MX_BLOCK == 0 && ld % 8 == 0 && ((uintptr_t)x & 15) == 0;
-    const long long want = (items + 255) / 256, most = (long long)sms * 8;
-    const dim3 grid((unsigned)(want < most ? want : most));
-    if (whole) return tnx_launch_ex(1, quantize_kernel<T, true>, grid, dim3(256), 0, stream, (const T*)x, ld, (uint32_t*)codes, (uint8_t*)scales, items, blocks, K);
-    return tnx_launch_ex(1, quantize_kernel<T, false>, grid, dim3(256), 0, stream, (const T*)x, ld, (uint32_t*)codes, (uint8_t*)scales, items, blocks, K);
+    const int vec = ld % 8 == 0 && ((uintptr_t)x & 15) == 0;
+    // a few rows: a piece a thread, so that all SMs have some
+    if (vec && K % MX_BLOCK == 0 && (ld == K || rows == 1))
+        return tnx_launch_ex(1, quantize_kernel<T, true>, dim3(grid_for(items, items > 256ll * 8 * sms ? PIECES : 1, sms)), dim3(256), 0, stream, (const T*)x, ld,
+                             (uint32_t*)codes, (uint8_t*)scales, items, blocks, K, vec);
+    return tnx_launch_ex(1, quantize_kernel<T, false>, dim3(grid_for(items, 1, sms)), dim3(256), 0, stream, (const T*)x, ld, (uint32_t*)codes,
+                         (uint8_t*)scales, items, blocks, K, vec);
 }
 
 template <typename T>
@@ -177,9 +221,11 @@ int launch_dequantize(const void* codes, const void* scales, void* out, long lon
     const int blocks = (K + MX_BLOCK - 1) / MX_BLOCK;
     const long long items = (long long)rows * blocks * 4;
     const int vec = ld % 8 == 0 && ((uintptr_t)out & 15) == 0;
-    const long long want = (items + 255) / 256, most = (long long)sms * 8;
-    const dim3 grid((unsigned)(want < most ? want : most));
-    return tnx_launch_ex(1, dequantize_kernel<T>, grid, dim3(256), 0, stream, (const uint32_t*)codes, (const uint8_t*)scales, (T*)out, ld, items, blocks, K, vec);
+    if (vec && K % MX_BLOCK == 0 && (ld == K || rows == 1))
+        return tnx_launch_ex(1, dequantize_kernel<T, true>, dim3(grid_for(items, items > 256ll * 8 * sms ? PIECES : 1, sms)), dim3(256), 0, stream,
+                             (const uint32_t*)codes, (const uint8_t*)scales, (T*)out, ld, items, blocks, K, vec);
+    return tnx_launch_ex(1, dequantize_kernel<T, false>, dim3(grid_for(items, 1, sms)), dim3(256), 0, stream, (const uint32_t*)codes, (const uint8_t*)scales,
+                         (T*)out, ld, items, blocks, K, vec);
 }
 
 }  // namespace
