@@ -7,10 +7,8 @@
 // lanes of the accumulator, the tokens its columns, so that a step of few tokens pads tokens to 16 and streams W once.  K may be split
 // over the CTAs of a cluster.
 //
-// gemm16 (16-bit activations): W's codes come through TMA into shared memory, 256 columns of K a box; eight warps turn 64 columns at a
-// time into 16-bit values and put them into tensor memory, whence the MMAs take them as their A operand; activations come through
-// TMA.  Looking the values up by byte permutation costs 2.1 instructions a value; a K block of 64 x 128 values is needed every 512 cycles at 256
-// tokens, so a quarter of the issue slots go there.
+// gemm16 (16-bit activations): W's codes come through TMA into shared memory, 256 columns of K a box; sixteen warps turn them into 16-bit
+// values and put those into tensor memory, whence the MMAs take them as their A operand; activations come through TMA.
 //
 // gemm4 (activations in 4 bits too): both operands' codes come through TMA, 256 columns of K a stage, and are multiplied as they are
 // (tcgen05.mma kind::mxf4, a scale for 32 columns of K).  The MMAs read scales from tensor memory, where lane l of every quarter holds the
@@ -171,25 +169,25 @@ __device__ __forceinline__ void finish_tile(const Params& p, uint8_t* smem, bool
     }
 }
 
-template <int BN> __host__ __device__ constexpr int x_stage_bytes() { return BN * KB * 2; }
+// A stage is a box of codes: 256 columns of K, 16 MMAs.  (With 64 columns a stage, the waits and commits of the MMAs' warp, 250 to 300 cycles a stage
+// whatever it multiplies, were half of the kernel: one to 64 tokens by 16,384 x 4,096 22 us.)
+template <int BN> __host__ __device__ constexpr int x_stage_bytes() { return BN * CODE_K * 2; }
 template <int BN, int STAGES, int BOXES> __host__ __device__ constexpr int gemm16_smem() { return BOXES * CODE_BYTES + STAGES * x_stage_bytes<BN>() + 1024; }
-template <int BN> __host__ __device__ constexpr int gemm16_accs() { return BN <= 32 ? 4 : BN <= 64 ? 2 : 1; }
-template <int BN, int STAGES> __host__ __device__ constexpr uint32_t gemm16_tmem() { return gemm16_accs<BN>() * BN + STAGES * 32 <= 256 ? 256u : 512u; }
+template <int BN> __host__ __device__ constexpr int gemm16_accs() { return BN <= 32 ? 4 : BN <= 64 ? 2 : 1; }       // shorter chains of additions where there is room
 
-// BN tokens; STAGES: K blocks of activations and values in flight; BOXES: boxes of codes.
-template <int BN, int STAGES, int BOXES, int CTAS>
-__global__ void __launch_bounds__(THREADS16, CTAS)
+// BN tokens; STAGES: stages of activations and values in flight; BOXES: boxes of codes.
+template <int BN, int STAGES, int BOXES>
+__global__ void __launch_bounds__(THREADS16, 1)
 gemm16_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const Params p) {
-    constexpr int X_BYTES = x_stage_bytes<BN>();
-    constexpr uint32_t TMEM_COLS = gemm16_tmem<BN, STAGES>();
-    constexpr int ACCS = gemm16_accs<BN>();
-    static_assert(GROUPS16 == CODE_K / KB, "a group of warps for every K block of a box");
+    constexpr int X_BYTES = x_stage_bytes<BN>(), ACCS = gemm16_accs<BN>(), PARTS = CODE_K / KB, A_COLS = CODE_K / 2;
+    static_assert(ACCS * BN + STAGES * A_COLS <= 512, "tensor memory");
+    static_assert(GROUPS16 == PARTS, "a group of warps for every K block of a box");
     static_assert(BN * ROW_LD * 4 <= BOXES * CODE_BYTES + STAGES * X_BYTES, "the staged sums take the place of the stages");
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
     uint8_t* sW = smem;                                   // [BOXES]
-    uint8_t* sX = smem + BOXES * CODE_BYTES;              // [STAGES]
-    __shared__ uint64_t w_full[BOXES], w_empty[BOXES], x_full[STAGES], a_full[STAGES], empty[STAGES], done;
+    uint8_t* sX = smem + BOXES * CODE_BYTES;              // [STAGES][K blocks]
+    __shared__ uint64_t w_full[BOXES], w_empty[BOXES], full[STAGES], empty[STAGES], done;
     __shared__ uint32_t tmem_base_smem;
 #ifdef TNX_F16
     __shared__ int row_ref[TILE_W];
@@ -198,24 +196,21 @@ gemm16_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int token0 = blockIdx.x * BN, row0 = blockIdx.y * TILE_W;
     const int box0 = (int)blockIdx.z * p.boxes_per_split;
-    const int kb0 = box0 * (CODE_K / KB);
-    const int num_kb = min(p.num_kb - kb0, p.boxes_per_split * (CODE_K / KB));       // at least one
-    const int num_boxes = (num_kb + CODE_K / KB - 1) / (CODE_K / KB);
+    const int kb0 = box0 * PARTS;
+    const int num_kb = min(p.num_kb - kb0, p.boxes_per_split * PARTS);               // at least one
+    const int num_boxes = (num_kb + PARTS - 1) / PARTS;
 
     pdl_launch_dependents();
     if (threadIdx.x == 0) {
         for (int i = 0; i < BOXES; ++i) { mbar_init(&w_full[i], 1); mbar_init(&w_empty[i], 4 * GROUPS16); }
-        for (int i = 0; i < STAGES; ++i) { mbar_init(&x_full[i], 1); mbar_init(&a_full[i], 4); mbar_init(&empty[i], 1); }
+        for (int i = 0; i < STAGES; ++i) { mbar_init(&full[i], 1 + 4 * GROUPS16); mbar_init(&empty[i], 1); }         // full: activations and all warps' values
         mbar_init(&done, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("prefetch.tensormap [%0];" ::"l"((unsigned long long)&map_w) : "memory");
         asm volatile("prefetch.tensormap [%0];" ::"l"((unsigned long long)&map_x) : "memory");
     }
-    if (warp == 1) { tmem_alloc(&tmem_base_smem, TMEM_COLS); tmem_relinquish(); }
+    if (warp == 1) { tmem_alloc(&tmem_base_smem, 512u); tmem_relinquish(); }
     pdl_wait();                                           // codes, scales and activations may be the preceding kernel's
-#ifdef TNX_F16
-    if (threadIdx.x < TILE_W) row_ref[threadIdx.x] = 0;
-#endif
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -224,11 +219,12 @@ gemm16_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__
 
     if (warp == 0) {
         if (lane == 0) {
-            for (int i = 0; i < num_kb && ok; ++i) {
-                const int s = i % STAGES;
+            for (int i = 0; i < num_boxes && ok; ++i) {
+                const int s = i % STAGES, parts = min(PARTS, num_kb - i * PARTS);
                 if (i >= STAGES) { ok = mbar_wait(&empty[s], (uint32_t)(i / STAGES - 1) & 1u, p.err, 62); if (!ok) break; }
-                mbar_expect_tx(&x_full[s], X_BYTES);
-                tma_load_2d(sX + s * X_BYTES, &map_x, &x_full[s], (kb0 + i) * KB, token0);
+                mbar_expect_tx(&full[s], (uint32_t)(parts * BN * KB * 2));
+                for (int j = 0; j < parts; ++j)
+                    tma_load_2d(sX + s * X_BYTES + j * (BN * KB * 2), &map_x, &full[s], (kb0 + i * PARTS + j) * KB, token0);
             }
         }
         __syncwarp();
@@ -249,27 +245,27 @@ gemm16_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__
         constexpr uint32_t idesc = idesc16(BN);
         const uint64_t desc0 = smem_desc_sw128(smem_u32(sX));
         Ring<STAGES> r;
-        for (int i = 0; i < num_kb && ok;) {
-            int ready = min(ready_stages(x_full, r.slot, r.pass, STAGES, a_full, r.slot, r.pass, STAGES), num_kb - i);
-            if (ready == 0) {
-                ok = __all_sync(0xffffffffu, mbar_wait(&x_full[r.slot], r.pass, p.err, 63) && mbar_wait(&a_full[r.slot], r.pass, p.err, 64));
-                if (!ok) break;
-                ready = 1;
-            }
+        for (int i = 0; i < num_boxes && ok; ++i) {
+            ok = __all_sync(0xffffffffu, mbar_wait(&full[r.slot], r.pass, p.err, 63));
+            if (!ok) break;
             tc_fence_after();
-            for (; ready > 0; --ready, ++i) {
-                const uint64_t bdesc = desc0 + (uint64_t)(r.slot * (X_BYTES >> 4));
-                const uint32_t a = tmem_a + (uint32_t)(r.slot * 32);
-                if (elected()) {
+            const int parts = min(PARTS, num_kb - i * PARTS);
+            const uint64_t bdesc = desc0 + (uint64_t)(r.slot * (X_BYTES >> 4));
+            const uint32_t a = tmem_a + (uint32_t)(r.slot * A_COLS);
+            if (elected()) {
+#pragma unroll
+                for (int j = 0; j < PARTS; ++j) {
+                    if (j >= parts) break;
 #pragma unroll
                     for (int k = 0; k < KB / 16; ++k)
-                        umma_a_tmem(tmem_d + (uint32_t)(k % ACCS * BN), a + 8u * k, bdesc + (uint64_t)(2 * k), idesc, (i > 0 || k >= ACCS) ? 1u : 0u);
-                    umma_commit(&empty[r.slot]);
-                    if (i == num_kb - 1) umma_commit(&done);
+                        umma_a_tmem(tmem_d + (uint32_t)(k % ACCS * BN), a + (uint32_t)(32 * j + 8 * k), bdesc + (uint64_t)(j * (BN * KB * 2 >> 4) + 2 * k), idesc,
+                                    (i > 0 || j > 0 || k >= ACCS) ? 1u : 0u);
                 }
-                __syncwarp();
-                r.next();
+                umma_commit(&empty[r.slot]);
+                if (i == num_boxes - 1) umma_commit(&done);
             }
+            __syncwarp();
+            r.next();
         }
     } else if (warp >= 4) {
         // Values: warp w fills the lanes of quarter w % 4 (which its tensor memory accesses are confined to), each group of four
@@ -284,6 +280,11 @@ gemm16_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__
             if (even) return __ldg((const uint16_t*)(sc + b));
             return (uint32_t)__ldg(sc + b) | (b + 1 < p.blocks ? (uint32_t)__ldg(sc + b + 1) << 8 : 0u);
         };
+        // Asked for four boxes ahead: a trip to memory takes longer than a box.  (The loop is unrolled so that a register waits for its load
+        // where the scale is used: handing the values on would wait for the newest.)
+        uint32_t ahead[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) ahead[j] = load_scales(j);
         int ref = 0;
 #ifdef TNX_F16
         // the largest scale of every row over this CTA's share of K, which becomes a factor of the row's sums
@@ -310,54 +311,47 @@ gemm16_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__
             ref = row_ref[r];
         }
 #endif
-        // Asked for four boxes ahead: one box ahead, every box took a trip to memory (one token by 16,384 x 4,096 24 us).
-        // (The loop is unrolled so that a register waits for its load where the scale is used: handing the values on would wait for the newest.)
-        uint32_t ahead[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) ahead[j] = load_scales(j);
         for (int box4 = 0; box4 < num_boxes && ok; box4 += 4) {
 #pragma unroll
-          for (int u = 0; u < 4; ++u) {
-            const int box = box4 + u;
-            if (box >= num_boxes || !ok) break;
-            const uint32_t two = ahead[u];
-            ahead[u] = load_scales(box + 4);
-            const int ws = box % BOXES;
-            ok = __all_sync(0xffffffffu, mbar_wait(&w_full[ws], (uint32_t)(box / BOXES) & 1u, p.err, 65));
-            if (!ok) break;
-            // group j takes the box's K block j
-            const uint32_t row_addr = smem_u32(sW + ws * CODE_BYTES) + (uint32_t)r * 128u;
-            const int i = box * 4 + group;
-            if (i >= num_kb) break;
-            uint4 q[2];
-#pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                const uint32_t at = row_addr + ((uint32_t)((2 * group + c) ^ (r & 7)) << 4);
-                asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(q[c].x), "=r"(q[c].y), "=r"(q[c].z), "=r"(q[c].w) : "r"(at) : "memory");
-            }
-            uint32_t v[32];
-#pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                const MxValues t((two >> (8 * c)) & 255u, ref);
-                t.decode8(q[c].x, &v[16 * c]);
-                t.decode8(q[c].y, &v[16 * c + 4]);
-                t.decode8(q[c].z, &v[16 * c + 8]);
-                t.decode8(q[c].w, &v[16 * c + 12]);
-            }
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&w_empty[ws]);                             // this warp has read its share of the box
-            const int s = i % STAGES;
-            if (i >= STAGES) {
-                ok = __all_sync(0xffffffffu, mbar_wait(&empty[s], (uint32_t)(i / STAGES - 1) & 1u, p.err, 66));
+            for (int u = 0; u < 4; ++u) {
+                const int box = box4 + u, ws = box % BOXES, s = box % STAGES;
+                if (box >= num_boxes || !ok) break;
+                const uint32_t two = ahead[u];
+                ahead[u] = load_scales(box + 4);
+                ok = __all_sync(0xffffffffu, mbar_wait(&w_full[ws], (uint32_t)(box / BOXES) & 1u, p.err, 65));
                 if (!ok) break;
-                tc_fence_after();
+                const bool has = box * PARTS + group < num_kb;       // the last box may end before this group's K block
+                const uint32_t row_addr = smem_u32(sW + ws * CODE_BYTES) + (uint32_t)r * 128u;
+                uint4 q[2];
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    const uint32_t at = row_addr + ((uint32_t)((2 * group + c) ^ (r & 7)) << 4);
+                    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(q[c].x), "=r"(q[c].y), "=r"(q[c].z), "=r"(q[c].w) : "r"(at) : "memory");
+                }
+                uint32_t v[32];
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    const MxValues t((two >> (8 * c)) & 255u, ref);
+                    t.decode8(q[c].x, &v[16 * c]);
+                    t.decode8(q[c].y, &v[16 * c + 4]);
+                    t.decode8(q[c].z, &v[16 * c + 8]);
+                    t.decode8(q[c].w, &v[16 * c + 12]);
+                }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&w_empty[ws]);                             // this warp has read its share of the box
+                if (box >= STAGES) {
+                    ok = __all_sync(0xffffffffu, mbar_wait(&empty[s], (uint32_t)(box / STAGES - 1) & 1u, p.err, 66));
+                    if (!ok) break;
+                    tc_fence_after();
+                }
+                if (has) {
+                    tmem_st32(tmem_a + (uint32_t)(s * A_COLS + group * 32) + ((uint32_t)(quad * 32) << 16), v);
+                    tmem_st_wait();
+                }
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&full[s]);
             }
-            tmem_st32(tmem_a + (uint32_t)(s * 32) + ((uint32_t)(quad * 32) << 16), v);
-            tmem_st_wait();
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&a_full[s]);
-          }
         }
         ok = __all_sync(0xffffffffu, ok && mbar_wait(&done, 0, p.err, 67));
         tc_fence_after();
@@ -368,7 +362,7 @@ gemm16_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__
 #endif
     }
     finish_tile<BN, THREADS16>(p, smem, ok, row0, token0);
-    if (warp == 1) { tc_fence_after(); tmem_dealloc(tmem_base_smem, TMEM_COLS); }
+    if (warp == 1) { tc_fence_after(); tmem_dealloc(tmem_base_smem, 512u); }
 }
 
 // ---- both operands in 4 bits -----------------------------------------------------------------------
@@ -537,12 +531,12 @@ int launch(Kernel kernel, TnxSmemLimit& limit, int threads, int smem, int bn, co
     if (p.splits > 1) return tnx_launch_cluster(1, dim3(1, 1, p.splits), kernel, grid, dim3(threads), smem, stream, mw, mx, p);
     return tnx_launch_ex(1, kernel, grid, dim3(threads), smem, stream, mw, mx, p);
 }
-template <int BN, int STAGES, int BOXES, int CTAS>
+template <int BN, int STAGES, int BOXES>
 int launch16(const void* a, long long lda, const void* codes, int K, const Params& p, int tiles_w, cudaStream_t stream) {
     CUtensorMap mw, mx;
     if (!map_bytes(&mw, codes, p.w_rows, p.blocks * 16, 64) || !map_h16(&mx, a, p.e.M, K, lda, BN)) return TNX_ERR_UNSUPPORTED;
     static TnxSmemLimit limit;
-    return launch(gemm16_kernel<BN, STAGES, BOXES, CTAS>, limit, THREADS16, gemm16_smem<BN, STAGES, BOXES>(), BN, mw, mx, p, tiles_w, stream);
+    return launch(gemm16_kernel<BN, STAGES, BOXES>, limit, THREADS16, gemm16_smem<BN, STAGES, BOXES>(), BN, mw, mx, p, tiles_w, stream);
 }
 template <int BN, int STAGES, int CTAS>
 int launch4(const void* a, const void* codes, const Params& p, int tiles_w, cudaStream_t stream) {
@@ -564,7 +558,7 @@ void fill(Params& p, const void* scales, const void* a_scales, const float* bias
 // Tokens of a tile and the split of K over a cluster's CTAs.
 int plan(Params& p, int K, int n_sms, int tiles_w, int ctas_few) {
     const int M = p.e.M, boxes = (K + CODE_K - 1) / CODE_K;
-    int bn = M <= 16 ? 16 : M <= 32 ? 32 : M <= 64 ? 64 : M <= 128 ? 128 : 256;
+    int bn = M <= 16 ? 16 : M <= 32 ? 32 : M <= 64 ? 64 : 128;
     if (g_forced_bn) bn = g_forced_bn;
     const long long tiles = (long long)tiles_w * ((M + bn - 1) / bn);
     const int room = n_sms * (bn >= 128 ? 1 : ctas_few);
@@ -592,11 +586,10 @@ TNX_EXPORT int tnx_gemm_mxfp4_16(const void* a, long long lda, const void* codes
     Params p;
     fill(p, scales, nullptr, bias, residual, out, out_h16, ldc, M, N, K, act, gated, err);
     switch (plan(p, K, n_sms, tiles_w, 1)) {
-        case 16: return launch16<16, 8, 6, 1>(a, lda, codes, K, p, tiles_w, stream);
-        case 32: return launch16<32, 8, 6, 1>(a, lda, codes, K, p, tiles_w, stream);
-        case 64: return launch16<64, 8, 6, 1>(a, lda, codes, K, p, tiles_w, stream);
-        case 128: return launch16<128, 8, 4, 1>(a, lda, codes, K, p, tiles_w, stream);
-        default: return launch16<256, 5, 3, 1>(a, lda, codes, K, p, tiles_w, stream);
+        case 16: return launch16<16, 3, 6>(a, lda, codes, K, p, tiles_w, stream);
+        case 32: return launch16<32, 3, 6>(a, lda, codes, K, p, tiles_w, stream);
+        case 64: return launch16<64, 3, 6>(a, lda, codes, K, p, tiles_w, stream);
+        default: return launch16<128, 2, 4>(a, lda, codes, K, p, tiles_w, stream);
     }
 }
 
@@ -613,8 +606,7 @@ TNX_EXPORT int tnx_gemm_mxfp4_4(const void* a, const void* a_scales, const void*
         case 16: return launch4<16, 4, 2>(a, codes, p, tiles_w, stream);
         case 32: return launch4<32, 4, 2>(a, codes, p, tiles_w, stream);
         case 64: return launch4<64, 4, 2>(a, codes, p, tiles_w, stream);
-        case 128: return launch4<128, 4, 1>(a, codes, p, tiles_w, stream);
-        default: return launch4<256, 4, 1>(a, codes, p, tiles_w, stream);
+        default: return launch4<128, 4, 1>(a, codes, p, tiles_w, stream);
     }
 }
 
