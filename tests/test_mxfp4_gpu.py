@@ -326,3 +326,19 @@ def test_many_tiles(M, N, K, dtype):
             gate, up = exact[:, :F].clamp_min(0), exact[:, F:]
             both = bound[:, :F] * up.abs() + gate * bound[:, F:] + bound[:, :F] * bound[:, F:] + 2.0 ** -23 * (gate * up).abs()
             _check(out, gate * up, both, dtype)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("M,N,K", [(64, 256, 20480), (200, 300, 20480), (300, 512, 6144)])
+def test_long_sums_in_32_bits(M, N, K, dtype):
+    """Long sums into 32-bit results: random operands, whose additions round either way, lose less than 2^-20 of the result."""
+    from transformers_neuronx_b200.kernels import build
+    m = mx()
+    assert build.load("gemm_mxfp4", dtype).tnx_gemm_mxfp4_chain() == m._CHAIN[dtype]
+    w, wv = _matrix(N, K, M + K, spread=2.0)
+    a = torch.randn(M, K, generator=torch.Generator().manual_seed(K)).to(dtype).to(DEV)
+    out = torch.empty(M, N, device=DEV)
+    m.gemm_mxfp4(a, w, out)
+    ops().raise_on_device_error()
+    want = a.double() @ wv.t()
+    assert float((out.double() - want).norm() / want.norm()) <= 2.0 ** -20

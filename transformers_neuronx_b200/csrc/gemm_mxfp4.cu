@@ -546,6 +546,10 @@ int launch4(const void* a, const void* codes, const Params& p, int tiles_w, cuda
     return launch(gemm4_kernel<BN, STAGES, CTAS>, limit, THREADS4, gemm4_smem<BN, STAGES>(), BN, mw, mx, p, tiles_w, stream);
 }
 
+// Random operands, relative errors of 32-bit results: float16 3.8e-7 over chains of 4,096 columns, 1.2e-6 over 8,192, 5.5e-6 over 20,480; bfloat16, whose
+// products have fewer bits, 0.8e-7, 2.2e-7 and 1e-6 to 2e-6.
+constexpr int MX_CHAIN = 5120;
+
 int g_forced_splits = 0, g_forced_bn = 0;
 
 void fill(Params& p, const void* scales, const void* a_scales, const float* bias, const float* residual, void* out, int out_h16, long long ldc, int M, int N,
@@ -555,8 +559,9 @@ void fill(Params& p, const void* scales, const void* a_scales, const float* bias
     p.w_rows = gated ? 2 * N : N; p.blocks = (K + MX_BLOCK - 1) / MX_BLOCK; p.err = err;
     p.num_kb = (K + KB - 1) / KB;
 }
-// Tokens of a tile and the split of K over a cluster's CTAs.
-int plan(Params& p, int K, int n_sms, int tiles_w, int ctas_few) {
+// Tokens of a tile and the split of K over a cluster's CTAs.  chain: the most columns of K that one accumulator of a tile of 128 tokens should add up
+// (0: any number): an addition cuts off what it shifts out, so what a sum loses grows with its chain.
+int plan(Params& p, int K, int n_sms, int tiles_w, int ctas_few, int chain) {
     const int M = p.e.M, boxes = (K + CODE_K - 1) / CODE_K;
     int bn = M <= 16 ? 16 : M <= 32 ? 32 : M <= 64 ? 64 : 128;
     if (g_forced_bn) bn = g_forced_bn;
@@ -564,6 +569,7 @@ int plan(Params& p, int K, int n_sms, int tiles_w, int ctas_few) {
     const int room = n_sms * (bn >= 128 ? 1 : ctas_few);
     int splits = 1;
     while (splits < 8 && tiles * splits * 2 <= room && boxes >= splits * 2) splits *= 2;
+    while (chain && bn == 128 && splits < 8 && K > chain * splits && boxes >= splits * 2) splits *= 2;
     if (g_forced_splits) splits = g_forced_splits;
     p.boxes_per_split = (boxes + splits - 1) / splits;
     while (splits > 1 && p.boxes_per_split * (splits - 1) >= boxes) { splits /= 2; p.boxes_per_split = (boxes + splits - 1) / splits; }   // no CTA without work
@@ -572,6 +578,9 @@ int plan(Params& p, int K, int n_sms, int tiles_w, int ctas_few) {
 }
 
 }  // namespace
+
+// The most columns of K for whose 32-bit sums a tile's one accumulator is near enough (gemm_mxfp4_tiles.cu has one a tile).
+TNX_EXPORT int tnx_gemm_mxfp4_chain() { return MX_CHAIN; }
 
 // For sweeps and tests: the split of K (1, 2, 4 or 8) and the tokens of a tile whatever the sizes (0: the plan's own).
 TNX_EXPORT void tnx_gemm_mxfp4_force(int bn, int splits) { g_forced_bn = bn; g_forced_splits = splits; }
@@ -585,7 +594,7 @@ TNX_EXPORT int tnx_gemm_mxfp4_16(const void* a, long long lda, const void* codes
     if (lda % 8 || ((uintptr_t)a & 15) || ((uintptr_t)codes & 15) || tiles_w > 65535) return TNX_ERR_UNSUPPORTED;
     Params p;
     fill(p, scales, nullptr, bias, residual, out, out_h16, ldc, M, N, K, act, gated, err);
-    switch (plan(p, K, n_sms, tiles_w, 1)) {
+    switch (plan(p, K, n_sms, tiles_w, 1, out_h16 ? 0 : MX_CHAIN)) {
         case 16: return launch16<16, 3, 6>(a, lda, codes, K, p, tiles_w, stream);
         case 32: return launch16<32, 3, 6>(a, lda, codes, K, p, tiles_w, stream);
         case 64: return launch16<64, 3, 6>(a, lda, codes, K, p, tiles_w, stream);
@@ -602,7 +611,7 @@ TNX_EXPORT int tnx_gemm_mxfp4_4(const void* a, const void* a_scales, const void*
     if (((uintptr_t)a & 15) || ((uintptr_t)codes & 15) || tiles_w > 65535) return TNX_ERR_UNSUPPORTED;
     Params p;
     fill(p, scales, a_scales, bias, residual, out, out_h16, ldc, M, N, K, act, gated, err);
-    switch (plan(p, K, n_sms, tiles_w, 2)) {
+    switch (plan(p, K, n_sms, tiles_w, 2, 0)) {
         case 16: return launch4<16, 4, 2>(a, codes, p, tiles_w, stream);
         case 32: return launch4<32, 4, 2>(a, codes, p, tiles_w, stream);
         case 64: return launch4<64, 4, 2>(a, codes, p, tiles_w, stream);

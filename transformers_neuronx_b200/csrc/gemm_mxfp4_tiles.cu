@@ -173,10 +173,11 @@ __device__ __forceinline__ void teardown(bool ok, uint32_t tmem, int warp) {
 }
 
 // ---- 16-bit activations ------------------------------------------------------------------------------
-constexpr int STAGES16 = 4, BOXES = 4, GROUPS = 4;
+constexpr int BOXES = 4, GROUPS = 4;          // boxes of codes in flight; groups of four warps, one for each of a box's four K blocks
+constexpr int PARTS = 2, A_STAGES = 2, X_STAGES = 3;       // K blocks a stage; stages of values (tensor memory) and of activations
 constexpr int THREADS16 = 256 + 128 * GROUPS;        // warps 0: activations, 1: MMAs, 2: codes, 3: rows' references, 4..7: epilogue, 8..23: values
-constexpr int X16_BYTES = MAX_BN * KB * 2;
-constexpr int SMEM16 = BOXES * CODE_BYTES + STAGES16 * X16_BYTES + 1024;
+constexpr int X16_BYTES = MAX_BN * KB * 2;   // of a K block
+constexpr int SMEM16 = BOXES * CODE_BYTES + X_STAGES * PARTS * X16_BYTES + 1024;
 
 __global__ void __launch_bounds__(THREADS16, 1)
 gemm16_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const Params p) {
@@ -184,7 +185,7 @@ gemm16_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__
     uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
     uint8_t* sW = smem;
     uint8_t* sX = smem + BOXES * CODE_BYTES;
-    __shared__ uint64_t w_full[BOXES], w_empty[BOXES], full[STAGES16], empty[STAGES16];
+    __shared__ uint64_t w_full[BOXES], w_empty[BOXES], x_full[X_STAGES], x_empty[X_STAGES], a_full[A_STAGES], a_empty[A_STAGES];
     __shared__ Rings d;
     __shared__ uint32_t tmem_base_smem;
 #ifdef TNX_F16
@@ -192,12 +193,13 @@ gemm16_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__
     __shared__ int row_ref[2][TILE_W];
 #endif
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int num = p.num, boxes = (num + 3) / 4;
+    const int num = p.num, stages = (num + PARTS - 1) / PARTS, boxes = (num + 3) / 4;             // K blocks, stages and boxes a tile
 
     pdl_launch_dependents();
     if (threadIdx.x == 0) {
         for (int i = 0; i < BOXES; ++i) { mbar_init(&w_full[i], 1); mbar_init(&w_empty[i], 4 * GROUPS); }
-        for (int i = 0; i < STAGES16; ++i) { mbar_init(&full[i], 5); mbar_init(&empty[i], 1); }       // full: activations and four warps' values
+        for (int i = 0; i < X_STAGES; ++i) { mbar_init(&x_full[i], 1); mbar_init(&x_empty[i], 1); }
+        for (int i = 0; i < A_STAGES; ++i) { mbar_init(&a_full[i], 4 * PARTS); mbar_init(&a_empty[i], 1); }
         for (int i = 0; i < 2; ++i) { mbar_init(&d.full[i], 1); mbar_init(&d.empty[i], 4); }
 #ifdef TNX_F16
         for (int i = 0; i < 2; ++i) { mbar_init(&ref_full[i], 1); mbar_init(&ref_empty[i], 4 + 4 * GROUPS); }
@@ -218,15 +220,19 @@ gemm16_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__
         if (threadIdx.x == 0) atomicExch(p.err, 90);
     } else if (warp == 0) {
         if (lane == 0) {
-            Ring<STAGES16> r;
+            Ring<X_STAGES> r;
             int n = 0;
-            for (int tile = blockIdx.x; tile < p.tiles && ok; tile += gridDim.x)
-                for (int i = 0; i < num; ++i, ++n) {
-                    if (n >= STAGES16) { ok = mbar_wait(&empty[r.slot], r.pass ^ 1u, p.err, 92); if (!ok) break; }
-                    mbar_expect_tx(&full[r.slot], (uint32_t)(p.bn * KB * 2));
-                    tma_load_2d(sX + r.slot * X16_BYTES, &map_x, &full[r.slot], i * KB, tile % p.tiles_t * p.bn);
+            for (int tile = blockIdx.x; tile < p.tiles && ok; tile += gridDim.x) {
+                const int token0 = tile % p.tiles_t * p.bn;
+                for (int i = 0; i < stages; ++i, ++n) {
+                    if (n >= X_STAGES) { ok = mbar_wait(&x_empty[r.slot], r.pass ^ 1u, p.err, 92); if (!ok) break; }
+                    const int parts = min(PARTS, num - i * PARTS);
+                    mbar_expect_tx(&x_full[r.slot], (uint32_t)(parts * p.bn * KB * 2));
+                    for (int j = 0; j < parts; ++j)
+                        tma_load_2d(sX + (r.slot * PARTS + j) * X16_BYTES, &map_x, &x_full[r.slot], (i * PARTS + j) * KB, token0);
                     r.next();
                 }
+            }
         }
         __syncwarp();
     } else if (warp == 2) {
@@ -242,39 +248,39 @@ gemm16_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__
         }
         __syncwarp();
     } else if (warp == 1) {
-        // Two stages a turn: a wait costs this warp 200 cycles even where the barrier is ready (it queues behind the MMAs issued before it), the
-        // MMAs of a stage take 256 to 384; a wait and other turn's work for every stage took 600 to 700.
+        // A stage is 128 columns of K: the waits cost this warp 200 to 250 cycles a stage even where the barriers are ready (they queue behind the MMAs
+        // issued before them), eight MMAs take 512 to 768.  With 64 columns a stage the warp was what the kernel waited for.
         const uint32_t idesc = idesc16(p.bn);
         const uint64_t desc0 = smem_desc_sw128(smem_u32(sX));
-        const int total = (p.tiles - (int)blockIdx.x + (int)gridDim.x - 1) / (int)gridDim.x * num;
-        int i = 0, it = 0;
-        for (int n0 = 0; n0 < total && ok; n0 += STAGES16) {
-            const uint32_t pass = (uint32_t)(n0 / STAGES16) & 1u;
-#pragma unroll
-            for (int s0 = 0; s0 < STAGES16; s0 += 2) {
-                if (n0 + s0 >= total || !ok) break;
-                const bool both = n0 + s0 + 1 < total;
-                ok = mbar_wait(&full[s0], pass, p.err, 95) && (!both || mbar_wait(&full[s0 + 1], pass, p.err, 96));
+        Ring<X_STAGES> r;
+        Ring<A_STAGES> q;
+        int it = 0;
+        for (int tile = blockIdx.x; tile < p.tiles && ok; tile += gridDim.x, ++it) {
+            if (it >= 2) ok = __all_sync(0xffffffffu, mbar_wait(&d.empty[it & 1], (uint32_t)((it >> 1) - 1) & 1u, p.err, 94));
+            const uint32_t acc = tmem_d + (it & 1 ? MAX_BN : 0);
+            for (int i = 0; i < stages && ok; ++i) {
+                ok = mbar_wait(&x_full[r.slot], r.pass, p.err, 95) && mbar_wait(&a_full[q.slot], q.pass, p.err, 96);
                 ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                tc_fence_after();
+                const int parts = min(PARTS, num - i * PARTS);
+                const uint64_t bdesc = desc0 + (uint64_t)(r.slot * (PARTS * X16_BYTES >> 4));
+                const uint32_t a = tmem_a + (uint32_t)(q.slot * 32 * PARTS);
+                if (elected()) {
 #pragma unroll
-                for (int s = s0; s < s0 + 2; ++s) {
-                    if (!ok || (s > s0 && !both)) break;
-                    if (i == 0 && it >= 2) {
-                        ok = __all_sync(0xffffffffu, mbar_wait(&d.empty[it & 1], (uint32_t)((it >> 1) - 1) & 1u, p.err, 94));
-                        if (!ok) break;
-                    }
-                    tc_fence_after();
-                    if (elected()) {
-                        const uint32_t acc = tmem_d + (it & 1 ? MAX_BN : 0);
+                    for (int j = 0; j < PARTS; ++j) {
+                        if (j >= parts) break;
 #pragma unroll
                         for (int k = 0; k < KB / 16; ++k)
-                            umma_a_tmem(acc, tmem_a + (uint32_t)(s * 32 + 8 * k), desc0 + (uint64_t)(s * (X16_BYTES >> 4) + 2 * k), idesc, (i > 0 || k > 0) ? 1u : 0u);
-                        umma_commit(&empty[s]);
-                        if (i == num - 1) umma_commit(&d.full[it & 1]);
+                            umma_a_tmem(acc, a + (uint32_t)(32 * j + 8 * k), bdesc + (uint64_t)(j * (X16_BYTES >> 4) + 2 * k), idesc, (i > 0 || j > 0 || k > 0) ? 1u : 0u);
                     }
-                    __syncwarp();
-                    if (++i == num) { i = 0; ++it; }
+                    umma_commit(&x_empty[r.slot]);
+                    umma_commit(&a_empty[q.slot]);
+                    if (i == stages - 1) umma_commit(&d.full[it & 1]);
                 }
+                __syncwarp();
+                r.next();
+                q.next();
             }
         }
     } else if (warp == 3) {
@@ -385,7 +391,7 @@ gemm16_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__
 #endif
                 ok = __all_sync(0xffffffffu, mbar_wait(&w_full[ws], (uint32_t)(g / BOXES) & 1u, p.err, 100));
                 if (!ok) break;
-                const int i = box * 4 + group, n = it * num + i;
+                const int i = box * 4 + group, stage = box * (4 / PARTS) + group / PARTS, n = it * stages + stage;
                 if (++box == boxes) { box = 0; ++it; }
                 uint32_t v[32];
                 if (i < num) {
@@ -407,18 +413,20 @@ gemm16_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__
                 }
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&w_empty[ws]);                 // this warp has read its share of the box
-                if (i >= num) continue;
-                const int s = n % STAGES16;
-                if (n >= STAGES16) {
-                    ok = __all_sync(0xffffffffu, mbar_wait(&empty[s], (uint32_t)(n / STAGES16 - 1) & 1u, p.err, 101));
+                if (stage >= stages) continue;                            // the tile's last box ends before this stage
+                const int s = n % A_STAGES;
+                if (n >= A_STAGES) {
+                    ok = __all_sync(0xffffffffu, mbar_wait(&a_empty[s], (uint32_t)(n / A_STAGES - 1) & 1u, p.err, 101));
                     if (!ok) break;
                     tc_fence_after();
                 }
-                tmem_st32(tmem_a + (uint32_t)(s * 32) + ((uint32_t)(quad * 32) << 16), v);
-                tmem_st_wait();
+                if (i < num) {
+                    tmem_st32(tmem_a + (uint32_t)(s * 32 * PARTS + group % PARTS * 32) + ((uint32_t)(quad * 32) << 16), v);
+                    tmem_st_wait();
+                }
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&full[s]);
+                if (lane == 0) mbar_arrive(&a_full[s]);
             }
         }
     }
@@ -544,7 +552,7 @@ gemm4_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ 
         }
         __syncwarp();
     } else if (warp == 1) {
-        // Two stages a turn, as above.  Copies of scales and MMAs are carried out in the order in which they are issued.
+        // Two stages a turn: waits for barriers that are ready cost this warp 200 to 250 cycles a turn.  Copies of scales and MMAs are carried out in the order in which they are issued.
         const uint32_t idesc0 = idesc4(p.bn, 0), idesc2 = idesc4(p.bn, 2);
         const uint64_t desc0 = smem_desc_sw128(smem_u32(smem)), sfdesc0 = atom_desc(smem_u32(sSF));
         const int total = (p.tiles - (int)blockIdx.x + (int)gridDim.x - 1) / (int)gridDim.x * num;

@@ -27,6 +27,8 @@ from .ops import ACTIVATIONS, KernelError, _FLOATS, _H16, _check, _state, activa
 
 BLOCK = 32                                    # values that share a scale
 TILE_TOKENS = 128                             # beyond these persistent blocks walk over tiles of up to 192 tokens (gemm_mxfp4_tiles.cu)
+# 32-bit results: the columns that one accumulator of the tensor cores adds up without a visible loss; beyond them K is split (gemm_mxfp4.cu)
+_CHAIN = {torch.float16: 5120, torch.bfloat16: 5120}
 FEW_TOKENS = 16                               # up to here the matrix is streamed through registers (gemv_mxfp4.cu)
 
 
@@ -282,7 +284,7 @@ def _product(a, w, out, bias, residual, activation, gated):
             code = _entry("gemm_mxfp4_tiles", "tnx_gemm_mxfp4_tiles_4", kind)(
                 _PACK[18](a_p, as_p, *tail, scratch.data_ptr(), sms, err, _stream(device)))
             kernels = 2
-        elif M > TILE_TOKENS:
+        elif M > TILE_TOKENS and (out_h16 or K <= _CHAIN[kind]):
             code = _entry("gemm_mxfp4_tiles", "tnx_gemm_mxfp4_tiles_16", kind)(_PACK[17](a_p, lda, *tail, sms, err, _stream(device)))
         elif quantized:
             code = _entry("gemm_mxfp4", "tnx_gemm_mxfp4_4", kind)(_PACK[17](a_p, as_p, *tail, sms, err, _stream(device)))
