@@ -579,6 +579,19 @@ int plan(Params& p, int K, int n_sms, int tiles_w, int ctas_few, int chain) {
 
 }  // namespace
 
+// What a call would take, in ns, for a choice between this file's kernels and gemm_mxfp4_tiles.cu's: rounds of CTAs, each its boxes of 256 columns and what a
+// CTA costs beside them (fitted to more than 128 tokens, whose tiles are 128 wide; `quantized`: 4-bit activations).
+TNX_EXPORT long long tnx_gemm_mxfp4_estimate(int M, int N, int K, int gated, int quantized, int out_h16, int n_sms) {
+    Params p;
+    p.e.M = M;
+    const int tiles_w = gated ? (N + 63) / 64 : (N + TILE_W - 1) / TILE_W;
+    if (tiles_w > 65535) return 1ll << 60;
+    const int bn = plan(p, K, n_sms, tiles_w, 1, quantized || out_h16 ? 0 : MX_CHAIN);
+    const long long ctas = (long long)tiles_w * ((M + bn - 1) / bn) * p.splits;
+    const int places = p.splits <= 2 ? n_sms : p.splits == 4 ? n_sms * 9 / 10 : n_sms * 7 / 10;
+    return (ctas + places - 1) / places * (p.boxes_per_split * (quantized ? 650ll : 1150ll) + (quantized ? 4500 : 5000));
+}
+
 // The most columns of K for whose 32-bit sums a tile's one accumulator is near enough (gemm_mxfp4_tiles.cu has one a tile).
 TNX_EXPORT int tnx_gemm_mxfp4_chain() { return MX_CHAIN; }
 

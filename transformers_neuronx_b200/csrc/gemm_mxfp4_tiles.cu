@@ -640,6 +640,17 @@ void plan(Params& p, int n_sms, int tiles_w, int extra) {
 
 }  // namespace
 
+// What a call would take, in ns (see the function of the same kind in gemm_mxfp4.cu): rounds of tiles, each its stages, whose time grows with the tile's
+// tokens only in part.
+TNX_EXPORT long long tnx_gemm_mxfp4_tiles_estimate(int M, int N, int K, int gated, int quantized, int n_sms) {
+    Params p;
+    p.e.M = M;
+    const int tiles_w = gated ? (N + 63) / 64 : (N + TILE_W - 1) / TILE_W;
+    plan(p, n_sms, tiles_w, quantized ? 430 : 360);
+    const long long rounds = ((long long)p.tiles + n_sms - 1) / n_sms;
+    return quantized ? rounds * ((K + CODE_K - 1) / CODE_K) * (300 + p.bn * 7 / 10) + 8000 : rounds * ((K + 127) / 128) * (500 + p.bn * 14 / 10) + 6000;
+}
+
 // For sweeps: the tokens of a tile (a multiple of 16 from 64 to 192) whatever the sizes (0: the plan's own).
 TNX_EXPORT void tnx_gemm_mxfp4_tiles_force(int bn) { g_forced_bn = bn; }
 
@@ -654,7 +665,7 @@ TNX_EXPORT int tnx_gemm_mxfp4_tiles_16(const void* a, long long lda, const void*
     fill_epilogue(p.e, bias, residual, out, out_h16, ldc, M, N, act, gated);
     p.scales = (const uint8_t*)scales; p.a_scales = nullptr; p.err = err;
     p.w_rows = gated ? 2 * N : N; p.blocks = (K + MX_BLOCK - 1) / MX_BLOCK; p.num = (K + KB - 1) / KB;
-    plan(p, n_sms, tiles_w, 400);
+    plan(p, n_sms, tiles_w, 360);
     CUtensorMap mw, mx;
     if (!map_w(&mw, codes, p) || !map_h16(&mx, a, M, K, lda, p.bn)) return TNX_ERR_UNSUPPORTED;
     static TnxSmemLimit limit;
@@ -676,7 +687,7 @@ TNX_EXPORT int tnx_gemm_mxfp4_tiles_4(const void* a, const void* a_scales, const
     fill_epilogue(p.e, bias, residual, out, out_h16, ldc, M, N, act, gated);
     p.scales = (const uint8_t*)scales; p.a_scales = (const uint8_t*)a_scales; p.err = err;
     p.w_rows = gated ? 2 * N : N; p.blocks = (K + MX_BLOCK - 1) / MX_BLOCK; p.num = (K + CODE_K - 1) / CODE_K;
-    plan(p, n_sms, tiles_w, 200);
+    plan(p, n_sms, tiles_w, 430);
     CUtensorMap mw, mx;
     if (!map_w(&mw, codes, p) || !map_bytes(&mx, a, M, p.blocks * 16, p.bn)) return TNX_ERR_UNSUPPORTED;
     static TnxSmemLimit limit;

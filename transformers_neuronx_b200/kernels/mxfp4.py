@@ -15,7 +15,7 @@ keeps 8-bit matrices beside scales per column (src/transformers_neuronx/quantize
 """
 from __future__ import annotations
 
-from ctypes import c_char_p
+from ctypes import c_char_p, c_longlong
 from struct import Struct
 from typing import Optional
 
@@ -27,8 +27,7 @@ from .ops import ACTIVATIONS, KernelError, _FLOATS, _H16, _check, _state, activa
 
 BLOCK = 32                                    # values that share a scale
 TILE_TOKENS = 128                             # beyond these persistent blocks walk over tiles of up to 192 tokens (gemm_mxfp4_tiles.cu)
-# 32-bit results: the columns that one accumulator of the tensor cores adds up without a visible loss; beyond them K is split (gemm_mxfp4.cu)
-_CHAIN = {torch.float16: 5120, torch.bfloat16: 5120}
+CHAIN = 5120                                  # 32-bit results: the columns that one accumulator adds up without a visible loss; beyond them K is split
 FEW_TOKENS = 16                               # up to here the matrix is streamed through registers (gemv_mxfp4.cu)
 
 
@@ -227,6 +226,28 @@ def gated_gemm_mxfp4(a, w: Mxfp4Matrix, out: torch.Tensor, bias=None, activation
     return _product(a, w, out, bias, None, activation, True)
 
 
+_tiles = {}                                   # sizes -> whether persistent tiles are the faster kernel
+
+
+def _in_tiles(M, N, K, gated, quantized, out_h16, kind, sms) -> bool:
+    """More than TILE_TOKENS tokens: whether the kernel of persistent tiles takes them, or (few tiles, long K; 32-bit results of a long K) the one that
+    splits K over clusters.  Whichever is estimated to be faster; 2,048 tokens by 16,384 x 4,096 245 us in tiles, 330 split; 200 by 5,120 x 20,480 121 and 78."""
+    key = (M, N, K, gated, quantized, out_h16, kind, sms)
+    have = _tiles.get(key)
+    if have is None:
+        if not quantized and not out_h16 and K > CHAIN:
+            have = False
+        else:
+            few, many = _build.load("gemm_mxfp4", kind), _build.load("gemm_mxfp4_tiles", kind)
+            few.tnx_gemm_mxfp4_estimate.restype = many.tnx_gemm_mxfp4_tiles_estimate.restype = c_longlong
+            g, q = int(gated), int(quantized)
+            have = (many.tnx_gemm_mxfp4_tiles_estimate(M, N, K, g, q, sms) <= few.tnx_gemm_mxfp4_estimate(M, N, K, g, q, out_h16, sms))
+        if len(_tiles) > 4096:
+            _tiles.clear()
+        _tiles[key] = have
+    return have
+
+
 def _product(a, w, out, bias, residual, activation, gated):
     act = ACTIVATIONS.get(activation)
     if act is None:
@@ -277,14 +298,15 @@ def _product(a, w, out, bias, residual, activation, gated):
     if M <= FEW_TOKENS and w_p % 16 == 0 and (a_kind != 2 or a_p % 4 == 0):
         code = _entry("gemv_mxfp4", "tnx_gemv_mxfp4", kind)(_PACK[19](a_p, a_kind, as_p, lda, *tail, sms, err, _stream(device)))
     elif (a_p | w_p) % 16 == 0 and (a_kind == 2 or (a_kind == 0 and lda % 8 == 0)):
-        if M > TILE_TOKENS and quantized:
+        tiles = M > TILE_TOKENS and _in_tiles(M, N, K, gated, quantized, out_h16, kind, sms)
+        if tiles and quantized:
             # scales as the tensor cores read them: 1,024 bytes for 128 rows of W, 2,048 for 64 tokens, for every 256 columns
             nbytes = ((rows + 127) // 128 * 1024 + (M + 63) // 64 * 2048) * ((K + 255) // 256)
             scratch = torch.empty_strided((nbytes,), (1,), dtype=torch.uint8, device=out.device)
             code = _entry("gemm_mxfp4_tiles", "tnx_gemm_mxfp4_tiles_4", kind)(
                 _PACK[18](a_p, as_p, *tail, scratch.data_ptr(), sms, err, _stream(device)))
             kernels = 2
-        elif M > TILE_TOKENS and (out_h16 or K <= _CHAIN[kind]):
+        elif tiles:
             code = _entry("gemm_mxfp4_tiles", "tnx_gemm_mxfp4_tiles_16", kind)(_PACK[17](a_p, lda, *tail, sms, err, _stream(device)))
         elif quantized:
             code = _entry("gemm_mxfp4", "tnx_gemm_mxfp4_4", kind)(_PACK[17](a_p, as_p, *tail, sms, err, _stream(device)))
