@@ -401,15 +401,14 @@ int launch(const void* codes, const Params& p, int smem, cudaStream_t stream) {
 template <int TERMS, bool SCALED>
 int launch_terms(const void* codes, const Params& p, int smem, cudaStream_t stream) {
     if (p.M <= 8) return launch<TERMS, 1, SCALED>(codes, p, smem, stream);
-    if (p.M <= 16) return launch<TERMS, 2, SCALED>(codes, p, smem, stream);
-    return launch<TERMS, 4, SCALED>(codes, p, smem, stream);
+    return launch<TERMS, 2, SCALED>(codes, p, smem, stream);
 }
 
 int g_forced_wf = 0, g_forced_splits = 0;
 
 }  // namespace
 
-constexpr int FEW_TOKENS = 32;
+constexpr int FEW_TOKENS = 16;               // of a launch; more go in slices
 // For sweeps and tests: groups of 16 rows a block (1 to 16) and the split of K (1, 2, 4 or 8) whatever the sizes (0: the plan's own).
 TNX_EXPORT void tnx_gemv_mxfp4_force(int wf, int splits) { g_forced_wf = wf; g_forced_splits = splits; }
 
@@ -419,7 +418,18 @@ TNX_EXPORT int tnx_gemv_mxfp4(const void* a, int a_kind, const void* a_scales, l
                               cudaStream_t stream) {
     if (M <= 0 || N <= 0) return 0;
     if (K <= 0 || a_kind < 0 || a_kind > 2 || act < 0 || act >= TNX_ACT_COUNT || n_sms <= 0) return TNX_ERR_BAD_ARG;
-    if (M > FEW_TOKENS || ((uintptr_t)codes & 15) || (a_kind == 2 && ((uintptr_t)a & 3))) return TNX_ERR_UNSUPPORTED;
+    if (((uintptr_t)codes & 15) || (a_kind == 2 && ((uintptr_t)a & 3))) return TNX_ERR_UNSUPPORTED;
+    if (M > FEW_TOKENS) {
+        const long long blocks = (K + MX_BLOCK - 1) / MX_BLOCK;
+        for (int m = 0; m < M; m += FEW_TOKENS) {
+            const void* a_m = a_kind == 2 ? (const void*)((const uint8_t*)a + m * blocks * 16) : (const void*)((const char*)a + m * lda * (a_kind ? 4 : 2));
+            const int r = tnx_gemv_mxfp4(a_m, a_kind, a_scales ? (const void*)((const uint8_t*)a_scales + m * blocks) : nullptr, lda, codes, scales, bias,
+                                         residual ? residual + m * ldc : nullptr, (void*)((char*)out + m * ldc * (out_h16 ? 2 : 4)), out_h16, ldc,
+                                         M - m < FEW_TOKENS ? M - m : FEW_TOKENS, N, K, act, gated, n_sms, err, stream);
+            if (r) return r;
+        }
+        return 0;
+    }
     Params p;
     p.a = a; p.a_scales = (const uint8_t*)a_scales; p.lda = lda; p.a_kind = a_kind;
     p.a_vec = ((uintptr_t)a & 15) == 0 && lda % (a_kind == 1 ? 4 : 8) == 0;
@@ -429,7 +439,7 @@ TNX_EXPORT int tnx_gemv_mxfp4(const void* a, int a_kind, const void* a_scales, l
     p.act = act; p.out_h16 = out_h16; p.gated = gated;
     p.words = p.blocks % 8 == 0 && ((uintptr_t)scales & 7) == 0;
     const int terms = a_kind == 1 ? 3 : 1, groups = (N + (gated ? 8 : 16) - 1) / (gated ? 8 : 16);
-    const int nt = M <= 8 ? 1 : M <= 16 ? 2 : 4;
+    const int nt = M <= 8 ? 1 : 2;
     const int box_x = SLOT_K * 2 * nt * 8 * terms, box_s = nt * 8 * 4;      // shared memory of a box's activations, for one share of K
     auto scale_bytes = [&](int wf, int boxes) { return 16 * wf * ((boxes * 8 + 127) / 128 * 128 + 8); };        // eight rows lie in all banks
     // The last plans by their sizes: working one out takes longer than a launch.

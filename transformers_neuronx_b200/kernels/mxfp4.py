@@ -28,7 +28,7 @@ from .ops import ACTIVATIONS, KernelError, _FLOATS, _H16, _check, _state, activa
 BLOCK = 32                                    # values that share a scale
 TILE_TOKENS = 128                             # beyond these persistent blocks walk over tiles of up to 192 tokens (gemm_mxfp4_tiles.cu)
 CHAIN = 5120                                  # 32-bit results: the columns that one accumulator adds up without a visible loss; beyond them K is split
-FEW_TOKENS = 16                               # up to here the matrix is streamed through registers (gemv_mxfp4.cu)
+FEW_TOKENS = 16                               # the most that the kernel which streams the matrix through registers takes at a time (gemv_mxfp4.cu)
 
 
 class Mxfp4Matrix:
@@ -295,9 +295,14 @@ def _product(a, w, out, bias, residual, activation, gated):
     sms, err = _device_info(device, out.device)
     kernels = 1
     tail = (w_p, s_p, bias_p, res_p, out.data_ptr(), out_h16, ldc, M, N, K, act, 1 if gated else 0)
-    if M <= FEW_TOKENS and w_p % 16 == 0 and (a_kind != 2 or a_p % 4 == 0):
+    few = w_p % 16 == 0 and (a_kind != 2 or a_p % 4 == 0)
+    tensor = (a_p | w_p) % 16 == 0 and (a_kind == 2 or (a_kind == 0 and lda % 8 == 0))
+    # 4-bit activations are always faster on the tensor cores (one to 16 tokens by 16,384 x 4,096 9 us, 13 to 27 streamed); 16-bit ones from nine tokens
+    # on (12 tokens 17 to 20 us, 19 to 22 streamed), or 17 where the matrix is small (16 by 2,048 x 2,048 11 and 8 to 9); 32-bit ones are streamed
+    if few and (not tensor or (a_kind == 0 and (M <= 8 or (M <= FEW_TOKENS and rows * K <= 1 << 23)))) and (M <= FEW_TOKENS or a_kind == 1):
         code = _entry("gemv_mxfp4", "tnx_gemv_mxfp4", kind)(_PACK[19](a_p, a_kind, as_p, lda, *tail, sms, err, _stream(device)))
-    elif (a_p | w_p) % 16 == 0 and (a_kind == 2 or (a_kind == 0 and lda % 8 == 0)):
+        kernels = -(-M // FEW_TOKENS)
+    elif tensor:
         tiles = M > TILE_TOKENS and _in_tiles(M, N, K, gated, quantized, out_h16, kind, sms)
         if tiles and quantized:
             # scales as the tensor cores read them: 1,024 bytes for 128 rows of W, 2,048 for 64 tokens, for every 256 columns
