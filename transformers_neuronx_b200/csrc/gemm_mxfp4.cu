@@ -14,6 +14,8 @@
 // (tcgen05.mma kind::mxf4, a scale for 32 columns of K).  The MMAs read scales from tensor memory, where lane l of every quarter holds the
 // scales of rows l, 32 + l, 64 + l ... in neighbouring columns, four blocks of K a column: eight warps load them row by row, exchange
 // them through shared memory and store them there.
+#include <atomic>
+
 #include "gemm_mxfp4.cuh"
 
 namespace {
@@ -523,34 +525,100 @@ gemm4_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ 
 }
 
 // ---- host -----------------------------------------------------------------------------------------
+// How many CTAs of a kernel the device holds at a time in clusters of S, asked for once a device and kernel.
+struct Places {
+    std::atomic<int> known[64][9];
+    template <typename Kernel> int of(Kernel kernel, int threads, int smem, int S, int n_sms) {
+        int dev = 0;
+        cudaGetDevice(&dev);
+        if (dev < 0 || dev >= 64) return n_sms;
+        int n = known[dev][S].load();
+        if (n) return n;
+        if (S == 1) {
+            if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, threads, smem) != cudaSuccess) { cudaGetLastError(); n = 1; }
+            n = (n < 1 ? 1 : n) * n_sms;
+        } else {
+            cudaLaunchConfig_t cfg = {};
+            cfg.gridDim = dim3(1, 1, S); cfg.blockDim = dim3(threads); cfg.dynamicSmemBytes = smem;
+            cudaLaunchAttribute attr[1];
+            attr[0].id = cudaLaunchAttributeClusterDimension;
+            attr[0].val.clusterDim.x = 1; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = S;
+            cfg.attrs = attr; cfg.numAttrs = 1;
+            if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess) { cudaGetLastError(); n = 0; }
+            n = n < 1 ? n_sms / 2 : n * S;
+        }
+        known[dev][S].store(n);
+        return n;
+    }
+};
+
+int g_forced_splits = 0, g_forced_bn = 0;
+
+// The split of K over a cluster's CTAs, any number up to eight that leaves none without work: rounds of CTAs, each its boxes of 256 columns and what it
+// costs beside them, as much as `fixed` boxes (13 tokens by 5,120 x 20,480: 64 us unsplit, 35 in two, 28 in three, 42 in four, which need two
+// rounds).  chain: the most columns of K that one accumulator should add up (0: any number): an addition cuts off what it shifts out, so what a
+// sum loses grows with its chain.  Returns the estimate in boxes.
+template <typename PlacesOf>
+long long split(Params& p, int bn, int tiles_w, int fixed, int chain, PlacesOf places_of) {
+    const int boxes = (p.blocks + CODE_K / MX_BLOCK - 1) / (CODE_K / MX_BLOCK);
+    const long long tiles = (long long)tiles_w * ((p.e.M + bn - 1) / bn);
+    int least = 1;
+    while (chain && least < 8 && p.blocks * MX_BLOCK > chain * least) ++least;
+    long long best = -1;
+    p.splits = 1; p.boxes_per_split = boxes;
+    for (int S = 1; S <= 8; ++S) {
+        const int per = (boxes + S - 1) / S;
+        if ((boxes + per - 1) / per != S) continue;
+        if (g_forced_splits ? S != g_forced_splits : S < least && boxes >= least) continue;
+        const int places = places_of(S);
+        const long long rounds = (tiles * S + places - 1) / places, cost = rounds * (per + fixed) + (S > 1 ? 1 : 0);
+        if (best < 0 || cost < best) { best = cost; p.splits = S; p.boxes_per_split = per; }
+    }
+    return best < 0 ? boxes + fixed : best;
+}
+
 template <typename Kernel>
-int launch(Kernel kernel, TnxSmemLimit& limit, int threads, int smem, int bn, const CUtensorMap& mw, const CUtensorMap& mx, const Params& p, int tiles_w, cudaStream_t stream) {
-    const int r = limit.allow(kernel, smem);
-    if (r) return r;
+int launch(Kernel kernel, int threads, int smem, int bn, const CUtensorMap& mw, const CUtensorMap& mx, const Params& p, int tiles_w, cudaStream_t stream) {
     const dim3 grid((p.e.M + bn - 1) / bn, tiles_w, p.splits);
     if (p.splits > 1) return tnx_launch_cluster(1, dim3(1, 1, p.splits), kernel, grid, dim3(threads), smem, stream, mw, mx, p);
     return tnx_launch_ex(1, kernel, grid, dim3(threads), smem, stream, mw, mx, p);
 }
+
+constexpr int FIXED16 = 8, FIXED4 = 20;      // what a CTA costs beside its boxes, in boxes
+
+// cost: only the estimate is wanted, nothing is launched.
 template <int BN, int STAGES, int BOXES>
-int launch16(const void* a, long long lda, const void* codes, int K, const Params& p, int tiles_w, cudaStream_t stream) {
+int launch16(const void* a, long long lda, const void* codes, int K, Params& p, int tiles_w, int chain, int n_sms, cudaStream_t stream, long long* cost = nullptr) {
+    static TnxSmemLimit limit;
+    static Places places;
+    auto kernel = gemm16_kernel<BN, STAGES, BOXES>;
+    constexpr int SMEM = gemm16_smem<BN, STAGES, BOXES>();
+    const int r = limit.allow(kernel, SMEM);
+    if (r) return r;
+    const long long boxes = split(p, BN, tiles_w, FIXED16, chain, [&](int S) { return places.of(kernel, THREADS16, SMEM, S, n_sms); });
+    if (cost) { *cost = boxes; return 0; }
     CUtensorMap mw, mx;
     if (!map_bytes(&mw, codes, p.w_rows, p.blocks * 16, 64) || !map_h16(&mx, a, p.e.M, K, lda, BN)) return TNX_ERR_UNSUPPORTED;
-    static TnxSmemLimit limit;
-    return launch(gemm16_kernel<BN, STAGES, BOXES>, limit, THREADS16, gemm16_smem<BN, STAGES, BOXES>(), BN, mw, mx, p, tiles_w, stream);
+    return launch(kernel, THREADS16, SMEM, BN, mw, mx, p, tiles_w, stream);
 }
 template <int BN, int STAGES, int CTAS>
-int launch4(const void* a, const void* codes, const Params& p, int tiles_w, cudaStream_t stream) {
+int launch4(const void* a, const void* codes, Params& p, int tiles_w, int n_sms, cudaStream_t stream, long long* cost = nullptr) {
+    static TnxSmemLimit limit;
+    static Places places;
+    auto kernel = gemm4_kernel<BN, STAGES, CTAS>;
+    constexpr int SMEM = gemm4_smem<BN, STAGES>();
+    const int r = limit.allow(kernel, SMEM);
+    if (r) return r;
+    const long long boxes = split(p, BN, tiles_w, FIXED4, 0, [&](int S) { return places.of(kernel, THREADS4, SMEM, S, n_sms); });
+    if (cost) { *cost = boxes; return 0; }
     CUtensorMap mw, mx;
     if (!map_bytes(&mw, codes, p.w_rows, p.blocks * 16, 64) || !map_bytes(&mx, a, p.e.M, p.blocks * 16, BN)) return TNX_ERR_UNSUPPORTED;
-    static TnxSmemLimit limit;
-    return launch(gemm4_kernel<BN, STAGES, CTAS>, limit, THREADS4, gemm4_smem<BN, STAGES>(), BN, mw, mx, p, tiles_w, stream);
+    return launch(kernel, THREADS4, SMEM, BN, mw, mx, p, tiles_w, stream);
 }
 
 // Random operands, relative errors of 32-bit results: float16 3.8e-7 over chains of 4,096 columns, 1.2e-6 over 8,192, 5.5e-6 over 20,480; bfloat16, whose
 // products have fewer bits, 0.8e-7, 2.2e-7 and 1e-6 to 2e-6.
 constexpr int MX_CHAIN = 5120;
-
-int g_forced_splits = 0, g_forced_bn = 0;
 
 void fill(Params& p, const void* scales, const void* a_scales, const float* bias, const float* residual, void* out, int out_h16, long long ldc, int M, int N,
           int K, int act, int gated, int* err) {
@@ -559,23 +627,7 @@ void fill(Params& p, const void* scales, const void* a_scales, const float* bias
     p.w_rows = gated ? 2 * N : N; p.blocks = (K + MX_BLOCK - 1) / MX_BLOCK; p.err = err;
     p.num_kb = (K + KB - 1) / KB;
 }
-// Tokens of a tile and the split of K over a cluster's CTAs.  chain: the most columns of K that one accumulator of a tile of 128 tokens should add up
-// (0: any number): an addition cuts off what it shifts out, so what a sum loses grows with its chain.
-int plan(Params& p, int K, int n_sms, int tiles_w, int ctas_few, int chain) {
-    const int M = p.e.M, boxes = (K + CODE_K - 1) / CODE_K;
-    int bn = M <= 16 ? 16 : M <= 32 ? 32 : M <= 64 ? 64 : 128;
-    if (g_forced_bn) bn = g_forced_bn;
-    const long long tiles = (long long)tiles_w * ((M + bn - 1) / bn);
-    const int room = n_sms * (bn >= 128 ? 1 : ctas_few);
-    int splits = 1;
-    while (splits < 8 && tiles * splits * 2 <= room && boxes >= splits * 2) splits *= 2;
-    while (chain && bn == 128 && splits < 8 && K > chain * splits && boxes >= splits * 2) splits *= 2;
-    if (g_forced_splits) splits = g_forced_splits;
-    p.boxes_per_split = (boxes + splits - 1) / splits;
-    while (splits > 1 && p.boxes_per_split * (splits - 1) >= boxes) { splits /= 2; p.boxes_per_split = (boxes + splits - 1) / splits; }   // no CTA without work
-    p.splits = splits;
-    return bn;
-}
+int tile_tokens(int M) { return g_forced_bn ? g_forced_bn : M <= 16 ? 16 : M <= 32 ? 32 : M <= 64 ? 64 : 128; }
 
 }  // namespace
 
@@ -586,16 +638,20 @@ TNX_EXPORT long long tnx_gemm_mxfp4_estimate(int M, int N, int K, int gated, int
     p.e.M = M;
     const int tiles_w = gated ? (N + 63) / 64 : (N + TILE_W - 1) / TILE_W;
     if (tiles_w > 65535) return 1ll << 60;
-    const int bn = plan(p, K, n_sms, tiles_w, 1, quantized || out_h16 ? 0 : MX_CHAIN);
-    const long long ctas = (long long)tiles_w * ((M + bn - 1) / bn) * p.splits;
-    const int places = p.splits <= 2 ? n_sms : p.splits == 4 ? n_sms * 9 / 10 : n_sms * 7 / 10;
-    return (ctas + places - 1) / places * (p.boxes_per_split * (quantized ? 650ll : 1150ll) + (quantized ? 4500 : 5000));
+    p.blocks = (K + MX_BLOCK - 1) / MX_BLOCK;
+    long long boxes = 0;
+    const int r = quantized ? launch4<128, 4, 1>(nullptr, nullptr, p, tiles_w, n_sms, nullptr, &boxes)
+                            : launch16<128, 2, 4>(nullptr, 0, nullptr, K, p, tiles_w, out_h16 ? 0 : MX_CHAIN, n_sms, nullptr, &boxes);
+    if (r) return 1ll << 60;
+    // a box takes 650 (4-bit activations) or 1,150 ns; what a CTA costs beside them is 4.5 and 5 us
+    const long long rounds = (boxes - (p.splits > 1 ? 1 : 0)) / (p.boxes_per_split + (quantized ? FIXED4 : FIXED16));
+    return rounds * (p.boxes_per_split * (quantized ? 650ll : 1150ll) + (quantized ? 4500 : 5000));
 }
 
 // The most columns of K for whose 32-bit sums a tile's one accumulator is near enough (gemm_mxfp4_tiles.cu has one a tile).
 TNX_EXPORT int tnx_gemm_mxfp4_chain() { return MX_CHAIN; }
 
-// For sweeps and tests: the split of K (1, 2, 4 or 8) and the tokens of a tile whatever the sizes (0: the plan's own).
+// For sweeps and tests: the split of K (1 to 8) and the tokens of a tile whatever the sizes (0: the plan's own).
 TNX_EXPORT void tnx_gemm_mxfp4_force(int bn, int splits) { g_forced_bn = bn; g_forced_splits = splits; }
 
 // 16-bit activations [M, K] (pitch lda, a multiple of 8 elements, 16-byte aligned) by codes [w_rows][blocks * 16] (16-byte aligned).
@@ -607,11 +663,12 @@ TNX_EXPORT int tnx_gemm_mxfp4_16(const void* a, long long lda, const void* codes
     if (lda % 8 || ((uintptr_t)a & 15) || ((uintptr_t)codes & 15) || tiles_w > 65535) return TNX_ERR_UNSUPPORTED;
     Params p;
     fill(p, scales, nullptr, bias, residual, out, out_h16, ldc, M, N, K, act, gated, err);
-    switch (plan(p, K, n_sms, tiles_w, 1, out_h16 ? 0 : MX_CHAIN)) {
-        case 16: return launch16<16, 3, 6>(a, lda, codes, K, p, tiles_w, stream);
-        case 32: return launch16<32, 3, 6>(a, lda, codes, K, p, tiles_w, stream);
-        case 64: return launch16<64, 3, 6>(a, lda, codes, K, p, tiles_w, stream);
-        default: return launch16<128, 2, 4>(a, lda, codes, K, p, tiles_w, stream);
+    const int chain = out_h16 ? 0 : MX_CHAIN;
+    switch (tile_tokens(M)) {
+        case 16: return launch16<16, 3, 6>(a, lda, codes, K, p, tiles_w, 4 * chain, n_sms, stream);         // four accumulators share a sum
+        case 32: return launch16<32, 3, 6>(a, lda, codes, K, p, tiles_w, 4 * chain, n_sms, stream);
+        case 64: return launch16<64, 3, 6>(a, lda, codes, K, p, tiles_w, 2 * chain, n_sms, stream);
+        default: return launch16<128, 2, 4>(a, lda, codes, K, p, tiles_w, chain, n_sms, stream);
     }
 }
 
@@ -624,11 +681,11 @@ TNX_EXPORT int tnx_gemm_mxfp4_4(const void* a, const void* a_scales, const void*
     if (((uintptr_t)a & 15) || ((uintptr_t)codes & 15) || tiles_w > 65535) return TNX_ERR_UNSUPPORTED;
     Params p;
     fill(p, scales, a_scales, bias, residual, out, out_h16, ldc, M, N, K, act, gated, err);
-    switch (plan(p, K, n_sms, tiles_w, 2, 0)) {
-        case 16: return launch4<16, 4, 2>(a, codes, p, tiles_w, stream);
-        case 32: return launch4<32, 4, 2>(a, codes, p, tiles_w, stream);
-        case 64: return launch4<64, 4, 2>(a, codes, p, tiles_w, stream);
-        default: return launch4<128, 4, 1>(a, codes, p, tiles_w, stream);
+    switch (tile_tokens(M)) {
+        case 16: return launch4<16, 4, 2>(a, codes, p, tiles_w, n_sms, stream);
+        case 32: return launch4<32, 4, 2>(a, codes, p, tiles_w, n_sms, stream);
+        case 64: return launch4<64, 4, 2>(a, codes, p, tiles_w, n_sms, stream);
+        default: return launch4<128, 4, 1>(a, codes, p, tiles_w, n_sms, stream);
     }
 }
 
