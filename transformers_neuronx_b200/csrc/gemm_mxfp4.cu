@@ -525,7 +525,7 @@ gemm4_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ 
 }
 
 // ---- host -----------------------------------------------------------------------------------------
-// How many CTAs of a kernel the device holds at a time in clusters of S, asked for once a device and kernel.
+// How many CTAs of a kernel the device holds at a time in clusters of S when an SM has one of them, asked for once a device and kernel.
 struct Places {
     std::atomic<int> known[64][9];
     template <typename Kernel> int of(Kernel kernel, int threads, int smem, int S, int n_sms) {
@@ -535,8 +535,7 @@ struct Places {
         int n = known[dev][S].load();
         if (n) return n;
         if (S == 1) {
-            if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, threads, smem) != cudaSuccess) { cudaGetLastError(); n = 1; }
-            n = (n < 1 ? 1 : n) * n_sms;
+            n = n_sms;
         } else {
             cudaLaunchConfig_t cfg = {};
             cfg.gridDim = dim3(1, 1, S); cfg.blockDim = dim3(threads); cfg.dynamicSmemBytes = smem;
@@ -555,7 +554,7 @@ struct Places {
 int g_forced_splits = 0, g_forced_bn = 0;
 
 // The split of K over a cluster's CTAs, any number up to eight that leaves none without work: rounds of CTAs, each its boxes of 256 columns and what it
-// costs beside them, as much as `fixed` boxes (13 tokens by 5,120 x 20,480: 64 us unsplit, 35 in two, 28 in three, 42 in four, which need two
+// costs beside them, as much as `fixed` boxes; a part of a sum to be joined costs about one (13 tokens by 5,120 x 20,480: 64 us unsplit, 35 in two, 28 in three, 42 in four, which need two
 // rounds).  chain: the most columns of K that one accumulator should add up (0: any number): an addition cuts off what it shifts out, so what a
 // sum loses grows with its chain.  Returns the estimate in boxes.
 template <typename PlacesOf>
@@ -571,10 +570,10 @@ long long split(Params& p, int bn, int tiles_w, int fixed, int chain, PlacesOf p
         if ((boxes + per - 1) / per != S) continue;
         if (g_forced_splits ? S != g_forced_splits : S < least && boxes >= least) continue;
         const int places = places_of(S);
-        const long long rounds = (tiles * S + places - 1) / places, cost = rounds * (per + fixed) + (S > 1 ? 1 : 0);
+        const long long rounds = (tiles * S + places - 1) / places, cost = rounds * (per + fixed) + S;
         if (best < 0 || cost < best) { best = cost; p.splits = S; p.boxes_per_split = per; }
     }
-    return best < 0 ? boxes + fixed : best;
+    return best < 0 ? boxes + fixed + 1 : best;
 }
 
 template <typename Kernel>
@@ -609,7 +608,7 @@ int launch4(const void* a, const void* codes, Params& p, int tiles_w, int n_sms,
     constexpr int SMEM = gemm4_smem<BN, STAGES>();
     const int r = limit.allow(kernel, SMEM);
     if (r) return r;
-    const long long boxes = split(p, BN, tiles_w, FIXED4, 0, [&](int S) { return places.of(kernel, THREADS4, SMEM, S, n_sms); });
+    const long long boxes = split(p, BN, tiles_w, FIXED4, 0, [&](int S) { return CTAS * places.of(kernel, THREADS4, SMEM, S, n_sms); });
     if (cost) { *cost = boxes; return 0; }
     CUtensorMap mw, mx;
     if (!map_bytes(&mw, codes, p.w_rows, p.blocks * 16, 64) || !map_bytes(&mx, a, p.e.M, p.blocks * 16, BN)) return TNX_ERR_UNSUPPORTED;
@@ -644,7 +643,7 @@ TNX_EXPORT long long tnx_gemm_mxfp4_estimate(int M, int N, int K, int gated, int
                             : launch16<128, 2, 4>(nullptr, 0, nullptr, K, p, tiles_w, out_h16 ? 0 : MX_CHAIN, n_sms, nullptr, &boxes);
     if (r) return 1ll << 60;
     // a box takes 650 (4-bit activations) or 1,150 ns; what a CTA costs beside them is 4.5 and 5 us
-    const long long rounds = (boxes - (p.splits > 1 ? 1 : 0)) / (p.boxes_per_split + (quantized ? FIXED4 : FIXED16));
+    const long long rounds = (boxes - p.splits) / (p.boxes_per_split + (quantized ? FIXED4 : FIXED16));
     return rounds * (p.boxes_per_split * (quantized ? 650ll : 1150ll) + (quantized ? 4500 : 5000));
 }
 
