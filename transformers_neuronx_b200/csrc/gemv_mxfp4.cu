@@ -442,6 +442,10 @@ TNX_EXPORT int tnx_gemv_mxfp4(const void* a, int a_kind, const void* a_scales, l
     const int nt = M <= 8 ? 1 : 2;
     const int box_x = SLOT_K * 2 * nt * 8 * terms, box_s = nt * 8 * 4;      // shared memory of a box's activations, for one share of K
     auto scale_bytes = [&](int wf, int boxes) { return 16 * wf * ((boxes * 8 + 127) / 128 * 128 + 8); };        // eight rows lie in all banks
+    auto phase_of = [&](int wf, int wk, int boxes) {                          // boxes a warp can take before its activations are replaced
+        while (boxes > 1 && wf * wk * AHEAD * SLOT_BYTES + boxes * wk * (box_x + box_s) + scale_bytes(wf, boxes * wk) + 1024 > SMEM_MOST) --boxes;
+        return boxes;
+    };
     // The last plans by their sizes: working one out takes longer than a launch.
     struct Plan { int M, N, slots, gated, terms, sms, wf, wk, splits, sps; };
     static thread_local Plan known[64];
@@ -450,7 +454,8 @@ TNX_EXPORT int tnx_gemv_mxfp4(const void* a, int a_kind, const void* a_scales, l
     if (!forced && k.M == M && k.N == N && k.slots == p.slots && k.gated == gated && k.terms == terms && k.sms == n_sms) {
         p.wf = k.wf; p.wk = k.wk; p.splits = k.splits; p.slots_per_split = k.sps;
     } else {
-        // The busiest SM's boxes of codes, and what a block costs beside them (its activations, sums and barriers: as much as 16 boxes).
+        // The busiest SM's boxes of codes, and what a block costs beside them (its activations, sums and barriers: as much as 16 boxes; activations that
+        // come in two phases 12 more: 8 tokens by 2,048 x 4,096 12.8 us so, 8.3 by two parts of K in one phase each).
         long long best = -1;
         for (int splits = 1; splits <= 8; splits *= 2) {
             if (g_forced_splits && splits != g_forced_splits) continue;
@@ -467,7 +472,8 @@ TNX_EXPORT int tnx_gemv_mxfp4(const void* a, int a_kind, const void* a_scales, l
                 // clusters of four find places on nine SMs in ten at a time, of eight on seven
                 const int places = splits <= 2 ? n_sms : splits == 4 ? n_sms * 9 / 10 : n_sms * 7 / 10;
                 const long long rounds = (blocks + places - 1) / places;
-                const long long cost = rounds * ((long long)wf * wk * ((sps + wk - 1) / wk) + 16 + (splits > 1 ? 8 : 0));
+                const int each = (sps + wk - 1) / wk, phases = (each + phase_of(wf, wk, each) - 1) / phase_of(wf, wk, each);
+                const long long cost = rounds * ((long long)wf * wk * each + 16 + 12 * (phases - 1) + (splits > 1 ? 8 : 0));
                 if (best < 0 || cost < best) { best = cost; p.splits = splits; p.wf = wf; p.wk = wk; p.slots_per_split = sps; }
             }
         }
@@ -476,8 +482,7 @@ TNX_EXPORT int tnx_gemv_mxfp4(const void* a, int a_kind, const void* a_scales, l
     }
     const int ring = p.wf * p.wk * AHEAD * SLOT_BYTES;
     const int per = (p.slots_per_split + p.wk - 1) / p.wk;
-    p.phase = per;
-    while (p.phase > 1 && ring + p.phase * p.wk * (box_x + box_s) + scale_bytes(p.wf, p.phase * p.wk) + 1024 > SMEM_MOST) --p.phase;
+    p.phase = phase_of(p.wf, p.wk, per);
     p.phase = (per + (per + p.phase - 1) / p.phase - 1) / ((per + p.phase - 1) / p.phase);           // as many phases, equal ones
     p.x_at = ring;
     p.sx_at = ring + p.phase * p.wk * box_x;

@@ -297,9 +297,10 @@ def _product(a, w, out, bias, residual, activation, gated):
     tail = (w_p, s_p, bias_p, res_p, out.data_ptr(), out_h16, ldc, M, N, K, act, 1 if gated else 0)
     few = w_p % 16 == 0 and (a_kind != 2 or a_p % 4 == 0)
     tensor = (a_p | w_p) % 16 == 0 and (a_kind == 2 or (a_kind == 0 and lda % 8 == 0))
-    # 4-bit activations are always faster on the tensor cores (one to 16 tokens by 16,384 x 4,096 9 us, 13 to 27 streamed); 16-bit ones from nine tokens
-    # on (12 tokens 17 to 20 us, 19 to 22 streamed), or 17 where the matrix is small (16 by 2,048 x 2,048 11 and 8 to 9); 32-bit ones are streamed
-    if few and (not tensor or (a_kind == 0 and (M <= 8 or (M <= FEW_TOKENS and rows * K <= 1 << 23)))) and (M <= FEW_TOKENS or a_kind == 1):
+    # 4-bit activations are always faster on the tensor cores (one to 16 tokens by 16,384 x 4,096 9 us, 13 to 27 streamed), 16-bit ones from nine tokens
+    # on (8 tokens by 16,384 x 4,096 14 to 16 us streamed, 17 to 20 on the tensor cores, 12 tokens 19 to 22 and 17 to 20; by 2,304 x 768 5 to 6 and 6,
+    # then 6 to 7.6 and 6); 32-bit ones are streamed, 16 tokens at a time
+    if few and (not tensor or (a_kind == 0 and M <= 8)) and (M <= FEW_TOKENS or a_kind == 1):
         code = _entry("gemv_mxfp4", "tnx_gemv_mxfp4", kind)(_PACK[19](a_p, a_kind, as_p, lda, *tail, sms, err, _stream(device)))
         kernels = -(-M // FEW_TOKENS)
     elif tensor:
