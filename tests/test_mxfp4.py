@@ -72,3 +72,15 @@ def test_quantized_models_need_16_bits():
         model.quantize(QuantizationConfig())
     model.quantization = QuantizationConfig()
     assert {"mxfp4", "gemv_mxfp4", "gemm_mxfp4", "gemm_mxfp4_tiles"} <= set(model.libraries(torch.bfloat16))
+
+
+def test_sizes_that_kernels_do_not_count_are_refused():
+    """Rows and columns are counted in 32 bits: larger ones are refused before anything runs."""
+    m = mx()
+    with pytest.raises(m.KernelError, match="at most"):
+        m.Mxfp4Matrix(torch.empty(2 ** 31, 16, dtype=torch.uint8, device="meta"), torch.empty(2 ** 31, 1, dtype=torch.uint8, device="meta"))
+    x = torch.empty(1, 32).expand(2 ** 31, 32)
+    with pytest.raises(m.KernelError, match="at most"):
+        m._floats(x, "x", x.get_device())
+    one = torch.empty_strided((1, 20), (3, 1))
+    assert m._floats(one, "x", one.get_device()) == (1, 20, 24)            # the pitch of one row means nothing

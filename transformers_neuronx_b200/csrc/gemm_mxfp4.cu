@@ -171,6 +171,11 @@ __device__ __forceinline__ void finish_tile(const Params& p, uint8_t* smem, bool
     }
 }
 
+// Tensor memory is asked for behind the wait for the preceding kernel and before the next one may start, and what else an SM can hold beside a CTA
+// leaves it enough: whoever waits for tensor memory then waits for CTAs that end by themselves.  (A CTA of the next kernel that held some while it
+// waited for this one, or CTAs of two kernels on two streams whose clusters each hold what the other's want, would never end.)  gemm16 takes all of
+// it, so a CTA of a cluster takes the SM's shared memory too; gemm4's CTAs take a quarter and half of the shared memory, or (128 tokens) half.
+
 // A stage is a box of codes: 256 columns of K, 16 MMAs.  (With 64 columns a stage, the waits and commits of the MMAs' warp, 250 to 300 cycles a stage
 // whatever it multiplies, were half of the kernel: one to 64 tokens by 16,384 x 4,096 22 us.)
 template <int BN> __host__ __device__ constexpr int x_stage_bytes() { return BN * CODE_K * 2; }
@@ -202,7 +207,6 @@ gemm16_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__
     const int num_kb = min(p.num_kb - kb0, p.boxes_per_split * PARTS);               // at least one
     const int num_boxes = (num_kb + PARTS - 1) / PARTS;
 
-    pdl_launch_dependents();
     if (threadIdx.x == 0) {
         for (int i = 0; i < BOXES; ++i) { mbar_init(&w_full[i], 1); mbar_init(&w_empty[i], 4 * GROUPS16); }
         for (int i = 0; i < STAGES; ++i) { mbar_init(&full[i], 1 + 4 * GROUPS16); mbar_init(&empty[i], 1); }         // full: activations and all warps' values
@@ -211,11 +215,12 @@ gemm16_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__
         asm volatile("prefetch.tensormap [%0];" ::"l"((unsigned long long)&map_w) : "memory");
         asm volatile("prefetch.tensormap [%0];" ::"l"((unsigned long long)&map_x) : "memory");
     }
-    if (warp == 1) { tmem_alloc(&tmem_base_smem, 512u); tmem_relinquish(); }
     pdl_wait();                                           // codes, scales and activations may be the preceding kernel's
+    if (warp == 1) { tmem_alloc(&tmem_base_smem, 512u); tmem_relinquish(); }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
+    pdl_launch_dependents();                              // see Tensor memory, above
     const uint32_t tmem_d = tmem_base_smem, tmem_a = tmem_d + ACCS * BN;
     bool ok = true;
 
@@ -368,12 +373,12 @@ gemm16_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__
 }
 
 // ---- both operands in 4 bits -----------------------------------------------------------------------
-template <int BN> __host__ __device__ constexpr int sf_cols_x() { return BN < 32 ? 1 : BN / 32; }         // columns of an atom (four blocks of K) with rows in them
-template <int BN> __host__ __device__ constexpr int sf_step_x() { return BN < 128 ? 4 : BN / 32; }         // columns from one atom to the next
-template <int BN> __host__ __device__ constexpr int sf_stage_cols() { return BN == 256 ? 32 : 16; }       // W: 8 columns, activations: 2 atoms
+// A stage's scales in tensor memory: two atoms (four blocks of K) of four columns for W, two for the activations.
+constexpr int SF_COLS = 16;
+template <int BN> __host__ __device__ constexpr int sf_cols_x() { return BN < 32 ? 1 : BN / 32; }         // columns of an atom with tokens in them
 template <int BN, int STAGES> __host__ __device__ constexpr int gemm4_smem() { return STAGES * (CODE_BYTES + BN * CODE_K / 2) + 1024; }
 template <int BN, int STAGES> __host__ __device__ constexpr uint32_t gemm4_tmem() {
-    return BN + STAGES * sf_stage_cols<BN>() <= 128 ? 128u : BN + STAGES * sf_stage_cols<BN>() <= 256 ? 256u : 512u;
+    return BN + STAGES * SF_COLS <= 128 ? 128u : BN + STAGES * SF_COLS <= 256 ? 256u : 512u;
 }
 
 __device__ __forceinline__ void group_sync(int group) {
@@ -386,22 +391,21 @@ __global__ void __launch_bounds__(THREADS4, CTAS)
 gemm4_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const Params p) {
     constexpr int STAGE_BYTES = CODE_BYTES + BN * CODE_K / 2;
     constexpr uint32_t TMEM_COLS = gemm4_tmem<BN, STAGES>();
-    constexpr int XC = sf_cols_x<BN>(), XS = sf_step_x<BN>(), SF_COLS = sf_stage_cols<BN>();
+    constexpr int XC = sf_cols_x<BN>();
     static_assert(BN * ROW_LD * 4 <= STAGES * STAGE_BYTES, "the staged sums take the place of the stages");
     static_assert(STAGES % 2 == 0, "two groups of warps fill the scales in turn");
-    static_assert(8 + 2 * XS <= SF_COLS, "a stage's scales");
+    static_assert(BN <= 128, "a thread loads a row of the activations' scales");
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
     __shared__ uint64_t full[STAGES], sf_full[STAGES], empty[STAGES], done;
     __shared__ uint32_t tmem_base_smem;
-    __shared__ uint32_t sf_smem[2][(8 + 2 * XS) * 32];
+    __shared__ uint32_t sf_smem[2][SF_COLS * 32];
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int token0 = blockIdx.x * BN, row0 = blockIdx.y * TILE_W;
     const int st0 = (int)blockIdx.z * p.boxes_per_split;                           // stages of 256 columns
     const int num = min((p.blocks + 7) / 8 - st0, p.boxes_per_split);               // at least one
 
-    pdl_launch_dependents();
     if (threadIdx.x == 0) {
         for (int i = 0; i < STAGES; ++i) { mbar_init(&full[i], 1); mbar_init(&sf_full[i], 4); mbar_init(&empty[i], 1); }
         mbar_init(&done, 1);
@@ -409,11 +413,12 @@ gemm4_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ 
         asm volatile("prefetch.tensormap [%0];" ::"l"((unsigned long long)&map_w) : "memory");
         asm volatile("prefetch.tensormap [%0];" ::"l"((unsigned long long)&map_x) : "memory");
     }
+    pdl_wait();                                           // codes, scales and activations may be the preceding kernel's
     if (warp == 1) { tmem_alloc(&tmem_base_smem, TMEM_COLS); tmem_relinquish(); }
-    pdl_wait();
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
+    pdl_launch_dependents();                              // see Tensor memory, above
     const uint32_t tmem_d = tmem_base_smem, tmem_sf = tmem_d + BN;
     bool ok = true;
 
@@ -450,7 +455,7 @@ gemm4_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ 
 #pragma unroll
                     for (int k = 0; k < 4; ++k)           // 64 columns of K = 32 bytes = 2 units of the address field
                         umma_mxf4(tmem_d, adesc + (uint64_t)(2 * k), bdesc + (uint64_t)(2 * k), idesc4(BN, (k & 1) * 2), sf + 4u * (k >> 1),
-                                  sf + 8u + (uint32_t)(XS * (k >> 1)), (i > 0 || k > 0) ? 1u : 0u);
+                                  sf + 8u + 4u * (k >> 1), (i > 0 || k > 0) ? 1u : 0u);
                     umma_commit(&empty[r.slot]);
                     if (i == num - 1) umma_commit(&done);
                 }
@@ -459,22 +464,20 @@ gemm4_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ 
             }
         }
     } else if (warp >= 4) {
-        // Scales: two groups of four warps take stages in turn; a thread loads a row of W's and up to two of the activations', eight scales each,
+        // Scales: two groups of four warps take stages in turn; a thread loads a row of W's and one of the activations', eight scales each,
         // three turns ahead (a trip to memory takes longer than a stage); then every warp stores all of them to the lanes of its quarter.
         const int quad = warp & 3, group = (warp - 4) >> 2, r = quad * 32 + lane;
         const uint8_t* w_end = p.scales + (long long)p.w_rows * p.blocks;
         const uint8_t* x_end = p.a_scales + (long long)p.e.M * p.blocks;
         const uint8_t* ws = p.scales + (long long)tile_row(p.e, row0, r, p.w_rows) * p.blocks;
-        const uint8_t* xs[2];
-#pragma unroll
-        for (int j = 0; j < 2; ++j) { const int t = token0 + r + 128 * j; xs[j] = p.a_scales + (long long)(t < p.e.M ? t : p.e.M - 1) * p.blocks; }
-        struct Scales { uint2 w, x[2]; };
+        const int t = token0 + r < p.e.M ? token0 + r : p.e.M - 1;
+        const uint8_t* xs = p.a_scales + (long long)t * p.blocks;
+        struct Scales { uint2 w, x; };
         auto load = [&](int i) {
             Scales q;
             const int b = (st0 + i) * 8, n = i < num ? p.blocks - b : 0;
             q.w = load8(ws + b, p.scales, w_end, n);
-#pragma unroll
-            for (int j = 0; j < 2; ++j) if (r + 128 * j < 32 * XC) q.x[j] = load8(xs[j] + b, p.a_scales, x_end, n);
+            if (r < 32 * XC) q.x = load8(xs + b, p.a_scales, x_end, n);
             return q;
         };
         uint32_t* buf = sf_smem[group];
@@ -487,13 +490,11 @@ gemm4_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ 
             const Scales now = ahead[u];
             ahead[u] = load(i + 6);
             buf[quad * 32 + lane] = now.w.x; buf[(4 + quad) * 32 + lane] = now.w.y;
-#pragma unroll
-            for (int j = 0; j < 2; ++j)
-                if (r + 128 * j < 32 * XC) { buf[(8 + 4 * j + quad) * 32 + lane] = now.x[j].x; buf[(8 + XS + 4 * j + quad) * 32 + lane] = now.x[j].y; }
+            if (r < 32 * XC) { buf[(8 + quad) * 32 + lane] = now.x.x; buf[(12 + quad) * 32 + lane] = now.x.y; }
             group_sync(group);
-            uint32_t v[8 + 2 * XS];
+            uint32_t v[SF_COLS];
 #pragma unroll
-            for (int c = 0; c < 8 + 2 * XS; ++c) v[c] = c < 8 || (c - 8) % XS < XC ? buf[c * 32 + lane] : 0u;
+            for (int c = 0; c < SF_COLS; ++c) v[c] = c < 8 || c % 4 < XC ? buf[c * 32 + lane] : 0u;
             const int s = i % STAGES;
             if (ok && i >= STAGES) {
                 ok = __all_sync(0xffffffffu, mbar_wait(&empty[s], (uint32_t)(i / STAGES - 1) & 1u, p.err, 74));
@@ -502,7 +503,7 @@ gemm4_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ 
             if (ok) {
                 const uint32_t at = tmem_sf + (uint32_t)(s * SF_COLS) + ((uint32_t)(quad * 32) << 16);
 #pragma unroll
-                for (int c = 0; c < 8 + 2 * XS; c += 8) {
+                for (int c = 0; c < SF_COLS; c += 8) {
                     uint32_t q[8];
 #pragma unroll
                     for (int j = 0; j < 8; ++j) q[j] = v[c + j];
@@ -553,10 +554,10 @@ struct Places {
 
 int g_forced_splits = 0, g_forced_bn = 0;
 
-// The split of K over a cluster's CTAs, any number up to eight that leaves none without work: rounds of CTAs, each its boxes of 256 columns and what it
-// costs beside them, as much as `fixed` boxes; a part of a sum to be joined costs about one (13 tokens by 5,120 x 20,480: 64 us unsplit, 35 in two, 28 in three, 42 in four, which need two
-// rounds).  chain: the most columns of K that one accumulator should add up (0: any number): an addition cuts off what it shifts out, so what a
-// sum loses grows with its chain.  Returns the estimate in boxes.
+// The split of K over a cluster's CTAs, any number up to eight that leaves none without work: rounds of CTAs, each its boxes of 256 columns and what
+// it costs beside them, as much as `fixed` boxes; a part of a sum to be joined costs about one (13 float16 tokens by 5,120 x 20,480: 64 us unsplit,
+// 35 in two, 28 in three, 42 in four, which need two rounds).  chain: the most columns of K that one accumulator should add up (0: any number): an
+// addition cuts off what it shifts out, so what a sum loses grows with its chain.  Returns the estimate in boxes.
 template <typename PlacesOf>
 long long split(Params& p, int bn, int tiles_w, int fixed, int chain, PlacesOf places_of) {
     const int boxes = (p.blocks + CODE_K / MX_BLOCK - 1) / (CODE_K / MX_BLOCK);
@@ -583,6 +584,7 @@ int launch(Kernel kernel, int threads, int smem, int bn, const CUtensorMap& mw, 
     return tnx_launch_ex(1, kernel, grid, dim3(threads), smem, stream, mw, mx, p);
 }
 
+constexpr int SMEM_ALONE = 220 * 1024, SMEM_HALF = 106 * 1024;        // beside them: nothing that uses tensor memory; one more
 constexpr int FIXED16 = 8, FIXED4 = 20;      // what a CTA costs beside its boxes, in boxes
 
 // cost: only the estimate is wanted, nothing is launched.
@@ -592,20 +594,22 @@ int launch16(const void* a, long long lda, const void* codes, int K, Params& p, 
     static Places places;
     auto kernel = gemm16_kernel<BN, STAGES, BOXES>;
     constexpr int SMEM = gemm16_smem<BN, STAGES, BOXES>();
-    const int r = limit.allow(kernel, SMEM);
+    static_assert(SMEM <= SMEM_ALONE, "shared memory");
+    const int r = limit.allow(kernel, SMEM_ALONE);
     if (r) return r;
-    const long long boxes = split(p, BN, tiles_w, FIXED16, chain, [&](int S) { return places.of(kernel, THREADS16, SMEM, S, n_sms); });
+    const long long boxes = split(p, BN, tiles_w, FIXED16, chain, [&](int S) { return places.of(kernel, THREADS16, SMEM_ALONE, S, n_sms); });
     if (cost) { *cost = boxes; return 0; }
     CUtensorMap mw, mx;
     if (!map_bytes(&mw, codes, p.w_rows, p.blocks * 16, 64) || !map_h16(&mx, a, p.e.M, K, lda, BN)) return TNX_ERR_UNSUPPORTED;
-    return launch(kernel, THREADS16, SMEM, BN, mw, mx, p, tiles_w, stream);
+    return launch(kernel, THREADS16, p.splits > 1 ? SMEM_ALONE : SMEM, BN, mw, mx, p, tiles_w, stream);
 }
 template <int BN, int STAGES, int CTAS>
 int launch4(const void* a, const void* codes, Params& p, int tiles_w, int n_sms, cudaStream_t stream, long long* cost = nullptr) {
     static TnxSmemLimit limit;
     static Places places;
     auto kernel = gemm4_kernel<BN, STAGES, CTAS>;
-    constexpr int SMEM = gemm4_smem<BN, STAGES>();
+    constexpr int SMEM = CTAS == 2 ? SMEM_HALF : gemm4_smem<BN, STAGES>();
+    static_assert(gemm4_smem<BN, STAGES>() <= SMEM, "shared memory");
     const int r = limit.allow(kernel, SMEM);
     if (r) return r;
     const long long boxes = split(p, BN, tiles_w, FIXED4, 0, [&](int S) { return CTAS * places.of(kernel, THREADS4, SMEM, S, n_sms); });
@@ -630,8 +634,8 @@ int tile_tokens(int M) { return g_forced_bn ? g_forced_bn : M <= 16 ? 16 : M <= 
 
 }  // namespace
 
-// What a call would take, in ns, for a choice between this file's kernels and gemm_mxfp4_tiles.cu's: rounds of CTAs, each its boxes of 256 columns and what a
-// CTA costs beside them (fitted to more than 128 tokens, whose tiles are 128 wide; `quantized`: 4-bit activations).
+// What a call would take, in ns, for a choice between this file's kernels and gemm_mxfp4_tiles.cu's: rounds of CTAs, each its boxes of 256 columns and
+// what a CTA costs beside them (fitted to more than 128 tokens, whose tiles are 128 wide; `quantized`: 4-bit activations).
 TNX_EXPORT long long tnx_gemm_mxfp4_estimate(int M, int N, int K, int gated, int quantized, int out_h16, int n_sms) {
     Params p;
     p.e.M = M;

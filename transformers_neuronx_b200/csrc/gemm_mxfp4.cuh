@@ -23,8 +23,8 @@ __device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
 // How many of the next stages (up to four) are ready: lane j looks at stage j of one ring, lane 4 + j at stage j of the other, all in one trip
-// to shared memory.  An MMA's issue blocks until the ones ahead of it have almost been executed, and a look at a barrier takes 150 to 200
-// cycles even when it is ready: a look at both rings for every stage left the tensor cores idle for half of the time.
+// to shared memory.  A look at a barrier queues behind the MMAs issued before it and takes 150 to 250 cycles even when the stage is ready: a
+// look at both rings for every stage left the tensor cores idle for half of the time.
 __device__ __forceinline__ int ready_stages(uint64_t* a, int a_slot, uint32_t a_pass, int a_stages, uint64_t* b, int b_slot, uint32_t b_pass, int b_stages) {
     const int lane = threadIdx.x & 31;
     const bool second = lane & 4;
@@ -118,7 +118,6 @@ bool map_h16(CUtensorMap* out, const void* ptr, int rows, int cols, long long ld
     return fn(out, TNX_TMA_H16, 2, const_cast<void*>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
-
 
 inline void fill_epilogue(Epilogue& e, const float* bias, const float* residual, void* out, int out_h16, long long ldc, int M, int N, int act, int gated) {
     e.bias = bias; e.residual = residual; e.out = out; e.ldc = ldc;

@@ -195,7 +195,6 @@ gemm16_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int num = p.num, stages = (num + PARTS - 1) / PARTS, boxes = (num + 3) / 4;             // K blocks, stages and boxes a tile
 
-    pdl_launch_dependents();
     if (threadIdx.x == 0) {
         for (int i = 0; i < BOXES; ++i) { mbar_init(&w_full[i], 1); mbar_init(&w_empty[i], 4 * GROUPS); }
         for (int i = 0; i < X_STAGES; ++i) { mbar_init(&x_full[i], 1); mbar_init(&x_empty[i], 1); }
@@ -208,11 +207,12 @@ gemm16_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__
         asm volatile("prefetch.tensormap [%0];" ::"l"((unsigned long long)&map_w) : "memory");
         asm volatile("prefetch.tensormap [%0];" ::"l"((unsigned long long)&map_x) : "memory");
     }
-    if (warp == 3) { tmem_alloc(&tmem_base_smem, 512u); tmem_relinquish(); }
     pdl_wait();                                           // codes, scales and activations may be the preceding kernel's
+    if (warp == 3) { tmem_alloc(&tmem_base_smem, 512u); tmem_relinquish(); }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
+    pdl_launch_dependents();             // a kernel that started before all CTAs have their tensor memory might hold some and wait for them
     // The whole of tensor memory is this CTA's, so it begins at column 0: addresses that the compiler knows.
     constexpr uint32_t tmem_d = 0u, tmem_a = 2 * MAX_BN;
     bool ok = tmem_base_smem == 0u;                       // never anything else
@@ -508,7 +508,6 @@ gemm4_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int num = p.num;
 
-    pdl_launch_dependents();
     if (threadIdx.x == 0) {
         for (int i = 0; i < STAGES4; ++i) { mbar_init(&full[i], 2); mbar_init(&empty[i], 1); }
         for (int i = 0; i < 2; ++i) { mbar_init(&d.full[i], 1); mbar_init(&d.empty[i], 8); }
@@ -516,11 +515,12 @@ gemm4_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ 
         asm volatile("prefetch.tensormap [%0];" ::"l"((unsigned long long)&map_w) : "memory");
         asm volatile("prefetch.tensormap [%0];" ::"l"((unsigned long long)&map_x) : "memory");
     }
-    if (warp == 3) { tmem_alloc(&tmem_base_smem, 512u); tmem_relinquish(); }
     pdl_wait();
+    if (warp == 3) { tmem_alloc(&tmem_base_smem, 512u); tmem_relinquish(); }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
+    pdl_launch_dependents();
     constexpr uint32_t tmem_d = 0u, tmem_sf = 2 * MAX_BN;            // the whole of tensor memory is this CTA's
     bool ok = tmem_base_smem == 0u;                       // never anything else
     if (!ok) {
@@ -552,7 +552,8 @@ gemm4_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ 
         }
         __syncwarp();
     } else if (warp == 1) {
-        // Two stages a turn: waits for barriers that are ready cost this warp 200 to 250 cycles a turn.  Copies of scales and MMAs are carried out in the order in which they are issued.
+        // Two stages a turn: waits for barriers that are ready cost this warp 200 to 250 cycles a turn.  Copies of scales and MMAs are carried out in
+        // the order in which they are issued.
         const uint32_t idesc0 = idesc4(p.bn, 0), idesc2 = idesc4(p.bn, 2);
         const uint64_t desc0 = smem_desc_sw128(smem_u32(smem)), sfdesc0 = atom_desc(smem_u32(sSF));
         const int total = (p.tiles - (int)blockIdx.x + (int)gridDim.x - 1) / (int)gridDim.x * num;

@@ -84,7 +84,8 @@ __global__ void __launch_bounds__(256) quantize_kernel(const T* __restrict__ x, 
     }
 }
 
-// Eight values a thread; no kernel behind it starts early, because a product may take the values for a matrix that no kernel writes.  In 32 bits and in bfloat16 every value is exact; float16 rounds what lies outside its range.
+// Eight values a thread; bound by memory.  In 32 bits and in bfloat16 every value is exact; float16 rounds what lies outside its range.  No kernel
+// behind it starts early: a product may take the values for a matrix that no kernel writes.
 template <typename T, bool FLAT>
 __global__ void __launch_bounds__(256) dequantize_kernel(const uint32_t* __restrict__ codes, const uint8_t* __restrict__ scales, T* __restrict__ out, long long ld,
                                                          long long items, int blocks, int K, int vec) {

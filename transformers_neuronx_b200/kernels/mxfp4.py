@@ -28,6 +28,7 @@ from .ops import ACTIVATIONS, KernelError, _FLOATS, _H16, _check, _state, activa
 BLOCK = 32                                    # values that share a scale
 TILE_TOKENS = 128                             # beyond these persistent blocks walk over tiles of up to 192 tokens (gemm_mxfp4_tiles.cu)
 CHAIN = 5120                                  # 32-bit results: the columns that one accumulator adds up without a visible loss; beyond them K is split
+MOST = 2**31 - 4096                           # rows or columns: kernels count both, rounded up to tiles, in 32 bits
 FEW_TOKENS = 16                               # the most that the kernel which streams the matrix through registers takes at a time (gemv_mxfp4.cu)
 
 
@@ -46,6 +47,8 @@ class Mxfp4Matrix:
         if codes.shape != (rows, blocks * 16) or codes.device != scales.device:
             raise KernelError(f"codes {tuple(codes.shape)} and scales {tuple(scales.shape)} do not fit: 16 bytes of codes a scale, one device")
         columns = blocks * BLOCK if columns is None else int(columns)
+        if rows > MOST or columns > MOST:
+            raise KernelError(f"{rows} x {columns} values: at most {MOST} either way")
         if blocks < 1 or not (blocks - 1) * BLOCK < columns <= blocks * BLOCK:
             raise KernelError(f"{columns} columns do not make {blocks} blocks of {BLOCK}")
         self._codes, self._scales, self._buffer = codes, scales, None
@@ -164,6 +167,16 @@ def _floats(t, name: str, device: int):
     pitch, step = t.stride()
     if step != 1 and columns > 1:
         raise KernelError(f"{name} must have contiguous rows")
+    if rows > MOST or columns > MOST:
+        raise KernelError(f"{name} is {rows} x {columns}: at most {MOST} either way")
+    return rows, columns, pitch if rows > 1 else (columns + 7) // 8 * 8         # the pitch of one row means nothing
+
+
+def _writable(t, name: str, device: int):
+    """_floats() of a tensor that a kernel writes."""
+    rows, columns, pitch = _floats(t, name, device)
+    if pitch < columns and rows > 1:
+        raise KernelError(f"{name}'s rows overlap: a pitch of {pitch} for {columns} columns")
     return rows, columns, pitch
 
 
@@ -202,7 +215,7 @@ def dequantize_mxfp4(m: Mxfp4Matrix, dtype=torch.bfloat16, out: Optional[torch.T
             raise KernelError(f"dtype {dtype}: expected one of {_FLOATS}")
         out, pitch = torch.empty_strided((rows, columns), (columns, 1), dtype=dtype, device=m.device), columns
     else:
-        have, width, pitch = _floats(out, "out", device)
+        have, width, pitch = _writable(out, "out", device)
         if have != rows or width != columns:
             raise KernelError(f"out is {tuple(out.shape)}, the matrix {rows} x {columns}")
         dtype = out.dtype
@@ -216,7 +229,10 @@ def dequantize_mxfp4(m: Mxfp4Matrix, dtype=torch.bfloat16, out: Optional[torch.T
 def gemm_mxfp4(a, w: Mxfp4Matrix, out: torch.Tensor, bias=None, residual=None, activation=None) -> torch.Tensor:
     """out = act(a @ w^T + bias) + residual.  a: [tokens, columns] 16- or 32-bit floats, or an Mxfp4Matrix (quantize_mxfp4); out:
     [tokens, rows of w], 32-bit or 16-bit (float activations in 16 bits: the same type); bias: 32-bit; residual: 32-bit with the shape and
-    row pitch of a 32-bit out, which it may be.  Sums are 32-bit; each result is rounded once."""
+    row pitch of a 32-bit out, which it may be.  Sums are 32-bit; each result is rounded once.  out overlaps no other operand.
+
+    Where operands become 16-bit ones, values far below their neighbours lose bits: with float16 activations values of a row of w below 2^-36 of
+    the row's largest scale, and where few tokens are streamed (kernels' choice) activations below 2^-39 of the largest of the 256 around them."""
     return _product(a, w, out, bias, residual, activation, False)
 
 
@@ -267,7 +283,7 @@ def _product(a, w, out, bias, residual, activation, gated):
         kind = a.dtype
         a_kind = 1 if kind is torch.float32 else 0
         a_p, as_p = a.data_ptr(), 0
-    Mo, N, ldc = _floats(out, "out", device)
+    Mo, N, ldc = _writable(out, "out", device)
     if gated and rows % 2:
         raise KernelError(f"a gated product needs as many gate rows as up rows, got {rows} in all")
     if w.columns != K or Mo != M or (2 * N if gated else N) != rows:
@@ -296,7 +312,7 @@ def _product(a, w, out, bias, residual, activation, gated):
     kernels = 1
     tail = (w_p, s_p, bias_p, res_p, out.data_ptr(), out_h16, ldc, M, N, K, act, 1 if gated else 0)
     few = w_p % 16 == 0 and (a_kind != 2 or a_p % 4 == 0)
-    tensor = (a_p | w_p) % 16 == 0 and (a_kind == 2 or (a_kind == 0 and lda % 8 == 0))
+    tensor = (a_p | w_p) % 16 == 0 and (a_kind == 2 or (a_kind == 0 and lda % 8 == 0 and lda >= K))
     # 4-bit activations are always faster on the tensor cores (one to 16 tokens by 16,384 x 4,096 9 us, 13 to 27 streamed), 16-bit ones from nine tokens
     # on (8 tokens by 16,384 x 4,096 14 to 16 us streamed, 17 to 20 on the tensor cores, 12 tokens 19 to 22 and 17 to 20; by 2,304 x 768 5 to 6 and 6,
     # then 6 to 7.6 and 6); 32-bit ones are streamed, 16 tokens at a time
