@@ -24,8 +24,6 @@ from .base import NormedInput, Part, to_device, weight_to_device
 from .spec import LinearSpec
 
 
-
-
 class Linear(Part):
     graph_safe = True
     def __init__(self, spec: LinearSpec):
