@@ -229,3 +229,22 @@ def test_values_beyond_4_gigabytes():
         for at in (0, 53687, 65535, 69990):
             _check(out[at:at + 11], av[at:at + 11] @ wv.t(), _sum_bound(av[at:at + 11], wv), torch.bfloat16)
         del out
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("M,N,K", [(1040, 6000, 288), (700, 20000, 160), (1500, 9001, 544)])
+def test_tiles_of_an_odd_number_of_stages(M, N, K, dtype):
+    """Blocks that walk over several tiles whose stages fill their places unevenly: the first result is right, all others are the same."""
+    m = mx()
+    w, wv = _matrix(N, K, 11)
+    a = torch.randn(M, K, generator=torch.Generator().manual_seed(K)).to(dtype).to(DEV)
+    first = torch.empty(M, N, device=DEV, dtype=dtype)
+    m.gemm_mxfp4(a, w, first)
+    _check(first, a.double() @ wv.t(), _sum_bound(a.double(), wv), dtype)
+    out = torch.empty_like(first)
+    for i in range(40):
+        if i % 4 == 0:
+            out.fill_(float("nan"))                       # a kernel between them: blocks begin at other times
+        m.gemm_mxfp4(a, w, out)
+        assert torch.equal(out, first)
+    ops().raise_on_device_error()

@@ -174,7 +174,7 @@ __device__ __forceinline__ void teardown(bool ok, uint32_t tmem, int warp) {
 
 // ---- 16-bit activations ------------------------------------------------------------------------------
 constexpr int BOXES = 4, GROUPS = 4;          // boxes of codes in flight; groups of four warps, one for each of a box's four K blocks
-constexpr int PARTS = 2, A_STAGES = 2, X_STAGES = 3;       // K blocks a stage; stages of values (tensor memory) and of activations
+constexpr int PARTS = 2, A_STAGES = GROUPS / PARTS, X_STAGES = 3;       // K blocks a stage; stages of values (tensor memory) and of activations
 constexpr int THREADS16 = 256 + 128 * GROUPS;        // warps 0: activations, 1: MMAs, 2: codes, 3: rows' references, 4..7: epilogue, 8..23: values
 constexpr int X16_BYTES = MAX_BN * KB * 2;   // of a K block
 constexpr int SMEM16 = BOXES * CODE_BYTES + X_STAGES * PARTS * X16_BYTES + 1024;
@@ -253,19 +253,20 @@ gemm16_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__
         const uint32_t idesc = idesc16(p.bn);
         const uint64_t desc0 = smem_desc_sw128(smem_u32(sX));
         Ring<X_STAGES> r;
-        Ring<A_STAGES> q;
+        uint32_t passes = 0u;                             // of the places of values, a bit each
         int it = 0;
         for (int tile = blockIdx.x; tile < p.tiles && ok; tile += gridDim.x, ++it) {
             if (it >= 2) ok = __all_sync(0xffffffffu, mbar_wait(&d.empty[it & 1], (uint32_t)((it >> 1) - 1) & 1u, p.err, 94));
             const uint32_t acc = tmem_d + (it & 1 ? MAX_BN : 0);
             for (int i = 0; i < stages && ok; ++i) {
-                ok = mbar_wait(&x_full[r.slot], r.pass, p.err, 95) && mbar_wait(&a_full[q.slot], q.pass, p.err, 96);
+                const int place = i % A_STAGES;
+                ok = mbar_wait(&x_full[r.slot], r.pass, p.err, 95) && mbar_wait(&a_full[place], (passes >> place) & 1u, p.err, 96);
                 ok = __all_sync(0xffffffffu, ok);
                 if (!ok) break;
                 tc_fence_after();
                 const int parts = min(PARTS, num - i * PARTS);
                 const uint64_t bdesc = desc0 + (uint64_t)(r.slot * (PARTS * X16_BYTES >> 4));
-                const uint32_t a = tmem_a + (uint32_t)(q.slot * 32 * PARTS);
+                const uint32_t a = tmem_a + (uint32_t)(place * 32 * PARTS);
                 if (elected()) {
 #pragma unroll
                     for (int j = 0; j < PARTS; ++j) {
@@ -275,12 +276,12 @@ gemm16_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__
                             umma_a_tmem(acc, a + (uint32_t)(32 * j + 8 * k), bdesc + (uint64_t)(j * (X16_BYTES >> 4) + 2 * k), idesc, (i > 0 || j > 0 || k > 0) ? 1u : 0u);
                     }
                     umma_commit(&x_empty[r.slot]);
-                    umma_commit(&a_empty[q.slot]);
+                    umma_commit(&a_empty[place]);
                     if (i == stages - 1) umma_commit(&d.full[it & 1]);
                 }
                 __syncwarp();
                 r.next();
-                q.next();
+                passes ^= 1u << place;
             }
         }
     } else if (warp == 3) {
@@ -350,7 +351,9 @@ gemm16_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__
 #endif
         });
     } else {
-        // Values: a thread owns a row, group j takes K block j of every box.
+        // Values: a thread owns a row, group j takes K block j of every box and so always fills the same place in tensor memory, where a tile's even (or
+        // odd) stages stand: a group that changed places between tiles of an odd number of stages would not see all of a place's turns, of which
+        // a barrier tells only every other apart.
         const int quad = warp & 3, group = (warp - 8) >> 2, r = quad * 32 + lane;
         const bool even = p.blocks % 2 == 0 && ((uintptr_t)p.scales & 1) == 0;
         // The two scales of this group's K block, asked for four boxes ahead (a trip to memory takes longer than a box), over the tiles' ends.
@@ -372,7 +375,7 @@ gemm16_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__
 #pragma unroll
         for (int j = 0; j < 4; ++j) ahead[j] = load_scales();
         const int total = (p.tiles - (int)blockIdx.x + (int)gridDim.x - 1) / (int)gridDim.x * boxes;
-        int box = 0, it = 0, ref = 0;
+        int box = 0, it = 0, ref = 0, use = 0;            // use: stages that this group has filled
         for (int g0 = 0; g0 < total && ok; g0 += 4) {
 #pragma unroll
             for (int u = 0; u < 4; ++u) {
@@ -391,7 +394,7 @@ gemm16_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__
 #endif
                 ok = __all_sync(0xffffffffu, mbar_wait(&w_full[ws], (uint32_t)(g / BOXES) & 1u, p.err, 100));
                 if (!ok) break;
-                const int i = box * 4 + group, stage = box * (4 / PARTS) + group / PARTS, n = it * stages + stage;
+                const int i = box * 4 + group, stage = box * A_STAGES + group / PARTS;
                 if (++box == boxes) { box = 0; ++it; }
                 uint32_t v[32];
                 if (i < num) {
@@ -414,12 +417,13 @@ gemm16_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&w_empty[ws]);                 // this warp has read its share of the box
                 if (stage >= stages) continue;                            // the tile's last box ends before this stage
-                const int s = n % A_STAGES;
-                if (n >= A_STAGES) {
-                    ok = __all_sync(0xffffffffu, mbar_wait(&a_empty[s], (uint32_t)(n / A_STAGES - 1) & 1u, p.err, 101));
+                const int s = group / PARTS;
+                if (use > 0) {
+                    ok = __all_sync(0xffffffffu, mbar_wait(&a_empty[s], (uint32_t)(use - 1) & 1u, p.err, 101));
                     if (!ok) break;
                     tc_fence_after();
                 }
+                ++use;
                 if (i < num) {
                     tmem_st32(tmem_a + (uint32_t)(s * 32 * PARTS + group % PARTS * 32) + ((uint32_t)(quad * 32) << 16), v);
                     tmem_st_wait();
