@@ -110,7 +110,13 @@ __device__ __forceinline__ void write16(const Epilogue& e, const float (&v)[16],
     }
 }
 
-struct Rings {                               // both kernels' barriers between MMAs and epilogue
+// Two warps issue the MMAs, a stage each in turn: a warp's waits for a stage cost 200 to 250 cycles even where the barriers are ready (they queue behind
+// the MMAs that it issued before), which the other one's MMAs then cover.  The turn is handed on when a stage's MMAs have been issued, so they are
+// carried out in the order of the stages.  (Also by a warp whose wait ran out: the other one must not wait for ever.)
+__device__ __forceinline__ void await_turn(int who) { asm volatile("bar.sync %0, 64;" ::"r"(2 + who) : "memory"); tc_fence_after(); }
+__device__ __forceinline__ void hand_on(int who) { tc_fence_before(); __syncwarp(); asm volatile("bar.arrive %0, 64;" ::"r"(3 - who) : "memory"); }
+
+struct Rings {                               // both kernels' barriers between MMAs and epilogue; full: one arrival from either warp of the MMAs
     uint64_t full[2], empty[2];
 };
 
@@ -175,7 +181,7 @@ __device__ __forceinline__ void teardown(bool ok, uint32_t tmem, int warp) {
 // ---- 16-bit activations ------------------------------------------------------------------------------
 constexpr int BOXES = 4, GROUPS = 4;          // boxes of codes in flight; groups of four warps, one for each of a box's four K blocks
 constexpr int PARTS = 2, A_STAGES = GROUPS / PARTS, X_STAGES = 3;       // K blocks a stage; stages of values (tensor memory) and of activations
-constexpr int THREADS16 = 256 + 128 * GROUPS;        // warps 0: activations, 1: MMAs, 2: codes, 3: rows' references, 4..7: epilogue, 8..23: values
+constexpr int THREADS16 = 256 + 128 * GROUPS;        // warps 0: activations, 1, 3: MMAs, 2: codes, 4..7: rows' references and epilogue, 8..23: values
 constexpr int X16_BYTES = MAX_BN * KB * 2;   // of a K block
 constexpr int SMEM16 = BOXES * CODE_BYTES + X_STAGES * PARTS * X16_BYTES + 1024;
 
@@ -199,9 +205,9 @@ gemm16_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__
         for (int i = 0; i < BOXES; ++i) { mbar_init(&w_full[i], 1); mbar_init(&w_empty[i], 4 * GROUPS); }
         for (int i = 0; i < X_STAGES; ++i) { mbar_init(&x_full[i], 1); mbar_init(&x_empty[i], 1); }
         for (int i = 0; i < A_STAGES; ++i) { mbar_init(&a_full[i], 4 * PARTS); mbar_init(&a_empty[i], 1); }
-        for (int i = 0; i < 2; ++i) { mbar_init(&d.full[i], 1); mbar_init(&d.empty[i], 4); }
+        for (int i = 0; i < 2; ++i) { mbar_init(&d.full[i], 2); mbar_init(&d.empty[i], 4); }
 #ifdef TNX_F16
-        for (int i = 0; i < 2; ++i) { mbar_init(&ref_full[i], 1); mbar_init(&ref_empty[i], 4 + 4 * GROUPS); }
+        for (int i = 0; i < 2; ++i) { mbar_init(&ref_full[i], 4); mbar_init(&ref_empty[i], 4 * GROUPS); }
 #endif
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("prefetch.tensormap [%0];" ::"l"((unsigned long long)&map_w) : "memory");
@@ -247,27 +253,31 @@ gemm16_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__
                 }
         }
         __syncwarp();
-    } else if (warp == 1) {
-        // A stage is 128 columns of K: the waits cost this warp 200 to 250 cycles a stage even where the barriers are ready (they queue behind the MMAs
-        // issued before them), eight MMAs take 512 to 768.  With 64 columns a stage the warp was what the kernel waited for.
+    } else if (warp == 1 || warp == 3) {
+        // A stage is 128 columns of K, eight MMAs.
+        const int who = warp == 1 ? 0 : 1;
         const uint32_t idesc = idesc16(p.bn);
         const uint64_t desc0 = smem_desc_sw128(smem_u32(sX));
+        const int total = (p.tiles - (int)blockIdx.x + (int)gridDim.x - 1) / (int)gridDim.x * stages;
         Ring<X_STAGES> r;
         uint32_t passes = 0u;                             // of the places of values, a bit each
-        int it = 0;
-        for (int tile = blockIdx.x; tile < p.tiles && ok; tile += gridDim.x, ++it) {
-            if (it >= 2) ok = __all_sync(0xffffffffu, mbar_wait(&d.empty[it & 1], (uint32_t)((it >> 1) - 1) & 1u, p.err, 94));
-            const uint32_t acc = tmem_d + (it & 1 ? MAX_BN : 0);
-            for (int i = 0; i < stages && ok; ++i) {
-                const int place = i % A_STAGES;
-                ok = mbar_wait(&x_full[r.slot], r.pass, p.err, 95) && mbar_wait(&a_full[place], (passes >> place) & 1u, p.err, 96);
+        int it = 0, i = 0;
+        for (int n = 0; n < total; ++n) {
+            const int place = i % A_STAGES;
+            if ((n & 1) == who) {
+                // (an odd tile's last stage stands in the same place, so it has to be the turn of this one before its barrier tells anything)
+                const bool early = i == 0 && n > 0;
+                if (early) await_turn(who);
+                if (ok && it >= 2 && i < 2) ok = mbar_wait(&d.empty[it & 1], (uint32_t)((it >> 1) - 1) & 1u, p.err, 94);
+                ok = ok && mbar_wait(&x_full[r.slot], r.pass, p.err, 95) && mbar_wait(&a_full[place], (passes >> place) & 1u, p.err, 96);
                 ok = __all_sync(0xffffffffu, ok);
-                if (!ok) break;
+                if (n && !early) await_turn(who);
                 tc_fence_after();
+                const uint32_t acc = tmem_d + (it & 1 ? MAX_BN : 0);
                 const int parts = min(PARTS, num - i * PARTS);
                 const uint64_t bdesc = desc0 + (uint64_t)(r.slot * (PARTS * X16_BYTES >> 4));
                 const uint32_t a = tmem_a + (uint32_t)(place * 32 * PARTS);
-                if (elected()) {
+                if (ok && elected()) {
 #pragma unroll
                     for (int j = 0; j < PARTS; ++j) {
                         if (j >= parts) break;
@@ -277,73 +287,74 @@ gemm16_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__
                     }
                     umma_commit(&x_empty[r.slot]);
                     umma_commit(&a_empty[place]);
-                    if (i == stages - 1) umma_commit(&d.full[it & 1]);
+                    if (i >= stages - 2) umma_commit(&d.full[it & 1]);
+                    if (stages == 1) umma_commit(&d.full[it & 1]);
                 }
                 __syncwarp();
-                r.next();
-                passes ^= 1u << place;
+                if (n + 1 < total) hand_on(who);
             }
+            r.next();
+            passes ^= 1u << place;
+            if (++i == stages) { i = 0; ++it; }
         }
-    } else if (warp == 3) {
+    } else if (warp < 8) {
 #ifdef TNX_F16
-        // The largest scale of every row of the next tiles, which becomes a factor of the row's sums.
-        int it = 0;
+        // The largest scale of every row of a tile, which becomes a factor of the row's sums: found two tiles ahead, each warp for the rows that it writes
+        // out.
         const bool wide = p.blocks % 16 == 0 && ((uintptr_t)p.scales & 15) == 0;
-        for (int tile = blockIdx.x; tile < p.tiles && ok; tile += gridDim.x, ++it) {
-            const int buf = it & 1, tw = tile / p.tiles_t;
-            if (it >= 2) ok = __all_sync(0xffffffffu, mbar_wait(&ref_empty[buf], (uint32_t)((it >> 1) - 1) & 1u, p.err, 97));
-            if (!ok) break;
+        auto find_refs = [&](int it) {
+            const int tile = (int)blockIdx.x + it * (int)gridDim.x, buf = it & 1, r0 = (warp & 3) * 32 + (lane >> 2);
+            if (tile >= p.tiles) return;
             auto largest = [](uint32_t m, uint32_t w) {               // of four bytes; 255 (NaN) is no size
 #pragma unroll
                 for (int k = 0; k < 4; ++k) { const uint32_t E = (w >> (8 * k)) & 255u; m = max(m, E == 255u ? 0u : E); }
                 return m;
             };
-            // eight rows of four lanes at a time and eight of those in flight: the first tile waits for this
-#pragma unroll 1
-            for (int half = 0; half < 2; ++half) {
-                const uint8_t* q[8];
-                uint32_t m[8];
+            // four rows of eight lanes' in flight at a time: the first tile waits for this
+            const uint8_t* q[4];
+            uint32_t m[4];
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    q[e] = p.scales + (long long)tile_row(p, tw, half * 64 + e * 8 + (lane >> 2)) * p.blocks;
-                    m[e] = 0u;
+            for (int e = 0; e < 4; ++e) {
+                q[e] = p.scales + (long long)tile_row(p, tile / p.tiles_t, r0 + e * 8) * p.blocks;
+                m[e] = 0u;
+            }
+            if (wide) {
+#pragma unroll 2
+                for (int j = (lane & 3) * 16; j < p.blocks; j += 64) {
+                    uint4 v[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) v[e] = __ldg((const uint4*)(q[e] + j));
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) m[e] = largest(largest(largest(largest(m[e], v[e].x), v[e].y), v[e].z), v[e].w);
                 }
-                if (wide) {
-                    for (int j = (lane & 3) * 16; j < p.blocks; j += 64) {
-                        uint4 v[8];
+            } else {
+#pragma unroll 2
+                for (int j = lane & 3; j < p.blocks; j += 4) {
+                    uint32_t v[4];
 #pragma unroll
-                        for (int e = 0; e < 8; ++e) v[e] = __ldg((const uint4*)(q[e] + j));
+                    for (int e = 0; e < 4; ++e) v[e] = __ldg(q[e] + j);
 #pragma unroll
-                        for (int e = 0; e < 8; ++e) m[e] = largest(largest(largest(largest(m[e], v[e].x), v[e].y), v[e].z), v[e].w);
-                    }
-                } else {
-                    for (int j = lane & 3; j < p.blocks; j += 4) {
-                        uint32_t v[8];
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) v[e] = __ldg(q[e] + j);
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) m[e] = max(m[e], v[e] == 255u ? 0u : v[e]);
-                    }
+                    for (int e = 0; e < 4; ++e) m[e] = max(m[e], v[e] == 255u ? 0u : v[e]);
                 }
+            }
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    m[e] = max(m[e], __shfl_xor_sync(0xffffffffu, m[e], 1));
-                    m[e] = max(m[e], __shfl_xor_sync(0xffffffffu, m[e], 2));
-                    if ((lane & 3) == 0) row_ref[buf][half * 64 + e * 8 + (lane >> 2)] = (int)m[e];
-                }
+            for (int e = 0; e < 4; ++e) {
+                m[e] = max(m[e], __shfl_xor_sync(0xffffffffu, m[e], 1));
+                m[e] = max(m[e], __shfl_xor_sync(0xffffffffu, m[e], 2));
+                if ((lane & 3) == 0) row_ref[buf][r0 + e * 8] = (int)m[e];
             }
             __syncwarp();
             if (lane == 0) mbar_arrive(&ref_full[buf]);
-        }
+        };
+        find_refs(0);
+        find_refs(1);
 #endif
-    } else if (warp < 8) {
         ok = epilogue<1>(p, d, tmem_d, MAX_BN, 0, [&](int it) {
 #ifdef TNX_F16
             const int buf = it & 1;
-            if (!__all_sync(0xffffffffu, mbar_wait(&ref_full[buf], (uint32_t)(it >> 1) & 1u, p.err, 98))) return 0.f;
             const uint32_t E = (uint32_t)row_ref[buf][(warp & 3) * 32 + lane];
             __syncwarp();
-            if (lane == 0) mbar_arrive(&ref_empty[buf]);
+            if (__all_sync(0xffffffffu, mbar_wait(&ref_empty[buf], (uint32_t)(it >> 1) & 1u, p.err, 97))) find_refs(it + 2);
             return mx_scale(E) * (1.f / (float)(1 << MX_F16_TOP));
 #else
             (void)it;
@@ -439,7 +450,7 @@ gemm16_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__
 
 // ---- 4-bit activations -------------------------------------------------------------------------------
 constexpr int STAGES4 = 5;
-constexpr int THREADS4 = 384;                // warps 0, 2: TMA, 1: MMAs, 4..11: epilogue
+constexpr int THREADS4 = 384;                // warps 0, 2: TMA, 1, 3: MMAs, 4..11: epilogue
 constexpr int X4_BYTES = MAX_BN * CODE_K / 2, STAGE4_BYTES = CODE_BYTES + X4_BYTES;
 constexpr int SF_ATOM = 512;                 // scales of 128 rows and 128 columns of K: [32 lanes][rows l, 32 + l, 64 + l, 96 + l][4 blocks]
 constexpr int SFW_BYTES = 2 * SF_ATOM, SFX_BYTES = 4 * SF_ATOM;        // a stage's for W and for up to 256 tokens
@@ -514,7 +525,7 @@ gemm4_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ 
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < STAGES4; ++i) { mbar_init(&full[i], 2); mbar_init(&empty[i], 1); }
-        for (int i = 0; i < 2; ++i) { mbar_init(&d.full[i], 1); mbar_init(&d.empty[i], 8); }
+        for (int i = 0; i < 2; ++i) { mbar_init(&d.full[i], 2); mbar_init(&d.empty[i], 8); }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("prefetch.tensormap [%0];" ::"l"((unsigned long long)&map_w) : "memory");
         asm volatile("prefetch.tensormap [%0];" ::"l"((unsigned long long)&map_x) : "memory");
@@ -555,32 +566,25 @@ gemm4_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ 
             }
         }
         __syncwarp();
-    } else if (warp == 1) {
-        // Two stages a turn: waits for barriers that are ready cost this warp 200 to 250 cycles a turn.  Copies of scales and MMAs are carried out in
-        // the order in which they are issued.
+    } else if (warp < 4) {
+        // Copies of scales and MMAs are carried out in the order in which they are issued.
+        const int who = warp == 1 ? 0 : 1;
         const uint32_t idesc0 = idesc4(p.bn, 0), idesc2 = idesc4(p.bn, 2);
         const uint64_t desc0 = smem_desc_sw128(smem_u32(smem)), sfdesc0 = atom_desc(smem_u32(sSF));
         const int total = (p.tiles - (int)blockIdx.x + (int)gridDim.x - 1) / (int)gridDim.x * num;
         int i = 0, it = 0;
         Ring<STAGES4> r;
-        for (int n = 0; n < total && ok; n += 2) {
-            Ring<STAGES4> q = r;
-            q.next();
-            const bool both = n + 1 < total;
-            ok = mbar_wait(&full[r.slot], r.pass, p.err, 113) && (!both || mbar_wait(&full[q.slot], q.pass, p.err, 114));
-            ok = __all_sync(0xffffffffu, ok);
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                if (!ok || (h && !both)) break;
-                if (i == 0 && it >= 2) {
-                    ok = __all_sync(0xffffffffu, mbar_wait(&d.empty[it & 1], (uint32_t)((it >> 1) - 1) & 1u, p.err, 112));
-                    if (!ok) break;
-                }
+        for (int n = 0; n < total; ++n) {
+            if ((n & 1) == who) {
+                if (ok && it >= 2 && i < 2) ok = mbar_wait(&d.empty[it & 1], (uint32_t)((it >> 1) - 1) & 1u, p.err, 112);
+                ok = ok && mbar_wait(&full[r.slot], r.pass, p.err, 113);
+                ok = __all_sync(0xffffffffu, ok);
+                if (n) await_turn(who);
                 tc_fence_after();
                 const uint64_t adesc = desc0 + (uint64_t)(r.slot * (STAGE4_BYTES >> 4)), bdesc = adesc + (uint64_t)(CODE_BYTES >> 4);
                 const uint64_t sfdesc = sfdesc0 + (uint64_t)(r.slot * ((SFW_BYTES + SFX_BYTES) >> 4));
                 const uint32_t sf = tmem_sf + (uint32_t)(r.slot * SF_COLS), acc = tmem_d + (it & 1 ? MAX_BN : 0);
-                if (elected()) {
+                if (ok && elected()) {
 #pragma unroll
                     for (int k = 0; k < 2; ++k) {         // 128 columns of K
                         copy_atom(sf + 4u * k, sfdesc + (uint64_t)(k * (SF_ATOM >> 4)));
@@ -592,12 +596,14 @@ gemm4_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ 
                         umma_mxf4(acc, adesc + (uint64_t)(2 * k), bdesc + (uint64_t)(2 * k), k & 1 ? idesc2 : idesc0, sf + 4u * (k >> 1),
                                   sf + 8u + 8u * (k >> 1), (i > 0 || k > 0) ? 1u : 0u);
                     umma_commit(&empty[r.slot]);
-                    if (i == num - 1) umma_commit(&d.full[it & 1]);
+                    if (i >= num - 2) umma_commit(&d.full[it & 1]);
+                    if (num == 1) umma_commit(&d.full[it & 1]);
                 }
                 __syncwarp();
-                r.next();
-                if (++i == num) { i = 0; ++it; }
+                if (n + 1 < total) hand_on(who);
             }
+            r.next();
+            if (++i == num) { i = 0; ++it; }
         }
     } else if (warp >= 4) {
         ok = epilogue<2>(p, d, tmem_d, MAX_BN, (warp - 4) >> 2, [](int) { return 1.f; });
