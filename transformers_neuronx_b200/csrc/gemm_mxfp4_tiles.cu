@@ -1,15 +1,17 @@
 // Products of many tokens with a 4-bit matrix on the 5th-generation tensor cores (what is computed: gemm_mxfp4.cu).
 //
 // Persistent CTAs, one an SM, walk over tiles of 128 rows of W (the lanes of an accumulator) by up to 192 tokens (its columns).  Two accumulators:
-// while one is written out by four warps of their own, the MMAs fill the other.  (A CTA a tile, whose sums went through shared memory,
-// spent 11 us a tile outside of its main loop: 2,048 tokens by 16,384 x 4,096 229 us with 16-bit activations, 153 with 4-bit ones.)
+// while one is written out by warps of their own, the MMAs fill the other.  (A CTA a tile, whose sums went through shared memory, spent 11 us a tile
+// outside of its main loop.)  2,048 tokens by 16,384 x 4,096: 223 us with 16-bit activations, 1.23 PFLOP/s, where the tensor cores are busy for
+// 61% of the time at 1.6 GHz, which the power limit leaves (no MMAs: 171 to 186 us, no decoding: 195 to 211, neither of them: 121, which is what the
+// activations' way from L2 takes); 69 us with 4-bit ones, 3.98 PFLOP/s, of which the loads alone take 56.
 // Sums go straight from tensor memory to memory: a warp's lanes are 32 neighbouring features, so that a token's store is 64 or 128 bytes.
 // Gated tiles alternate eight gate rows and their eight up rows: gate and up values meet by one exchange of lanes eight apart.
 //
 // gemm16 (16-bit activations): codes come through TMA, 256 columns of K a box; sixteen warps turn them into 16-bit values in tensor memory, 64 columns a
 // group of four warps; the MMAs take them from there as their A operand, activations from shared memory.
-// gemm4 (4-bit activations): both operands' codes come through TMA and are multiplied as they are (kind::mxf4); eight warps bring the scales to tensor
-// memory.
+// gemm4 (4-bit activations): both operands' codes come through TMA and are multiplied as they are (kind::mxf4); so do the scales, which a kernel before
+// this one has put into the order in which they are copied on to tensor memory.
 #include "gemm_mxfp4.cuh"
 
 namespace {
@@ -180,7 +182,7 @@ __device__ __forceinline__ void teardown(bool ok, uint32_t tmem, int warp) {
 
 // ---- 16-bit activations ------------------------------------------------------------------------------
 constexpr int BOXES = 4, GROUPS = 4;          // boxes of codes in flight; groups of four warps, one for each of a box's four K blocks
-constexpr int PARTS = 2, A_STAGES = GROUPS / PARTS, X_STAGES = 3;       // K blocks a stage; stages of values (tensor memory) and of activations
+constexpr int PARTS = 2, X_STAGES = 3;       // K blocks a stage; stages of activations (of values, in tensor memory: a K block a group)
 constexpr int THREADS16 = 256 + 128 * GROUPS;        // warps 0: activations, 1, 3: MMAs, 2: codes, 4..7: rows' references and epilogue, 8..23: values
 constexpr int X16_BYTES = MAX_BN * KB * 2;   // of a K block
 constexpr int SMEM16 = BOXES * CODE_BYTES + X_STAGES * PARTS * X16_BYTES + 1024;
@@ -191,7 +193,7 @@ gemm16_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__
     uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
     uint8_t* sW = smem;
     uint8_t* sX = smem + BOXES * CODE_BYTES;
-    __shared__ uint64_t w_full[BOXES], w_empty[BOXES], x_full[X_STAGES], x_empty[X_STAGES], a_full[A_STAGES], a_empty[A_STAGES];
+    __shared__ uint64_t w_full[BOXES], w_empty[BOXES], x_full[X_STAGES], x_empty[X_STAGES], a_full[GROUPS / PARTS], a_empty[GROUPS];
     __shared__ Rings d;
     __shared__ uint32_t tmem_base_smem;
 #ifdef TNX_F16
@@ -204,7 +206,8 @@ gemm16_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__
     if (threadIdx.x == 0) {
         for (int i = 0; i < BOXES; ++i) { mbar_init(&w_full[i], 1); mbar_init(&w_empty[i], 4 * GROUPS); }
         for (int i = 0; i < X_STAGES; ++i) { mbar_init(&x_full[i], 1); mbar_init(&x_empty[i], 1); }
-        for (int i = 0; i < A_STAGES; ++i) { mbar_init(&a_full[i], 4 * PARTS); mbar_init(&a_empty[i], 1); }
+        for (int i = 0; i < GROUPS; ++i) mbar_init(&a_empty[i], 1);
+        for (int i = 0; i < GROUPS / PARTS; ++i) mbar_init(&a_full[i], 4 * PARTS);
         for (int i = 0; i < 2; ++i) { mbar_init(&d.full[i], 2); mbar_init(&d.empty[i], 4); }
 #ifdef TNX_F16
         for (int i = 0; i < 2; ++i) { mbar_init(&ref_full[i], 4); mbar_init(&ref_empty[i], 4 * GROUPS); }
@@ -263,30 +266,30 @@ gemm16_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__
         uint32_t passes = 0u;                             // of the places of values, a bit each
         int it = 0, i = 0;
         for (int n = 0; n < total; ++n) {
-            const int place = i % A_STAGES;
+            const int place = i * PARTS % GROUPS, parts = min(PARTS, num - i * PARTS);
             if ((n & 1) == who) {
-                // (an odd tile's last stage stands in the same place, so it has to be the turn of this one before its barrier tells anything)
+                // (a tile's last stage may have had the same place, so it has to be the turn of this one before its barrier tells anything)
                 const bool early = i == 0 && n > 0;
                 if (early) await_turn(who);
                 if (ok && it >= 2 && i < 2) ok = mbar_wait(&d.empty[it & 1], (uint32_t)((it >> 1) - 1) & 1u, p.err, 94);
-                ok = ok && mbar_wait(&x_full[r.slot], r.pass, p.err, 95) && mbar_wait(&a_full[place], (passes >> place) & 1u, p.err, 96);
+                ok = ok && mbar_wait(&x_full[r.slot], r.pass, p.err, 95) && mbar_wait(&a_full[place / PARTS], (passes >> place) & 1u, p.err, 96);
                 ok = __all_sync(0xffffffffu, ok);
                 if (n && !early) await_turn(who);
                 tc_fence_after();
                 const uint32_t acc = tmem_d + (it & 1 ? MAX_BN : 0);
-                const int parts = min(PARTS, num - i * PARTS);
                 const uint64_t bdesc = desc0 + (uint64_t)(r.slot * (PARTS * X16_BYTES >> 4));
-                const uint32_t a = tmem_a + (uint32_t)(place * 32 * PARTS);
+                const uint32_t a = tmem_a + (uint32_t)(place * 32);
                 if (ok && elected()) {
 #pragma unroll
                     for (int j = 0; j < PARTS; ++j) {
-                        if (j >= parts) break;
+                        if (j < parts) {
 #pragma unroll
-                        for (int k = 0; k < KB / 16; ++k)
-                            umma_a_tmem(acc, a + (uint32_t)(32 * j + 8 * k), bdesc + (uint64_t)(j * (X16_BYTES >> 4) + 2 * k), idesc, (i > 0 || j > 0 || k > 0) ? 1u : 0u);
+                            for (int k = 0; k < KB / 16; ++k)
+                                umma_a_tmem(acc, a + (uint32_t)(32 * j + 8 * k), bdesc + (uint64_t)(j * (X16_BYTES >> 4) + 2 * k), idesc, (i > 0 || j > 0 || k > 0) ? 1u : 0u);
+                        }
+                        umma_commit(&a_empty[place + j]);
                     }
                     umma_commit(&x_empty[r.slot]);
-                    umma_commit(&a_empty[place]);
                     if (i >= stages - 2) umma_commit(&d.full[it & 1]);
                     if (stages == 1) umma_commit(&d.full[it & 1]);
                 }
@@ -362,9 +365,9 @@ gemm16_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__
 #endif
         });
     } else {
-        // Values: a thread owns a row, group j takes K block j of every box and so always fills the same place in tensor memory, where a tile's even (or
-        // odd) stages stand: a group that changed places between tiles of an odd number of stages would not see all of a place's turns, of which
-        // a barrier tells only every other apart.
+        // Values: a thread owns a row, group j takes K block j of every box and keeps a place of its own in tensor memory, which is free as soon as that K
+        // block's four MMAs are done.  (Places that the groups took in turn: a group that did not see all of a place's turns, of which a barrier tells
+        // only every other apart, could overwrite values in use.)
         const int quad = warp & 3, group = (warp - 8) >> 2, r = quad * 32 + lane;
         const bool even = p.blocks % 2 == 0 && ((uintptr_t)p.scales & 1) == 0;
         // The two scales of this group's K block, asked for four boxes ahead (a trip to memory takes longer than a box), over the tiles' ends.
@@ -386,7 +389,7 @@ gemm16_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__
 #pragma unroll
         for (int j = 0; j < 4; ++j) ahead[j] = load_scales();
         const int total = (p.tiles - (int)blockIdx.x + (int)gridDim.x - 1) / (int)gridDim.x * boxes;
-        int box = 0, it = 0, ref = 0, use = 0;            // use: stages that this group has filled
+        int box = 0, it = 0, ref = 0, use = 0;            // use: K blocks that this group has filled
         for (int g0 = 0; g0 < total && ok; g0 += 4) {
 #pragma unroll
             for (int u = 0; u < 4; ++u) {
@@ -405,10 +408,10 @@ gemm16_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__
 #endif
                 ok = __all_sync(0xffffffffu, mbar_wait(&w_full[ws], (uint32_t)(g / BOXES) & 1u, p.err, 100));
                 if (!ok) break;
-                const int i = box * 4 + group, stage = box * A_STAGES + group / PARTS;
+                const bool has = box * 4 + group < num, stage = box * 4 + group / PARTS * PARTS < num;       // the tile's last box may end before them
                 if (++box == boxes) { box = 0; ++it; }
                 uint32_t v[32];
-                if (i < num) {
+                if (has) {
                     const uint32_t row_addr = smem_u32(sW + ws * CODE_BYTES) + (uint32_t)r * 128u;
                     uint4 q[2];
 #pragma unroll
@@ -427,21 +430,20 @@ gemm16_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__
                 }
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&w_empty[ws]);                 // this warp has read its share of the box
-                if (stage >= stages) continue;                            // the tile's last box ends before this stage
-                const int s = group / PARTS;
+                if (!stage) continue;
                 if (use > 0) {
-                    ok = __all_sync(0xffffffffu, mbar_wait(&a_empty[s], (uint32_t)(use - 1) & 1u, p.err, 101));
+                    ok = __all_sync(0xffffffffu, mbar_wait(&a_empty[group], (uint32_t)(use - 1) & 1u, p.err, 101));
                     if (!ok) break;
                     tc_fence_after();
                 }
                 ++use;
-                if (i < num) {
-                    tmem_st32(tmem_a + (uint32_t)(s * 32 * PARTS + group % PARTS * 32) + ((uint32_t)(quad * 32) << 16), v);
+                if (has) {
+                    tmem_st32(tmem_a + (uint32_t)(group * 32) + ((uint32_t)(quad * 32) << 16), v);
                     tmem_st_wait();
                 }
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&a_full[s]);
+                if (lane == 0) mbar_arrive(&a_full[group / PARTS]);
             }
         }
     }
