@@ -646,9 +646,9 @@ TNX_EXPORT long long tnx_gemm_mxfp4_estimate(int M, int N, int K, int gated, int
     const int r = quantized ? launch4<128, 4, 1>(nullptr, nullptr, p, tiles_w, n_sms, nullptr, &boxes)
                             : launch16<128, 2, 4>(nullptr, 0, nullptr, K, p, tiles_w, out_h16 ? 0 : MX_CHAIN, n_sms, nullptr, &boxes);
     if (r) return 1ll << 60;
-    // a box takes 650 (4-bit activations) or 1,150 ns; what a CTA costs beside them is 4.5 and 5 us
+    // a box takes 650 (4-bit activations) or 1,150 ns; what a CTA costs beside them is 6.5 us, with 4-bit activations 0.3 more for every part of a sum
     const long long rounds = (boxes - p.splits) / (p.boxes_per_split + (quantized ? FIXED4 : FIXED16));
-    return rounds * (p.boxes_per_split * (quantized ? 650ll : 1150ll) + (quantized ? 4500 : 5000));
+    return rounds * (p.boxes_per_split * (quantized ? 650ll : 1150ll) + 6500 + (quantized ? 300 * p.splits : 0));
 }
 
 // The most columns of K for whose 32-bit sums a tile's one accumulator is near enough (gemm_mxfp4_tiles.cu has one a tile).

@@ -661,7 +661,7 @@ TNX_EXPORT long long tnx_gemm_mxfp4_tiles_estimate(int M, int N, int K, int gate
     const int tiles_w = gated ? (N + 63) / 64 : (N + TILE_W - 1) / TILE_W;
     plan(p, n_sms, tiles_w, quantized ? 430 : 360);
     const long long rounds = ((long long)p.tiles + n_sms - 1) / n_sms;
-    return quantized ? rounds * ((K + CODE_K - 1) / CODE_K) * (300 + p.bn * 7 / 10) + 8000 : rounds * ((K + 127) / 128) * (500 + p.bn * 14 / 10) + 6000;
+    return quantized ? rounds * ((K + CODE_K - 1) / CODE_K) * (300 + p.bn * 7 / 10) + 6500 : rounds * ((K + 127) / 128) * (500 + p.bn * 14 / 10) + 5000;
 }
 
 // For sweeps: the tokens of a tile (a multiple of 16 from 64 to 192) whatever the sizes (0: the plan's own).
