@@ -15,30 +15,75 @@ __device__ __forceinline__ uint32_t pack_e2m1x8(const float (&v)[8]) {
     return r;
 }
 
-// Four neighbouring lanes hold a block, eight values each.  The block's exponent is the smallest e with max |x| <= 6 * 2^e, read off the
-// largest value's bits: m = 1.f * 2^x needs e = x - 2 up to f = 1.5 and x - 1 beyond.  Bits compared as whole numbers put infinities and
-// NaN above every finite value, so one comparison finds them.  x * 2^-e is exact (or far below the smallest code), its conversion rounds
-// to the nearest code, ties to even.
-__device__ __forceinline__ uint32_t quantize8(const float (&v)[8], uint32_t& E) {
+// The bits of the largest magnitude of eight values, as a 32-bit float's.  Bits compared as whole numbers put infinities and NaN above every finite value, so
+// one comparison finds them.  16-bit values are compared two at a time; four neighbouring lanes hold a block.
+__device__ __forceinline__ uint32_t block_max(const Vec8<float>& q) {
+    float v[8];
+    q.get(v);
     uint32_t m = 0;
 #pragma unroll
     for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(v[i]) & 0x7FFFFFFFu);
     m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
-    m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
+    return max(m, __shfl_xor_sync(0xffffffffu, m, 2));
+}
+__device__ __forceinline__ uint32_t block_max(const Vec8<h16>& q) {
+    const uint32_t s = 0x7FFF7FFFu;
+    uint32_t m = __vmaxu2(__vmaxu2(q.raw.x & s, q.raw.y & s), __vmaxu2(q.raw.z & s, q.raw.w & s));
+    m = __vmaxu2(m, __shfl_xor_sync(0xffffffffu, m, 1));
+    m = __vmaxu2(m, __shfl_xor_sync(0xffffffffu, m, 2));
+    m = max(m & 0xFFFFu, m >> 16);
+#ifdef TNX_F16
+    return __float_as_uint(h16_to_float(__ushort_as_half((unsigned short)m)));
+#else
+    return m << 16;
+#endif
+}
+
+// Eight values times 2^-e, exactly (or far below the smallest code).
+__device__ __forceinline__ void scaled(const Vec8<float>& q, float by, float (&s)[8]) {
+    q.get(s);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) s[i] *= by;
+}
+__device__ __forceinline__ void scaled(const Vec8<h16>& q, float by, float (&s)[8]) {
+#ifdef TNX_F16
+    q.get(s);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) s[i] *= by;
+#else
+    // bfloat16 halves as operands of a 32-bit multiply-add: nothing to unpack; -0 added leaves the sign of a zero alone
+    const uint32_t w[4] = {q.raw.x, q.raw.y, q.raw.z, q.raw.w};
+    const unsigned short b = (unsigned short)(__float_as_uint(by) >> 16);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        asm("{\n\t.reg .b16 l, h;\n\t"
+            "mov.b32 {l, h}, %2;\n\t"
+            "fma.rn.f32.bf16 %0, l, %3, %4;\n\t"
+            "fma.rn.f32.bf16 %1, h, %3, %4;\n\t}"
+            : "=f"(s[2 * i]), "=f"(s[2 * i + 1]) : "r"(w[i]), "h"(b), "f"(-0.f));
+#endif
+}
+
+// The block's exponent is the smallest e with max |x| <= 6 * 2^e, read off the largest value's bits: m = 1.f * 2^x needs e = x - 2 up to f = 1.5 and
+// x - 1 beyond.  The conversion of x * 2^-e rounds to the nearest code, ties to even.
+template <typename T>
+__device__ __forceinline__ uint32_t quantize8(const Vec8<T>& q, uint32_t& E) {
+    const uint32_t m = block_max(q);
     const int e = (int)(m >> 23) - 2 + ((m & 0x7FFFFFu) > 0x400000u ? 1 : 0);
     if (m >= 0x7F800000u) { E = 255u; return 0u; }
     E = (uint32_t)max(e, 0);
-    const float inv = __uint_as_float((254u - E) << 23);          // E <= 253 for finite values
     float s[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) s[i] = v[i] * inv;
+    scaled(q, __uint_as_float((254u - E) << 23), s);              // E <= 253 for finite values
     return pack_e2m1x8(s);
 }
 
 // Rows to 4 bits: one read of the values, one write of codes and scales; bound by memory.  `items` = rows * blocks * 4 pieces of eight values, whose
-// codes lie in their order.  FLAT: so do the values (whole blocks, no gap between rows, 16-byte aligned), and a thread asks for four pieces
+// codes lie in their order.  FLAT: so do the values (whole blocks, no gap between rows, 16-byte aligned), and a thread asks for several pieces
 // before it uses the first.  Otherwise a piece's row and column are worked out, and values are read one by one where 16 bytes at a time cannot be.
-constexpr int PIECES = 4;
+// 16,384 x 4,096 from bfloat16 29 us, 5.8 TB/s, from 32 bits 45, 6.7 TB/s of which the second-level cache keeps some (bfloat16 with one piece a thread
+// 32, three 32, four 37; with each value unpacked and compared alone, four pieces 42); back to bfloat16 28, to 32 bits 65 (two pieces 31 and 65,
+// four 28 and 70; 8 blocks an SM that walk 30 and 77).
+constexpr int TO_PIECES = 2, TO_BLOCKS = 16, BACK_PIECES = 3, BACK_BLOCKS = 128;          // pieces a thread, blocks an SM at most
 
 template <typename T, bool FLAT>
 __global__ void __launch_bounds__(256) quantize_kernel(const T* __restrict__ x, long long ld, uint32_t* __restrict__ codes, uint8_t* __restrict__ scales,
@@ -46,41 +91,49 @@ __global__ void __launch_bounds__(256) quantize_kernel(const T* __restrict__ x, 
     pdl_launch_dependents();             // the products read codes behind their own wait
     pdl_wait();
     const long long stride = (long long)gridDim.x * blockDim.x;
-    constexpr int U = FLAT ? PIECES : 1;
+    constexpr int U = FLAT ? TO_PIECES : 1;
     // whole warps walk the loop: the block's largest value is found by lanes together
     for (long long i0 = (long long)blockIdx.x * blockDim.x + (threadIdx.x & ~31u); i0 < items; i0 += stride * U) {
         const long long i = i0 + (threadIdx.x & 31u);
-        float v[U][8];
+        Vec8<T> q[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) q[u].zero();
         if (FLAT) {
-            Vec8<T> q[U];
 #pragma unroll
-            for (int u = 0; u < U; ++u) { q[u].zero(); if (i + u * stride < items) q[u].load(x + (i + u * stride) * 8); }
+            for (int u = 0; u < U; ++u) if (i + u * stride < items) q[u].load(x + (i + u * stride) * 8);
+        } else if (i < items) {
+            const long long row = i / (4 * blocks);
+            const int k = (int)(i - row * (4 * blocks)) * 8;
+            const T* src = x + row * ld + k;
+            if (vec && k + 8 <= K) q[0].load(src);
+            else {
+                T v[8];
 #pragma unroll
-            for (int u = 0; u < U; ++u) q[u].get(v[u]);
-        } else {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) v[0][j] = 0.f;
-            if (i < items) {
-                const long long row = i / (4 * blocks);
-                const int k = (int)(i - row * (4 * blocks)) * 8;
-                const T* src = x + row * ld + k;
-                if (vec && k + 8 <= K) { Vec8<T> q; q.load(src); q.get(v[0]); }
-                else {
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) if (k + j < K) v[0][j] = to_float(src[j]);
-                }
+                for (int j = 0; j < 8; ++j) v[j] = k + j < K ? src[j] : from_float<T>(0.f);
+                memcpy(&q[0], v, sizeof v);
             }
         }
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const long long at = i + u * stride;
             uint32_t E;
-            const uint32_t c = quantize8(v[u], E);
+            const uint32_t c = quantize8(q[u], E);
             if (at < items) {
                 codes[at] = c;
                 if ((at & 3) == 0) scales[at >> 2] = (uint8_t)E;
             }
         }
+    }
+}
+
+// Eight codes as 32-bit numbers, without a scale.
+__device__ __forceinline__ void codes_to_float(uint32_t w, float (&v)[8]) {
+    uint32_t h[4];
+    codes_to_f16(w, h);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const float2 f = __half22float2(*(const __half2*)&h[j]);
+        v[2 * j] = f.x; v[2 * j + 1] = f.y;
     }
 }
 
@@ -91,7 +144,7 @@ __global__ void __launch_bounds__(256) dequantize_kernel(const uint32_t* __restr
                                                          long long items, int blocks, int K, int vec) {
     pdl_wait();
     const long long stride = (long long)gridDim.x * blockDim.x;
-    constexpr int U = FLAT ? PIECES : 1;
+    constexpr int U = FLAT ? BACK_PIECES : 1;
     for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < items; i += stride * U) {
         uint32_t c[U], E[U];
 #pragma unroll
@@ -106,8 +159,9 @@ __global__ void __launch_bounds__(256) dequantize_kernel(const uint32_t* __restr
             if (at >= items) break;
             const float s = mx_scale(E[u]);
             float v[8];
+            codes_to_float(c[u], v);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] = mx_code(c[u] >> (4 * j)) * s;
+            for (int j = 0; j < 8; ++j) v[j] *= s;
             if (FLAT) {
                 Vec8<T> q;
                 q.set(v);
@@ -198,10 +252,10 @@ __global__ void __launch_bounds__(32 * SIMT_WARPS) simt_kernel(const SimtParams 
     }
 }
 
-// Blocks of 256 threads: enough for one piece a thread, at most eight an SM.
-inline unsigned grid_for(long long items, int pieces, int sms) {
-    const long long want = (items + 256 * pieces - 1) / (256 * pieces), most = (long long)sms * 8;
-    return (unsigned)(want < most ? want : most);
+// Blocks of 256 threads, `most` an SM at most.
+inline unsigned grid_for(long long items, int pieces, int most, int sms) {
+    const long long want = (items + 256 * pieces - 1) / (256 * pieces), limit = (long long)sms * most;
+    return (unsigned)(want < limit ? want : limit);
 }
 
 template <typename T>
@@ -211,9 +265,9 @@ int launch_quantize(const void* x, long long ld, void* codes, void* scales, int 
     const int vec = ld % 8 == 0 && ((uintptr_t)x & 15) == 0;
     // a few rows: a piece a thread, so that all SMs have some
     if (vec && K % MX_BLOCK == 0 && (ld == K || rows == 1))
-        return tnx_launch_ex(1, quantize_kernel<T, true>, dim3(grid_for(items, items > 256ll * 8 * sms ? PIECES : 1, sms)), dim3(256), 0, stream, (const T*)x, ld,
+        return tnx_launch_ex(1, quantize_kernel<T, true>, dim3(grid_for(items, items > 256ll * 8 * sms ? TO_PIECES : 1, TO_BLOCKS, sms)), dim3(256), 0, stream, (const T*)x, ld,
                              (uint32_t*)codes, (uint8_t*)scales, items, blocks, K, vec);
-    return tnx_launch_ex(1, quantize_kernel<T, false>, dim3(grid_for(items, 1, sms)), dim3(256), 0, stream, (const T*)x, ld, (uint32_t*)codes,
+    return tnx_launch_ex(1, quantize_kernel<T, false>, dim3(grid_for(items, 1, TO_BLOCKS, sms)), dim3(256), 0, stream, (const T*)x, ld, (uint32_t*)codes,
                          (uint8_t*)scales, items, blocks, K, vec);
 }
 
@@ -223,9 +277,9 @@ int launch_dequantize(const void* codes, const void* scales, void* out, long lon
     const long long items = (long long)rows * blocks * 4;
     const int vec = ld % 8 == 0 && ((uintptr_t)out & 15) == 0;
     if (vec && K % MX_BLOCK == 0 && (ld == K || rows == 1))
-        return tnx_launch_ex(1, dequantize_kernel<T, true>, dim3(grid_for(items, items > 256ll * 8 * sms ? PIECES : 1, sms)), dim3(256), 0, stream,
+        return tnx_launch_ex(1, dequantize_kernel<T, true>, dim3(grid_for(items, items > 256ll * 8 * sms ? BACK_PIECES : 1, BACK_BLOCKS, sms)), dim3(256), 0, stream,
                              (const uint32_t*)codes, (const uint8_t*)scales, (T*)out, ld, items, blocks, K, vec);
-    return tnx_launch_ex(1, dequantize_kernel<T, false>, dim3(grid_for(items, 1, sms)), dim3(256), 0, stream, (const uint32_t*)codes, (const uint8_t*)scales,
+    return tnx_launch_ex(1, dequantize_kernel<T, false>, dim3(grid_for(items, 1, BACK_BLOCKS, sms)), dim3(256), 0, stream, (const uint32_t*)codes, (const uint8_t*)scales,
                          (T*)out, ld, items, blocks, K, vec);
 }
 

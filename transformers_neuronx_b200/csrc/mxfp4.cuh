@@ -27,6 +27,17 @@ __device__ __forceinline__ float mx_code(uint32_t c) {
     return __uint_as_float(((c & 8u) << 28) | ((c & 7u) << 22)) * 8.507059173023462e37f;
 }
 
+// Eight codes as eight float16 numbers, without a scale.
+__device__ __forceinline__ void codes_to_f16(uint32_t w, uint32_t (&o)[4]) {
+    asm("{\n\t.reg .b8 b0, b1, b2, b3;\n\t"
+        "mov.b32 {b0, b1, b2, b3}, %4;\n\t"
+        "cvt.rn.f16x2.e2m1x2 %0, b0;\n\t"
+        "cvt.rn.f16x2.e2m1x2 %1, b1;\n\t"
+        "cvt.rn.f16x2.e2m1x2 %2, b2;\n\t"
+        "cvt.rn.f16x2.e2m1x2 %3, b3;\n\t}"
+        : "=r"(o[0]), "=r"(o[1]), "=r"(o[2]), "=r"(o[3]) : "r"(w));
+}
+
 __device__ __forceinline__ uint32_t mul_h16x2(uint32_t a, uint32_t b) {
     h16x2 r = __hmul2(*(h16x2*)&a, *(h16x2*)&b);
     return *(uint32_t*)&r;
@@ -48,13 +59,7 @@ struct MxValues {
     }
     __device__ __forceinline__ void decode8(uint32_t w, uint32_t* o) const {
         uint32_t c[4];
-        asm("{\n\t.reg .b8 b0, b1, b2, b3;\n\t"
-            "mov.b32 {b0, b1, b2, b3}, %4;\n\t"
-            "cvt.rn.f16x2.e2m1x2 %0, b0;\n\t"
-            "cvt.rn.f16x2.e2m1x2 %1, b1;\n\t"
-            "cvt.rn.f16x2.e2m1x2 %2, b2;\n\t"
-            "cvt.rn.f16x2.e2m1x2 %3, b3;\n\t}"
-            : "=r"(c[0]), "=r"(c[1]), "=r"(c[2]), "=r"(c[3]) : "r"(w));
+        codes_to_f16(w, c);
 #pragma unroll
         for (int j = 0; j < 4; ++j) o[j] = mul_h16x2(c[j], s);
     }
