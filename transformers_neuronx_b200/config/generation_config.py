@@ -4,7 +4,7 @@
 (src/transformers_neuronx/config.py:106-131) with the same defaults and meanings;
 `NeuronConfig(on_device_generation=GenerationConfig(...))` is how a caller of the reference hands it to
 a model (config.py:220, opt/model.py:47-48, :187-189).  Every other option of the reference's
-NeuronConfig describes its compiler, its tensor layouts, quantization or several devices; they are
+NeuronConfig, but for those that the class here names, describes its compiler, its tensor layouts or several devices; they are
 accepted and reported as ignored.
 """
 from __future__ import annotations
