@@ -76,6 +76,11 @@ __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
+// Eight bytes to shared memory, the first n of them from src, the others zero; cp.async.wait_all waits for them.
+__device__ __forceinline__ void copy8_async(void* dst, const void* src, uint32_t n) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(n) : "memory");
+}
+
 // Eight activations of a token from column k on, as they lie in memory.
 struct Raw { uint4 a, b; };
 __device__ __forceinline__ Raw load_raw(const Params& p, int token, int k) {
@@ -210,21 +215,22 @@ __global__ void __launch_bounds__(32 * (MAX_WARPS + 1), 1) gemv_kernel(const __g
         for (int f0 = 0; f0 < per; f0 += p.phase) {
             if (f0) asm volatile("bar.sync 1, %0;" ::"r"(32 * warps) : "memory");
             const int len = min(p.phase, per - f0);       // boxes of a share
-            // W's scales, as they lie in memory: a trip there for every box would take longer than the box.
+            // W's scales, as they lie in memory: a trip there for every box would take longer than the box.  Copied without waiting for each: a thread
+            // has several, whose trips one after the other took 3 to 4 us.
             for (int q = threadIdx.x; q < 16 * p.wf * p.wk * len; q += 32 * warps) {
                 const int row = q / (p.wk * len), rest = q - row * (p.wk * len), share = rest / len, f = rest - share * len;
                 const int w_row = min(row < 8 * p.wf ? first + row : (p.gated ? p.N + first : first + 8 * p.wf) + row - 8 * p.wf, p.w_rows - 1);
                 const int blk = (s_begin + share * per + f0 + f) * SLOT_BLOCKS;
                 const uint8_t* src = p.scales + (long long)w_row * p.blocks + blk;
-                uint2 v = make_uint2(0u, 0u);
-                if (p.words) {
-                    if (blk < p.blocks) v = __ldg((const uint2*)src);
-                } else {
+                uint8_t* to = sw + row * p.sw_ld + (share * p.phase + f) * 8;
+                if (p.words) copy8_async(to, blk < p.blocks ? src : p.scales, blk < p.blocks ? 8u : 0u);
+                else {
+                    uint2 v = make_uint2(0u, 0u);
 #pragma unroll
                     for (int j = 0; j < 8; ++j)
                         if (blk + j < p.blocks) { const uint32_t E = (uint32_t)__ldg(src + j) << (8 * (j & 3)); if (j < 4) v.x |= E; else v.y |= E; }
+                    *(uint2*)to = v;
                 }
-                *(uint2*)(sw + row * p.sw_ld + (share * p.phase + f) * 8) = v;
             }
             // A warp brings a token's share of a box, a lane eight columns; four boxes are asked for before the first is used.
             const int units = len * p.wk * p.M;
@@ -249,6 +255,7 @@ __global__ void __launch_bounds__(32 * (MAX_WARPS + 1), 1) gemv_kernel(const __g
                     if (SCALED && lane == 0) sx[at[j] * (NT * 8) + tok[j]] = scale;
                 }
             }
+            asm volatile("cp.async.wait_all;" ::: "memory");
             asm volatile("bar.sync 1, %0;" ::"r"(32 * warps) : "memory");
             const int last = min(e, b + f0 + len);
             uint32_t xb = smem_u32(xs) + (uint32_t)(wk * p.phase * BOX_X + lane) * 16u;
