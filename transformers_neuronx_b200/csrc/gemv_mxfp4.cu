@@ -81,6 +81,10 @@ __device__ __forceinline__ void copy8_async(void* dst, const void* src, uint32_t
     asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(n) : "memory");
 }
 
+__device__ __forceinline__ void copy16_async(void* dst, const void* src, uint32_t n) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(n) : "memory");
+}
+
 // Eight activations of a token from column k on, as they lie in memory.
 struct Raw { uint4 a, b; };
 __device__ __forceinline__ Raw load_raw(const Params& p, int token, int k) {
@@ -232,9 +236,20 @@ __global__ void __launch_bounds__(32 * (MAX_WARPS + 1), 1) gemv_kernel(const __g
                     *(uint2*)to = v;
                 }
             }
-            // A warp brings a token's share of a box, a lane eight columns; four boxes are asked for before the first is used.
+            // A warp brings a token's share of a box, a lane eight columns; float16 values are copied as they are, of others four boxes are asked for
+            // before the first is used.
             const int units = len * p.wk * p.M;
-            for (int q0 = warp; q0 < units; q0 += 4 * warps) {
+            int q0 = warp;
+            if (!SCALED && p.a_vec) {
+                for (; q0 < units; q0 += warps) {
+                    const int box = q0 / p.M, share = box / len, f = box - share * len, token = q0 - box * p.M;
+                    const int k = (s_begin + share * per + f0 + f) * SLOT_K + lane * 8;
+                    uint4* to = xs + (share * p.phase + f) * BOX_X + (lane >> 2) * BLOCK_X + token * 4 + (lane & 3);
+                    if (k < p.K && k + 8 > p.K) *to = load_raw(p, token, k).a;
+                    else copy16_async(to, k < p.K ? (const h16*)p.a + token * p.lda + k : (const h16*)p.a, k < p.K ? 16u : 0u);
+                }
+            }
+            for (; q0 < units; q0 += 4 * warps) {
                 Raw raw[4];
                 int at[4], tok[4];
 #pragma unroll
