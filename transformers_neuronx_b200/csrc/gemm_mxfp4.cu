@@ -301,21 +301,38 @@ gemm16_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__
         {
             const bool wide = p.blocks % 8 == 0 && ((uintptr_t)p.scales & 7) == 0;
             const int n = blk_end - blk0, t = (warp - 4) * 32 + lane;
-            for (int row = t >> 3; row < TILE_W; row += 16 * GROUPS16) {
-                const uint8_t* q = p.scales + (long long)tile_row(p.e, row0, row, p.w_rows) * p.blocks + blk0;
-                int m = 0;
-                if (wide)
-                    for (int j = (t & 7) * 8; j < n; j += 64) {
-                        const uint2 v = __ldg((const uint2*)(q + j));
+            static_assert(2 * 16 * GROUPS16 == TILE_W, "eight threads a row, two rows each");
+            const uint8_t* q[2];
+            int m[2] = {0, 0};
 #pragma unroll
-                        for (int k = 0; k < 8; ++k) { const int E = (int)(((k < 4 ? v.x : v.y) >> (8 * (k & 3))) & 255u); if (E < 255) m = max(m, E); }
-                    }
-                else
-                    for (int j = t & 7; j < n; j += 8) { const int E = __ldg(q + j); if (E < 255) m = max(m, E); }
-                m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
-                m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
-                m = max(m, __shfl_xor_sync(0xffffffffu, m, 4));
-                if ((t & 7) == 0) row_ref[row] = m;
+            for (int h = 0; h < 2; ++h) q[h] = p.scales + (long long)tile_row(p.e, row0, (t >> 3) + h * (TILE_W / 2), p.w_rows) * p.blocks + blk0;
+            if (wide) {
+#pragma unroll 4
+                for (int j = (t & 7) * 8; j < n; j += 64) {
+                    uint2 v[2];
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) v[h] = __ldg((const uint2*)(q[h] + j));
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) { const int E = (int)(((k < 4 ? v[h].x : v[h].y) >> (8 * (k & 3))) & 255u); if (E < 255) m[h] = max(m[h], E); }
+                }
+            } else {
+#pragma unroll 4
+                for (int j = t & 7; j < n; j += 8) {
+                    int E[2];
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) E[h] = __ldg(q[h] + j);
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) if (E[h] < 255) m[h] = max(m[h], E[h]);
+                }
+            }
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                m[h] = max(m[h], __shfl_xor_sync(0xffffffffu, m[h], 1));
+                m[h] = max(m[h], __shfl_xor_sync(0xffffffffu, m[h], 2));
+                m[h] = max(m[h], __shfl_xor_sync(0xffffffffu, m[h], 4));
+                if ((t & 7) == 0) row_ref[(t >> 3) + h * (TILE_W / 2)] = m[h];
             }
             asm volatile("bar.sync 1, %0;" ::"n"(128 * GROUPS16) : "memory");
             ref = row_ref[r];

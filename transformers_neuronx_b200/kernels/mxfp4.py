@@ -314,7 +314,7 @@ def _product(a, w, out, bias, residual, activation, gated):
     few = w_p % 16 == 0 and (a_kind != 2 or a_p % 4 == 0)
     tensor = (a_p | w_p) % 16 == 0 and (a_kind == 2 or (a_kind == 0 and lda % 8 == 0 and lda >= K))
     # 4-bit activations are always faster on the tensor cores (one to 16 tokens by 16,384 x 4,096 9 us, 13 to 27 streamed), 16-bit ones from nine tokens
-    # on (8 tokens by 16,384 x 4,096 14 to 16 us streamed, 17 to 20 on the tensor cores, 12 tokens 19 to 22 and 17 to 20; by 2,304 x 768 5 to 6 and 6,
+    # on (8 tokens by 16,384 x 4,096 13 to 16 us streamed, 17 to 20 on the tensor cores, 12 tokens 19 to 22 and 17 to 20; by 2,304 x 768 5 to 6 and 6,
     # then 6 to 7.6 and 6); 32-bit ones are streamed, 16 tokens at a time
     if few and (not tensor or (a_kind == 0 and M <= 8)) and (M <= FEW_TOKENS or a_kind == 1):
         code = _entry("gemv_mxfp4", "tnx_gemv_mxfp4", kind)(_PACK[19](a_p, a_kind, as_p, lda, *tail, sms, err, _stream(device)))
