@@ -9,8 +9,9 @@
 //
 // gemm16 (16-bit activations): W's codes come through TMA into shared memory, 256 columns of K a box; sixteen warps turn them into 16-bit
 // values and put those into tensor memory, whence the MMAs take them as their A operand; activations come through TMA.  That turning is what
-// bounds it, 0.75 us a box, beside 5 us a CTA has before its first box and behind its last: 24 tokens by 16,384 x 4,096 17.5 us (float16) and 20
-// (bfloat16, whose values take more instructions), 13 by 5,120 x 20,480 28 and 32 (1.9 and 1.7 TB/s), 128 by 2,048 x 8,192 15.
+// bounds it, 0.75 us a box, beside 5 us a CTA has before its first box and behind its last: 16 tokens by 16,384 x 4,096 17 us (float16) and 20.5
+// (bfloat16, whose values take more instructions), 14.7 and 13.4 without it, 13 and 11.4 also without MMAs; 13 by 5,120 x 20,480 27.5 and 31.5
+// (2 and 1.8 TB/s), 128 by 2,048 x 8,192 15.  (Two warps that issue the MMAs in turn, as in gemm_mxfp4_tiles.cu, changed nothing here.)
 //
 // gemm4 (activations in 4 bits too): both operands' codes come through TMA, 256 columns of K a stage, and are multiplied as they are
 // (tcgen05.mma kind::mxf4, a scale for 32 columns of K).  The MMAs read scales from tensor memory, where lane l of every quarter holds the
