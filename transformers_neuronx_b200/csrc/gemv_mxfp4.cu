@@ -13,7 +13,8 @@
 //
 // Activations are float16 operands too: float16 as they are, others divided by a power of two that brings the largest of a box's 256 to
 // 2^14..2^15, in one term (bfloat16's eight bits and 4-bit values fit) or three (32 bits).  What is lost is below 2^-39 of the largest of
-// the 256, where float16 ends.
+// the 256, where float16 ends.  A block's sum of such operands may reach 2^23, so a box with a scale byte of 228 (2^101) or more takes another way, on
+// which the sum meets both powers of two as one: multiplied by the block's alone it could leave 32 bits where the result does not.
 //
 // The warps of a block: wf groups of 16 rows by wk shares of K, whose sums meet in shared memory; K may be split further over the blocks of a
 // cluster.  The plan chooses them so that one round of blocks, one an SM, covers the GPU as evenly as the sizes allow.
@@ -56,6 +57,18 @@ __device__ __forceinline__ uint4 lds128(uint32_t a) {
     return v;
 }
 __device__ __forceinline__ float2 lds_f2(uint32_t a) { float2 v; asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(a)); return v; }
+
+// The sums of a block of 32 columns: a lane's eight columns of two rows by eight tokens' activations, which lie at `at`, their terms x_term bytes apart.
+template <int TERMS>
+__device__ __forceinline__ void block_sums(float (&c)[4], const uint32_t (&A)[4], const uint32_t (&B)[4], uint32_t at, uint32_t x_term) {
+#pragma unroll
+    for (int k = 0; k < TERMS; ++k) {
+        const uint4 x = lds128(at + k * x_term);
+        if (k == 0) mma_first(c, A[0], B[0], A[1], B[1], x.x, x.y);
+        else mma(c, A[0], B[0], A[1], B[1], x.x, x.y);
+        mma(c, A[2], B[2], A[3], B[3], x.z, x.w);
+    }
+}
 
 __device__ __forceinline__ uint32_t pack_f16(float a, float b) {
     const __half2 r = __floats2half2_rn(a, b);
@@ -166,6 +179,14 @@ __device__ __forceinline__ void make_terms(const Params& p, const Raw& r, uint4 
 __device__ __forceinline__ float scale_at(uint32_t w, int at) {
     const float f = __uint_as_float(max((at < 3 ? w << (23 - 8 * at) : w >> 1) & 0x7F800000u, 0x00400000u));
     return fmaf(f, 0.f, f);
+}
+
+// c * 2^(E - 127) * f, f a power of two from 2^-127 to 2^114, rounded once at the most: the two exponents are added up and applied in halves of one sign,
+// so that what lies between c and the result is no larger and no smaller than both.
+constexpr uint32_t HIGH_SCALE = 228u;        // eight blocks' sums, 2^26, times a smaller scale stay in 32 bits
+__device__ __forceinline__ float times_powers(float c, uint32_t E, float f) {
+    const int e = (int)E - 254 + (int)(__float_as_uint(f) >> 23), h = e >> 1;            // -254 .. 241
+    return c * mx_scale(E == 255u ? 255u : (uint32_t)(h + 127)) * mx_scale((uint32_t)(e - h + 127));
 }
 
 // NT: groups of eight tokens; SCALED: the activations have scales.  Warps 0 .. wf * wk - 1 multiply, the last one fetches codes.
@@ -289,6 +310,30 @@ __global__ void __launch_bounds__(32 * (MAX_WARPS + 1), 1) gemv_kernel(const __g
                 if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&full[wk][place], pass, p.err, 81));
                 if (!ok) break;
                 const uint32_t row = ring + (uint32_t)(place * box_bytes);
+                auto release = [&]() {                               // the box has been read
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&empty[wk][place]);
+                    if (++place == AHEAD) { place = 0; pass ^= 1u; }
+                };
+                if (SCALED && __any_sync(0xffffffffu, ((two & 0x7F7F7F7Fu) + 0x01010101u * (256u - HIGH_SCALE)) & two & 0x80808080u)) {
+#pragma unroll 1
+                    for (int i = 0; i < SLOT_BLOCKS; ++i) {
+                        uint32_t A[4], B[4];
+                        codes_to_f16(lds32(row + (uint32_t)((i ^ g) << 4)), A);
+                        codes_to_f16(lds32(row + (uint32_t)((i ^ g) << 4) + half), B);
+                        const uint32_t E = __shfl_sync(0xffffffffu, two, (lane & ~3) | (i >> 1)) >> (8 * (i & 1)), Ea = E & 255u, Eb = (E >> 16) & 255u;
+#pragma unroll
+                        for (int n = 0; n < NT; ++n) {
+                            float c[4];
+                            block_sums<TERMS>(c, A, B, xb + (uint32_t)(i * BLOCK_X + n * 32) * 16u, x_term);
+                            const float2 f = lds_f2(sxb + (uint32_t)n * 32u);
+                            acc[n][0] += times_powers(c[0], Ea, f.x); acc[n][1] += times_powers(c[1], Ea, f.y);
+                            acc[n][2] += times_powers(c[2], Eb, f.x); acc[n][3] += times_powers(c[3], Eb, f.y);
+                        }
+                    }
+                    release();
+                    continue;
+                }
                 uint32_t wa[SLOT_BLOCKS], wb[SLOT_BLOCKS];
 #pragma unroll
                 for (int i = 0; i < SLOT_BLOCKS; ++i) {
@@ -296,9 +341,7 @@ __global__ void __launch_bounds__(32 * (MAX_WARPS + 1), 1) gemv_kernel(const __g
                     wa[i] = lds32(at);
                     wb[i] = lds32(at + half);
                 }
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&empty[wk][place]);       // the box has been read
-                if (++place == AHEAD) { place = 0; pass ^= 1u; }
+                release();
                 float sum[NT][4];
 #pragma unroll
                 for (int i = 0; i < SLOT_BLOCKS; ++i) {
@@ -310,13 +353,7 @@ __global__ void __launch_bounds__(32 * (MAX_WARPS + 1), 1) gemv_kernel(const __g
 #pragma unroll
                     for (int n = 0; n < NT; ++n) {
                         float c[4];
-#pragma unroll
-                        for (int k = 0; k < TERMS; ++k) {
-                            const uint4 x = lds128(xb + k * x_term + (uint32_t)(i * BLOCK_X + n * 32) * 16u);
-                            if (k == 0) mma_first(c, A[0], B[0], A[1], B[1], x.x, x.y);
-                            else mma(c, A[0], B[0], A[1], B[1], x.x, x.y);
-                            mma(c, A[2], B[2], A[3], B[3], x.z, x.w);
-                        }
+                        block_sums<TERMS>(c, A, B, xb + (uint32_t)(i * BLOCK_X + n * 32) * 16u, x_term);
                         if (SCALED && i == 0) {
                             sum[n][0] = c[0] * ga; sum[n][1] = c[1] * ga; sum[n][2] = c[2] * gb; sum[n][3] = c[3] * gb;
                         } else {

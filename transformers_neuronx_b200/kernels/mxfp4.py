@@ -232,7 +232,9 @@ def gemm_mxfp4(a, w: Mxfp4Matrix, out: torch.Tensor, bias=None, residual=None, a
     row pitch of a 32-bit out, which it may be.  Sums are 32-bit; each result is rounded once.  out overlaps no other operand.
 
     Where operands become 16-bit ones, values far below their neighbours lose bits: with float16 activations values of a row of w below 2^-36 of
-    the row's largest scale, and where few tokens are streamed (kernels' choice) activations below 2^-39 of the largest of the 256 around them."""
+    the row's largest scale, and where few tokens are streamed (kernels' choice) activations below 2^-39 of the largest of the 256 around them.
+    A value of the matrix that no 32-bit number holds (2^128 and more: codes 4 and 6 of scale byte 253, 2 to 6 of 254) counts as itself or as an infinity,
+    as the kernel has it; every other scale byte is as good as any, and no step on the way to a result leaves 32 bits unless the sums do."""
     return _product(a, w, out, bias, residual, activation, False)
 
 
