@@ -66,3 +66,72 @@ def test_low_scales_beside_high_ones(M, dtype):
         m.gemm_mxfp4(x, w, out)
         ops().raise_on_device_error()
         _check(out, av @ wv.t(), _sum_bound(av, wv), torch.float32)
+
+
+# ---- sums that are not finite, or far below zero, behind an activation ---------------------------------------------
+SUMS = [float("nan"), float("-inf"), float("inf"), -3e38, -1e30, -2e4, -200.0, -70.0, -20.0, -5.0, -0.5, 0.0, 0.5, 5.0, 20.0, 3e4, 1e30, 3e38]
+ACTS = ["none", "relu", "relu2", "sigmoid", "gelu"]
+
+
+def _sources(m, M, K, dtype, seed):
+    """The kinds of activations that different kernels take: `dtype`, rows that no tensor map takes, 4 bits."""
+    a = torch.randn(M, K + 3, generator=torch.Generator().manual_seed(seed)).to(dtype).to(DEV)
+    return [a[:, 3:], a[:, :K].contiguous(), m.quantize_mxfp4(a[:, :K])]
+
+
+def _check_sums(got, x, act, dtype):
+    """got = act(x) in `dtype`, x exact sums.  32-bit results: exp, tanh and erf within two units in the last place, an addition and a division (3 * 2^-23 in
+    all), 16-bit ones: an exp(x) with 2 + 1.2 |x| units, |x| <= 90.  Where 1 + tanh or 1 + erf nearly cancel, 2^-22 of the argument's size is left over (it
+    is whole beyond 100).  exp leaves its range at 88.7: 2^-120."""
+    want = plain.activation(x.double(), act).to(torch.float32).double()
+    there = want.to(dtype)
+    assert torch.equal(got.isnan(), there.isnan()), (got, there)
+    assert torch.equal(got.isinf(), there.isinf()) and torch.equal(got[there.isinf()] > 0, there[there.isinf()] > 0), (got, there)
+    rel = 2.0 ** -21 if dtype is torch.float32 else HALF_STEP[dtype] * (1 + 2.0 ** -7) + 2.0 ** -16
+    off = rel * want.abs() + 2.0 ** -120 + (2.0 ** -25 if dtype is torch.float16 else 0.0)
+    if act in ("gelu", "gelu_new"):
+        off = off + 2.0 ** -22 * x.double().abs().clamp_max(100)
+    fine = there.isfinite()
+    bad = ((got.double() - want).abs() > off) & fine
+    assert not bool(bad.any()), (act, x[bad], got[bad], want[bad])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("M", [2, 20, 200])
+@pytest.mark.parametrize("act", ACTS)
+def test_activations_of_given_sums(act, M, dtype):
+    """Zero products, so that the bias is the sum: infinities, NaN and numbers of every size through every activation."""
+    m = mx()
+    K = 96
+    x = torch.tensor(SUMS * 8, device=DEV)
+    F = len(x)
+    w = m.Mxfp4Matrix(torch.zeros(2 * F, K // 2, dtype=torch.uint8, device=DEV), torch.full((2 * F, K // 32), 127, dtype=torch.uint8, device=DEV))
+    half = m.Mxfp4Matrix(w.codes[:F], w.scales[:F])
+    for a in _sources(m, M, K, dtype, M):
+        out = torch.full((M, F), 7.0, device=DEV, dtype=dtype)
+        m.gemm_mxfp4(a, half, out, bias=x, activation=act)
+        ops().raise_on_device_error()
+        _check_sums(out, x.expand(M, F), act, dtype)
+        out = torch.full((M, F), 7.0, device=DEV, dtype=dtype)
+        m.gated_gemm_mxfp4(a, w, out, bias=torch.cat((x, torch.ones_like(x))), activation=act)
+        ops().raise_on_device_error()
+        _check_sums(out, x.expand(M, F), act, dtype)
+
+
+@pytest.mark.parametrize("act", ACTS + ["silu", "gelu_new"])
+@pytest.mark.parametrize("M", [1, 9, 200])
+def test_blocks_that_are_not_a_number_behind_activations(M, act):
+    """A block of scale byte 255 makes its feature NaN whatever the activation, in the gate's rows and in the up rows, and no other."""
+    m = mx()
+    K, F = 320, 90
+    for row, feature in ((7, 7), (F + 11, 11)):
+        w, _ = _matrix(2 * F, K, 3)
+        w.scales[row, 4] = 255
+        for a in _sources(m, M, K, torch.bfloat16, M):
+            out = torch.zeros(M, 2 * F, device=DEV)
+            m.gemm_mxfp4(a, w, out, activation=act)
+            assert bool(out[:, row].isnan().all()) and int(out.isnan().sum()) == M
+            out = torch.zeros(M, F, device=DEV, dtype=torch.bfloat16)
+            m.gated_gemm_mxfp4(a, w, out, activation=act)
+            assert bool(out[:, feature].isnan().all()) and int(out.isnan().sum()) == M
+    ops().raise_on_device_error()

@@ -58,7 +58,7 @@ __host__ __device__ constexpr uint32_t idesc16(int n) {
 __device__ __forceinline__ float activate(float v, int act) {
     if (act == TNX_ACT_SILU) return __fdividef(v, 1.f + __expf(fminf(-v, 80.f)));
     if (act == TNX_ACT_GELU_NEW) return gelu_new_fast(v);
-    return apply_activation(v, act);
+    return mx_activation(v, act);
 }
 
 __device__ __forceinline__ void umma_mxf4(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t sfa, uint32_t sfb, uint32_t accumulate) {

@@ -54,7 +54,7 @@ __device__ __forceinline__ void load_codes(const Params& p, uint8_t* at, const C
 
 // Sixteen columns (tokens from `token` on) of this lane's row.
 template <int ACT>
-__device__ __forceinline__ float act_of(float v, int act) { return ACT == TNX_ACT_COUNT ? apply_activation(v, act) : activate(v, ACT); }
+__device__ __forceinline__ float act_of(float v, int act) { return ACT == TNX_ACT_COUNT ? mx_activation(v, act) : activate(v, ACT); }
 
 __device__ __forceinline__ void put(void* at, float v, int h16_out) {
     if (h16_out) *(h16*)at = float_to_h16(v);

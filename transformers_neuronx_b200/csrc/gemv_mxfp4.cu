@@ -412,7 +412,7 @@ __global__ void __launch_bounds__(32 * (MAX_WARPS + 1), 1) gemv_kernel(const __g
         for (int token = (threadIdx.x / feats) * splits + rank; token < p.M; token += groups * splits) {
             const long long o = (long long)token * p.ldc + n;
             const float res = p.residual ? __ldcg(p.residual + o) : 0.f;
-            float v = apply_activation(total(token, f) + bias, p.act);
+            float v = mx_activation(total(token, f) + bias, p.act);
             if (p.gated) v *= total(token, feats + f) + bias_up;
             v += res;
             if (p.out_h16) ((h16*)p.out)[o] = float_to_h16(v);

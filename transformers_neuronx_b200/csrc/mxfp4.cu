@@ -273,7 +273,7 @@ __global__ void __launch_bounds__(32 * SIMT_WARPS) simt_kernel(const SimtParams 
         float v = warp_sum(sum[0][t]), u = p.gated ? warp_sum(sum[1][t]) : 0.f;
         if (lane == 0) {
             if (p.bias) { v += p.bias[n]; if (p.gated) u += p.bias[p.N + n]; }
-            v = apply_activation(v, p.act);
+            v = mx_activation(v, p.act);
             if (p.gated) v *= u;
             const long long o = (long long)(m0 + t) * p.ldc + n;
             if (p.residual) v += p.residual[o];

@@ -27,6 +27,15 @@ __device__ __forceinline__ float mx_code(uint32_t c) {
     return __uint_as_float(((c & 8u) << 28) | ((c & 7u) << 22)) * 8.507059173023462e37f;
 }
 
+// The products' activations (common.cuh), but for a sum that is NaN, as the values of a block of scale byte 255 make it: it stays NaN behind relu and its
+// square too.
+__device__ __forceinline__ float mx_activation(float v, int act) {
+    if (act != TNX_ACT_RELU && act != TNX_ACT_RELU2) return apply_activation(v, act);
+    float r;
+    asm("max.NaN.f32 %0, %1, 0f00000000;" : "=f"(r) : "f"(v));
+    return act == TNX_ACT_RELU ? r : r * r;
+}
+
 // Eight codes as eight float16 numbers, without a scale.
 __device__ __forceinline__ void codes_to_f16(uint32_t w, uint32_t (&o)[4]) {
     asm("{\n\t.reg .b8 b0, b1, b2, b3;\n\t"
