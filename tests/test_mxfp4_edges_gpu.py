@@ -70,7 +70,7 @@ def test_low_scales_beside_high_ones(M, dtype):
 
 # ---- sums that are not finite, or far below zero, behind an activation ---------------------------------------------
 SUMS = [float("nan"), float("-inf"), float("inf"), -3e38, -1e30, -2e4, -200.0, -70.0, -20.0, -5.0, -0.5, 0.0, 0.5, 5.0, 20.0, 3e4, 1e30, 3e38]
-ACTS = ["none", "relu", "relu2", "sigmoid", "gelu"]
+ACTS = ["none", "relu", "relu2", "silu", "sigmoid", "gelu", "gelu_new"]
 
 
 def _sources(m, M, K, dtype, seed):
@@ -101,6 +101,8 @@ def _check_sums(got, x, act, dtype):
 @pytest.mark.parametrize("act", ACTS)
 def test_activations_of_given_sums(act, M, dtype):
     """Zero products, so that the bias is the sum: infinities, NaN and numbers of every size through every activation."""
+    if act in ("silu", "gelu_new") and dtype is torch.float32:
+        pytest.skip("16-bit results only")
     m = mx()
     K = 96
     x = torch.tensor(SUMS * 8, device=DEV)
@@ -118,7 +120,7 @@ def test_activations_of_given_sums(act, M, dtype):
         _check_sums(out, x.expand(M, F), act, dtype)
 
 
-@pytest.mark.parametrize("act", ACTS + ["silu", "gelu_new"])
+@pytest.mark.parametrize("act", ACTS)
 @pytest.mark.parametrize("M", [1, 9, 200])
 def test_blocks_that_are_not_a_number_behind_activations(M, act):
     """A block of scale byte 255 makes its feature NaN whatever the activation, in the gate's rows and in the up rows, and no other."""

@@ -54,10 +54,15 @@ __host__ __device__ constexpr uint32_t idesc16(int n) {
     return (1u << 4) | IDESC_H16_AB | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(TILE_W >> 4) << 24);
 }
 
-// x / (1 + e^-x) and the tanh form of gelu by the same few instructions; the others as everywhere (common.cuh).
+// x / (1 + e^-u) by the same few instructions for silu (u = x) and the tanh form of gelu; the others as everywhere.  The exponential is that of -|u|, never
+// above one, so that far below zero the result goes to zero as it should (with e^-u held at e^80, -1e38 became -1,800) and is NaN at minus infinity.
+__device__ __forceinline__ float gate_fast(float x, float u) {
+    const float e = __expf(-fabsf(u));
+    return __fdividef(u >= 0.f ? x : x * e, 1.f + e);
+}
 __device__ __forceinline__ float activate(float v, int act) {
-    if (act == TNX_ACT_SILU) return __fdividef(v, 1.f + __expf(fminf(-v, 80.f)));
-    if (act == TNX_ACT_GELU_NEW) return gelu_new_fast(v);
+    if (act == TNX_ACT_SILU) return gate_fast(v, v);
+    if (act == TNX_ACT_GELU_NEW) return gate_fast(v, 1.5957691216057308f * (v + 0.044715f * v * v * v));
     return mx_activation(v, act);
 }
 
