@@ -97,7 +97,7 @@ __device__ __forceinline__ void write_tile(const Epilogue& e, uint32_t sums, int
         const float4 s = load(t, f);
         float v[4] = {s.x, s.y, s.z, s.w};
 #pragma unroll
-        for (int j = 0; j < 4; ++j) v[j] = activate(v[j] + b[j], e.act);
+        for (int j = 0; j < 4; ++j) v[j] = e.out_h16 ? activate(v[j] + b[j], e.act) : mx_activation(v[j] + b[j], e.act);
         if (e.gated) {
             const float4 u = load(t, 64 + f);
             v[0] *= u.x + bu[0]; v[1] *= u.y + bu[1]; v[2] *= u.z + bu[2]; v[3] *= u.w + bu[3];

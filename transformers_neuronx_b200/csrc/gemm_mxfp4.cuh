@@ -54,7 +54,8 @@ __host__ __device__ constexpr uint32_t idesc16(int n) {
     return (1u << 4) | IDESC_H16_AB | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(TILE_W >> 4) << 24);
 }
 
-// x / (1 + e^-u) by the same few instructions for silu (u = x) and the tanh form of gelu; the others as everywhere.  The exponential is that of -|u|, never
+// Activations of results that are rounded to 16 bits anyway (32-bit ones take mx_activation): x / (1 + e^-u) by the same few instructions for silu (u = x)
+// and the tanh form of gelu, whose exponential is within 2 + 1.2 |u| units of its last place.  The exponential is that of -|u|, never
 // above one, so that far below zero the result goes to zero as it should (with e^-u held at e^80, -1e38 became -1,800) and is NaN at minus infinity.
 __device__ __forceinline__ float gate_fast(float x, float u) {
     const float e = __expf(-fabsf(u));

@@ -52,7 +52,7 @@ __device__ __forceinline__ void load_codes(const Params& p, uint8_t* at, const C
         }
 }
 
-// Sixteen columns (tokens from `token` on) of this lane's row.
+// ACT: an activation known to the compiler, or TNX_ACT_COUNT: any, by its number and in full precision.
 template <int ACT>
 __device__ __forceinline__ float act_of(float v, int act) { return ACT == TNX_ACT_COUNT ? mx_activation(v, act) : activate(v, ACT); }
 
@@ -61,7 +61,8 @@ __device__ __forceinline__ void put(void* at, float v, int h16_out) {
     else *(float*)at = v;
 }
 
-// WHOLE: all of the columns are tokens and all of the warp's rows features: no comparisons, and an address is one addition.
+// Sixteen columns (tokens from `token` on) of this lane's row.  WHOLE: all of the columns are tokens and all of the warp's rows features: no
+// comparisons, and an address is one addition.
 template <int ACT, bool WHOLE, bool H16, bool RESIDUAL>
 __device__ __forceinline__ void write16_as(const Epilogue& e, const float (&v)[16], int n, int token, float bias) {
     const long long step = e.ldc * (H16 ? 2 : 4), o = (long long)token * e.ldc + n;
@@ -126,6 +127,8 @@ struct Rings {                               // both kernels' barriers between M
 template <int SETS, typename Factor>
 __device__ __forceinline__ bool epilogue(const Params& p, Rings& d, uint32_t tmem_d, int step, int set, Factor factor_of) {
     const int quad = (threadIdx.x >> 5) & 3, lane = threadIdx.x & 31, r = quad * 32 + lane;
+    // the few instructions' forms are for results that are rounded to 16 bits
+    const int act = p.e.out_h16 || p.e.act == TNX_ACT_NONE || p.e.act == TNX_ACT_RELU ? p.e.act : TNX_ACT_COUNT;
     bool ok = true;
     int it = 0;
     for (int tile = blockIdx.x; tile < p.tiles && ok; tile += gridDim.x, ++it) {
@@ -152,7 +155,7 @@ __device__ __forceinline__ bool epilogue(const Params& p, Rings& d, uint32_t tme
 #pragma unroll
             for (int j = 0; j < 16; ++j) v[j] = __uint_as_float(raw[j]) * factor;
             if (c + 16 * SETS < cols) tmem_ld16(at + (uint32_t)(c + 16 * SETS), raw);               // on its way while these are written
-            switch (p.e.act) {
+            switch (act) {
                 case TNX_ACT_NONE: write16<TNX_ACT_NONE>(p.e, v, n, token0 + c, bias, bias_up); break;
                 case TNX_ACT_RELU: write16<TNX_ACT_RELU>(p.e, v, n, token0 + c, bias, bias_up); break;
                 case TNX_ACT_SILU: write16<TNX_ACT_SILU>(p.e, v, n, token0 + c, bias, bias_up); break;
