@@ -13,8 +13,9 @@
 //
 // Activations are float16 operands too: float16 as they are, others divided by a power of two that brings the largest of a box's 256 to
 // 2^14..2^15, in one term (bfloat16's eight bits and 4-bit values fit) or three (32 bits).  What is lost is below 2^-39 of the largest of
-// the 256, where float16 ends.  A block's sum of such operands may reach 2^23, so a box with a scale byte of 228 (2^101) or more takes another way, on
-// which the sum meets both powers of two as one: multiplied by the block's alone it could leave 32 bits where the result does not.
+// the 256, where float16 ends.  A block's sum of such operands is up to 2^15 times too large when it meets the matrix's scale, so that by scale bytes from
+// 228 on it may leave 32 bits where the result does not: a sum that is not finite is worked out again, in 64 bits.  (Choosing another way for such
+// scales ahead, by a look at them, took 4 to 7% of one token by 16,384 x 4,096.)
 //
 // The warps of a block: wf groups of 16 rows by wk shares of K, whose sums meet in shared memory; K may be split further over the blocks of a
 // cluster.  The plan chooses them so that one round of blocks, one an SM, covers the GPU as evenly as the sizes allow.
@@ -30,7 +31,7 @@ constexpr int AHEAD = 4;                     // boxes a warp has asked for
 struct Params {
     const void* a; const uint8_t* a_scales; long long lda;
     int a_kind, a_vec;                       // 0: h16, 1: float, 2: codes; rows can be read 16 bytes at a time
-    const uint8_t* scales;
+    const uint8_t* codes; const uint8_t* scales;
     const float* bias; const float* residual; void* out; long long ldc;
     int M, N, K, w_rows, blocks, slots, act, out_h16, gated;
     int wf, wk, splits, slots_per_split, phase; // phase: boxes of K whose activations lie in shared memory at a time
@@ -57,18 +58,6 @@ __device__ __forceinline__ uint4 lds128(uint32_t a) {
     return v;
 }
 __device__ __forceinline__ float2 lds_f2(uint32_t a) { float2 v; asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(a)); return v; }
-
-// The sums of a block of 32 columns: a lane's eight columns of two rows by eight tokens' activations, which lie at `at`, their terms x_term bytes apart.
-template <int TERMS>
-__device__ __forceinline__ void block_sums(float (&c)[4], const uint32_t (&A)[4], const uint32_t (&B)[4], uint32_t at, uint32_t x_term) {
-#pragma unroll
-    for (int k = 0; k < TERMS; ++k) {
-        const uint4 x = lds128(at + k * x_term);
-        if (k == 0) mma_first(c, A[0], B[0], A[1], B[1], x.x, x.y);
-        else mma(c, A[0], B[0], A[1], B[1], x.x, x.y);
-        mma(c, A[2], B[2], A[3], B[3], x.z, x.w);
-    }
-}
 
 __device__ __forceinline__ uint32_t pack_f16(float a, float b) {
     const __half2 r = __floats2half2_rn(a, b);
@@ -181,12 +170,20 @@ __device__ __forceinline__ float scale_at(uint32_t w, int at) {
     return fmaf(f, 0.f, f);
 }
 
-// c * 2^(E - 127) * f, f a power of two from 2^-127 to 2^114, rounded once at the most: the two exponents are added up and applied in halves of one sign,
-// so that what lies between c and the result is no larger and no smaller than both.
-constexpr uint32_t HIGH_SCALE = 228u;        // eight blocks' sums, 2^26, times a smaller scale stay in 32 bits
-__device__ __forceinline__ float times_powers(float c, uint32_t E, float f) {
-    const int e = (int)E - 254 + (int)(__float_as_uint(f) >> 23), h = e >> 1;            // -254 .. 241
-    return c * mx_scale(E == 255u ? 255u : (uint32_t)(h + 127)) * mx_scale((uint32_t)(e - h + 127));
+// sum_k a[k] w[k] by one thread, in 64 bits: a row of codes and its scales, a token's activations (a_scales: of codes).  (Single parameters: the kernel's as a
+// whole would be copied to memory of its own at the kernel's start, 2 us.)
+__device__ __forceinline__ double power_of_two(uint32_t E) { return E == 255u ? (double)NAN : __hiloint2double((int)((E + 896u) << 20), 0); }      // 2^(E - 127)
+__device__ __noinline__ float sum_again(const uint8_t* codes, const uint8_t* scales, const void* a, const uint8_t* a_scales, int a_kind, int K) {
+    double v = 0.;
+#pragma unroll 1
+    for (int k = 0; k < K; ++k) {
+        float x;
+        if (a_kind == 2) x = mx_code(((const uint8_t*)a)[k / 2] >> (4 * (k & 1)));
+        else x = a_kind ? ((const float*)a)[k] : h16_to_float(((const h16*)a)[k]);
+        const double w = mx_code(codes[k / 2] >> (4 * (k & 1))) * power_of_two(scales[k / MX_BLOCK]);
+        v += w * (a_kind == 2 ? x * power_of_two(a_scales[k / MX_BLOCK]) : (double)x);
+    }
+    return (float)v;
 }
 
 // NT: groups of eight tokens; SCALED: the activations have scales.  Warps 0 .. wf * wk - 1 multiply, the last one fetches codes.
@@ -310,30 +307,6 @@ __global__ void __launch_bounds__(32 * (MAX_WARPS + 1), 1) gemv_kernel(const __g
                 if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&full[wk][place], pass, p.err, 81));
                 if (!ok) break;
                 const uint32_t row = ring + (uint32_t)(place * box_bytes);
-                auto release = [&]() {                               // the box has been read
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(&empty[wk][place]);
-                    if (++place == AHEAD) { place = 0; pass ^= 1u; }
-                };
-                if (SCALED && __any_sync(0xffffffffu, ((two & 0x7F7F7F7Fu) + 0x01010101u * (256u - HIGH_SCALE)) & two & 0x80808080u)) {
-#pragma unroll 1
-                    for (int i = 0; i < SLOT_BLOCKS; ++i) {
-                        uint32_t A[4], B[4];
-                        codes_to_f16(lds32(row + (uint32_t)((i ^ g) << 4)), A);
-                        codes_to_f16(lds32(row + (uint32_t)((i ^ g) << 4) + half), B);
-                        const uint32_t E = __shfl_sync(0xffffffffu, two, (lane & ~3) | (i >> 1)) >> (8 * (i & 1)), Ea = E & 255u, Eb = (E >> 16) & 255u;
-#pragma unroll
-                        for (int n = 0; n < NT; ++n) {
-                            float c[4];
-                            block_sums<TERMS>(c, A, B, xb + (uint32_t)(i * BLOCK_X + n * 32) * 16u, x_term);
-                            const float2 f = lds_f2(sxb + (uint32_t)n * 32u);
-                            acc[n][0] += times_powers(c[0], Ea, f.x); acc[n][1] += times_powers(c[1], Ea, f.y);
-                            acc[n][2] += times_powers(c[2], Eb, f.x); acc[n][3] += times_powers(c[3], Eb, f.y);
-                        }
-                    }
-                    release();
-                    continue;
-                }
                 uint32_t wa[SLOT_BLOCKS], wb[SLOT_BLOCKS];
 #pragma unroll
                 for (int i = 0; i < SLOT_BLOCKS; ++i) {
@@ -341,7 +314,9 @@ __global__ void __launch_bounds__(32 * (MAX_WARPS + 1), 1) gemv_kernel(const __g
                     wa[i] = lds32(at);
                     wb[i] = lds32(at + half);
                 }
-                release();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&empty[wk][place]);       // the box has been read
+                if (++place == AHEAD) { place = 0; pass ^= 1u; }
                 float sum[NT][4];
 #pragma unroll
                 for (int i = 0; i < SLOT_BLOCKS; ++i) {
@@ -353,7 +328,13 @@ __global__ void __launch_bounds__(32 * (MAX_WARPS + 1), 1) gemv_kernel(const __g
 #pragma unroll
                     for (int n = 0; n < NT; ++n) {
                         float c[4];
-                        block_sums<TERMS>(c, A, B, xb + (uint32_t)(i * BLOCK_X + n * 32) * 16u, x_term);
+#pragma unroll
+                        for (int k = 0; k < TERMS; ++k) {
+                            const uint4 x = lds128(xb + k * x_term + (uint32_t)(i * BLOCK_X + n * 32) * 16u);
+                            if (k == 0) mma_first(c, A[0], B[0], A[1], B[1], x.x, x.y);
+                            else mma(c, A[0], B[0], A[1], B[1], x.x, x.y);
+                            mma(c, A[2], B[2], A[3], B[3], x.z, x.w);
+                        }
                         if (SCALED && i == 0) {
                             sum[n][0] = c[0] * ga; sum[n][1] = c[1] * ga; sum[n][2] = c[2] * gb; sum[n][3] = c[3] * gb;
                         } else {
@@ -404,6 +385,13 @@ __global__ void __launch_bounds__(32 * (MAX_WARPS + 1), 1) gemv_kernel(const __g
                 for (int w = 0; w < p.wk; ++w) v += ld_cluster(at + w * p.M * ld, (uint32_t)s);
         return v;
     };
+    auto sum_of = [&](int token, int row, int w_row) {
+        const float v = total(token, row);
+        if (!SCALED || fabsf(v) < INFINITY) return v;
+        const long long wb = (long long)w_row * p.blocks, ab = (long long)token * p.blocks;
+        const char* a = (const char*)p.a + (p.a_kind == 2 ? ab * 16 : token * p.lda * (p.a_kind ? 4 : 2));
+        return sum_again(p.codes + wb * 16, p.scales + wb, a, p.a_scales + ab, p.a_kind, p.K);
+    };
     const int feats = p.gated ? rows / 2 : rows;
     const int f = threadIdx.x % feats;                    // a thread keeps its feature: blocks have at least as many threads as features
     const int n = first + f, groups = blockDim.x / feats;
@@ -412,8 +400,8 @@ __global__ void __launch_bounds__(32 * (MAX_WARPS + 1), 1) gemv_kernel(const __g
         for (int token = (threadIdx.x / feats) * splits + rank; token < p.M; token += groups * splits) {
             const long long o = (long long)token * p.ldc + n;
             const float res = p.residual ? __ldcg(p.residual + o) : 0.f;
-            float v = mx_activation(total(token, f) + bias, p.act);
-            if (p.gated) v *= total(token, feats + f) + bias_up;
+            float v = mx_activation(sum_of(token, f, n) + bias, p.act);
+            if (p.gated) v *= sum_of(token, feats + f, p.N + n) + bias_up;
             v += res;
             if (p.out_h16) ((h16*)p.out)[o] = float_to_h16(v);
             else ((float*)p.out)[o] = v;
@@ -484,7 +472,7 @@ TNX_EXPORT int tnx_gemv_mxfp4(const void* a, int a_kind, const void* a_scales, l
     Params p;
     p.a = a; p.a_scales = (const uint8_t*)a_scales; p.lda = lda; p.a_kind = a_kind;
     p.a_vec = ((uintptr_t)a & 15) == 0 && lda % (a_kind == 1 ? 4 : 8) == 0;
-    p.scales = (const uint8_t*)scales; p.bias = bias; p.residual = residual; p.out = out; p.ldc = ldc; p.err = err;
+    p.codes = (const uint8_t*)codes; p.scales = (const uint8_t*)scales; p.bias = bias; p.residual = residual; p.out = out; p.ldc = ldc; p.err = err;
     p.M = M; p.N = N; p.K = K; p.w_rows = gated ? 2 * N : N; p.blocks = (K + MX_BLOCK - 1) / MX_BLOCK;
     p.slots = (p.blocks + SLOT_BLOCKS - 1) / SLOT_BLOCKS;
     p.act = act; p.out_h16 = out_h16; p.gated = gated;
