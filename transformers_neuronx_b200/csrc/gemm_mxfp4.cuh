@@ -55,12 +55,10 @@ __host__ __device__ constexpr uint32_t idesc16(int n) {
 }
 
 // Activations of results that are rounded to 16 bits anyway (32-bit ones take mx_activation): x / (1 + e^-u) by the same few instructions for silu (u = x)
-// and the tanh form of gelu, whose exponential is within 2 + 1.2 |u| units of its last place.  The exponential is that of -|u|, never
-// above one, so that far below zero the result goes to zero as it should (with e^-u held at e^80, -1e38 became -1,800) and is NaN at minus infinity.
-__device__ __forceinline__ float gate_fast(float x, float u) {
-    const float e = __expf(-fabsf(u));
-    return __fdividef(u >= 0.f ? x : x * e, 1.f + e);
-}
+// and the tanh form of gelu, whose exponential is within 2 + 1.2 |u| units of its last place.  The division gives zero by a divisor of 2^126 and more (u
+// below -87.3), an infinity among them, and NaN for an infinity by one, so that nothing has to be held in a range: with e^-u held at e^80, -1e38 became
+// -1,800.
+__device__ __forceinline__ float gate_fast(float x, float u) { return __fdividef(x, 1.f + __expf(-u)); }
 __device__ __forceinline__ float activate(float v, int act) {
     if (act == TNX_ACT_SILU) return gate_fast(v, v);
     if (act == TNX_ACT_GELU_NEW) return gate_fast(v, 1.5957691216057308f * (v + 0.044715f * v * v * v));
