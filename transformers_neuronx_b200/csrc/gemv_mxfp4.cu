@@ -14,8 +14,8 @@
 // Activations are float16 operands too: float16 as they are, others divided by a power of two that brings the largest of a box's 256 to
 // 2^14..2^15, in one term (bfloat16's eight bits and 4-bit values fit) or three (32 bits).  What is lost is below 2^-39 of the largest of
 // the 256, where float16 ends.  A block's sum of such operands is up to 2^15 times too large when it meets the matrix's scale, so that by scale bytes from
-// 228 on it may leave 32 bits where the result does not: a sum that is not finite is worked out again, in 64 bits.  (Choosing another way for such
-// scales ahead, by a look at them, took 4 to 7% of one token by 16,384 x 4,096.)
+// 228 on it may leave 32 bits where the result does not: a sum that is not finite is worked out again in 64 bits, if its row has such a scale.
+// (Choosing another way for them ahead, by a look at the scales, took 4 to 7% of one token by 16,384 x 4,096.)
 //
 // The warps of a block: wf groups of 16 rows by wk shares of K, whose sums meet in shared memory; K may be split further over the blocks of a
 // cluster.  The plan chooses them so that one round of blocks, one an SM, covers the GPU as evenly as the sizes allow.
@@ -170,20 +170,31 @@ __device__ __forceinline__ float scale_at(uint32_t w, int at) {
     return fmaf(f, 0.f, f);
 }
 
-// sum_k a[k] w[k] by one thread, in 64 bits: a row of codes and its scales, a token's activations (a_scales: of codes).  (Single parameters: the kernel's as a
-// whole would be copied to memory of its own at the kernel's start, 2 us.)
+// sum_k a[k] w[k] by one thread, in 64 bits: a row of codes and its scales, a token's activations (a_scales: of codes).  `v`: the sum as it came out, not
+// finite, which is right where no scale is from HIGH_SCALE to 254 (activations or blocks that are not finite).  (Single parameters: the kernel's as a whole
+// would be copied to memory of its own at the kernel's start, 2 us.)
+constexpr uint32_t HIGH_SCALE = 228u;        // eight blocks' sums, 2^26 at the most, times a smaller scale stay in 32 bits
 __device__ __forceinline__ double power_of_two(uint32_t E) { return E == 255u ? (double)NAN : __hiloint2double((int)((E + 896u) << 20), 0); }      // 2^(E - 127)
-__device__ __noinline__ float sum_again(const uint8_t* codes, const uint8_t* scales, const void* a, const uint8_t* a_scales, int a_kind, int K) {
-    double v = 0.;
+__device__ __noinline__ float sum_again(float v, const uint8_t* codes, const uint8_t* scales, const void* a, const uint8_t* a_scales, int a_kind, int K) {
+    const int blocks = (K + MX_BLOCK - 1) / MX_BLOCK;
+    int b = 0;
+    if (((uintptr_t)scales & 3) == 0)                     // four bytes at a time up to the first of HIGH_SCALE or more
+        for (; b + 4 <= blocks; b += 4) {
+            const uint32_t w = __ldg((const uint32_t*)(scales + b));
+            if (((w & 0x7F7F7F7Fu) + 0x01010101u * (256u - HIGH_SCALE)) & w & 0x80808080u) break;
+        }
+    while (b < blocks && (scales[b] < HIGH_SCALE || scales[b] == 255u)) ++b;
+    if (b == blocks) return v;
+    double sum = 0.;
 #pragma unroll 1
     for (int k = 0; k < K; ++k) {
         float x;
         if (a_kind == 2) x = mx_code(((const uint8_t*)a)[k / 2] >> (4 * (k & 1)));
         else x = a_kind ? ((const float*)a)[k] : h16_to_float(((const h16*)a)[k]);
         const double w = mx_code(codes[k / 2] >> (4 * (k & 1))) * power_of_two(scales[k / MX_BLOCK]);
-        v += w * (a_kind == 2 ? x * power_of_two(a_scales[k / MX_BLOCK]) : (double)x);
+        sum += w * (a_kind == 2 ? x * power_of_two(a_scales[k / MX_BLOCK]) : (double)x);
     }
-    return (float)v;
+    return (float)sum;
 }
 
 // NT: groups of eight tokens; SCALED: the activations have scales.  Warps 0 .. wf * wk - 1 multiply, the last one fetches codes.
@@ -390,7 +401,7 @@ __global__ void __launch_bounds__(32 * (MAX_WARPS + 1), 1) gemv_kernel(const __g
         if (!SCALED || fabsf(v) < INFINITY) return v;
         const long long wb = (long long)w_row * p.blocks, ab = (long long)token * p.blocks;
         const char* a = (const char*)p.a + (p.a_kind == 2 ? ab * 16 : token * p.lda * (p.a_kind ? 4 : 2));
-        return sum_again(p.codes + wb * 16, p.scales + wb, a, p.a_scales + ab, p.a_kind, p.K);
+        return sum_again(v, p.codes + wb * 16, p.scales + wb, a, p.a_scales + ab, p.a_kind, p.K);
     };
     const int feats = p.gated ? rows / 2 : rows;
     const int f = threadIdx.x % feats;                    // a thread keeps its feature: blocks have at least as many threads as features
