@@ -135,3 +135,54 @@ def test_blocks_that_are_not_a_number_behind_activations(M, act):
             m.gated_gemm_mxfp4(a, w, out, activation=act)
             assert bool(out[:, feature].isnan().all()) and int(out.isnan().sum()) == M
     ops().raise_on_device_error()
+
+
+# ---- more rows of W than 65,535 tiles ------------------------------------------------------------------------------
+@pytest.mark.parametrize("quantized", [False, True])
+@pytest.mark.parametrize("M", [1, 16, 64, 130])
+def test_more_than_65535_tiles(M, quantized):
+    m = mx()
+    K, N = 32, 65535 * 128 + 200
+    g = torch.Generator(device=DEV).manual_seed(M)
+    codes = torch.empty(N, 16, device=DEV, dtype=torch.uint8).random_(0, 256, generator=g)
+    scales = torch.empty(N, 1, device=DEV, dtype=torch.uint8).random_(118, 126, generator=g)
+    w = m.Mxfp4Matrix(codes, scales)
+    a = torch.randn(M, K, generator=g, device=DEV).bfloat16()
+    x, av = (m.quantize_mxfp4(a), plain.rounded(a)) if quantized else (a, a.double())
+
+    def values(rows):
+        return m.dequantize_mxfp4(m.Mxfp4Matrix(codes[rows].contiguous(), scales[rows].contiguous()), torch.float32).double()
+    out = torch.full((M, N), float("nan"), device=DEV, dtype=torch.bfloat16)
+    m.gemm_mxfp4(x, w, out)
+    ops().raise_on_device_error()
+    at = torch.tensor([0, 127, 128, 65534 * 128, 65535 * 128 - 1, 65535 * 128, 65535 * 128 + 1, N - 1], device=DEV)
+    wv = values(at)
+    _check(out[:, at], av @ wv.t(), _sum_bound(av, wv), torch.bfloat16)
+    assert not bool(out.isnan().any())
+    F = N // 2                                             # more than 65,535 tiles of 64 features
+    out = torch.full((M, F), float("nan"), device=DEV, dtype=torch.bfloat16)
+    m.gated_gemm_mxfp4(x, w, out, activation="relu")
+    ops().raise_on_device_error()
+    at = torch.tensor([0, 63, 64, 65534 * 64, 65535 * 64 - 1, 65535 * 64, F - 1], device=DEV)
+    gv, uv = values(at), values(F + at)
+    gate, up, bg, bu = (av @ gv.t()).clamp_min(0), av @ uv.t(), _sum_bound(av, gv), _sum_bound(av, uv)
+    _check(out[:, at], gate * up, bg * up.abs() + gate * bu + bg * bu + 2.0 ** -23 * (gate * up).abs(), torch.bfloat16)
+    assert not bool(out.isnan().any())
+
+
+def test_more_than_65535_tiles_of_long_rows():
+    """32-bit results of more than 5,120 columns: 130 tokens, whose K is split (22 GB of codes)."""
+    m = mx()
+    M, K, N = 130, 5152, 65535 * 128 + 200
+    g = torch.Generator(device=DEV).manual_seed(1)
+    codes = torch.empty(N, K // 2, device=DEV, dtype=torch.uint8).random_(0, 256, generator=g)
+    scales = torch.empty(N, K // 32, device=DEV, dtype=torch.uint8).random_(118, 126, generator=g)
+    a = torch.randn(M, K, generator=g, device=DEV).bfloat16()
+    out = torch.full((M, N), float("nan"), device=DEV)
+    m.gemm_mxfp4(a, m.Mxfp4Matrix(codes, scales), out)
+    ops().raise_on_device_error()
+    at = torch.tensor([0, 128, 65535 * 128 - 1, 65535 * 128, N - 1], device=DEV)
+    wv = m.dequantize_mxfp4(m.Mxfp4Matrix(codes[at].contiguous(), scales[at].contiguous()), torch.float32).double()
+    _check(out[:, at], a.double() @ wv.t(), _sum_bound(a.double(), wv), torch.float32)
+    del codes, scales, out
+    torch.cuda.empty_cache()

@@ -33,6 +33,7 @@ struct Params {
     Epilogue e;
     const uint8_t* scales;
     const uint8_t* a_scales;                 // gemm4
+    int tiles_t;                             // tiles of tokens: blockIdx.x counts them within those of W, of which there may be more than a grid's other axes hold
     int w_rows, blocks;                      // rows of W and scales a row
     int num_kb, boxes_per_split;             // K in stages; boxes of codes a CTA of the cluster takes
     int splits;
@@ -205,7 +206,7 @@ gemm16_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__
 #endif
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int token0 = blockIdx.x * BN, row0 = blockIdx.y * TILE_W;
+    const int tile_w = (int)blockIdx.x / p.tiles_t, token0 = ((int)blockIdx.x - tile_w * p.tiles_t) * BN, row0 = tile_w * TILE_W;
     const int box0 = (int)blockIdx.z * p.boxes_per_split;
     const int kb0 = box0 * PARTS;
     const int num_kb = min(p.num_kb - kb0, p.boxes_per_split * PARTS);               // at least one
@@ -423,7 +424,7 @@ gemm4_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ 
     __shared__ uint32_t sf_smem[2][SF_COLS * 32];
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int token0 = blockIdx.x * BN, row0 = blockIdx.y * TILE_W;
+    const int tile_w = (int)blockIdx.x / p.tiles_t, token0 = ((int)blockIdx.x - tile_w * p.tiles_t) * BN, row0 = tile_w * TILE_W;
     const int st0 = (int)blockIdx.z * p.boxes_per_split;                           // stages of 256 columns
     const int num = min((p.blocks + 7) / 8 - st0, p.boxes_per_split);               // at least one
 
@@ -599,8 +600,10 @@ long long split(Params& p, int bn, int tiles_w, int fixed, int chain, PlacesOf p
 }
 
 template <typename Kernel>
-int launch(Kernel kernel, int threads, int smem, int bn, const CUtensorMap& mw, const CUtensorMap& mx, const Params& p, int tiles_w, cudaStream_t stream) {
-    const dim3 grid((p.e.M + bn - 1) / bn, tiles_w, p.splits);
+int launch(Kernel kernel, int threads, int smem, int bn, const CUtensorMap& mw, const CUtensorMap& mx, Params& p, int tiles_w, cudaStream_t stream) {
+    p.tiles_t = (p.e.M + bn - 1) / bn;
+    if ((long long)p.tiles_t * tiles_w > 0x7FFFFFFF) return TNX_ERR_UNSUPPORTED;
+    const dim3 grid(p.tiles_t * tiles_w, 1, p.splits);
     if (p.splits > 1) return tnx_launch_cluster(1, dim3(1, 1, p.splits), kernel, grid, dim3(threads), smem, stream, mw, mx, p);
     return tnx_launch_ex(1, kernel, grid, dim3(threads), smem, stream, mw, mx, p);
 }
@@ -661,7 +664,6 @@ TNX_EXPORT long long tnx_gemm_mxfp4_estimate(int M, int N, int K, int gated, int
     Params p;
     p.e.M = M;
     const int tiles_w = gated ? (N + 63) / 64 : (N + TILE_W - 1) / TILE_W;
-    if (tiles_w > 65535) return 1ll << 60;
     p.blocks = (K + MX_BLOCK - 1) / MX_BLOCK;
     long long boxes = 0;
     const int r = quantized ? launch4<128, 4, 1>(nullptr, nullptr, p, tiles_w, n_sms, nullptr, &boxes)
@@ -684,7 +686,7 @@ TNX_EXPORT int tnx_gemm_mxfp4_16(const void* a, long long lda, const void* codes
     if (M <= 0 || N <= 0) return 0;
     if (K <= 0 || act < 0 || act >= TNX_ACT_COUNT || n_sms <= 0) return TNX_ERR_BAD_ARG;
     const int tiles_w = gated ? (N + 63) / 64 : (N + TILE_W - 1) / TILE_W;
-    if (lda % 8 || ((uintptr_t)a & 15) || ((uintptr_t)codes & 15) || tiles_w > 65535) return TNX_ERR_UNSUPPORTED;
+    if (lda % 8 || ((uintptr_t)a & 15) || ((uintptr_t)codes & 15)) return TNX_ERR_UNSUPPORTED;
     Params p;
     fill(p, scales, nullptr, bias, residual, out, out_h16, ldc, M, N, K, act, gated, err);
     const int chain = out_h16 ? 0 : MX_CHAIN;
@@ -702,7 +704,7 @@ TNX_EXPORT int tnx_gemm_mxfp4_4(const void* a, const void* a_scales, const void*
     if (M <= 0 || N <= 0) return 0;
     if (K <= 0 || act < 0 || act >= TNX_ACT_COUNT || n_sms <= 0) return TNX_ERR_BAD_ARG;
     const int tiles_w = gated ? (N + 63) / 64 : (N + TILE_W - 1) / TILE_W;
-    if (((uintptr_t)a & 15) || ((uintptr_t)codes & 15) || tiles_w > 65535) return TNX_ERR_UNSUPPORTED;
+    if (((uintptr_t)a & 15) || ((uintptr_t)codes & 15)) return TNX_ERR_UNSUPPORTED;
     Params p;
     fill(p, scales, a_scales, bias, residual, out, out_h16, ldc, M, N, K, act, gated, err);
     switch (tile_tokens(M)) {
