@@ -186,3 +186,38 @@ def test_more_than_65535_tiles_of_long_rows():
     _check(out[:, at], a.double() @ wv.t(), _sum_bound(a.double(), wv), torch.float32)
     del codes, scales, out
     torch.cuda.empty_cache()
+
+
+# ---- which build of the kernels ------------------------------------------------------------------------------------
+def _loaded_flavours(m, monkeypatch, run):
+    """The flavours in which run() asks for this family's libraries."""
+    from transformers_neuronx_b200.kernels import build
+    asked, load = set(), build.load
+
+    def recording(name, dtype=None):
+        if "mxfp4" in name:
+            asked.add((name, build.flavour_of(dtype)))
+        return load(name, dtype)
+    with monkeypatch.context() as p:
+        p.setattr(build, "load", recording)
+        p.setattr(m, "_entries", {})
+        p.setattr(m, "_tiles", {})
+        run()
+    return asked
+
+
+@pytest.mark.parametrize("dtype,flavour", [(torch.float16, "f16"), (torch.bfloat16, "")])
+@pytest.mark.parametrize("M", [1, 16, 200])
+def test_flavour_of_4_bit_activations(M, dtype, flavour, monkeypatch):
+    """Operands that came from one 16-bit type go to the kernels built for it, into 32 bits too, whichever of the two tells."""
+    m = mx()
+    x, w = torch.randn(M, 256, device=DEV).to(dtype), torch.randn(300, 256, device=DEV).to(dtype)
+    out = torch.empty(M, 300, device=DEV)
+
+    def run():
+        q = m.quantize_mxfp4(w)
+        m.gemm_mxfp4(m.quantize_mxfp4(x), q, out)
+        m.gemm_mxfp4(m.quantize_mxfp4(x), m.Mxfp4Matrix(q.codes, q.scales), out)
+        m.gemm_mxfp4(m.Mxfp4Matrix(*(lambda p: (p.codes, p.scales))(m.quantize_mxfp4(x))), q, out)
+        m.gemm_mxfp4(m.quantize_mxfp4(x, out=m.quantize_mxfp4(x.clone())), q, out)
+    assert {f for _, f in _loaded_flavours(m, monkeypatch, run)} == {flavour}

@@ -119,3 +119,26 @@ def test_every_product_of_a_model(which, amp, activations, monkeypatch):
     assert max(tokens) > 128 and min(tokens) <= 2              # both ends: a prompt and single tokens
     if which == "Taborax-B":                                   # a shared expert with a gate of its own, whose width the routed ones do not divide
         assert scaled and any(kind == "gemm" for kind, _ in kinds)
+
+
+@pytest.mark.parametrize("amp", ["f16", "bf16"])
+@pytest.mark.parametrize("which", ["Vononex-Q", "Tutelix-B", "Vozirax-B", "Resatar-B", "Taborax-B"])
+def test_a_model_loads_only_the_libraries_it_names(which, amp, monkeypatch):
+    """4-bit inputs, whose type says nothing about the engine's: nothing is left to be compiled within a request."""
+    from transformers_neuronx_b200.kernels import build
+    m = mx()
+    tiny = _model(which)
+    model = _engine(tiny.folder, amp, "mxfp4")
+    named = set(build.with_flavour(model.model.libraries(model.model.act_dtype), model.model.act_dtype))
+    asked, load = set(), build.load
+
+    def recording(name, dtype=None):
+        if "mxfp4" in name:
+            f = build.flavour_of(dtype)
+            asked.add(f"{name}.{f}" if f else name)
+        return load(name, dtype)
+    monkeypatch.setattr(build, "load", recording)
+    monkeypatch.setattr(m, "_entries", {})
+    monkeypatch.setattr(m, "_tiles", {})
+    _steps(model, [tiny.random_ids(150, seed=s) for s in (1, 2)], 1)
+    assert asked and asked <= named, sorted(asked - named)

@@ -37,7 +37,8 @@ class Mxfp4Matrix:
     blocks = ceil(columns / 32).  Both contiguous and on one device; codes behind the last column are zeros (0 times whatever stands there
     is what the products add).  The tensors are used as they are, not copied."""
 
-    __slots__ = ("_codes", "_scales", "_buffer", "_device", "_blocks", "rows", "columns")
+    # _kind: the 16-bit type of the values that were brought into 4 bits, if it was one: where no 16-bit operand names it, it names the build of the kernels
+    __slots__ = ("_codes", "_scales", "_buffer", "_device", "_blocks", "_kind", "rows", "columns")
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor, columns: Optional[int] = None):
         for t, name in ((codes, "codes"), (scales, "scales")):
@@ -52,7 +53,7 @@ class Mxfp4Matrix:
         if blocks < 1 or not (blocks - 1) * BLOCK < columns <= blocks * BLOCK:
             raise KernelError(f"{columns} columns do not make {blocks} blocks of {BLOCK}")
         self._codes, self._scales, self._buffer = codes, scales, None
-        self._device, self._blocks, self.rows, self.columns = codes.get_device(), blocks, rows, columns
+        self._device, self._blocks, self._kind, self.rows, self.columns = codes.get_device(), blocks, None, rows, columns
 
     @classmethod
     def _empty(cls, rows: int, columns: int, device: torch.device, number: int) -> "Mxfp4Matrix":
@@ -61,7 +62,7 @@ class Mxfp4Matrix:
         blocks = (columns + BLOCK - 1) // BLOCK
         self._codes = self._scales = None
         self._buffer = torch.empty_strided((rows * blocks * 17,), (1,), dtype=torch.uint8, device=device)
-        self._device, self._blocks, self.rows, self.columns = number, blocks, rows, columns
+        self._device, self._blocks, self._kind, self.rows, self.columns = number, blocks, None, rows, columns
         return self
 
     def _split(self) -> None:
@@ -193,8 +194,9 @@ def quantize_mxfp4(x: torch.Tensor, out: Optional[Mxfp4Matrix] = None) -> Mxfp4M
     codes, scales = out._pointers()
     if codes % 4:
         raise KernelError("out's codes must be 4-byte aligned")
+    dtype = x.dtype
+    out._kind = dtype if dtype in _H16 else None
     if rows:
-        dtype = x.dtype
         _check(_entry("mxfp4", "tnx_mxfp4_quantize", dtype)(_PACK[9](
             x.data_ptr(), 0 if dtype is torch.float32 else 1, pitch, codes, scales, rows, columns, _device_info(device, x.device)[0], _stream(device))),
             "quantize_mxfp4")
@@ -278,12 +280,14 @@ def _product(a, w, out, bias, residual, activation, gated):
     if quantized:
         if a._device != device:
             raise KernelError(f"a is on {a.device}, w on {w.device}")
-        M, K, lda, kind, a_kind = a.rows, a.columns, 0, None, 2
+        M, K, lda, kind, a_kind = a.rows, a.columns, 0, a._kind or w._kind, 2
         a_p, as_p = a._pointers()
     else:
         M, K, lda = _floats(a, "a", device)
         kind = a.dtype
-        a_kind = 1 if kind is torch.float32 else 0
+        a_kind = 0
+        if kind is torch.float32:
+            a_kind, kind = 1, w._kind
         a_p, as_p = a.data_ptr(), 0
     Mo, N, ldc = _writable(out, "out", device)
     if gated and rows % 2:
