@@ -221,3 +221,23 @@ def test_flavour_of_4_bit_activations(M, dtype, flavour, monkeypatch):
         m.gemm_mxfp4(m.Mxfp4Matrix(*(lambda p: (p.codes, p.scales))(m.quantize_mxfp4(x))), q, out)
         m.gemm_mxfp4(m.quantize_mxfp4(x, out=m.quantize_mxfp4(x.clone())), q, out)
     assert {f for _, f in _loaded_flavours(m, monkeypatch, run)} == {flavour}
+
+
+# ---- the slices of a product on the multiply-add units -------------------------------------------------------------
+def test_most_tokens_of_one_column():
+    """2^31 - 4,096 tokens of one value by a matrix of one row (4.3 GB each way): the slices' counter stays in its range."""
+    m = mx()
+    M = m.MOST
+    w = m.Mxfp4Matrix(torch.tensor([[4] + [0] * 15], dtype=torch.uint8, device=DEV), torch.tensor([[127]], dtype=torch.uint8, device=DEV), 1)     # 2
+    a = torch.ones(M, 1, device=DEV, dtype=torch.float16)
+    a[-1] = 3
+    a[M // 2] = 5
+    out = torch.zeros(M, 1, device=DEV, dtype=torch.float16)
+    m.gemm_mxfp4(a, w, out)
+    ops().raise_on_device_error()
+    assert float(out[-1]) == 6 and float(out[M // 2]) == 10
+    out[-1] = out[M // 2] = 2
+    for part in out.split(1 << 28):
+        assert bool((part == 2).all())
+    del a, out, part
+    torch.cuda.empty_cache()

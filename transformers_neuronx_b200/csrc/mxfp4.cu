@@ -340,13 +340,13 @@ TNX_EXPORT int tnx_mxfp4_gemm_simt(const void* a, int a_kind, const void* a_scal
     p.M = M; p.N = N; p.K = K; p.blocks = (K + MX_BLOCK - 1) / MX_BLOCK; p.act = act; p.gated = gated; p.out_h16 = out_h16;
     // 65,535 blocks along y at most: more tokens go in slices
     const int slice = 65535 * SIMT_TOKENS;
-    for (int m = 0; m < M; m += slice) {
+    for (long long m = 0; m < M; m += slice) {            // (an int would pass its end behind the last slice of nearly 2^31 tokens)
         SimtParams q = p;
-        q.M = M - m < slice ? M - m : slice;
-        q.a = a_kind == 2 ? (const void*)((const uint8_t*)a + (long long)m * p.blocks * 16) : (const void*)((const char*)a + (long long)m * lda * (a_kind ? 4 : 2));
-        if (a_scales) q.a_scales = p.a_scales + (long long)m * p.blocks;
-        if (residual) q.residual = residual + (long long)m * ldc;
-        q.out = (char*)out + (long long)m * ldc * (out_h16 ? 2 : 4);
+        q.M = M - m < slice ? (int)(M - m) : slice;
+        q.a = a_kind == 2 ? (const void*)((const uint8_t*)a + m * p.blocks * 16) : (const void*)((const char*)a + m * lda * (a_kind ? 4 : 2));
+        if (a_scales) q.a_scales = p.a_scales + m * p.blocks;
+        if (residual) q.residual = residual + m * ldc;
+        q.out = (char*)out + m * ldc * (out_h16 ? 2 : 4);
         const int r = tnx_launch_ex(1, simt_kernel, dim3((N + SIMT_WARPS - 1) / SIMT_WARPS, (q.M + SIMT_TOKENS - 1) / SIMT_TOKENS), dim3(32 * SIMT_WARPS), 0, stream, q);
         if (r) return r;
     }
