@@ -241,3 +241,121 @@ def test_most_tokens_of_one_column():
         assert bool((part == 2).all())
     del a, out, part
     torch.cuda.empty_cache()
+
+
+# ---- 4-bit activations that no tensor map takes --------------------------------------------------------------------
+@pytest.mark.parametrize("M", [1, 8, 9, 16, 17])
+@pytest.mark.parametrize("spread", [4.0, 60.0])
+def test_4_bit_activations_off_16_bytes(M, spread):
+    """Codes of the activations that begin four bytes into a buffer: the streaming kernel takes up to 16 tokens of them, the multiply-add units more."""
+    m = mx()
+    N, K = 150, 1000
+    g = torch.Generator().manual_seed(M)
+    w, wv = _matrix(N, K, M)
+    a = torch.randn(M, K, generator=g) * torch.exp2(torch.round((torch.rand(M, 32, generator=g) - 0.5) * spread)).repeat_interleave(32, 1)[:, :K]
+    q = m.quantize_mxfp4(a.to(DEV))
+    n = q.codes.numel()
+    buf = torch.zeros(n + 16, dtype=torch.uint8, device=DEV)
+    buf[4:4 + n] = q.codes.flatten()
+    x = m.Mxfp4Matrix(buf[4:4 + n].view(M, -1), q.scales, K)
+    av = plain.rounded(a.to(DEV))
+    # values below 2^-39 of the largest of the 256 around them are not told from zero by the streaming kernel
+    pad = torch.nn.functional.pad(av.abs(), (0, -K % 256)).view(M, -1, 256).amax(-1)
+    wide = torch.nn.functional.pad(wv.abs(), (0, -K % 256)).view(N, -1, 256).sum(-1)
+    bound = _sum_bound(av, wv) + 2.0 ** -39 * (pad @ wide.t())
+    out = torch.empty(M, N, device=DEV)
+    m.gemm_mxfp4(x, w, out)
+    ops().raise_on_device_error()
+    _check(out, av @ wv.t(), bound, torch.float32)
+    gate, up = (av @ wv[:75].t()).clamp_min(0), av @ wv[75:].t()
+    out = torch.empty(M, 75, device=DEV)
+    m.gated_gemm_mxfp4(x, w, out, activation="relu")
+    ops().raise_on_device_error()
+    bg, bu = bound[:, :75], bound[:, 75:]
+    _check(out, gate * up, bg * up.abs() + gate * bu + bg * bu + 2.0 ** -23 * (gate * up).abs(), torch.float32)
+
+
+# ---- every plan ----------------------------------------------------------------------------------------------------
+def _force(library, dtype, name, *values):
+    from transformers_neuronx_b200.kernels import build
+    return getattr(build.load(library, dtype), name)(*values)
+
+
+def _all_results(m, w, wv, x, av, bias, dtype):
+    """The product and (an even number of rows) the gated one, checked."""
+    N = w.rows
+    exact, bound = av @ wv.t() + bias.double(), _sum_bound(av, wv)
+    bound = bound + 2.0 ** -23 * (exact.abs() + bias.double().abs())
+    out = torch.full((av.shape[0], N), float("nan"), device=DEV, dtype=dtype)
+    m.gemm_mxfp4(x, w, out, bias=bias)
+    ops().raise_on_device_error()
+    _check(out, exact, bound, dtype)
+    F = N // 2
+    out = torch.full((av.shape[0], F), float("nan"), device=DEV, dtype=dtype)
+    m.gated_gemm_mxfp4(x, w, out, bias=bias, activation="relu")
+    ops().raise_on_device_error()
+    gate, up, bg, bu = exact[:, :F].clamp_min(0), exact[:, F:], bound[:, :F], bound[:, F:]
+    _check(out, gate * up, bg * up.abs() + gate * bu + bg * bu + 2.0 ** -23 * (gate * up).abs(), dtype)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("splits", range(1, 9))
+def test_every_split_and_width_of_a_tile(splits, dtype):
+    m = mx()
+    N, K = 266, (2 * splits - 1) * 256 - 160               # two boxes a part, the last one's ragged
+    w, wv = _matrix(N, K, splits)
+    g = torch.Generator().manual_seed(splits)
+    bias = torch.randn(N, generator=g).to(DEV)
+    try:
+        for bn in (16, 32, 64, 128):
+            assert _force("gemm_mxfp4", dtype, "tnx_gemm_mxfp4_force", bn, splits) == 0
+            for M in (13, 117):
+                a = torch.randn(M, K, generator=g).to(dtype).to(DEV)
+                _all_results(m, w, wv, a, a.double(), bias, dtype)
+                _all_results(m, w, wv, m.quantize_mxfp4(a), plain.rounded(a), bias, dtype)
+    finally:
+        _force("gemm_mxfp4", dtype, "tnx_gemm_mxfp4_force", 0, 0)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("bn", range(64, 193, 16))
+def test_every_width_of_a_persistent_tile(bn, dtype, monkeypatch):
+    m = mx()
+    N, K = 1034, 544
+    w, wv = _matrix(N, K, bn)
+    g = torch.Generator().manual_seed(bn)
+    bias = torch.randn(N, generator=g).to(DEV)
+    monkeypatch.setattr(m, "_in_tiles", lambda *a: True)
+    try:
+        assert _force("gemm_mxfp4_tiles", dtype, "tnx_gemm_mxfp4_tiles_force", bn) == 0
+        for M in (129, 1500):
+            a = torch.randn(M, K, generator=g).to(dtype).to(DEV)
+            _all_results(m, w, wv, a, a.double(), bias, dtype)
+            _all_results(m, w, wv, m.quantize_mxfp4(a), plain.rounded(a), bias, dtype)
+    finally:
+        _force("gemm_mxfp4_tiles", dtype, "tnx_gemm_mxfp4_tiles_force", 0)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("splits", [1, 2, 4, 8])
+def test_every_plan_of_streamed_products(splits, dtype):
+    m = mx()
+    N, K = 266, 4000
+    w, wv = _matrix(N, K, splits)
+    g = torch.Generator().manual_seed(splits)
+    bias = torch.randn(N, generator=g).to(DEV)
+    try:
+        for wf in range(1, 16):
+            assert _force("gemv_mxfp4", dtype, "tnx_gemv_mxfp4_force", wf, splits) == 0
+            for M in (1, 7, 16) if dtype is torch.float32 else (1, 7):
+                a = torch.randn(M, K, generator=g).to(dtype).to(DEV)
+                _all_results(m, w, wv, a, a.double(), bias, dtype)
+    finally:
+        _force("gemv_mxfp4", dtype, "tnx_gemv_mxfp4_force", 0, 0)
+
+
+def test_forced_plans_that_are_none_are_refused():
+    for library, name, bad in (("gemm_mxfp4", "tnx_gemm_mxfp4_force", ((48, 0), (0, 9), (-16, 1))), ("gemm_mxfp4_tiles", "tnx_gemm_mxfp4_tiles_force", ((48,), (72,), (208,))),
+                               ("gemv_mxfp4", "tnx_gemv_mxfp4_force", ((16, 1), (1, 3), (-1, 0)))):
+        for values in bad:
+            assert _force(library, torch.bfloat16, name, *values) != 0

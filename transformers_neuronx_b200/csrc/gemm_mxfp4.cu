@@ -677,8 +677,12 @@ TNX_EXPORT long long tnx_gemm_mxfp4_estimate(int M, int N, int K, int gated, int
 // The most columns of K for whose 32-bit sums a tile's one accumulator is near enough (gemm_mxfp4_tiles.cu has one a tile).
 TNX_EXPORT int tnx_gemm_mxfp4_chain() { return MX_CHAIN; }
 
-// For sweeps and tests: the split of K (1 to 8) and the tokens of a tile whatever the sizes (0: the plan's own).
-TNX_EXPORT void tnx_gemm_mxfp4_force(int bn, int splits) { g_forced_bn = bn; g_forced_splits = splits; }
+// For tests: the tokens of a tile (16, 32, 64 or 128) and the split of K (1 to 8, where K allows it) whatever the sizes (0: the plan's own).
+TNX_EXPORT int tnx_gemm_mxfp4_force(int bn, int splits) {
+    if ((bn && bn != 16 && bn != 32 && bn != 64 && bn != 128) || splits < 0 || splits > 8) return TNX_ERR_BAD_ARG;
+    g_forced_bn = bn; g_forced_splits = splits;
+    return 0;
+}
 
 // 16-bit activations [M, K] (pitch lda, a multiple of 8 elements, 16-byte aligned) by codes [w_rows][blocks * 16] (16-byte aligned).
 TNX_EXPORT int tnx_gemm_mxfp4_16(const void* a, long long lda, const void* codes, const void* scales, const float* bias, const float* residual, void* out,

@@ -667,8 +667,12 @@ TNX_EXPORT long long tnx_gemm_mxfp4_tiles_estimate(int M, int N, int K, int gate
     return quantized ? rounds * ((K + CODE_K - 1) / CODE_K) * (300 + p.bn * 7 / 10) + 6500 : rounds * ((K + 127) / 128) * (500 + p.bn * 14 / 10) + 5000;
 }
 
-// For sweeps: the tokens of a tile (a multiple of 16 from 64 to 192) whatever the sizes (0: the plan's own).
-TNX_EXPORT void tnx_gemm_mxfp4_tiles_force(int bn) { g_forced_bn = bn; }
+// For tests: the tokens of a tile (a multiple of 16 from 64 to 192) whatever the sizes (0: the plan's own).
+TNX_EXPORT int tnx_gemm_mxfp4_tiles_force(int bn) {
+    if (bn && (bn < 64 || bn > MAX_BN || bn % 16)) return TNX_ERR_BAD_ARG;
+    g_forced_bn = bn;
+    return 0;
+}
 
 // 16-bit activations [M, K] (pitch lda, a multiple of 8 elements, 16-byte aligned) by codes [w_rows][blocks * 16] (16-byte aligned).
 TNX_EXPORT int tnx_gemm_mxfp4_tiles_16(const void* a, long long lda, const void* codes, const void* scales, const float* bias, const float* residual, void* out,

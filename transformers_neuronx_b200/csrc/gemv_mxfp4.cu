@@ -459,8 +459,12 @@ int g_forced_wf = 0, g_forced_splits = 0;
 }  // namespace
 
 constexpr int FEW_TOKENS = 16;               // of a launch; more go in slices
-// For sweeps and tests: groups of 16 rows a block (1 to 16) and the split of K (1, 2, 4 or 8) whatever the sizes (0: the plan's own).
-TNX_EXPORT void tnx_gemv_mxfp4_force(int wf, int splits) { g_forced_wf = wf; g_forced_splits = splits; }
+// For tests: groups of 16 rows a block (1 to 15) and the split of K (1, 2, 4 or 8, where K allows it) whatever the sizes (0: the plan's own).
+TNX_EXPORT int tnx_gemv_mxfp4_force(int wf, int splits) {
+    if (wf < 0 || wf > MAX_WARPS || splits < 0 || splits > 8 || (splits & (splits - 1))) return TNX_ERR_BAD_ARG;
+    g_forced_wf = wf; g_forced_splits = splits;
+    return 0;
+}
 
 // a_kind: 0 16-bit, 1 32-bit activations (pitch lda), 2 codes (4-byte aligned) with a_scales; codes of W 16-byte aligned.
 TNX_EXPORT int tnx_gemv_mxfp4(const void* a, int a_kind, const void* a_scales, long long lda, const void* codes, const void* scales, const float* bias,
