@@ -359,3 +359,20 @@ def test_forced_plans_that_are_none_are_refused():
                                ("gemv_mxfp4", "tnx_gemv_mxfp4_force", ((16, 1), (1, 3), (-1, 0)))):
         for values in bad:
             assert _force(library, torch.bfloat16, name, *values) != 0
+
+
+# ---- long sums of two 4-bit operands -------------------------------------------------------------------------------
+@pytest.mark.parametrize("M,N,K", [(16, 256, 20480), (64, 256, 65536), (200, 300, 20480), (300, 512, 65536)])
+def test_long_sums_of_4_bit_activations(M, N, K):
+    """One accumulator adds up all of K, 64 columns an addition: random operands whose scales spread over 2^8 lose less than 2^-20 of the result, as sums of
+    16-bit activations do in chains of a quarter of that."""
+    m = mx()
+    w, wv = _matrix(N, K, M + K, spread=8.0)
+    g = torch.Generator().manual_seed(K)
+    a = torch.randn(M, K, generator=g) * torch.exp2(torch.round((torch.rand(M, K // 32, generator=g) - 0.5) * 8)).repeat_interleave(32, 1)
+    a = a.bfloat16().to(DEV)
+    out = torch.empty(M, N, device=DEV)
+    m.gemm_mxfp4(m.quantize_mxfp4(a), w, out)
+    ops().raise_on_device_error()
+    want = plain.rounded(a) @ wv.t()
+    assert float((out.double() - want).norm() / want.norm()) <= 2.0 ** -20

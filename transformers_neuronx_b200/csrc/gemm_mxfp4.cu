@@ -644,7 +644,9 @@ int launch4(const void* a, const void* codes, Params& p, int tiles_w, int n_sms,
 }
 
 // Random operands, relative errors of 32-bit results: float16 3.8e-7 over chains of 4,096 columns, 1.2e-6 over 8,192, 5.5e-6 over 20,480; bfloat16, whose
-// products have fewer bits, 0.8e-7, 2.2e-7 and 1e-6 to 2e-6.
+// products have fewer bits, 0.8e-7, 2.2e-7 and 1e-6 to 2e-6.  With the limit, 100 bfloat16 tokens: 1.6e-7 over 20,480, 3.4e-7 over 40,960 where scales are alike,
+// 2.3e-6 and 4.5e-6 where they spread over 2^16; beyond eight chains, 40,960 columns, more again (6e-7 and 7.2e-6 over 65,536).  Both operands in 4 bits: an
+// addition for 64 columns; one accumulator's 0.7e-6 over 20,480 and 2.1e-6 over 65,536 (scales over 2^16; 0.5e-7 and 0.8e-7 over 2^8) need no limit.
 constexpr int MX_CHAIN = 5120;
 
 void fill(Params& p, const void* scales, const void* a_scales, const float* bias, const float* residual, void* out, int out_h16, long long ldc, int M, int N,

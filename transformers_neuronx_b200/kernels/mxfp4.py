@@ -27,7 +27,8 @@ from .ops import ACTIVATIONS, KernelError, _FLOATS, _H16, _check, _state, activa
 
 BLOCK = 32                                    # values that share a scale
 TILE_TOKENS = 128                             # beyond these persistent blocks walk over tiles of up to 192 tokens (gemm_mxfp4_tiles.cu)
-CHAIN = 5120                                  # 32-bit results: the columns that one accumulator adds up without a visible loss; beyond them K is split
+CHAIN = 5120                                  # 32-bit results of 16-bit activations: the columns that one accumulator adds up without a visible loss; beyond
+                                              # them K is split (up to eight ways); 4-bit ones take an addition for 64 columns instead of 16 and are not split for it
 MOST = 2**31 - 4096                           # rows or columns: kernels count both, rounded up to tiles, in 32 bits
 FEW_TOKENS = 16                               # the most that the kernel which streams the matrix through registers takes at a time (gemv_mxfp4.cu)
 
