@@ -142,3 +142,22 @@ def test_a_model_loads_only_the_libraries_it_names(which, amp, monkeypatch):
     monkeypatch.setattr(m, "_tiles", {})
     _steps(model, [tiny.random_ids(150, seed=s) for s in (1, 2)], 1)
     assert asked and asked <= named, sorted(asked - named)
+
+
+@pytest.mark.parametrize("amp", ["f16", "bf16", "f32"])
+def test_a_saved_model_keeps_the_builds_it_runs(amp, tmp_path):
+    """save() writes the libraries of the engine's own type, those of its 4-bit matrices among them."""
+    import os
+    from helpers import TinyModel
+    from transformers_neuronx_b200 import NeuronConfig, QuantizationConfig
+    from transformers_neuronx_b200.kernels import build
+    from transformers_neuronx_b200.opt.model import OPTForSampling
+    tiny = TinyModel("A", seed=1)
+    model = OPTForSampling.from_pretrained(tiny.folder, batch_size=1, amp=amp, n_positions=32,
+                                           neuron_config=NeuronConfig(quant=None if amp == "f32" else QuantizationConfig(activation_quant_dtype="mxfp4")))
+    model.to_neuron()
+    model.save(str(tmp_path))
+    act = model.model.act_dtype
+    named = build.with_flavour(model.model.libraries(act), act)
+    assert amp == "f32" or build.with_flavour(["gemm_mxfp4_tiles"], act)[0] in named
+    assert sorted(os.listdir(tmp_path)) == sorted(os.path.basename(build.library_path(n)) for n in named)

@@ -105,7 +105,8 @@ class OPTForSampling:
         """Writes the compiled kernel libraries this model uses into `directory`."""
         from ..kernels import build as kbuild
         self._ready()
-        kbuild.export_libraries(self.model.libraries(self.model.act_dtype), directory)
+        act = self.model.act_dtype
+        kbuild.export_libraries(kbuild.with_flavour(self.model.libraries(act), act), directory)
 
     def load(self, directory: str) -> None:
         """Call before to_neuron(): kernels compiled earlier (by save) from the same sources are
