@@ -6,7 +6,7 @@
 namespace {
 
 constexpr int TILE_W = 128;                  // rows of W a tile: the accumulator's lanes
-constexpr int KB = 64;                       // columns of K a pipeline stage holds in 16 bits
+constexpr int KB = 64;                       // columns of K in a block of 16-bit values, 128 bytes a row: stages hold two such blocks or a box's four
 constexpr int CODE_K = 256;                  // columns of K a box of codes holds: 128 bytes a row
 constexpr int CODE_BYTES = TILE_W * CODE_K / 2;
 

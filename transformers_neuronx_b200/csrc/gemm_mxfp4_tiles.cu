@@ -2,9 +2,10 @@
 //
 // Persistent CTAs, one an SM, walk over tiles of 128 rows of W (the lanes of an accumulator) by up to 192 tokens (its columns).  Two accumulators:
 // while one is written out by warps of their own, the MMAs fill the other.  (A CTA a tile, whose sums went through shared memory, spent 11 us a tile
-// outside of its main loop.)  2,048 tokens by 16,384 x 4,096: 223 us with 16-bit activations, 1.23 PFLOP/s, where the tensor cores are busy for
-// 61% of the time at 1.6 GHz, which the power limit leaves (no MMAs: 171 to 186 us, no decoding: 195 to 211, neither of them: 121, which is what the
-// activations' way from L2 takes); 69 us with 4-bit ones, 3.98 PFLOP/s, of which the loads alone take 56.
+// outside of its main loop.)  2,048 tokens by 16,384 x 4,096: 223 to 240 us with 16-bit activations, 1.15 to 1.23 PFLOP/s, where the tensor cores are busy
+// for 61% of the time at 1.6 GHz, which the power limit leaves (275 when run for seconds, 1 PFLOP/s; of 227, 186 or 171 are left without MMAs, 195 or 211
+// without decoding, 121 without either: what the activations' way from L2 takes); 69 to 73 us with 4-bit ones, 3.8 to 4 PFLOP/s, of which the loads alone
+// take 56.
 // Sums go straight from tensor memory to memory: a warp's lanes are 32 neighbouring features, so that a token's store is 64 or 128 bytes.
 // Gated tiles alternate eight gate rows and their eight up rows: gate and up values meet by one exchange of lanes eight apart.
 //

@@ -1,5 +1,5 @@
 // Products of a few tokens with a 4-bit matrix (formats: mxfp4.cuh; what is computed: gemm_mxfp4.cu).  The matrix is streamed once; what
-// bounds them is memory, or else the instructions that turn codes into operands, so these are few.  One token by 16,384 x 4,096 11.5 to 12 us,
+// bounds them is memory, or else the instructions that turn codes into operands, so these are few.  One token by 16,384 x 4,096 11 to 12 us,
 // 3 TB/s, of which 3.5 are what the smallest call takes (8.3 without scales, activations and arithmetic); eight 13 (float16) and 16 (bfloat16); one by
 // 5,120 x 20,480 18 us.
 //

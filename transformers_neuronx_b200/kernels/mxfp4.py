@@ -252,7 +252,8 @@ _tiles = {}                                   # sizes -> whether persistent tile
 
 def _in_tiles(M, N, K, gated, quantized, out_h16, kind, sms) -> bool:
     """More than TILE_TOKENS tokens: whether the kernel of persistent tiles takes them, or (few tiles, long K; 32-bit results of a long K) the one that
-    splits K over clusters.  Whichever is estimated to be faster; 2,048 tokens by 16,384 x 4,096 245 us in tiles, 330 split; 200 by 5,120 x 20,480 121 and 78."""
+    splits K over clusters.  Whichever is estimated to be faster; 2,048 tokens by 16,384 x 4,096 223 to 240 us in tiles, 323 split; 200 by 5,120 x 20,480
+    102 and 72."""
     key = (M, N, K, gated, quantized, out_h16, kind, sms)
     have = _tiles.get(key)
     if have is None:
